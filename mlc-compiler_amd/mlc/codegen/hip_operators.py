@@ -1,0 +1,315 @@
+"""Launches of the operators of ``mlc.ops``: rotary positions, attention with
+masks made from indices, the 8-bit cache and the attention over it.
+
+Their kernels are hand-written (``codegen/operators/*.hip``) and take every size
+and stride as an argument; what is fixed when they are compiled is the element
+type, the head size rounded up to a tile's, and which of the options the call
+uses. ``plan_*`` picks the kernel from sizes, types and alignment alone and lays
+its arguments out: pointers first, then what follows from the operands' shapes.
+The same plan serves a direct call and a compiled model.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+import pathlib
+import struct
+from dataclasses import dataclass
+
+import torch
+
+SOURCES = pathlib.Path(__file__).resolve().parent / "operators"
+NAMES = {torch.float16: "mlc::f16", torch.bfloat16: "__bf16", torch.float32: "float"}
+SHORT = {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
+LOG2E = math.log2(math.e)
+#: HIP takes fewer than 2^32 threads a launch
+MAX_THREADS = 2 ** 32 - 1
+#: compute units of an MI355X
+UNITS = 256
+
+
+class OperatorError(ValueError):
+    """Arguments that an operator of ``mlc.ops`` does not take."""
+
+
+@dataclass(frozen=True)
+class Operand:
+    """A tensor as a plan sees it; ``offset`` in bytes from the pointer that a
+    launch is given."""
+
+    shape: tuple
+    strides: tuple
+    dtype: torch.dtype
+    offset: int = 0
+    #: whether pointer and offset together are a multiple of 16
+    aligned: bool = True
+
+
+@dataclass(frozen=True)
+class Launch:
+    """One kernel launch: ``pointers`` names what its leading arguments point
+    to (None: a null pointer), ``tail`` are the bytes behind them."""
+
+    kernel: str  # the macro call that instantiates the kernel
+    file: str
+    symbol: str
+    grid: int
+    block: int
+    pointers: tuple
+    tail: bytes
+
+    def arguments(self, pointers: dict) -> bytes:
+        return struct.pack(f"<{len(self.pointers)}Q",
+                           *[0 if p is None else pointers[p] for p in self.pointers]) + self.tail
+
+
+@dataclass(frozen=True)
+class Plan:
+    launches: tuple
+    #: bytes of memory that the launches share and nobody reads afterwards
+    workspace: int = 0
+
+
+@functools.lru_cache(maxsize=None)
+def _text(file: str) -> str:
+    return (SOURCES / "common.hip").read_text() + (SOURCES / f"{file}.hip").read_text()
+
+
+def source(file: str, kernel: str) -> str:
+    """The module that holds one kernel."""
+    return f"{_text(file)}\n{kernel}\n"
+
+
+def _grid(blocks: int, threads: int, what: str) -> int:
+    if blocks * threads > MAX_THREADS:
+        raise OperatorError(f"{what}: {blocks} workgroups of {threads} threads are more than one "
+                            "launch takes; split the batch")
+    return blocks
+
+
+def _ceil(a: int, b: int) -> int:
+    return -(-a // b)
+
+
+def _numel(x: Operand) -> int:
+    return math.prod(x.shape)
+
+
+# --------------------------------------------------------------------------
+# rotary positions
+# --------------------------------------------------------------------------
+
+ROTARY_BLOCK, ROTARY_PAIRS = 256, 1024
+
+
+def rotary_kernel(dtype, v: int, interleaved: bool) -> tuple[str, str]:
+    name = f"rotary_{SHORT[dtype]}_v{v}_{'pairs' if interleaved else 'halves'}"
+    return f"ROTARY({name}, {NAMES[dtype]}, {v}, {str(bool(interleaved)).lower()})", name
+
+
+def plan_rotary(q: Operand, k: Operand, positions: Operand, frequencies: Operand,
+                interleaved: bool, magnitude: float) -> Plan:
+    batch, seq, heads, dim = q.shape
+    kv_heads = k.shape[2]
+    turned = 2 * frequencies.shape[0]
+    tokens = batch * seq
+    if tokens * (heads + kv_heads) * dim == 0:
+        return Plan(())
+    pack = 16 // q.dtype.itemsize
+    run = turned if interleaved else turned // 2
+    whole = all(n % pack == 0 for n in (dim, turned, run, *q.strides[:3], *k.strides[:3]))
+    v = pack if whole and q.aligned and k.aligned else 1
+    # enough workgroups first, then as many tokens of one as fill it
+    group = max(1, min(ROTARY_PAIRS // max(1, turned // 2), tokens // (4 * UNITS)))
+    blocks = min(_ceil(tokens, group), 1 << 22)
+    pb, pt = (0, positions.strides[0]) if len(positions.shape) == 1 else positions.strides
+    tail = struct.pack("<4q9q8ifi", q.offset, k.offset, positions.offset, frequencies.offset,
+                       *q.strides[:3], *k.strides[:3], pb, pt, frequencies.strides[0],
+                       tokens, seq, heads, kv_heads, dim, turned, group,
+                       positions.dtype == torch.int64, magnitude, 0)
+    kernel, name = rotary_kernel(q.dtype, v, interleaved)
+    return Plan((Launch(kernel, "rotary", name, blocks, ROTARY_BLOCK,
+                        ("q", "k", "positions", "frequencies", "out0", "out1"), tail),))
+
+
+# --------------------------------------------------------------------------
+# attention over keys and values in 16 bits
+# --------------------------------------------------------------------------
+
+ATTENTION_ROWS, ATTENTION_THREADS = 128, 256
+ATTENTION_DIMS = (64, 96, 128, 256)
+
+
+def _padded(dim: int, dims) -> int:
+    return next(d for d in dims if d >= dim)
+
+
+def score_scale(scale: float | None, dim: int) -> float:
+    return 1.0 / math.sqrt(max(dim, 1)) if scale is None else float(scale)
+
+
+def _factors(scale: float, cap: float) -> tuple[float, float]:
+    """What a score is multiplied by, and the cap in log2 units: the kernels'
+    exponentials are powers of two."""
+    return (scale / cap, cap * LOG2E) if cap else (scale * LOG2E, 0.0)
+
+
+def attention_kernel(dtype, dp: int, general: bool) -> tuple[str, str]:
+    name = f"attention_{SHORT[dtype]}_{dp}{'_general' if general else ''}"
+    return f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {str(general).lower()})", name
+
+
+def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
+                   documents: Operand | None, prefix: Operand | None, scale: float, causal: bool,
+                   cap: float) -> Plan:
+    batch, queries, heads, dim = q.shape
+    keys, kv_heads = k.shape[1:3]
+    if _numel(q) == 0:
+        return Plan(())
+    group = heads // kv_heads
+    tiles = _ceil(queries * group, ATTENTION_ROWS)
+    dp = _padded(dim, ATTENTION_DIMS)
+    general = bool(cap) or slopes is not None or documents is not None
+    some = lambda x, n: x.strides if x is not None else (0,) * n  # noqa: E731
+    off = lambda x: x.offset if x is not None else 0  # noqa: E731
+    tail = struct.pack("<6q13q8i2f", q.offset, k.offset, v.offset, off(slopes), off(documents),
+                       off(prefix), *q.strides[:3], *k.strides[:3], *v.strides[:3],
+                       *some(slopes, 1), *some(documents, 2), *some(prefix, 1),
+                       batch, queries, keys, kv_heads, group, dim, causal, tiles,
+                       *_factors(scale, cap))
+    kernel, name = attention_kernel(q.dtype, dp, general)
+    grid = _grid(tiles * batch * kv_heads, ATTENTION_THREADS, "attention")
+    pointers = ("q", "k", "v", "slopes" if slopes is not None else None,
+                "documents" if documents is not None else None,
+                "prefix" if prefix is not None else None, "out0")
+    return Plan((Launch(kernel, "attention", name, grid, ATTENTION_THREADS, pointers, tail),))
+
+
+# --------------------------------------------------------------------------
+# the 8-bit cache
+# --------------------------------------------------------------------------
+
+def append_kernel(dtype, align: int, n: int, waves: int) -> tuple[str, str]:
+    name = f"cache_append_{SHORT[dtype]}_a{align}_n{n}_w{waves}"
+    return f"CACHE_APPEND({name}, {NAMES[dtype]}, {align}, {n}, {waves})", name
+
+
+def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_scale: Operand,
+                      k: Operand, v: Operand, start: Operand, count: Operand | None) -> Plan:
+    batch, heads, capacity, dim = k_cache.shape
+    tokens = k.shape[1]
+    block = capacity // k_scale.shape[2] if k_scale.shape[2] else 1
+    if batch * heads * capacity * dim * tokens == 0:
+        return Plan(())
+    touched = min(capacity // block, (tokens + block - 2) // block + 1)
+    pack = 8
+    whole = all(n % pack == 0 for n in (*k.strides[:3], *v.strides[:3]))
+    align = 16 if whole and k.aligned and v.aligned else k.dtype.itemsize
+    # a workgroup's registers hold the new rows of a block: one wave where one
+    # item of 8 values for each lane is enough
+    items = min(tokens, block) * dim // 8
+    waves = 1 if items <= 64 else 4
+    n = 1 << (_ceil(items, 64 * waves) - 1).bit_length()
+    off = lambda x: x.offset if x is not None else 0  # noqa: E731
+    pair = lambda i: (k.strides[i], v.strides[i])  # noqa: E731
+    tail = struct.pack("<8q8q6i", k_cache.offset, v_cache.offset, k_scale.offset, v_scale.offset,
+                       k.offset, v.offset, start.offset, off(count), *pair(0), *pair(1), *pair(2),
+                       start.strides[0], count.strides[0] if count is not None else 0,
+                       tokens, heads, dim, capacity, block, touched)
+    kernel, name = append_kernel(k.dtype, align, n, waves)
+    grid = _grid(batch * touched * 2 * heads, 64 * waves, "cache_append")
+    pointers = ("k_cache", "v_cache", "k_scale", "v_scale", "k", "v", "start",
+                "count" if count is not None else None, "error")
+    return Plan((Launch(kernel, "cache_append", name, grid, 64 * waves, pointers, tail),))
+
+
+CACHED_DIMS = (64, 128, 256)
+
+
+def cached_kernel(dtype, dp: int, tall: int, step: int, waves: int, general: bool) -> tuple[str, str]:
+    name = f"cache_attention_{SHORT[dtype]}_{dp}_{tall}_{step}_{waves}{'_general' if general else ''}"
+    return (f"CACHE_ATTENTION({name}, {NAMES[dtype]}, {dp}, {tall}, {step}, {waves}, "
+            f"{str(general).lower()})"), name
+
+
+def join_kernel(dtype) -> tuple[str, str]:
+    name = f"cache_attention_join_{SHORT[dtype]}"
+    return f"CACHE_ATTENTION_JOIN({name}, {NAMES[dtype]})", name
+
+
+def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale: Operand,
+                         v_scale: Operand, start: Operand, count: Operand | None,
+                         slopes: Operand | None, scale: float, cap: float) -> Plan:
+    batch, tokens, heads, dim = q.shape
+    kv_heads, capacity = k_cache.shape[1:3]
+    if _numel(q) == 0:
+        return Plan(())
+    group, block = heads // kv_heads, capacity // k_scale.shape[2] if k_scale.shape[2] else 32
+    rows = tokens * group
+    dp = _padded(dim, CACHED_DIMS)
+    tall = 1 if rows <= 16 else 2 if rows <= 32 or dp == 256 else 4
+    row_tiles = _ceil(rows, 16 * tall)
+    step, waves = 64 if block % 64 == 0 else 32, 4
+    # items enough for the device, none shorter than two steps of every wave
+    shortest = 2 * 64 * waves
+    most = _ceil(capacity, shortest)
+    items = max(1, min(4 * UNITS // (kv_heads * row_tiles), batch * most))
+    slots = min(items + batch, batch * most)
+    general = bool(cap) or slopes is not None
+    off = lambda x: x.offset if x is not None else 0  # noqa: E731
+    tail = struct.pack("<8q6q8i2i2f", q.offset, k_cache.offset, v_cache.offset, k_scale.offset,
+                       v_scale.offset, off(slopes), start.offset, off(count), *q.strides[:3],
+                       slopes.strides[0] if slopes is not None else 0, start.strides[0],
+                       count.strides[0] if count is not None else 0, batch, tokens, kv_heads,
+                       group, dim, capacity, block.bit_length() - 1, row_tiles, items, shortest,
+                       *_factors(scale, cap))
+    kernel, name = cached_kernel(q.dtype, dp, tall, step, waves, general)
+    pointers = ("q", "k_cache", "v_cache", "k_scale", "v_scale",
+                "slopes" if slopes is not None else None, "start",
+                "count" if count is not None else None, "out0",
+                "workspace" if most > 1 else None, "error")
+    grid = _grid(slots * row_tiles * kv_heads, 64 * waves, "cache_attention")
+    launches = [Launch(kernel, "cache_attention", name, grid, 64 * waves, pointers, tail)]
+    workspace = 0
+    if most > 1:  # a sequence may be cut
+        workspace = slots * kv_heads * rows * (dim + 4) * 4
+        join, join_name = join_kernel(q.dtype)
+        launches.append(Launch(join, "cache_attention", join_name,
+                               _grid(batch * tokens * heads, 64, "cache_attention"), 64, pointers,
+                               tail))
+    return Plan(tuple(launches), workspace)
+
+
+#: operators of a captured graph -> the plan of their operands, by their names in
+#: the operator's schema
+PLANS = {
+    "mlc.rotary.default": plan_rotary,
+    "mlc.attention.default": lambda q, k, v, scale, causal, cap, slopes, documents, prefix:
+        plan_attention(q, k, v, slopes, documents, prefix, score_scale(scale, q.shape[3]), causal, cap),
+    "mlc.cache_append.default": plan_cache_append,
+    "mlc.cache_attention.default":
+        lambda q, k_cache, v_cache, k_scale, v_scale, start, count, scale, cap, slopes:
+        plan_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, slopes,
+                             score_scale(scale, q.shape[3]), cap),
+}
+#: those that can meet an invalid input
+FLAGGING = ("mlc.cache_append.default", "mlc.cache_attention.default")
+
+
+def all_kernels() -> list[tuple[str, str]]:
+    """``(file, kernel)`` of everything that a plan can ask for."""
+    out = []
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        out += [("rotary", rotary_kernel(dtype, v, i)[0]) for v in (16 // dtype.itemsize, 1)
+                for i in (False, True)]
+        out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
+                for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
+    for dtype in (torch.float16, torch.bfloat16):
+        out += [("attention", attention_kernel(dtype, dp, g)[0]) for dp in ATTENTION_DIMS
+                for g in (False, True)]
+        out += [("cache_attention", cached_kernel(dtype, dp, tall, step, 4, g)[0])
+                for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
+                for step in (32, 64) for g in (False, True)]
+        out.append(("cache_attention", join_kernel(dtype)[0]))
+    return out

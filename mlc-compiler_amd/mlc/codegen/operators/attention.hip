@@ -1,0 +1,320 @@
+// Attention of queries over keys and values in 16 bits, with the masks made from
+// indices instead of read: out = softmax(mask(bias(cap(scale q k^T)))) v, fp32
+// softmax, a row with nothing visible all zeros.
+//
+// Rows are (token, head of a group) pairs: all heads that share keys and values
+// go through one workgroup, which so reads them once. A workgroup of 4 waves has
+// 128 rows, a wave 32 of them, one row in lanes c and c + 32. Keys pass in tiles
+// of 64 through LDS.
+//  * S^T = K Q^T on 32x32x16 products: lane (c, h) ends with row c's scores. The
+//    rows of K are taken in the order that makes them tokens 16 i + 8 h .. + 7,
+//    the B operand of O^T = V^T P^T: probabilities never leave their lane.
+//  * V^T's operand is read transposed from V's rows (ds_read_b64_tr_b16).
+//  * The softmax is online: a running maximum, the sum and O scaled when it grows.
+
+namespace mlc {
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+struct AttentionArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* slopes;     // null: no bias by distance
+  const void* documents;  // null: one document
+  const void* prefix;     // null: none
+  void* out;
+  int64_t q_off, k_off, v_off, s_off, d_off, p_off;      // bytes
+  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ss, db, dt, ps;  // elements
+  int32_t batch, queries, keys, kv_heads, group, dim, causal, tiles;
+  float scale, cap;  // scale times log2 e where cap is 0, else 1/cap of it and cap log2 e
+};
+
+constexpr int ATT_WAVES = 4, ATT_ROWS = 32 * ATT_WAVES, ATT_KEYS = 64;
+
+template <class T> struct vec8;
+template <> struct vec8<f16> { typedef half8 type; static constexpr uint32_t exponent = 0x7c00u; };
+template <> struct vec8<__bf16> { typedef bf16x8 type; static constexpr uint32_t exponent = 0x7f80u; };
+
+__device__ __forceinline__ float16v mfma_32x32x16(half8 a, half8 b, float16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16v mfma_32x32x16(bf16x8 a, bf16x8 b, float16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// 16-byte slot of chunk ``c`` of row ``r``: a row is PC slots of 256 (DP 64: 128)
+// bytes and its slots are xor-ed with its number, so that 16 rows of one chunk,
+// and 4 rows of 4 chunks, each lie in 64 distinct banks.
+template <int PC> __device__ __forceinline__ int slot(int r, int c) {
+  if constexpr (PC == 8) return r * 8 + (c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)));
+  return r * PC + (c ^ (((r & 3) << 2) | ((r >> 2) & 3)));
+}
+
+// Four tokens of 16 values, one a lane: lane i of 16 gives the address of values
+// 4 (i % 4) .. + 3 of token i / 4 and gets value i of the four tokens.
+__device__ __forceinline__ h4 read_transposed(const void* p) {
+  return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) short4v*)p));
+}
+
+template <uint32_t E> __device__ __forceinline__ bool not_finite(uint4v x) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bad |= (x[i] & E) == E || (x[i] & (E << 16)) == (E << 16);
+  return bad;
+}
+
+template <class T, int DP, bool GENERAL>
+__device__ __forceinline__ void attention(const AttentionArgs& a) {
+  typedef typename vec8<T>::type v8;
+  constexpr int PC = DP == 64 ? 8 : DP <= 128 ? 16 : 32;  // 16-byte slots of an LDS row
+  constexpr int CH = DP / 8;                               // of which hold values
+  constexpr int THREADS = 64 * ATT_WAVES;
+  constexpr int N = ATT_KEYS * CH / THREADS;
+  static_assert(ATT_KEYS * CH % THREADS == 0, "staging");
+  __shared__ __attribute__((aligned(1024))) uint4v lk[ATT_KEYS * PC], lv[ATT_KEYS * PC];
+  __shared__ int ldoc[ATT_KEYS];
+  __shared__ int spoiled[2];  // whether a tile that is masked in part has V values not finite
+  __shared__ __attribute__((aligned(16))) T lp[ATT_WAVES][32][16];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int rows = a.queries * a.group;
+  // the tiles of one (batch, head) go to one XCD where there are enough, long ones first
+  const int pairs = a.batch * a.kv_heads;
+  int pair, tile;
+  if (pairs % 8 == 0) {
+    const int i = blockIdx.x / 8;
+    pair = i / a.tiles * 8 + blockIdx.x % 8;
+    tile = a.tiles - 1 - i % a.tiles;
+  } else {
+    pair = blockIdx.x % pairs;
+    tile = a.tiles - 1 - blockIdx.x / pairs;
+  }
+  const int b = pair / a.kv_heads, hk = pair % a.kv_heads;
+
+  const int shift = a.keys - a.queries;  // position of query 0
+  const int prefix = a.prefix ? at<int32_t>(a.prefix, a.p_off)[b * a.ps] : 0;
+  // last key that query ``t`` may see
+  auto last = [&](int t) {
+    int lim = a.keys - 1;
+    if (a.causal) {
+      const int own = t + shift > prefix - 1 ? t + shift : prefix - 1;
+      lim = own < lim ? own : lim;
+    }
+    return lim;
+  };
+  const int row = tile * ATT_ROWS + wave * 32 + c;
+  const int r = row < rows ? row : rows - 1;  // rows past the end repeat the last, and are not stored
+  const int t = r / a.group, head = hk * a.group + r % a.group;
+  const int32_t* const doc = at<int32_t>(a.documents, a.d_off) + b * a.db;
+  const int mine = GENERAL && a.documents ? doc[(t + shift) * a.dt] : 0;
+  const int lim = mine < 0 ? -1 : last(t);
+  const int first_row = tile * ATT_ROWS, end_row = first_row + ATT_ROWS < rows ? first_row + ATT_ROWS : rows;
+  const int wave_row = first_row + wave * 32;
+  const int lim_wg = last((end_row - 1) / a.group);
+  const int lim_wg_min = last(first_row / a.group);
+  const int lim_wave = wave_row < rows ? last(((wave_row + 31 < rows ? wave_row + 31 : rows - 1)) / a.group) : -1;
+  const int lim_wave_min = wave_row < rows ? last(wave_row / a.group) : -1;
+  const int tiles = lim_wg < 0 ? 0 : lim_wg / ATT_KEYS + 1;
+
+  v8 q[DP / 16];
+  {
+    const T* p = at<T>(a.q, a.q_off) + b * a.qb + (int64_t)t * a.qt + head * a.qh;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      T x[8] = {};
+      if (16 * s + 8 * h < a.dim) load_n<2>(x, p + 16 * s + 8 * h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[s][i] = x[i];
+    }
+  }
+  float slope = 0.0f;
+  if (GENERAL && a.slopes) slope = at<float>(a.slopes, a.s_off)[head * a.ss] * 0x1.715476p+0f;
+
+  const T* const kp = at<T>(a.k, a.k_off) + b * a.kb + hk * a.kh;
+  const T* const vp = at<T>(a.v, a.v_off) + b * a.vb + hk * a.vh;
+  T rk[N][8], rv[N][8];
+  auto load = [&](int kt) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = threadIdx.x + n * THREADS, key = kt * ATT_KEYS + i / CH, d = i % CH * 8;
+      if (key < a.keys && d < a.dim) {
+        load_n<2>(rk[n], kp + key * a.kt + d);
+        load_n<2>(rv[n], vp + key * a.vt + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rk[n][j] = rv[n][j] = (T)0.0f;
+      }
+    }
+  };
+
+  float16v o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+  float m = -__builtin_inff(), l = 0.0f;
+  // token of a 32-token half tile that row c of the score product is
+  const int token = ((c >> 4) << 4) | (((c >> 2) & 1) << 3) | (((c >> 3) & 1) << 2) | (c & 3);
+
+  if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
+  if (tiles > 0) load(0);
+  for (int kt = 0; kt < tiles; ++kt) {
+    const bool partial = GENERAL && a.documents ? true : lim_wg_min < (kt + 1) * ATT_KEYS - 1;
+    __syncthreads();
+    bool bad = false;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = threadIdx.x + n * THREADS, at_slot = slot<PC>(i / CH, i % CH);
+      lk[at_slot] = __builtin_bit_cast(uint4v, rk[n]);
+      const uint4v x = __builtin_bit_cast(uint4v, rv[n]);
+      lv[at_slot] = x;
+      if (partial) bad |= not_finite<vec8<T>::exponent>(x);
+    }
+    if (partial && bad) spoiled[kt & 1] = 1;
+    if (GENERAL && a.documents && threadIdx.x < ATT_KEYS) {
+      const int key = kt * ATT_KEYS + threadIdx.x;
+      ldoc[threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) spoiled[(kt + 1) & 1] = 0;
+    if (kt + 1 < tiles) load(kt + 1);
+    const int base = kt * ATT_KEYS;
+    if (base > lim_wave) continue;
+
+    float16v s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i)
+        s[u] = mfma_32x32x16(__builtin_bit_cast(v8, lk[slot<PC>(32 * u + token, 2 * i + h)]), q[i], s[u]);
+    }
+    float scale = a.scale;
+    if constexpr (GENERAL) {
+      // in log2 units: the cap, then the bias
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x = s[u][j] * a.scale;
+          if (a.cap != 0.0f) {
+            // tanh y = 1 - 2 / (e^2y + 1)
+            const float e = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
+            x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(e + 1.0f);
+          }
+          if (a.slopes) {
+            const int key = base + 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
+            x = __builtin_fmaf(-slope, __builtin_fabsf((float)(key - (t + shift))), x);
+          }
+          s[u][j] = x;
+        }
+      scale = 1.0f;
+    }
+    const bool masked = lim_wave_min < base + ATT_KEYS - 1 || (GENERAL && a.documents);
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int k = 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
+          bool seen = base + k <= lim;
+          if (GENERAL && a.documents) seen = seen && ldoc[k] == mine;
+          s[u][j] = seen ? s[u][j] : -__builtin_inff();
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = __builtin_fmaxf(top, s[u][j]);
+    top = xor32<OpMax>(top * scale);
+    if (top > m) {
+      const float alpha = __builtin_amdgcn_exp2f(m - top);  // m = -inf: 0, as O and l are
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
+      l *= alpha;
+      m = top;
+    }
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    v8 p[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], scale, -ref));
+        l += e;
+        p[2 * u + (j >> 3)][j & 7] = (T)e;
+      }
+    if (!(partial && spoiled[kt & 1])) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int g = lane & 15, d = 32 * i + 16 * ((lane >> 4) & 1) + 4 * (g & 3);
+          const int k = 16 * u + 8 * h + (g >> 2);
+          const h4 lo = read_transposed(reinterpret_cast<const char*>(lv + slot<PC>(k, d >> 3)) + (d & 7) * 2);
+          const h4 hi = read_transposed(reinterpret_cast<const char*>(lv + slot<PC>(k + 4, d >> 3)) + (d & 7) * 2);
+          const half8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[i] = mfma_32x32x16(__builtin_bit_cast(v8, w), p[u], o[i]);
+        }
+    } else {
+      // 0 times an infinity or NaN of a key that a row does not see is NaN in the
+      // product: row by row, over the keys it sees
+      const T* const value = reinterpret_cast<const T*>(lv);
+#pragma unroll 1
+      for (int u = 0; u < 4; ++u) {
+        // p[u] by a constant index only: it stays in registers
+        const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
+        *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j) {
+          const float x = element<T>::widen(lp[wave][c][j]);
+          if (x == 0.0f) continue;
+          const int k = 16 * u + j;
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int z = 0; z < 16; ++z) {
+              const int d = 32 * i + 8 * (z >> 2) + 4 * h + (z & 3);
+              o[i][z] += x * element<T>::widen(value[slot<PC>(k, d >> 3) * 8 + (d & 7)]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+  if (row >= rows) return;
+  l = xor32<OpSum>(l);
+  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+  T* const out = reinterpret_cast<T*>(a.out) +
+                 (((int64_t)b * a.queries + t) * a.kv_heads * a.group + head) * a.dim;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      const int d = 32 * i + 8 * z + 4 * h;
+      if (d < a.dim) {
+        T x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = element<T>::narrow(o[i][4 * z + j] * inverse);
+        store_n<8>(out + d, x);
+      }
+    }
+}
+
+}  // namespace mlc
+
+#define ATTENTION(NAME, T, DP, GENERAL)                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * mlc::ATT_WAVES) NAME(mlc::AttentionArgs a) { \
+    mlc::attention<T, DP, GENERAL>(a);                                                        \
+  }

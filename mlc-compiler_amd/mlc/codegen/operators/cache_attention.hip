@@ -1,0 +1,437 @@
+// Attention of the newest tokens over the 8-bit cache: token i of a sequence stands
+// at position start + i and sees the keys up to its own. Rows are (token, head of
+// a group) pairs, 16 * RT to a workgroup, so keys and values are read once for all
+// heads that share them.
+//
+// Bound by memory where rows are few: the cache is read once, 2 (dim + 4 / block)
+// bytes a key and head. A sequence's keys are cut into items; how long an item is
+// follows from the lengths that the sequences have on the device, so that every
+// workgroup has about as much to read whatever the lengths. Each wave of an item
+// takes its own keys straight into registers:
+//  * S^T = K Q^T on 16x16x32 products; the order of K's rows makes lane (c, g) end
+//    with row c's scores of keys 8 g .. 8 g + 7 of every 32, the B operand of
+//  * O^T = V^T P^T, whose V^T operand is made of V's rows by byte permutes. P is
+//    fp16 whatever the queries are: e4m3 is exact in it and P is below 1.
+//  * A key block's scales are powers of two outside the products: K's goes into the
+//    factor of its scores, V's multiplies the block's part of O.
+// The waves of a workgroup are joined in LDS, the items of a sequence by a second
+// kernel (cache_attention_join).
+
+namespace mlc {
+
+struct CacheAttentionArgs {
+  const void* q;
+  const void* cache[2];
+  const void* scale[2];
+  const void* slopes;  // null: no bias by distance
+  const void* start;
+  const void* count;  // null: every token is real
+  void* out;
+  float* part;  // [item][kv head][row][dim + 4]: O not normalised, its maximum and sum
+  int* error;
+  int64_t q_off, cache_off[2], scale_off[2], sl_off, start_off, count_off;  // bytes
+  int64_t qb, qt, qh, sls, ss, sc;                                          // elements
+  int32_t batch, tokens, kv_heads, group, dim, capacity, block_shift, row_tiles;
+  int32_t items, shortest;  // items wanted of all sequences; keys of the shortest one
+  float factor, cap;
+};
+
+// Keys of a sequence that its tokens may see; 0 for one that is refused.
+__device__ __forceinline__ int held(const CacheAttentionArgs& a, int b, int& start, int& count) {
+  start = at<int32_t>(a.start, a.start_off)[b * a.ss];
+  count = a.count ? at<int32_t>(a.count, a.count_off)[b * a.sc] : a.tokens;
+  const bool ok = start >= 0 && count >= 0 && count <= a.tokens &&
+                  (int64_t)start + count <= a.capacity;
+  if (!ok) count = -1;
+  return count > 0 ? start + count : 0;
+}
+
+struct Item {
+  int b, nth, of, length, keys;  // the nth of a sequence's items, ``length`` keys each
+};
+
+// How the sequences' keys are cut: every wave finds it again from the lengths.
+// ``want`` < 0: the first item of sequence -1 - want.
+__device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want, Item& found, int& first) {
+  const int lane = threadIdx.x & 63;
+  int start, count;
+  int64_t total = 0;
+  for (int b = lane; b < a.batch; b += 64) total += held(a, b, start, count);
+  total = group_reduce<64, OpSum, int64_t>(total);
+  int64_t length = (total + a.items - 1) / a.items;
+  length = (length + 63) / 64 * 64;
+  if (length > a.capacity) length = ((int64_t)a.capacity + 63) / 64 * 64;
+  const int c = length > a.shortest ? (int)length : a.shortest;
+  first = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane, keys = b < a.batch ? held(a, b, start, count) : 0;
+    const int n = b < a.batch ? (keys + c - 1) / c + (keys == 0) : 0;
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = __shfl_up(sum, d, 64);
+      sum += lane >= d ? other : 0;
+    }
+    const uint64_t past = want >= 0 ? __ballot(first + sum > want) : __ballot(b == -1 - want);
+    if (past) {
+      const int at_lane = __builtin_ctzll(past);
+      found.b = b0 + at_lane;
+      found.of = __shfl(n, at_lane, 64);
+      found.keys = __shfl(keys, at_lane, 64);
+      found.length = c;
+      first += __shfl(sum, at_lane, 64) - found.of;
+      found.nth = want >= 0 ? want - first : 0;
+      return true;
+    }
+    first += __shfl(sum, 63, 64);
+  }
+  return false;
+}
+
+template <class T> struct codes;
+template <> struct codes<f16> {
+  typedef half8 v8;
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
+};
+template <> struct codes<__bf16> {
+  typedef bf16x8 v8;
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  }
+};
+
+template <int W> struct words { uint32_t x[W]; };
+
+template <class T, int DP, int RT, int TOK, int WAVES, bool GENERAL>
+__device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
+  typedef typename codes<T>::v8 v8;
+  constexpr int KP = DP / 64;   // 16-byte pieces of a key's row per lane
+  constexpr int VB = DP / 16;   // bytes of a value's row per lane
+  constexpr int VW = VB / 4;    // and words
+  constexpr int CH = TOK / 32;  // chunks of 32 keys a step
+  __shared__ __attribute__((aligned(16))) float lo[WAVES][16][DP + 4];
+  __shared__ float lm[WAVES][16], ll[WAVES][16];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  uint32_t w = blockIdx.x;
+  const int hk = (int)(w % (uint32_t)a.kv_heads);
+  w /= (uint32_t)a.kv_heads;
+  const int rt0 = (int)(w % (uint32_t)a.row_tiles);
+  w /= (uint32_t)a.row_tiles;
+  Item item;
+  int first;
+  if (!find_item(a, (int)w, item, first)) return;
+  const int b = __builtin_amdgcn_readfirstlane(item.b);
+  int start, count;
+  held(a, b, start, count);
+  if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
+  const int lo_key = item.nth * item.length;
+  const int hi_key = lo_key + item.length < item.keys ? lo_key + item.length : item.keys;
+
+  const int rows = a.tokens * a.group;
+  v8 q[RT][2 * KP];
+  int lim[RT], pos[RT];
+  float slope[RT];
+  int lim_min = 0x7fffffff;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = (rt0 * RT + rt) * 16 + c, r = row < rows ? row : rows - 1;
+    const int t = r / a.group, head = hk * a.group + r % a.group;
+    pos[rt] = start + t;
+    lim[rt] = t < count ? start + t : -1;
+    lim_min = lim[rt] < lim_min ? lim[rt] : lim_min;
+    slope[rt] = GENERAL && a.slopes ? at<float>(a.slopes, a.sl_off)[head * a.sls] * 0x1.715476p+0f : 0.0f;
+    const T* p = at<T>(a.q, a.q_off) + b * a.qb + t * a.qt + head * a.qh;
+#pragma unroll
+    for (int s = 0; s < 2 * KP; ++s) {
+      const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      T x[8] = {};
+      if (d < a.dim) load_n<2>(x, p + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[rt][s][i] = x[i];
+    }
+  }
+  // the least of the rows' last keys: steps below it need no mask
+  for (int d = 1; d < 16; d <<= 1) {
+    const int other = __shfl_xor(lim_min, d, 64);
+    lim_min = other < lim_min ? other : lim_min;
+  }
+  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+
+  const int64_t head_at = ((int64_t)b * a.kv_heads + hk) * a.capacity;
+  const uint8_t* const kc = at<uint8_t>(a.cache[0], a.cache_off[0]) + head_at * a.dim;
+  const uint8_t* const vc = at<uint8_t>(a.cache[1], a.cache_off[1]) + head_at * a.dim;
+  const float* const ks = at<float>(a.scale[0], a.scale_off[0]) + (head_at >> a.block_shift);
+  const float* const vs = at<float>(a.scale[1], a.scale_off[1]) + (head_at >> a.block_shift);
+
+  float m[RT], l[RT];
+  float4v o[RT][VB];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -__builtin_inff();
+    l[rt] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VB; ++j) o[rt][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const int krow = 8 * (c >> 2) + (c & 3);
+  const bool v_mine = c * VB < a.dim;
+
+  for (int tb = lo_key + wave * TOK; tb < hi_key; tb += WAVES * TOK) {
+    uint4v kr[CH][2][KP];
+    words<VW> vr[CH][8];
+    const bool whole = tb + TOK <= hi_key;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int s = 0; s < KP; ++s) {
+          const int key = tb + 32 * ch + krow + 4 * u, d = 64 * s + 16 * g;
+          if (d < a.dim && (whole || key < hi_key))
+            kr[ch][u][s] = *reinterpret_cast<const uint4v*>(kc + (int64_t)key * a.dim + d);
+          else
+            kr[ch][u][s] = uint4v{0, 0, 0, 0};
+        }
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = tb + 32 * ch + 8 * g + i;
+        if (v_mine && (whole || key < hi_key))
+          vr[ch][i] = *reinterpret_cast<const words<VW>*>(vc + (int64_t)key * a.dim + c * VB);
+        else
+          vr[ch][i] = words<VW>{};
+      }
+    const float kscale = ks[tb >> a.block_shift], vscale = vs[tb >> a.block_shift];
+    const bool masked = tb + TOK - 1 > lim_min;
+
+    float4v s[RT][CH][2];
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 2 * KP; ++i) {
+          uint4v k;
+          const uint32_t w0 = kr[ch][u][i >> 1][(i & 1) * 2], w1 = kr[ch][u][i >> 1][(i & 1) * 2 + 1];
+          k.x = codes<T>::widen(w0, 0);
+          k.y = codes<T>::widen(w0, 1);
+          k.z = codes<T>::widen(w1, 0);
+          k.w = codes<T>::widen(w1, 1);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            if (i == 0) s[rt][ch][u] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            s[rt][ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[rt][i], s[rt][ch][u]);
+          }
+        }
+    half8 p[RT][CH];
+    float alpha[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float factor = a.factor * kscale;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = s[rt][ch][e >> 2][e & 3] * factor;
+          const int key = tb + 32 * ch + 8 * g + e;
+          if constexpr (GENERAL) {
+            if (a.cap != 0.0f) {
+              // tanh y = 1 - 2 / (e^2y + 1)
+              const float z = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
+              x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(z + 1.0f);
+            }
+            if (a.slopes) x = __builtin_fmaf(-slope[rt], __builtin_fabsf((float)(key - pos[rt])), x);
+          }
+          if (masked) x = key <= lim[rt] ? x : -__builtin_inff();
+          s[rt][ch][e >> 2][e & 3] = x;
+          top = __builtin_fmaxf(top, x);
+        }
+      top = xor32<OpMax>(xor16<OpMax>(top));
+      const float now = top > m[rt] ? top : m[rt];
+      const float ref = now == -__builtin_inff() ? 0.0f : now;
+      alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - ref);
+      m[rt] = now;
+      l[rt] *= alpha[rt];
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(s[rt][ch][e >> 2][e & 3] - ref);
+          l[rt] += x;
+          p[rt][ch][e] = (f16)x;
+        }
+    }
+    // a value that is NaN and that some row does not see would spoil the row: 0 * NaN
+    bool spoiled = false;
+    if (masked) {
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int z = 0; z < VW; ++z) {
+            // a byte of 0x7f carries into its top bit when 1 is added to its low seven
+            const uint32_t x = (vr[ch][i].x[z] & 0x7f7f7f7fu) + 0x01010101u;
+            spoiled |= (x & 0x80808080u) != 0;
+          }
+      spoiled = __any(spoiled);
+    }
+    float4v add[RT][VB];
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+      for (int z = 0; z < VW; ++z) {
+        uint32_t f[4][4];  // [byte][pair of tokens]
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t t0 = vr[ch][2 * i].x[z], t1 = vr[ch][2 * i + 1].x[z];
+          const uint32_t even = __builtin_amdgcn_perm(t1, t0, 0x05010400u);
+          const uint32_t odd = __builtin_amdgcn_perm(t1, t0, 0x07030602u);
+          f[0][i] = codes<f16>::widen(even, 0);
+          f[1][i] = codes<f16>::widen(even, 1);
+          f[2][i] = codes<f16>::widen(odd, 0);
+          f[3][i] = codes<f16>::widen(odd, 1);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          half8 v = __builtin_bit_cast(half8, uint4v{f[y][0], f[y][1], f[y][2], f[y][3]});
+          half8 nan = {};
+          if (spoiled) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              nan[i] = v[i] != v[i] ? (f16)1.0f : (f16)0.0f;
+              v[i] = v[i] != v[i] ? (f16)0.0f : v[i];
+            }
+          }
+          const int j = 4 * z + y;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            if (ch == 0) add[rt][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            add[rt][j] = mfma_16x16x32(v, p[rt][ch], add[rt][j]);
+            if (spoiled) {
+              // rows that see one of the NaN values get a NaN
+              half8 sees;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                sees[e] = tb + 32 * ch + 8 * g + e <= lim[rt] ? (f16)1.0f : (f16)0.0f;
+              const float4v hits = mfma_16x16x32(nan, sees, float4v{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (hits[i] > 0.0f) add[rt][j][i] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[rt][j][i] = __builtin_fmaf(add[rt][j][i], vscale, o[rt][j][i] * alpha[rt]);
+  }
+
+  // the waves' rows together; thread (row of 16, 4 values) at a time
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] = xor32<OpSum>(xor16<OpSum>(l[rt]));
+    if (rt > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < VB; j += 4)
+        *reinterpret_cast<float4v*>(&lo[wave][c][VB * (4 * g + i) + j]) =
+            float4v{o[rt][j][i], o[rt][j + 1][i], o[rt][j + 2][i], o[rt][j + 3][i]};
+    if (g == 0) {
+      lm[wave][c] = m[rt];
+      ll[wave][c] = l[rt];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (DP / 4); i += 64 * WAVES) {
+      const int y = i / (DP / 4), d = i % (DP / 4) * 4;
+      const int row = (rt0 * RT + rt) * 16 + y;
+      if (row >= rows || d >= a.dim) continue;
+      float top = lm[0][y];
+#pragma unroll
+      for (int z = 1; z < WAVES; ++z) top = __builtin_fmaxf(top, lm[z][y]);
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float4v x = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int z = 0; z < WAVES; ++z) {
+        const float f = __builtin_amdgcn_exp2f(lm[z][y] - ref);
+        sum = __builtin_fmaf(ll[z][y], f, sum);
+        const float4v v = *reinterpret_cast<const float4v*>(&lo[z][y][d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
+      }
+      if (item.of == 1) {
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int t = row / a.group, head = hk * a.group + row % a.group;
+        T v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(x[e] * inverse);
+        store_n<8>(reinterpret_cast<T*>(a.out) +
+                   (((int64_t)b * a.tokens + t) * a.kv_heads * a.group + head) * a.dim + d, v);
+      } else {
+        float* const part = a.part + (((int64_t)w * a.kv_heads + hk) * rows + row) * (a.dim + 4);
+        *reinterpret_cast<float4v*>(part + d) = x;
+        if (d == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{top, sum, 0.0f, 0.0f};
+      }
+    }
+  }
+}
+
+// One workgroup of 64 for each (sequence, token, head): its items' parts as one.
+template <class T> __device__ __forceinline__ void cache_attention_join(const CacheAttentionArgs& a) {
+  const int heads = a.kv_heads * a.group;
+  const int head = (int)(blockIdx.x % (uint32_t)heads);
+  const uint32_t w = blockIdx.x / (uint32_t)heads;
+  const int t = (int)(w % (uint32_t)a.tokens), b = (int)(w / (uint32_t)a.tokens);
+  Item item;
+  int first;
+  if (!find_item(a, -1 - b, item, first) || item.of == 1) return;
+  const int hk = head / a.group, rows = a.tokens * a.group, row = t * a.group + head % a.group;
+  const int64_t step = (int64_t)a.kv_heads * rows * (a.dim + 4);
+  const float* const part = a.part + (((int64_t)first * a.kv_heads + hk) * rows + row) * (a.dim + 4);
+  float top = -__builtin_inff();
+  for (int i = threadIdx.x; i < item.of; i += 64) top = __builtin_fmaxf(top, part[i * step + a.dim]);
+  top = group_reduce<64, OpMax>(top);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  float x[4] = {}, sum = 0.0f;
+  const int d = threadIdx.x * 4;
+  for (int i = 0; i < item.of; ++i) {
+    const float4v ml = *reinterpret_cast<const float4v*>(part + i * step + a.dim);
+    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+    sum = __builtin_fmaf(ml.y, f, sum);
+    if (d < a.dim) {
+      const float4v v = *reinterpret_cast<const float4v*>(part + i * step + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
+    }
+  }
+  if (d >= a.dim) return;
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(x[e] * inverse);
+  store_n<8>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.tokens + t) * heads + head) * a.dim + d, v);
+}
+
+}  // namespace mlc
+
+#define CACHE_ATTENTION(NAME, T, DP, RT, TOK, WAVES, GENERAL)                                     \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::CacheAttentionArgs a) {      \
+    mlc::cache_attention<T, DP, RT, TOK, WAVES, GENERAL>(a);                                      \
+  }
+#define CACHE_ATTENTION_JOIN(NAME, T)                                                             \
+  extern "C" __global__ void __launch_bounds__(64) NAME(mlc::CacheAttentionArgs a) {              \
+    mlc::cache_attention_join<T>(a);                                                              \
+  }

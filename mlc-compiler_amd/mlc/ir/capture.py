@@ -72,6 +72,8 @@ _ADDMM = "aten.addmm.default"
 _UNBIND = "aten.unbind.int"
 _SPLIT_BY_CHUNK = "aten.split.Tensor"
 _SPLIT_BY_SIZES = "aten.split_with_sizes.default"
+#: how the exporter writes an op that changes its operands
+_IN_PLACE = "auto_functionalized_v2"
 
 
 class CaptureError(Exception):
@@ -274,6 +276,9 @@ class _Translation:
         op = str(fx.target)
         if op in DROP_OPS:
             return
+        if op == _IN_PLACE:
+            self.bound[fx] = self._in_place(fx)
+            return
         args = [self._operand(a) for a in fx.args]
         kwargs = {key: self._operand(v) for key, v in fx.kwargs.items()}
         self.bound[fx] = self.routes[self._route(op, args, kwargs)](fx, op, args, kwargs)
@@ -314,6 +319,60 @@ class _Translation:
         self._emit(op, args, kwargs, outputs, export_val=recorded, target=fx.target,
                    types_from_export=True, opaque=True)
         return self._single_or_list(outputs)
+
+    def _in_place(self, fx) -> list:
+        """An operator of ``mlc.ops`` that changes its operands: they have to be
+        buffers of the module, whole, and the compiled schedule changes those.
+        Its results are values over the same buffers, which later readers of
+        them read, so that they run after it."""
+        target = fx.args[0]
+        if target.namespace != "mlc":
+            raise CaptureError(f"{target} changes its operands: only side-effect-free inference "
+                               "graphs and the operators of mlc.ops compile")
+        bases = [self._operand(x) for x in fx.kwargs["_all_bases"]]
+        args, changed = [], []
+        for a in target._schema.arguments:
+            if a.alias_info is None or not a.alias_info.is_write:
+                args.append(self._operand(fx.kwargs[a.name]))
+                continue
+            base: Value = bases[fx.kwargs[f"_{a.name}_base_index"]]
+            window = [n for n in fx.kwargs if n.startswith(f"_{a.name}_")
+                      and n != f"_{a.name}_base_index"]
+            if window or base.buffer.kind != "param" or base.layout != Layout.contiguous(base.buffer.shape):
+                raise CaptureError(f"{target}: {a.name} is changed in place, so it has to be a "
+                                   "whole buffer of the module (register_buffer)")
+            if any(base is v for v in changed):
+                raise CaptureError(f"{target}: one buffer is given for two operands that change")
+            args.append(base)
+            changed.append(base)
+        outputs = {id(v): Value(f"{fx.name}_{i}", v.buffer, v.layout) for i, v in enumerate(changed)}
+        self._emit(str(target), args, {}, list(outputs.values()), target=target,
+                   types_from_export=True, opaque=True, pin=True)
+        return [None] * max(1, len(target._schema.returns)) + [outputs.get(id(v), v) for v in bases]
+
+    def _check_changes(self) -> None:
+        """A buffer's old contents cannot be read beside the new ones: nothing
+        orders such a reader before the change."""
+        readers: dict[int, list[Node]] = self.graph.use_map()
+        windows: dict[int, list[Value]] = {}
+        for node in self.graph.nodes:
+            if node.meta.get("is_view"):
+                windows.setdefault(id(node.args[0]), []).append(node.out)
+        for node in self.graph.nodes:
+            if not node.meta.get("pin"):
+                continue
+            changed = {id(v.buffer) for v in node.outputs}
+            for v in node.unique_tensor_args():
+                if id(v.buffer) not in changed:
+                    continue
+                seen = [v]
+                while seen:
+                    at = seen.pop()
+                    seen += windows.get(id(at), [])
+                    if any(n is not node for n in readers.get(id(at), [])) or any(
+                            at is o for o in self.graph.outputs):
+                        raise CaptureError(f"{v.name} is read by another operator beside "
+                                           f"{node.op}, which changes it: read it after the change")
 
     def _view(self, fx, op, args, kwargs) -> Value:
         """A restride of the source's buffer. When the requested view needs
@@ -377,6 +436,9 @@ class _Translation:
         results = list(results) if isinstance(results, (list, tuple)) else [results]
         for position, result in enumerate(results):
             kind = specs[position].kind if position < len(specs) else OutputKind.USER_OUTPUT
+            if kind == OutputKind.BUFFER_MUTATION and self._operand(result).buffer.kind == "param" \
+                    and self._operand(result).producer.meta.get("pin"):
+                continue  # changed where it is
             if kind != OutputKind.USER_OUTPUT:
                 raise CaptureError(f"result {position} of the export is a {kind}, not a user "
                                    "output: only side-effect-free inference graphs compile")
@@ -386,3 +448,4 @@ class _Translation:
             self.graph.outputs.append(value)
             if value.buffer.kind == "intermediate":
                 value.buffer.kind = "output"
+        self._check_changes()

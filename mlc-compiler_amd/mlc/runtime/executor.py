@@ -128,7 +128,8 @@ class ExternCall:
 
 @dataclass
 class NativeCall:
-    """A library op the runtime implements with a kernel of its own."""
+    """A library op, or an operator of ``mlc.ops``, that the runtime implements with
+    a kernel of its own, or several (``bound`` is a list of them then)."""
 
     module: Any
     bound: Any
@@ -204,6 +205,15 @@ class _Buffers:
             self.live.update(v.buffer.name for v in (*k.reads(), *k.writes()))
         self.params = {v.buffer.name: graph.param_tensors[v.name].to(model.device).contiguous()
                        .reshape(-1) for v in graph.params}
+        #: buffers of the module that the schedule changes (``mlc.ops.cache_append``)
+        self.changed = {v.buffer.name for k in schedule.kernels for v in k.writes()
+                        if v.buffer.kind == "param"}
+        for v in graph.params:
+            own = graph.param_tensors[v.name]
+            if v.buffer.name in self.changed and self.params[v.buffer.name].data_ptr() != own.data_ptr():
+                raise ExecutionError(
+                    f"buffer {graph.param_origin[v.name]} is changed in place, and a copy of it would "
+                    f"be: it has to be contiguous and on {model.device} before the model is compiled")
         #: products of groups that run as one launch, which never stores them
         self.unstored = {schedule.kernels[i].outputs[0].buffer.name: schedule.kernels[i].outputs[0].buffer
                          for i in schedule.merged}
@@ -421,7 +431,9 @@ class CompiledModel:
                 and hasattr(self._module, "bind_inputs") and self._launch_directly()):
             self._module.bind_inputs(self._runs, {t.data_ptr(): i for i, t in
                                                   enumerate(self._buffers.inputs)})
-            mine = {id(t) for t in (*self._buffers.inputs, *self.params.values())}
+            changed = self._buffers.changed
+            mine = {id(t) for t in (*self._buffers.inputs,
+                                    *(t for n, t in self.params.items() if n not in changed))}
             held = [t for t in table.values() if id(t) not in mine]
             self._own = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
                          for t in (*held, *([self._arena] if self._arena is not None else []))]

@@ -33,10 +33,13 @@ from dataclasses import dataclass
 
 import torch
 
+from ..codegen import hip_operators
 from ..codegen.hip_backend import LaunchSpec, build_module, build_products
 from ..config import Config
+from ..ir.graph import Value
 from ..kernels import ExternKernel, Kernel, Schedule
 from . import native
+from .operators import INVALID, OperatorModules
 
 _CAPSULE_NAME = b"dltensor"
 _PyCapsule_New = ctypes.pythonapi.PyCapsule_New
@@ -104,12 +107,18 @@ class HipRuntime:
         self._plans: list[ctypes.c_void_p] = []
         #: native plan -> its launches, by entry
         self._launches: dict[int, list[Bound]] = {}
+        #: memory of operators that take several launches
+        self._workspaces: list[torch.Tensor] = []
         self._arena_tensor: torch.Tensor | None = None
         self._static_arena = bool(getattr(cfg, "static_arena", False))
         #: device address of the context's invalid-input word, if a kernel
         #: of this module can flag one (the native embedding gather)
         self._error_word: int | None = None
-        if any(spec.meta.get("error_word") for spec in self.launch_table.values()):
+        #: the kernels of ``mlc.ops`` that the schedule calls, in this context
+        self._operators = OperatorModules(self.index, self._ctx)
+        if any(spec.meta.get("error_word") for spec in self.launch_table.values()) or any(
+                isinstance(k, ExternKernel) and k.node.op in hip_operators.FLAGGING
+                for k in schedule.kernels):
             word = ctypes.c_void_p()
             native.check(self.lib.mlc_error_word(self._ctx, ctypes.byref(word)), "mlc_error_word")
             self._error_word = word.value
@@ -152,9 +161,13 @@ class HipRuntime:
         return Bound(k.name, self.functions[spec.symbol], spec.grid, spec.block, spec.lds_bytes,
                      args)
 
-    def bind_native_extern(self, k: ExternKernel, buffers: dict[str, torch.Tensor]) -> Bound | None:
-        """An extern op this module implements natively (``aten.embedding``),
-        resolved like a generated kernel; ``None`` leaves it to the library."""
+    def bind_native_extern(self, k: ExternKernel, buffers: dict[str, torch.Tensor]
+                           ) -> "Bound | list[Bound] | None":
+        """An extern op this module implements natively (``aten.embedding``, the
+        operators of ``mlc.ops``), resolved like a generated kernel; ``None``
+        leaves it to the library."""
+        if k.node.op in hip_operators.PLANS:
+            return self._bind_operator(k, buffers)
         return self._bind_extern(k, self.launch_table.get(k.name), buffers)
 
     def bind_product(self, k: ExternKernel, buffers: dict[str, torch.Tensor]) -> Bound | None:
@@ -189,6 +202,34 @@ class HipRuntime:
         return Bound(k.name, self.functions[spec.symbol], spec.grid, spec.block, spec.lds_bytes,
                      struct.pack(f"<{len(ptrs)}Q", *ptrs))
 
+    def _bind_operator(self, k: ExternKernel, buffers: dict[str, torch.Tensor]) -> list[Bound]:
+        """The launches of an operator of ``mlc.ops``. Memory they share is the
+        binding's own, held as long as the model."""
+        names = [a.name for a in k.node.meta["target"]._schema.arguments]
+        operands, pointers = {}, {}
+        for name, v in zip(names, k.node.args):
+            if not isinstance(v, Value):
+                operands[name] = v
+                continue
+            t = buffers[v.buffer.name]
+            if t.device.type != "cuda" or t.dtype != v.dtype or t.numel() < v.buffer.numel:
+                raise native.NativeError(f"{k.name}: buffer {v.buffer.name} is {t.dtype}[{t.numel()}] "
+                                         f"on {t.device}, expected {v.dtype}[{v.buffer.numel}] on the GPU")
+            offset = v.layout.offset * v.dtype.itemsize
+            pointers[name] = t.data_ptr()
+            operands[name] = hip_operators.Operand(v.shape, v.layout.strides, v.dtype, offset,
+                                                   (t.data_ptr() + offset) % 16 == 0)
+        for i, v in enumerate(k.outputs):
+            pointers[f"out{i}"] = buffers[v.buffer.name].data_ptr()
+        plan = hip_operators.PLANS[k.node.op](**operands)
+        if self._error_word is not None:
+            pointers["error"] = self._error_word
+        if plan.workspace:
+            self._workspaces.append(torch.empty(plan.workspace, dtype=torch.uint8, device=self.device))
+            pointers["workspace"] = self._workspaces[-1].data_ptr()
+        return [Bound(k.name, self._operators.function(x), x.grid, x.block, 0, x.arguments(pointers))
+                for x in plan.launches]
+
     # -- invalid inputs ------------------------------------------------------------
     @property
     def flags_errors(self) -> bool:
@@ -207,10 +248,7 @@ class HipRuntime:
             return None
         value = ctypes.c_int32()
         native.check(self.lib.mlc_error_poll(self._ctx, ctypes.byref(value)), "mlc_error_poll")
-        if value.value == 0:
-            return None
-        return ("an embedding id was outside its table (torch raises IndexError for such an "
-                "id); the rows it addressed were written as zeros")
+        return INVALID.get(value.value) if value.value else None
 
     def clear_errors(self) -> None:
         """Wait for the device, then zero the word."""
@@ -232,6 +270,10 @@ class HipRuntime:
         self.run_bound(self.bind(k, buffers))
 
     def run_bound(self, payload) -> None:
+        if isinstance(payload, list):
+            for bound in payload:
+                self.run_bound(bound)
+            return
         if isinstance(payload, Bound) and payload.grid == 0:
             return  # a reduction over zero rows: nothing to launch
         if isinstance(payload, Range):
@@ -248,12 +290,13 @@ class HipRuntime:
         generated kernels is one ``Range`` of a native launch plan."""
         def native_of(kind, payload):
             if kind == "kernel":
-                return payload if payload.grid else None
+                return [payload] if payload.grid else None
             if kind == "extern" and getattr(payload, "module", None) is self:
-                return payload.bound  # a library op this module claimed
+                bound = payload.bound  # a library op this module claimed
+                return bound if isinstance(bound, list) else [bound]
             return None
 
-        kernels = [b for b in (native_of(kind, p) for kind, p in plan) if b is not None]
+        kernels = [b for kind, p in plan for b in native_of(kind, p) or ()]
         handle = ctypes.c_void_p()
         native.check(self.lib.mlc_plan_create(self._ctx, len(kernels), ctypes.byref(handle)),
                      "mlc_plan_create")
@@ -265,12 +308,13 @@ class HipRuntime:
         runs: list = []
         i = 0
         for kind, payload in plan:
-            if native_of(kind, payload) is not None:
+            launches = native_of(kind, payload)
+            if launches is not None:
                 if runs and runs[-1][0] == "kernel":
-                    runs[-1][1].end = i + 1
+                    runs[-1][1].end = i + len(launches)
                 else:
-                    runs.append(("kernel", Range(handle.value, i, i + 1)))
-                i += 1
+                    runs.append(("kernel", Range(handle.value, i, i + len(launches))))
+                i += len(launches)
             else:
                 runs.append((kind, payload))
         return runs
@@ -388,6 +432,7 @@ class HipRuntime:
         for mod in getattr(self, "_mods", []):
             lib.mlc_module_unload(mod)
         self._mods = []
+        self._operators.close()
 
     def __del__(self) -> None:
         try:

@@ -65,6 +65,21 @@ def prebuild(items=None, verbose: bool = True) -> None:
         torch.cuda.empty_cache() if torch.cuda.is_available() else None
 
 
+def prebuild_operators(verbose: bool = True) -> None:
+    """The kernels of ``mlc.ops`` for every type, head size and option."""
+    import concurrent.futures
+    import os
+
+    from ..codegen import hip_operators
+
+    t0 = time.time()
+    texts = [hip_operators.source(file, kernel) for file, kernel in hip_operators.all_kernels()]
+    with concurrent.futures.ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(native.compile_code_object, texts))
+    if verbose:
+        print(f"prebuild operators: {len(texts)} kernels ({time.time() - t0:.1f}s)", flush=True)
+
+
 if __name__ == "__main__":
     keys = sys.argv[1:] or None
     prebuild([(k, Config()) for k in keys] if keys else None)
