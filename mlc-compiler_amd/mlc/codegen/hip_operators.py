@@ -137,7 +137,6 @@ def plan_rotary(q: Operand, k: Operand, positions: Operand, frequencies: Operand
 # attention over keys and values in 16 bits
 # --------------------------------------------------------------------------
 
-ATTENTION_ROWS, ATTENTION_THREADS = 128, 256
 ATTENTION_DIMS = (64, 96, 128, 256)
 
 
@@ -155,9 +154,11 @@ def _factors(scale: float, cap: float) -> tuple[float, float]:
     return (scale / cap, cap * LOG2E) if cap else (scale * LOG2E, 0.0)
 
 
-def attention_kernel(dtype, dp: int, general: bool) -> tuple[str, str]:
-    name = f"attention_{SHORT[dtype]}_{dp}{'_general' if general else ''}"
-    return f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {str(general).lower()})", name
+def attention_kernel(dtype, dp: int, waves: int, direct: bool, general: bool) -> tuple[str, str]:
+    name = (f"attention_{SHORT[dtype]}_{dp}_w{waves}{'_direct' if direct else ''}"
+            f"{'_general' if general else ''}")
+    return (f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {waves}, {str(direct).lower()}, "
+            f"{str(general).lower()})"), name
 
 
 def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
@@ -168,8 +169,11 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
     if _numel(q) == 0:
         return Plan(())
     group = heads // kv_heads
-    tiles = _ceil(queries * group, ATTENTION_ROWS)
     dp = _padded(dim, ATTENTION_DIMS)
+    direct = (dp == dim and keys > 0 and k.aligned and v.aligned
+              and all(n % 8 == 0 for n in (*k.strides[:3], *v.strides[:3])))
+    waves = 4
+    tiles = _ceil(queries * group, 32 * waves)
     general = bool(cap) or slopes is not None or documents is not None
     some = lambda x, n: x.strides if x is not None else (0,) * n  # noqa: E731
     off = lambda x: x.offset if x is not None else 0  # noqa: E731
@@ -178,12 +182,12 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
                        *some(slopes, 1), *some(documents, 2), *some(prefix, 1),
                        batch, queries, keys, kv_heads, group, dim, causal, tiles,
                        *_factors(scale, cap))
-    kernel, name = attention_kernel(q.dtype, dp, general)
-    grid = _grid(tiles * batch * kv_heads, ATTENTION_THREADS, "attention")
+    kernel, name = attention_kernel(q.dtype, dp, waves, direct, general)
+    grid = _grid(tiles * batch * kv_heads, 64 * waves, "attention")
     pointers = ("q", "k", "v", "slopes" if slopes is not None else None,
                 "documents" if documents is not None else None,
                 "prefix" if prefix is not None else None, "out0")
-    return Plan((Launch(kernel, "attention", name, grid, ATTENTION_THREADS, pointers, tail),))
+    return Plan((Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail),))
 
 
 # --------------------------------------------------------------------------
@@ -306,8 +310,8 @@ def all_kernels() -> list[tuple[str, str]]:
         out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
                 for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
     for dtype in (torch.float16, torch.bfloat16):
-        out += [("attention", attention_kernel(dtype, dp, g)[0]) for dp in ATTENTION_DIMS
-                for g in (False, True)]
+        out += [("attention", attention_kernel(dtype, dp, 4, direct, g)[0]) for dp in ATTENTION_DIMS
+                for direct in (False, True) for g in (False, True)]
         out += [("cache_attention", cached_kernel(dtype, dp, tall, step, 4, g)[0])
                 for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
                 for step in (32, 64) for g in (False, True)]

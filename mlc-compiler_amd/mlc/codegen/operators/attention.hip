@@ -32,7 +32,7 @@ struct AttentionArgs {
   float scale, cap;  // scale times log2 e where cap is 0, else 1/cap of it and cap log2 e
 };
 
-constexpr int ATT_WAVES = 4, ATT_ROWS = 32 * ATT_WAVES, ATT_KEYS = 64;
+constexpr int ATT_KEYS = 64;
 
 template <class T> struct vec8;
 template <> struct vec8<f16> { typedef half8 type; static constexpr uint32_t exponent = 0x7c00u; };
@@ -68,18 +68,28 @@ template <uint32_t E> __device__ __forceinline__ bool not_finite(uint4v x) {
   return bad;
 }
 
-template <class T, int DP, bool GENERAL>
+
+// 16 bytes of a lane from ``g`` straight to LDS at ``lds`` + 16 * lane.
+__device__ __forceinline__ void to_lds(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// DIRECT: rows of 16-byte aligned pieces, dim == DP: tiles go from memory to LDS
+// without passing registers. Otherwise through registers, zeros past dim.
+template <class T, int DP, int WAVES, bool DIRECT, bool GENERAL>
 __device__ __forceinline__ void attention(const AttentionArgs& a) {
   typedef typename vec8<T>::type v8;
   constexpr int PC = DP == 64 ? 8 : DP <= 128 ? 16 : 32;  // 16-byte slots of an LDS row
   constexpr int CH = DP / 8;                               // of which hold values
-  constexpr int THREADS = 64 * ATT_WAVES;
-  constexpr int N = ATT_KEYS * CH / THREADS;
-  static_assert(ATT_KEYS * CH % THREADS == 0, "staging");
-  __shared__ __attribute__((aligned(1024))) uint4v lk[ATT_KEYS * PC], lv[ATT_KEYS * PC];
-  __shared__ int ldoc[ATT_KEYS];
-  __shared__ int spoiled[2];  // whether a tile that is masked in part has V values not finite
-  __shared__ __attribute__((aligned(16))) T lp[ATT_WAVES][32][16];
+  constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+  constexpr int BUFFERS = DIRECT ? 2 : 1;
+  constexpr int N = ATT_KEYS * CH / THREADS;               // pieces of a tile for a thread
+  constexpr int NL = ATT_KEYS * PC / THREADS;              // slots of a tile for a thread
+  static_assert(ATT_KEYS * CH % THREADS == 0 && ATT_KEYS * PC % THREADS == 0, "staging");
+  __shared__ __attribute__((aligned(1024))) uint4v lk[BUFFERS][ATT_KEYS * PC], lv[BUFFERS][ATT_KEYS * PC];
+  __shared__ __attribute__((aligned(16))) int ldoc[2][ATT_KEYS];
+  __shared__ __attribute__((aligned(16))) T lp[WAVES][32][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -108,17 +118,16 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
     return lim;
   };
-  const int row = tile * ATT_ROWS + wave * 32 + c;
+  const int first_row = tile * ROWS, wave_row = first_row + wave * 32;
+  const int row = wave_row + c;
   const int r = row < rows ? row : rows - 1;  // rows past the end repeat the last, and are not stored
   const int t = r / a.group, head = hk * a.group + r % a.group;
   const int32_t* const doc = at<int32_t>(a.documents, a.d_off) + b * a.db;
   const int mine = GENERAL && a.documents ? doc[(t + shift) * a.dt] : 0;
   const int lim = mine < 0 ? -1 : last(t);
-  const int first_row = tile * ATT_ROWS, end_row = first_row + ATT_ROWS < rows ? first_row + ATT_ROWS : rows;
-  const int wave_row = first_row + wave * 32;
+  const int end_row = first_row + ROWS < rows ? first_row + ROWS : rows;
   const int lim_wg = last((end_row - 1) / a.group);
-  const int lim_wg_min = last(first_row / a.group);
-  const int lim_wave = wave_row < rows ? last(((wave_row + 31 < rows ? wave_row + 31 : rows - 1)) / a.group) : -1;
+  const int lim_wave = wave_row < rows ? last((wave_row + 31 < rows ? wave_row + 31 : rows - 1) / a.group) : -1;
   const int lim_wave_min = wave_row < rows ? last(wave_row / a.group) : -1;
   const int tiles = lim_wg < 0 ? 0 : lim_wg / ATT_KEYS + 1;
 
@@ -138,18 +147,34 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 
   const T* const kp = at<T>(a.k, a.k_off) + b * a.kb + hk * a.kh;
   const T* const vp = at<T>(a.v, a.v_off) + b * a.vb + hk * a.vh;
-  T rk[N][8], rv[N][8];
-  auto load = [&](int kt) {
+  T rk[DIRECT ? 1 : N][8], rv[DIRECT ? 1 : N][8];
+  auto load = [&](int kt, int into) {
+    if constexpr (DIRECT) {
+      // slot i of a tile is row i / PC; past the last key the last one again
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = threadIdx.x + n * THREADS, key = kt * ATT_KEYS + i / CH, d = i % CH * 8;
-      if (key < a.keys && d < a.dim) {
-        load_n<2>(rk[n], kp + key * a.kt + d);
-        load_n<2>(rv[n], vp + key * a.vt + d);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rk[n][j] = rv[n][j] = (T)0.0f;
+      for (int n = 0; n < NL; ++n) {
+        const int i = threadIdx.x + n * THREADS, kr = i / PC;
+        const int key = kt * ATT_KEYS + kr, at_key = key < a.keys ? key : a.keys - 1;
+        const int chunk = (slot<PC>(kr, i % PC) % PC) % CH;  // slots past the row: anything of it
+        to_lds(kp + at_key * a.kt + chunk * 8, lk[into] + wave * 64 + n * THREADS);
+        to_lds(vp + at_key * a.vt + chunk * 8, lv[into] + wave * 64 + n * THREADS);
       }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int i = threadIdx.x + n * THREADS, key = kt * ATT_KEYS + i / CH, d = i % CH * 8;
+        if (key < a.keys && d < a.dim) {
+          load_n<2>(rk[n], kp + key * a.kt + d);
+          load_n<2>(rv[n], vp + key * a.vt + d);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) rk[n][j] = rv[n][j] = (T)0.0f;
+        }
+      }
+    }
+    if (GENERAL && a.documents && threadIdx.x < ATT_KEYS) {
+      const int key = kt * ATT_KEYS + threadIdx.x;
+      ldoc[kt & 1][threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
     }
   };
 
@@ -161,29 +186,27 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   float m = -__builtin_inff(), l = 0.0f;
   // token of a 32-token half tile that row c of the score product is
   const int token = ((c >> 4) << 4) | (((c >> 2) & 1) << 3) | (((c >> 3) & 1) << 2) | (c & 3);
+  // where this lane reads V^T: token 8 h + group / 4 of 16 and value 16 (lane / 16 % 2) + 4 (lane % 4) of 32
+  const int vk = 8 * h + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
-  if (threadIdx.x < 2) spoiled[threadIdx.x] = 0;
-  if (tiles > 0) load(0);
+  if (tiles > 0) load(0, 0);
   for (int kt = 0; kt < tiles; ++kt) {
-    const bool partial = GENERAL && a.documents ? true : lim_wg_min < (kt + 1) * ATT_KEYS - 1;
-    __syncthreads();
-    bool bad = false;
+    const int now = DIRECT ? kt & 1 : 0;
+    if constexpr (DIRECT) {
+      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      __syncthreads();
+      if (kt + 1 < tiles) load(kt + 1, now ^ 1);
+    } else {
+      __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = threadIdx.x + n * THREADS, at_slot = slot<PC>(i / CH, i % CH);
-      lk[at_slot] = __builtin_bit_cast(uint4v, rk[n]);
-      const uint4v x = __builtin_bit_cast(uint4v, rv[n]);
-      lv[at_slot] = x;
-      if (partial) bad |= not_finite<vec8<T>::exponent>(x);
+      for (int n = 0; n < N; ++n) {
+        const int i = threadIdx.x + n * THREADS, at_slot = slot<PC>(i / CH, i % CH);
+        lk[0][at_slot] = __builtin_bit_cast(uint4v, rk[n]);
+        lv[0][at_slot] = __builtin_bit_cast(uint4v, rv[n]);
+      }
+      __syncthreads();
+      if (kt + 1 < tiles) load(kt + 1, 0);
     }
-    if (partial && bad) spoiled[kt & 1] = 1;
-    if (GENERAL && a.documents && threadIdx.x < ATT_KEYS) {
-      const int key = kt * ATT_KEYS + threadIdx.x;
-      ldoc[threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) spoiled[(kt + 1) & 1] = 0;
-    if (kt + 1 < tiles) load(kt + 1);
     const int base = kt * ATT_KEYS;
     if (base > lim_wave) continue;
 
@@ -194,28 +217,35 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
-        s[u] = mfma_32x32x16(__builtin_bit_cast(v8, lk[slot<PC>(32 * u + token, 2 * i + h)]), q[i], s[u]);
+        s[u] = mfma_32x32x16(__builtin_bit_cast(v8, lk[now][slot<PC>(32 * u + token, 2 * i + h)]), q[i], s[u]);
     }
     float scale = a.scale;
     if constexpr (GENERAL) {
       // in log2 units: the cap, then the bias
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float x = s[u][j] * a.scale;
-          if (a.cap != 0.0f) {
-            // tanh y = 1 - 2 / (e^2y + 1)
-            const float e = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
-            x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(e + 1.0f);
-          }
-          if (a.slopes) {
-            const int key = base + 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
-            x = __builtin_fmaf(-slope, __builtin_fabsf((float)(key - (t + shift))), x);
-          }
-          s[u][j] = x;
-        }
       scale = 1.0f;
+      if (a.cap != 0.0f) {
+        // cap tanh y = cap - 2 cap / (e^2y + 1)
+        const float by = a.scale * (2.0f * 0x1.715476p+0f);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            s[u][j] = __builtin_fmaf(-2.0f * a.cap,
+                                     __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][j] * by) + 1.0f), a.cap);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[u][j] *= a.scale;
+      }
+      if (a.slopes) {
+        const float away = (float)(base + 8 * h - (t + shift));
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            s[u][j] = __builtin_fmaf(-slope, __builtin_fabsf(away + (float)(32 * u + 16 * (j >> 3) + (j & 7))), s[u][j]);
+      }
     }
     const bool masked = lim_wave_min < base + ATT_KEYS - 1 || (GENERAL && a.documents);
     if (masked) {
@@ -225,7 +255,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         for (int j = 0; j < 16; ++j) {
           const int k = 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
           bool seen = base + k <= lim;
-          if (GENERAL && a.documents) seen = seen && ldoc[k] == mine;
+          if (GENERAL && a.documents) seen = seen && ldoc[kt & 1][k] == mine;
           s[u][j] = seen ? s[u][j] : -__builtin_inff();
         }
     }
@@ -235,14 +265,17 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = __builtin_fmaxf(top, s[u][j]);
     top = xor32<OpMax>(top * scale);
-    if (top > m) {
-      const float alpha = __builtin_amdgcn_exp2f(m - top);  // m = -inf: 0, as O and l are
+    // the reference of the exponentials follows the maximum in steps of at least 2^8:
+    // weights stay below 2^8 and O is seldom scaled
+    if (__any(top > m + 8.0f)) {
+      const float next = top > m ? top : m;
+      const float alpha = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - next);
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
       l *= alpha;
-      m = top;
+      m = next;
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m;
     v8 p[4];
@@ -254,25 +287,35 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         l += e;
         p[2 * u + (j >> 3)][j & 7] = (T)e;
       }
-    if (!(partial && spoiled[kt & 1])) {
+    auto values = [&](int i, int u) {
+      const h4 lo = read_transposed(reinterpret_cast<const char*>(
+          lv[now] + slot<PC>(16 * u + vk, (32 * i + vd) >> 3)) + (vd & 7) * 2);
+      const h4 hi = read_transposed(reinterpret_cast<const char*>(
+          lv[now] + slot<PC>(16 * u + vk + 4, (32 * i + vd) >> 3)) + (vd & 7) * 2);
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    bool spoiled = false;
+    if (masked) {
+      // 0 times an infinity or NaN of a key that a row does not see would be NaN
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int g = lane & 15, d = 32 * i + 16 * ((lane >> 4) & 1) + 4 * (g & 3);
-          const int k = 16 * u + 8 * h + (g >> 2);
-          const h4 lo = read_transposed(reinterpret_cast<const char*>(lv + slot<PC>(k, d >> 3)) + (d & 7) * 2);
-          const h4 hi = read_transposed(reinterpret_cast<const char*>(lv + slot<PC>(k + 4, d >> 3)) + (d & 7) * 2);
-          const half8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          o[i] = mfma_32x32x16(__builtin_bit_cast(v8, w), p[u], o[i]);
-        }
+        for (int u = 0; u < 4; ++u)
+          spoiled |= not_finite<vec8<T>::exponent>(__builtin_bit_cast(uint4v, values(i, u)));
+      spoiled = __any(spoiled);
+    }
+    if (!spoiled) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          o[i] = mfma_32x32x16(__builtin_bit_cast(v8, values(i, u)), p[u], o[i]);
     } else {
-      // 0 times an infinity or NaN of a key that a row does not see is NaN in the
-      // product: row by row, over the keys it sees
-      const T* const value = reinterpret_cast<const T*>(lv);
+      // key by key, over those that a row sees
+      const T* const value = reinterpret_cast<const T*>(lv[now]);
 #pragma unroll 1
       for (int u = 0; u < 4; ++u) {
-        // p[u] by a constant index only: it stays in registers
+        // p by a constant index only: it stays in registers
         const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
         *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
         __builtin_amdgcn_wave_barrier();
@@ -314,7 +357,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 
 }  // namespace mlc
 
-#define ATTENTION(NAME, T, DP, GENERAL)                                                       \
-  extern "C" __global__ void __launch_bounds__(64 * mlc::ATT_WAVES) NAME(mlc::AttentionArgs a) { \
-    mlc::attention<T, DP, GENERAL>(a);                                                        \
+#define ATTENTION(NAME, T, DP, WAVES, DIRECT, GENERAL)                                            \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, 2) NAME(mlc::AttentionArgs a) { \
+    mlc::attention<T, DP, WAVES, DIRECT, GENERAL>(a);                                             \
   }
