@@ -60,14 +60,20 @@ __device__ __forceinline__ h4 read_transposed(const void* p) {
       (__attribute__((address_space(3))) short4v*)p));
 }
 
-template <uint32_t E> __device__ __forceinline__ bool not_finite(uint4v x) {
-  bool bad = false;
+// Zeros in the place of what is infinite or NaN (all of exponent E set) among 8
+// values of 16 bits; whether there was any.
+template <uint32_t E> __device__ __forceinline__ bool drop_not_finite(uint4v& x) {
+  bool found = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    bad |= (x[i] & E) == E || (x[i] & (E << 16)) == (E << 16);
-  return bad;
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (x[i] & E) == E, hi = (x[i] & (E << 16)) == (E << 16);
+    found |= lo || hi;
+    x[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+  }
+  return found;
 }
 
+template <bool B> struct bool_constant { static constexpr bool value = B; };
 
 // 16 bytes of a lane from ``g`` straight to LDS at ``lds`` + 16 * lane.
 __device__ __forceinline__ void to_lds(const void* g, void* lds) {
@@ -128,7 +134,6 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int end_row = first_row + ROWS < rows ? first_row + ROWS : rows;
   const int lim_wg = last((end_row - 1) / a.group);
   const int lim_wave = wave_row < rows ? last((wave_row + 31 < rows ? wave_row + 31 : rows - 1) / a.group) : -1;
-  const int lim_wave_min = wave_row < rows ? last(wave_row / a.group) : -1;
   const int tiles = lim_wg < 0 ? 0 : lim_wg / ATT_KEYS + 1;
 
   v8 q[DP / 16];
@@ -147,22 +152,43 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 
   const T* const kp = at<T>(a.k, a.k_off) + b * a.kb + hk * a.kh;
   const T* const vp = at<T>(a.v, a.v_off) + b * a.vb + hk * a.vh;
+  // slot i = thread + n * THREADS of a tile is chunk (i % PC) ^ swizzle of row i / PC;
+  // rows of one thread are STEP apart, which the swizzle of 16 slots does not see
+  constexpr int STEP = THREADS / PC, KINDS = PC == 32 ? 2 : 1;
+  static_assert(PC == 32 ? STEP % 8 == 0 : STEP % 16 == 0, "swizzle");
+  uint32_t kv[KINDS], vv[KINDS];
+  auto chunk_of = [&](int kr) { return (slot<PC>(kr, threadIdx.x % PC) % PC) % CH; };
+#pragma unroll
+  for (int i = 0; i < KINDS; ++i) {
+    const int kr = threadIdx.x / PC, chunk = chunk_of(kr + i * STEP);
+    kv[i] = (kr * (uint32_t)a.kt + chunk * 8) * (uint32_t)sizeof(T);
+    vv[i] = (kr * (uint32_t)a.vt + chunk * 8) * (uint32_t)sizeof(T);
+  }
   T rk[DIRECT ? 1 : N][8], rv[DIRECT ? 1 : N][8];
   auto load = [&](int kt, int into) {
+    const int base = kt * ATT_KEYS;
     if constexpr (DIRECT) {
-      // slot i of a tile is row i / PC; past the last key the last one again
+      if (base + ATT_KEYS <= a.keys) {
+        const char* const kb = reinterpret_cast<const char*>(kp + base * a.kt);
+        const char* const vb = reinterpret_cast<const char*>(vp + base * a.vt);
 #pragma unroll
-      for (int n = 0; n < NL; ++n) {
-        const int i = threadIdx.x + n * THREADS, kr = i / PC;
-        const int key = kt * ATT_KEYS + kr, at_key = key < a.keys ? key : a.keys - 1;
-        const int chunk = (slot<PC>(kr, i % PC) % PC) % CH;  // slots past the row: anything of it
-        to_lds(kp + at_key * a.kt + chunk * 8, lk[into] + wave * 64 + n * THREADS);
-        to_lds(vp + at_key * a.vt + chunk * 8, lv[into] + wave * 64 + n * THREADS);
+        for (int n = 0; n < NL; ++n) {
+          to_lds(kb + n * STEP * a.kt * sizeof(T) + kv[n % KINDS], lk[into] + wave * 64 + n * THREADS);
+          to_lds(vb + n * STEP * a.vt * sizeof(T) + vv[n % KINDS], lv[into] + wave * 64 + n * THREADS);
+        }
+      } else {  // past the last key the last one again
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+          const int kr = threadIdx.x / PC + n * STEP, key = base + kr < a.keys ? base + kr : a.keys - 1;
+          const int chunk = chunk_of(kr);
+          to_lds(kp + key * a.kt + chunk * 8, lk[into] + wave * 64 + n * THREADS);
+          to_lds(vp + key * a.vt + chunk * 8, lv[into] + wave * 64 + n * THREADS);
+        }
       }
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int i = threadIdx.x + n * THREADS, key = kt * ATT_KEYS + i / CH, d = i % CH * 8;
+        const int i = threadIdx.x + n * THREADS, key = base + i / CH, d = i % CH * 8;
         if (key < a.keys && d < a.dim) {
           load_n<2>(rk[n], kp + key * a.kt + d);
           load_n<2>(rv[n], vp + key * a.vt + d);
@@ -173,8 +199,8 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
     }
     if (GENERAL && a.documents && threadIdx.x < ATT_KEYS) {
-      const int key = kt * ATT_KEYS + threadIdx.x;
-      ldoc[kt & 1][threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
+      const int key = base + threadIdx.x;
+      ldoc[into][threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
     }
   };
 
@@ -189,13 +215,13 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   // where this lane reads V^T: token 8 h + group / 4 of 16 and value 16 (lane / 16 % 2) + 4 (lane % 4) of 32
   const int vk = 8 * h + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
-  if (tiles > 0) load(0, 0);
-  for (int kt = 0; kt < tiles; ++kt) {
-    const int now = DIRECT ? kt & 1 : 0;
+  int it = 0;  // tiles so far
+  // waits for tile ``kt``, which is on its way, and starts on ``next``
+  auto arrive = [&](int next) {
     if constexpr (DIRECT) {
       asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
       __syncthreads();
-      if (kt + 1 < tiles) load(kt + 1, now ^ 1);
+      if (next < tiles) load(next, (it + 1) & 1);
     } else {
       __syncthreads();
 #pragma unroll
@@ -205,10 +231,12 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         lv[0][at_slot] = __builtin_bit_cast(uint4v, rv[n]);
       }
       __syncthreads();
-      if (kt + 1 < tiles) load(kt + 1, 0);
+      if (next < tiles) load(next, (it + 1) & 1);
     }
-    const int base = kt * ATT_KEYS;
-    if (base > lim_wave) continue;
+  };
+  auto compute = [&](int kt, auto is_masked, auto is_safe) {
+    constexpr bool MASKED = decltype(is_masked)::value, SAFE = decltype(is_safe)::value;
+    const int now = DIRECT ? it & 1 : 0, base = kt * ATT_KEYS;
 
     float16v s[2];
 #pragma unroll
@@ -247,15 +275,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
             s[u][j] = __builtin_fmaf(-slope, __builtin_fabsf(away + (float)(32 * u + 16 * (j >> 3) + (j & 7))), s[u][j]);
       }
     }
-    const bool masked = lim_wave_min < base + ATT_KEYS - 1 || (GENERAL && a.documents);
-    if (masked) {
+    if constexpr (MASKED) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int k = 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
           bool seen = base + k <= lim;
-          if (GENERAL && a.documents) seen = seen && ldoc[kt & 1][k] == mine;
+          if (GENERAL && a.documents) seen = seen && ldoc[it & 1][k] == mine;
           s[u][j] = seen ? s[u][j] : -__builtin_inff();
         }
     }
@@ -295,45 +322,77 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     bool spoiled = false;
-    if (masked) {
-      // 0 times an infinity or NaN of a key that a row does not see would be NaN
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          spoiled |= not_finite<vec8<T>::exponent>(__builtin_bit_cast(uint4v, values(i, u)));
-      spoiled = __any(spoiled);
-    }
-    if (!spoiled) {
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          o[i] = mfma_32x32x16(__builtin_bit_cast(v8, values(i, u)), p[u], o[i]);
-    } else {
-      // key by key, over those that a row sees
-      const T* const value = reinterpret_cast<const T*>(lv[now]);
-#pragma unroll 1
       for (int u = 0; u < 4; ++u) {
-        // p by a constant index only: it stays in registers
-        const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
-        *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int j = 0; j < 16; ++j) {
-          const float x = element<T>::widen(lp[wave][c][j]);
-          if (x == 0.0f) continue;
-          const int k = 16 * u + j;
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int z = 0; z < 16; ++z) {
-              const int d = 32 * i + 8 * (z >> 2) + 4 * h + (z & 3);
-              o[i][z] += x * element<T>::widen(value[slot<PC>(k, d >> 3) * 8 + (d & 7)]);
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
+        uint4v w = __builtin_bit_cast(uint4v, values(i, u));
+        if constexpr (SAFE) spoiled |= drop_not_finite<vec8<T>::exponent>(w);
+        o[i] = mfma_32x32x16(__builtin_bit_cast(v8, w), p[u], o[i]);
       }
+    if constexpr (SAFE) {
+      if (__any(spoiled)) {
+        const T* const value = reinterpret_cast<const T*>(lv[now]);
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          // p by a constant index only: it stays in registers
+          const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
+          *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {
+            const float x = element<T>::widen(lp[wave][c][j]);
+            const int k = 16 * u + j;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+              for (int z = 0; z < 16; ++z) {
+                const int d = 32 * i + 8 * (z >> 2) + 4 * h + (z & 3);
+                const float y = element<T>::widen(value[slot<PC>(k, d >> 3) * 8 + (d & 7)]);
+                if (x != 0.0f && !(__builtin_fabsf(y) < __builtin_inff())) o[i][z] += x * y;
+              }
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+  };
+
+  // tiles that every row sees whole, then those that need a mask
+  int whole = 0;
+  if (!(GENERAL && a.documents)) {
+    whole = (last(first_row / a.group) + 1) / ATT_KEYS;
+    whole = whole < 0 ? 0 : whole < tiles ? whole : tiles;
+  }
+  if (tiles > 0) load(0, 0);
+  int kt = 0;
+  for (; kt < whole; ++kt, ++it) {
+    arrive(kt + 1);
+    compute(kt, bool_constant<false>{}, bool_constant<false>{});
+  }
+  for (; kt < tiles; ++kt, ++it) {
+    arrive(kt + 1);
+    if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
+  }
+  // 0 times an infinity or NaN of a key that a row does not see is NaN in the products.
+  // Where something came out not finite, all is done again with such values left out
+  // of the products and added key by key to the rows that see them.
+  float check = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) check = __builtin_fmaf(o[i][j], 0.0f, check);
+  if (__syncthreads_or(check != 0.0f)) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    m = -__builtin_inff();
+    l = 0.0f;
+    load(0, it & 1);
+    for (kt = 0; kt < tiles; ++kt, ++it) {
+      arrive(kt + 1);
+      if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
     }
   }
   if (row >= rows) return;
