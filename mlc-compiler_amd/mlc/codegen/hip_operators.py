@@ -171,7 +171,7 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
     group = heads // kv_heads
     dp = _padded(dim, ATTENTION_DIMS)
     direct = (dp == dim and keys > 0 and k.aligned and v.aligned
-              and all(n % 8 == 0 for n in (*k.strides[:3], *v.strides[:3])))
+              and all(n % 8 == 0 and n < 1 << 24 for n in (*k.strides[:3], *v.strides[:3])))
     waves = 4
     tiles = _ceil(queries * group, 32 * waves)
     general = bool(cap) or slopes is not None or documents is not None

@@ -81,8 +81,9 @@ __device__ __forceinline__ void to_lds(const void* g, void* lds) {
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// DIRECT: rows of 16-byte aligned pieces, dim == DP: tiles go from memory to LDS
-// without passing registers. Otherwise through registers, zeros past dim.
+// DIRECT: rows of 16-byte aligned pieces, dim == DP: tiles go from memory to LDS without
+// passing registers, the next one while one is in use. Otherwise through registers, with
+// zeros past dim.
 template <class T, int DP, int WAVES, bool DIRECT, bool GENERAL>
 __device__ __forceinline__ void attention(const AttentionArgs& a) {
   typedef typename vec8<T>::type v8;
@@ -93,20 +94,22 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   constexpr int N = ATT_KEYS * CH / THREADS;               // pieces of a tile for a thread
   constexpr int NL = ATT_KEYS * PC / THREADS;              // slots of a tile for a thread
   static_assert(ATT_KEYS * CH % THREADS == 0 && ATT_KEYS * PC % THREADS == 0, "staging");
-  __shared__ __attribute__((aligned(1024))) uint4v lk[BUFFERS][ATT_KEYS * PC], lv[BUFFERS][ATT_KEYS * PC];
-  __shared__ __attribute__((aligned(16))) int ldoc[2][ATT_KEYS];
+  constexpr int TILE = ATT_KEYS * PC * 16;                 // bytes of LDS, a power of two
+  __shared__ __attribute__((aligned(BUFFERS * TILE))) char lds[2 * BUFFERS * TILE];  // keys, then values
+  __shared__ __attribute__((aligned(16))) int ldoc[GENERAL ? BUFFERS : 1][GENERAL ? WAVES : 1][ATT_KEYS];
   __shared__ __attribute__((aligned(16))) T lp[WAVES][32][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
   const int rows = a.queries * a.group;
-  // the tiles of one (batch, head) go to one XCD where there are enough, long ones first
+  // Workgroups go to the 8 XCDs in turn: a pair of batch and key head stays on one where
+  // there are enough of them, and long tiles come first
   const int pairs = a.batch * a.kv_heads;
   int pair, tile;
   if (pairs % 8 == 0) {
     const int i = blockIdx.x / 8;
-    pair = i / a.tiles * 8 + blockIdx.x % 8;
-    tile = a.tiles - 1 - i % a.tiles;
+    pair = i % (pairs / 8) * 8 + blockIdx.x % 8;
+    tile = a.tiles - 1 - i / (pairs / 8);
   } else {
     pair = blockIdx.x % pairs;
     tile = a.tiles - 1 - blockIdx.x / pairs;
@@ -165,24 +168,26 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     vv[i] = (kr * (uint32_t)a.vt + chunk * 8) * (uint32_t)sizeof(T);
   }
   T rk[DIRECT ? 1 : N][8], rv[DIRECT ? 1 : N][8];
+  int rdoc = 0;
   auto load = [&](int kt, int into) {
     const int base = kt * ATT_KEYS;
     if constexpr (DIRECT) {
+      char* const to = lds + into * TILE + wave * 1024;
       if (base + ATT_KEYS <= a.keys) {
         const char* const kb = reinterpret_cast<const char*>(kp + base * a.kt);
         const char* const vb = reinterpret_cast<const char*>(vp + base * a.vt);
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-          to_lds(kb + n * STEP * a.kt * sizeof(T) + kv[n % KINDS], lk[into] + wave * 64 + n * THREADS);
-          to_lds(vb + n * STEP * a.vt * sizeof(T) + vv[n % KINDS], lv[into] + wave * 64 + n * THREADS);
+          to_lds(kb + n * STEP * a.kt * sizeof(T) + kv[n % KINDS], to + n * THREADS * 16);
+          to_lds(vb + n * STEP * a.vt * sizeof(T) + vv[n % KINDS], to + BUFFERS * TILE + n * THREADS * 16);
         }
       } else {  // past the last key the last one again
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
           const int kr = threadIdx.x / PC + n * STEP, key = base + kr < a.keys ? base + kr : a.keys - 1;
           const int chunk = chunk_of(kr);
-          to_lds(kp + key * a.kt + chunk * 8, lk[into] + wave * 64 + n * THREADS);
-          to_lds(vp + key * a.vt + chunk * 8, lv[into] + wave * 64 + n * THREADS);
+          to_lds(kp + key * a.kt + chunk * 8, to + n * THREADS * 16);
+          to_lds(vp + key * a.vt + chunk * 8, to + BUFFERS * TILE + n * THREADS * 16);
         }
       }
     } else {
@@ -198,9 +203,15 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         }
       }
     }
-    if (GENERAL && a.documents && threadIdx.x < ATT_KEYS) {
-      const int key = base + threadIdx.x;
-      ldoc[into][threadIdx.x] = key < a.keys ? doc[key * a.dt] : -1;
+    if (GENERAL && a.documents) {
+      // every wave its own copy, so that all have as many loads on their way; what lies
+      // behind the last key is masked by its index
+      const int key = base + lane < a.keys ? base + lane : a.keys - 1;
+      if constexpr (DIRECT)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(doc + key * a.dt),
+                                         (__attribute__((address_space(3))) void*)ldoc[into][wave], 4, 0, 0);
+      else
+        rdoc = doc[key * a.dt];
     }
   };
 
@@ -212,31 +223,38 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   float m = -__builtin_inff(), l = 0.0f;
   // token of a 32-token half tile that row c of the score product is
   const int token = ((c >> 4) << 4) | (((c >> 2) & 1) << 3) | (((c >> 3) & 1) << 2) | (c & 3);
-  // where this lane reads V^T: token 8 h + group / 4 of 16 and value 16 (lane / 16 % 2) + 4 (lane % 4) of 32
+  // where this lane reads K, and V^T (token 8 h + group / 4 of 16 and value 16 (lane / 16 % 2)
+  // + 4 (lane % 4) of 32): the other pieces of a tile are an xor or a constant away, since a
+  // slot's number is, and the other buffer too
   const int vk = 8 * h + ((lane & 15) >> 2), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  uint32_t k_at = slot<PC>(token, h) * 16, v_at = slot<PC>(vk, vd >> 3) * 16 + (vd & 7) * 2;
+  constexpr int PITCH = PC * 16;
 
-  int it = 0;  // tiles so far
-  // waits for tile ``kt``, which is on its way, and starts on ``next``
-  auto arrive = [&](int next) {
+  int it = 0;  // the buffer of the tile in use
+  // waits for tile ``kt``, which is on its way, and for this wave's reads of the one before,
+  // whose buffer is the next to be filled, and starts on the next one
+  auto arrive = [&](int kt) {
     if constexpr (DIRECT) {
-      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-      __syncthreads();
-      if (next < tiles) load(next, (it + 1) & 1);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : : : "memory");
+      if (kt + 1 < tiles) load(kt + 1, it ^ 1);
     } else {
       __syncthreads();
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         const int i = threadIdx.x + n * THREADS, at_slot = slot<PC>(i / CH, i % CH);
-        lk[0][at_slot] = __builtin_bit_cast(uint4v, rk[n]);
-        lv[0][at_slot] = __builtin_bit_cast(uint4v, rv[n]);
+        reinterpret_cast<uint4v*>(lds)[at_slot] = __builtin_bit_cast(uint4v, rk[n]);
+        reinterpret_cast<uint4v*>(lds + TILE)[at_slot] = __builtin_bit_cast(uint4v, rv[n]);
       }
+      if (GENERAL && a.documents) ldoc[0][wave][lane] = rdoc;
       __syncthreads();
-      if (next < tiles) load(next, (it + 1) & 1);
+      if (kt + 1 < tiles) load(kt + 1, 0);
     }
   };
   auto compute = [&](int kt, auto is_masked, auto is_safe) {
     constexpr bool MASKED = decltype(is_masked)::value, SAFE = decltype(is_safe)::value;
-    const int now = DIRECT ? it & 1 : 0, base = kt * ATT_KEYS;
+    const int base = kt * ATT_KEYS;
 
     float16v s[2];
 #pragma unroll
@@ -245,7 +263,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
-        s[u] = mfma_32x32x16(__builtin_bit_cast(v8, lk[now][slot<PC>(32 * u + token, 2 * i + h)]), q[i], s[u]);
+        s[u] = mfma_32x32x16(*reinterpret_cast<const v8*>(lds + (k_at ^ (i << 5)) + u * 32 * PITCH), q[i], s[u]);
     }
     float scale = a.scale;
     if constexpr (GENERAL) {
@@ -276,13 +294,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
     }
     if constexpr (MASKED) {
+      const int own = lim - base - 8 * h;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const int k = 32 * u + 16 * (j >> 3) + 8 * h + (j & 7);
-          bool seen = base + k <= lim;
-          if (GENERAL && a.documents) seen = seen && ldoc[it & 1][k] == mine;
+          const int k = 32 * u + 16 * (j >> 3) + (j & 7);
+          bool seen = k <= own;
+          if (GENERAL && a.documents) seen = seen && ldoc[it][wave][k + 8 * h] == mine;
           s[u][j] = seen ? s[u][j] : -__builtin_inff();
         }
     }
@@ -315,10 +334,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         p[2 * u + (j >> 3)][j & 7] = (T)e;
       }
     auto values = [&](int i, int u) {
-      const h4 lo = read_transposed(reinterpret_cast<const char*>(
-          lv[now] + slot<PC>(16 * u + vk, (32 * i + vd) >> 3)) + (vd & 7) * 2);
-      const h4 hi = read_transposed(reinterpret_cast<const char*>(
-          lv[now] + slot<PC>(16 * u + vk + 4, (32 * i + vd) >> 3)) + (vd & 7) * 2);
+      const char* const at = lds + BUFFERS * TILE + u * 16 * PITCH;
+      const h4 lo = read_transposed(at + (v_at ^ (i << 6)));
+      const h4 hi = read_transposed(at + (v_at ^ (i << 6) ^ 16) + 4 * PITCH);
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     bool spoiled = false;
@@ -332,7 +350,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
     if constexpr (SAFE) {
       if (__any(spoiled)) {
-        const T* const value = reinterpret_cast<const T*>(lv[now]);
+        const T* const value = reinterpret_cast<const T*>(lds + (BUFFERS + it) * TILE);
 #pragma unroll 1
         for (int u = 0; u < 4; ++u) {
           // p by a constant index only: it stays in registers
@@ -364,14 +382,21 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     whole = (last(first_row / a.group) + 1) / ATT_KEYS;
     whole = whole < 0 ? 0 : whole < tiles ? whole : tiles;
   }
-  if (tiles > 0) load(0, 0);
+  auto turn = [&] {  // to the other buffer
+    if constexpr (DIRECT) {
+      k_at ^= TILE;
+      v_at ^= TILE;
+      it ^= 1;
+    }
+  };
+  if (tiles > 0) load(0, it);
   int kt = 0;
-  for (; kt < whole; ++kt, ++it) {
-    arrive(kt + 1);
+  for (; kt < whole; ++kt, turn()) {
+    arrive(kt);
     compute(kt, bool_constant<false>{}, bool_constant<false>{});
   }
-  for (; kt < tiles; ++kt, ++it) {
-    arrive(kt + 1);
+  for (; kt < tiles; ++kt, turn()) {
+    arrive(kt);
     if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
   }
   // 0 times an infinity or NaN of a key that a row does not see is NaN in the products.
@@ -389,9 +414,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
     m = -__builtin_inff();
     l = 0.0f;
-    load(0, it & 1);
-    for (kt = 0; kt < tiles; ++kt, ++it) {
-      arrive(kt + 1);
+    if (tiles > 0) load(0, it);
+    for (kt = 0; kt < tiles; ++kt, turn()) {
+      arrive(kt);
       if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
     }
   }
@@ -417,6 +442,6 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 }  // namespace mlc
 
 #define ATTENTION(NAME, T, DP, WAVES, DIRECT, GENERAL)                                            \
-  extern "C" __global__ void __launch_bounds__(64 * WAVES, 2) NAME(mlc::AttentionArgs a) { \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, 2) NAME(mlc::AttentionArgs a) {        \
     mlc::attention<T, DP, WAVES, DIRECT, GENERAL>(a);                                             \
   }
