@@ -161,6 +161,14 @@ def attention_kernel(dtype, dp: int, waves: int, direct: bool, general: bool) ->
             f"{str(general).lower()})"), name
 
 
+def attention_waves(rows: int, pairs: int) -> int:
+    """Waves of a workgroup, each with 32 rows."""
+    for waves in (4, 2):
+        if _ceil(rows, 32 * waves) * pairs >= UNITS:
+            return waves
+    return 1
+
+
 def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
                    documents: Operand | None, prefix: Operand | None, scale: float, causal: bool,
                    cap: float) -> Plan:
@@ -172,7 +180,7 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
     dp = _padded(dim, ATTENTION_DIMS)
     direct = (dp == dim and keys > 0 and k.aligned and v.aligned
               and all(n % 8 == 0 and n < 1 << 24 for n in (*k.strides[:3], *v.strides[:3])))
-    waves = 4
+    waves = attention_waves(queries * group, batch * kv_heads)
     tiles = _ceil(queries * group, 32 * waves)
     general = bool(cap) or slopes is not None or documents is not None
     some = lambda x, n: x.strides if x is not None else (0,) * n  # noqa: E731
@@ -310,8 +318,8 @@ def all_kernels() -> list[tuple[str, str]]:
         out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
                 for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
     for dtype in (torch.float16, torch.bfloat16):
-        out += [("attention", attention_kernel(dtype, dp, 4, direct, g)[0]) for dp in ATTENTION_DIMS
-                for direct in (False, True) for g in (False, True)]
+        out += [("attention", attention_kernel(dtype, dp, w, direct, g)[0]) for dp in ATTENTION_DIMS
+                for w in (1, 2, 4) for direct in (False, True) for g in (False, True)]
         out += [("cache_attention", cached_kernel(dtype, dp, tall, step, 4, g)[0])
                 for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
                 for step in (32, 64) for g in (False, True)]

@@ -32,7 +32,10 @@ struct AttentionArgs {
   float scale, cap;  // scale times log2 e where cap is 0, else 1/cap of it and cap log2 e
 };
 
-constexpr int ATT_KEYS = 64;
+// Keys of a tile: with heads of 256, rows of 64 scores would not fit the registers
+// beside O and Q, and O would move between vector and accumulation registers twice a
+// tile (2048 causal tokens, 4 x 8 heads: 136 us; 32 keys: see the table of sizes).
+template <int DP> constexpr int tile_keys = DP == 256 ? 32 : 64;
 
 template <class T> struct vec8;
 template <> struct vec8<f16> { typedef half8 type; static constexpr uint32_t exponent = 0x7c00u; };
@@ -91,12 +94,15 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   constexpr int CH = DP / 8;                               // of which hold values
   constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
   constexpr int BUFFERS = DIRECT ? 2 : 1;
-  constexpr int N = ATT_KEYS * CH / THREADS;               // pieces of a tile for a thread
-  constexpr int NL = ATT_KEYS * PC / THREADS;              // slots of a tile for a thread
-  static_assert(ATT_KEYS * CH % THREADS == 0 && ATT_KEYS * PC % THREADS == 0, "staging");
-  constexpr int TILE = ATT_KEYS * PC * 16;                 // bytes of LDS, a power of two
+  constexpr int KEYS = tile_keys<DP>, U = KEYS / 32;
+  constexpr int N = KEYS * CH / THREADS;               // pieces of a tile for a thread
+  constexpr int NL = KEYS * PC / THREADS;              // slots of a tile for a thread
+  static_assert(KEYS * CH % THREADS == 0 && KEYS * PC % THREADS == 0, "staging");
+  constexpr int TILE = KEYS * PC * 16;                 // bytes of LDS, a power of two
   __shared__ __attribute__((aligned(BUFFERS * TILE))) char lds[2 * BUFFERS * TILE];  // keys, then values
-  __shared__ __attribute__((aligned(16))) int ldoc[GENERAL ? BUFFERS : 1][GENERAL ? WAVES : 1][ATT_KEYS];
+  __shared__ __attribute__((aligned(16))) int ldoc[GENERAL ? BUFFERS : 1][GENERAL ? WAVES : 1][64];
+  __shared__ uint64_t lbits[WAVES];
+  __shared__ int lrange[3][WAVES];
   __shared__ __attribute__((aligned(16))) T lp[WAVES][32][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -137,7 +143,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int end_row = first_row + ROWS < rows ? first_row + ROWS : rows;
   const int lim_wg = last((end_row - 1) / a.group);
   const int lim_wave = wave_row < rows ? last((wave_row + 31 < rows ? wave_row + 31 : rows - 1) / a.group) : -1;
-  const int tiles = lim_wg < 0 ? 0 : lim_wg / ATT_KEYS + 1;
+  const int tiles = lim_wg < 0 ? 0 : lim_wg / KEYS + 1;
 
   v8 q[DP / 16];
   {
@@ -155,10 +161,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 
   const T* const kp = at<T>(a.k, a.k_off) + b * a.kb + hk * a.kh;
   const T* const vp = at<T>(a.v, a.v_off) + b * a.vb + hk * a.vh;
-  // slot i = thread + n * THREADS of a tile is chunk (i % PC) ^ swizzle of row i / PC;
-  // rows of one thread are STEP apart, which the swizzle of 16 slots does not see
-  constexpr int STEP = THREADS / PC, KINDS = PC == 32 ? 2 : 1;
-  static_assert(PC == 32 ? STEP % 8 == 0 : STEP % 16 == 0, "swizzle");
+  // slot i = thread + n * THREADS of a tile is chunk (i % PC) ^ swizzle of row i / PC; rows of
+  // one thread are STEP apart, and the swizzle comes again after 16 rows
+  constexpr int STEP = THREADS / PC, KINDS = STEP >= 16 ? 1 : 16 / STEP < NL ? 16 / STEP : NL;
   uint32_t kv[KINDS], vv[KINDS];
   auto chunk_of = [&](int kr) { return (slot<PC>(kr, threadIdx.x % PC) % PC) % CH; };
 #pragma unroll
@@ -170,10 +175,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   T rk[DIRECT ? 1 : N][8], rv[DIRECT ? 1 : N][8];
   int rdoc = 0;
   auto load = [&](int kt, int into) {
-    const int base = kt * ATT_KEYS;
+    const int base = kt * KEYS;
     if constexpr (DIRECT) {
       char* const to = lds + into * TILE + wave * 1024;
-      if (base + ATT_KEYS <= a.keys) {
+      if (base + KEYS <= a.keys) {
         const char* const kb = reinterpret_cast<const char*>(kp + base * a.kt);
         const char* const vb = reinterpret_cast<const char*>(vp + base * a.vt);
 #pragma unroll
@@ -206,7 +211,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     if (GENERAL && a.documents) {
       // every wave its own copy, so that all have as many loads on their way; what lies
       // behind the last key is masked by its index
-      const int key = base + lane < a.keys ? base + lane : a.keys - 1;
+      const int key = base + lane % KEYS < a.keys ? base + lane % KEYS : a.keys - 1;
       if constexpr (DIRECT)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(doc + key * a.dt),
                                          (__attribute__((address_space(3))) void*)ldoc[into][wave], 4, 0, 0);
@@ -231,14 +236,16 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   constexpr int PITCH = PC * 16;
 
   int it = 0;  // the buffer of the tile in use
-  // waits for tile ``kt``, which is on its way, and for this wave's reads of the one before,
-  // whose buffer is the next to be filled, and starts on the next one
-  auto arrive = [&](int kt) {
+  // waits for the tile that is on its way, and for this wave's reads of the one before,
+  // whose buffer is the next to be filled, and starts on the one after ``kt``; which it is
+  auto arrive = [&](int kt, auto after) {
+    int next;
     if constexpr (DIRECT) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" : : : "memory");
-      if (kt + 1 < tiles) load(kt + 1, it ^ 1);
+      next = after(kt + 1);
+      if (next < tiles) load(next, it ^ 1);
     } else {
       __syncthreads();
 #pragma unroll
@@ -249,16 +256,18 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
       if (GENERAL && a.documents) ldoc[0][wave][lane] = rdoc;
       __syncthreads();
-      if (kt + 1 < tiles) load(kt + 1, 0);
+      next = after(kt + 1);
+      if (next < tiles) load(next, 0);
     }
+    return next;
   };
   auto compute = [&](int kt, auto is_masked, auto is_safe) {
     constexpr bool MASKED = decltype(is_masked)::value, SAFE = decltype(is_safe)::value;
-    const int base = kt * ATT_KEYS;
+    const int base = kt * KEYS;
 
-    float16v s[2];
+    float16v s[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
 #pragma unroll
@@ -273,21 +282,21 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         // cap tanh y = cap - 2 cap / (e^2y + 1)
         const float by = a.scale * (2.0f * 0x1.715476p+0f);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             s[u][j] = __builtin_fmaf(-2.0f * a.cap,
                                      __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][j] * by) + 1.0f), a.cap);
       } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int j = 0; j < 16; ++j) s[u][j] *= a.scale;
       }
       if (a.slopes) {
         const float away = (float)(base + 8 * h - (t + shift));
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             s[u][j] = __builtin_fmaf(-slope, __builtin_fabsf(away + (float)(32 * u + 16 * (j >> 3) + (j & 7))), s[u][j]);
@@ -296,7 +305,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     if constexpr (MASKED) {
       const int own = lim - base - 8 * h;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int k = 32 * u + 16 * (j >> 3) + (j & 7);
@@ -307,7 +316,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
     float top = s[0][0];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = __builtin_fmaxf(top, s[u][j]);
     top = xor32<OpMax>(top * scale);
@@ -324,9 +333,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       m = next;
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m;
-    v8 p[4];
+    v8 p[2 * U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], scale, -ref));
@@ -343,7 +352,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2 * U; ++u) {
         uint4v w = __builtin_bit_cast(uint4v, values(i, u));
         if constexpr (SAFE) spoiled |= drop_not_finite<vec8<T>::exponent>(w);
         o[i] = mfma_32x32x16(__builtin_bit_cast(v8, w), p[u], o[i]);
@@ -352,9 +361,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       if (__any(spoiled)) {
         const T* const value = reinterpret_cast<const T*>(lds + (BUFFERS + it) * TILE);
 #pragma unroll 1
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2 * U; ++u) {
           // p by a constant index only: it stays in registers
-          const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
+          const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2 * U - 2] : p[2 * U - 1];
           *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
           __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
@@ -376,12 +385,6 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
   };
 
-  // tiles that every row sees whole, then those that need a mask
-  int whole = 0;
-  if (!(GENERAL && a.documents)) {
-    whole = (last(first_row / a.group) + 1) / ATT_KEYS;
-    whole = whole < 0 ? 0 : whole < tiles ? whole : tiles;
-  }
   auto turn = [&] {  // to the other buffer
     if constexpr (DIRECT) {
       k_at ^= TILE;
@@ -389,15 +392,118 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       it ^= 1;
     }
   };
-  if (tiles > 0) load(0, it);
-  int kt = 0;
-  for (; kt < whole; ++kt, turn()) {
-    arrive(kt);
-    compute(kt, bool_constant<false>{}, bool_constant<false>{});
+  // tiles that every row sees whole
+  int whole = (last(first_row / a.group) + 1) / KEYS;
+  whole = whole < 0 ? 0 : whole < tiles ? whole : tiles;
+  auto every = [](int kt) { return kt; };
+  if (!(GENERAL && a.documents)) {
+    // those first, then the ones that need a mask
+    if (tiles > 0) load(0, it);
+    int kt = 0;
+    while (kt < whole) {
+      const int next = arrive(kt, every);
+      compute(kt, bool_constant<false>{}, bool_constant<false>{});
+      turn();
+      kt = next;
+    }
+    while (kt < tiles) {
+      const int next = arrive(kt, every);
+      if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
+      turn();
+      kt = next;
+    }
   }
-  for (; kt < tiles; ++kt, turn()) {
-    arrive(kt);
-    if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
+  if constexpr (GENERAL) {
+    if (a.documents) {
+      // The documents of the workgroup's rows, least and largest, and whether a row has none.
+      // A tile whose documents lie outside is left out, one that is of the rows' only
+      // document needs no mask: tiles are looked through SPAN at a time, 8 keys a lane.
+      constexpr int LANES = KEYS / 8, PER_WAVE = 64 / LANES, SPAN = PER_WAVE * WAVES;
+      static_assert(SPAN <= 64, "bits");
+      auto least = [](int x, int y) { return x < y ? x : y; };
+      auto largest = [](int x, int y) { return x > y ? x : y; };
+      int lo = mine < 0 ? 0x7fffffff : mine, hi = mine, none = mine < 0;
+      for (int d = 1; d < 32; d <<= 1) {
+        lo = least(lo, __shfl_xor(lo, d, 64));
+        hi = largest(hi, __shfl_xor(hi, d, 64));
+        none |= __shfl_xor(none, d, 64);
+      }
+      if (lane == 0) lrange[0][wave] = lo, lrange[1][wave] = hi, lrange[2][wave] = none;
+      __syncthreads();
+      for (int i = 0; i < WAVES; ++i) {
+        lo = least(lo, lrange[0][i]);
+        hi = largest(hi, lrange[1][i]);
+        none |= lrange[2][i];
+      }
+      lo = __builtin_amdgcn_readfirstlane(lo);
+      hi = __builtin_amdgcn_readfirstlane(hi);
+      const bool one = __builtin_amdgcn_readfirstlane(none) == 0 && lo == hi;
+      int looked = -1;
+      uint64_t open = 0, full = 0;
+      // the first tile from ``kt`` on that rows see some of, all of (FULL), or not all of
+      auto find = [&](int kt, bool any, bool want_full) {
+        while (kt < tiles) {
+          if (kt / SPAN != looked) {
+            looked = kt / SPAN;
+            const int tile = looked * SPAN + wave * PER_WAVE + lane / LANES;
+            int dl = 0x7fffffff, dh = -1;
+            bool gap = false;  // a token of no document
+            for (int j = 0; j < 8; ++j) {
+              const int key = tile * KEYS + lane % LANES * 8 + j;
+              const int x = key < a.keys ? doc[key * a.dt] : -1;
+              gap |= x < 0;
+              dl = x < 0 ? dl : least(dl, x);
+              dh = largest(dh, x);
+            }
+            int holes = gap;
+            for (int d = 1; d < LANES; d <<= 1) {
+              dl = least(dl, __shfl_xor(dl, d, 64));
+              dh = largest(dh, __shfl_xor(dh, d, 64));
+              holes |= __shfl_xor(holes, d, 64);
+            }
+            const bool first = lane % LANES == 0;
+            const uint64_t some = __ballot(first && dh >= lo && dl <= hi);
+            const uint64_t all = __ballot(first && one && !holes && dl == lo && dh == lo && tile < whole);
+            uint64_t bits = 0;
+            for (int i = 0; i < PER_WAVE; ++i) {
+              bits |= ((some >> (i * LANES)) & 1) << i;
+              bits |= ((all >> (i * LANES)) & 1) << (i + 32);
+            }
+            __syncthreads();  // everyone is done with the span before
+            if (lane == 0) lbits[wave] = bits;
+            __syncthreads();
+            open = full = 0;
+            for (int i = 0; i < WAVES; ++i) {
+              const uint64_t w = lbits[i];
+              open |= (w & 0xffffffffu) << (i * PER_WAVE);
+              full |= (w >> 32) << (i * PER_WAVE);
+            }
+          }
+          const uint64_t left = (any ? open : want_full ? full : open & ~full) >> (kt % SPAN);
+          if (left) return kt + __builtin_ctzll(left);
+          kt = (looked + 1) * SPAN;
+        }
+        return tiles;
+      };
+      auto full_ones = [&](int kt) { return find(kt, false, true); };
+      auto other_ones = [&](int kt) { return find(kt, false, false); };
+      int kt = full_ones(0);
+      if (kt < tiles) load(kt, it);
+      while (kt < tiles) {
+        const int next = arrive(kt, full_ones);
+        compute(kt, bool_constant<false>{}, bool_constant<false>{});
+        turn();
+        kt = next;
+      }
+      kt = other_ones(0);
+      if (kt < tiles) load(kt, it);
+      while (kt < tiles) {
+        const int next = arrive(kt, other_ones);
+        if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
+        turn();
+        kt = next;
+      }
+    }
   }
   // 0 times an infinity or NaN of a key that a row does not see is NaN in the products.
   // Where something came out not finite, all is done again with such values left out
@@ -415,9 +521,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     m = -__builtin_inff();
     l = 0.0f;
     if (tiles > 0) load(0, it);
-    for (kt = 0; kt < tiles; ++kt, turn()) {
-      arrive(kt);
-      if (kt * ATT_KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
+    for (int kt = 0; kt < tiles; ++kt) {
+      arrive(kt, every);
+      if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
+      turn();
     }
   }
   if (row >= rows) return;
