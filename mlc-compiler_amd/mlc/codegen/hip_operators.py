@@ -161,12 +161,25 @@ def attention_kernel(dtype, dp: int, waves: int, direct: bool, general: bool) ->
             f"{str(general).lower()})"), name
 
 
-def attention_waves(rows: int, pairs: int) -> int:
-    """Waves of a workgroup, each with 32 rows."""
-    for waves in (4, 2):
-        if _ceil(rows, 32 * waves) * pairs >= UNITS:
-            return waves
-    return 1
+def join_kernel(op: str, dtype, waves: int) -> tuple[str, str]:
+    name = f"{op}_join_{SHORT[dtype]}_w{waves}"
+    return f"{op.upper()}_JOIN({name}, {NAMES[dtype]}, {waves})", name
+
+
+def _join(op: str, dtype, parts: int, rows: int, pointers: tuple, tail: bytes) -> Launch:
+    """The launch that makes one of up to ``parts`` parts of each of ``rows`` rows: four
+    waves a row take the latency of many parts side by side where rows are few."""
+    waves = 4 if parts > 8 and rows <= 1 << 16 else 1
+    kernel, name = join_kernel(op, dtype, waves)
+    return Launch(kernel, op, name, _grid(rows, 64 * waves, op), 64 * waves, pointers, tail)
+
+
+def attention_split(rows: int, pairs: int, key_tiles: int, dp: int) -> tuple[int, int]:
+    """Waves of a workgroup, each with 32 rows, and splits of the keys."""
+    waves = 4 if rows > 64 else 2 if rows > 32 else 1
+    blocks = _ceil(rows, 32 * waves) * pairs
+    splits = max(1, min(2 * UNITS // blocks, key_tiles // 4)) if blocks < UNITS else 1
+    return waves, splits
 
 
 def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
@@ -180,22 +193,28 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
     dp = _padded(dim, ATTENTION_DIMS)
     direct = (dp == dim and keys > 0 and k.aligned and v.aligned
               and all(n % 8 == 0 and n < 1 << 24 for n in (*k.strides[:3], *v.strides[:3])))
-    waves = attention_waves(queries * group, batch * kv_heads)
-    tiles = _ceil(queries * group, 32 * waves)
+    rows, pairs = queries * group, batch * kv_heads
+    waves, splits = attention_split(rows, pairs, _ceil(keys, 32 if dp == 256 else 64), dp)
+    tiles = _ceil(rows, 32 * waves)
     general = bool(cap) or slopes is not None or documents is not None
     some = lambda x, n: x.strides if x is not None else (0,) * n  # noqa: E731
     off = lambda x: x.offset if x is not None else 0  # noqa: E731
-    tail = struct.pack("<6q13q8i2f", q.offset, k.offset, v.offset, off(slopes), off(documents),
+    tail = struct.pack("<6q13q10i2f", q.offset, k.offset, v.offset, off(slopes), off(documents),
                        off(prefix), *q.strides[:3], *k.strides[:3], *v.strides[:3],
                        *some(slopes, 1), *some(documents, 2), *some(prefix, 1),
-                       batch, queries, keys, kv_heads, group, dim, causal, tiles,
+                       batch, queries, keys, kv_heads, group, dim, causal, tiles, splits, 0,
                        *_factors(scale, cap))
     kernel, name = attention_kernel(q.dtype, dp, waves, direct, general)
-    grid = _grid(tiles * batch * kv_heads, 64 * waves, "attention")
+    grid = _grid(tiles * pairs * splits, 64 * waves, "attention")
     pointers = ("q", "k", "v", "slopes" if slopes is not None else None,
                 "documents" if documents is not None else None,
-                "prefix" if prefix is not None else None, "out0")
-    return Plan((Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail),))
+                "prefix" if prefix is not None else None, "out0",
+                "workspace" if splits > 1 else None)
+    launch = Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail)
+    if splits == 1:
+        return Plan((launch,))
+    return Plan((launch, _join("attention", q.dtype, splits, batch * queries * heads, pointers, tail)),
+                splits * pairs * rows * (dim + 4) * 4)
 
 
 # --------------------------------------------------------------------------
@@ -245,11 +264,6 @@ def cached_kernel(dtype, dp: int, tall: int, step: int, waves: int, general: boo
             f"{str(general).lower()})"), name
 
 
-def join_kernel(dtype) -> tuple[str, str]:
-    name = f"cache_attention_join_{SHORT[dtype]}"
-    return f"CACHE_ATTENTION_JOIN({name}, {NAMES[dtype]})", name
-
-
 def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale: Operand,
                          v_scale: Operand, start: Operand, count: Operand | None,
                          slopes: Operand | None, scale: float, cap: float) -> Plan:
@@ -286,10 +300,8 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
     workspace = 0
     if most > 1:  # a sequence may be cut
         workspace = slots * kv_heads * rows * (dim + 4) * 4
-        join, join_name = join_kernel(q.dtype)
-        launches.append(Launch(join, "cache_attention", join_name,
-                               _grid(batch * tokens * heads, 64, "cache_attention"), 64, pointers,
-                               tail))
+        launches.append(_join("cache_attention", q.dtype, min(most, slots), batch * tokens * heads,
+                              pointers, tail))
     return Plan(tuple(launches), workspace)
 
 
@@ -323,5 +335,6 @@ def all_kernels() -> list[tuple[str, str]]:
         out += [("cache_attention", cached_kernel(dtype, dp, tall, step, 4, g)[0])
                 for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
                 for step in (32, 64) for g in (False, True)]
-        out.append(("cache_attention", join_kernel(dtype)[0]))
+        out += [(op, join_kernel(op, dtype, w)[0]) for op in ("attention", "cache_attention")
+                for w in (1, 4)]
     return out

@@ -26,9 +26,11 @@ struct AttentionArgs {
   const void* documents;  // null: one document
   const void* prefix;     // null: none
   void* out;
+  float* part;  // where keys are split: [split][pair][row][dim + 4], see join_parts
   int64_t q_off, k_off, v_off, s_off, d_off, p_off;      // bytes
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ss, db, dt, ps;  // elements
-  int32_t batch, queries, keys, kv_heads, group, dim, causal, tiles;
+  int32_t batch, queries, keys, kv_heads, group, dim, causal, tiles;  // tiles of rows
+  int32_t splits, pad;  // of keys
   float scale, cap;  // scale times log2 e where cap is 0, else 1/cap of it and cap log2 e
 };
 
@@ -108,18 +110,19 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
   const int rows = a.queries * a.group;
-  // Workgroups go to the 8 XCDs in turn: a pair of batch and key head stays on one where
-  // there are enough of them, and long tiles come first
-  const int pairs = a.batch * a.kv_heads;
-  int pair, tile;
-  if (pairs % 8 == 0) {
+  // Workgroups go to the 8 XCDs in turn: a unit (batch, key head, split of the keys) stays on
+  // one where there are enough of them, and long tiles come first
+  const int units = a.batch * a.kv_heads * a.splits;
+  int unit, tile;
+  if (units % 8 == 0) {
     const int i = blockIdx.x / 8;
-    pair = i % (pairs / 8) * 8 + blockIdx.x % 8;
-    tile = a.tiles - 1 - i / (pairs / 8);
+    unit = i % (units / 8) * 8 + blockIdx.x % 8;
+    tile = a.tiles - 1 - i / (units / 8);
   } else {
-    pair = blockIdx.x % pairs;
-    tile = a.tiles - 1 - blockIdx.x / pairs;
+    unit = blockIdx.x % units;
+    tile = a.tiles - 1 - blockIdx.x / units;
   }
+  const int pair = unit / a.splits, split = unit % a.splits;
   const int b = pair / a.kv_heads, hk = pair % a.kv_heads;
 
   const int shift = a.keys - a.queries;  // position of query 0
@@ -143,6 +146,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int end_row = first_row + ROWS < rows ? first_row + ROWS : rows;
   const int lim_wg = last((end_row - 1) / a.group);
   const int lim_wave = wave_row < rows ? last((wave_row + 31 < rows ? wave_row + 31 : rows - 1) / a.group) : -1;
+  // Tiles of keys before ``tiles`` are seen. A split takes every splits-th of them: those that
+  // are read at one time then lie side by side. (Splits of adjacent tiles lie a power of two
+  // apart and meet in few memory channels: one query, 16384 keys, 8 heads of 128, 64 splits
+  // 58 us; 16000 keys 20.)
   const int tiles = lim_wg < 0 ? 0 : lim_wg / KEYS + 1;
 
   v8 q[DP / 16];
@@ -244,7 +251,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" : : : "memory");
-      next = after(kt + 1);
+      next = after(kt + a.splits);
       if (next < tiles) load(next, it ^ 1);
     } else {
       __syncthreads();
@@ -256,7 +263,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
       if (GENERAL && a.documents) ldoc[0][wave][lane] = rdoc;
       __syncthreads();
-      next = after(kt + 1);
+      next = after(kt + a.splits);
       if (next < tiles) load(next, 0);
     }
     return next;
@@ -394,12 +401,12 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   };
   // tiles that every row sees whole
   int whole = (last(first_row / a.group) + 1) / KEYS;
-  whole = whole < 0 ? 0 : whole < tiles ? whole : tiles;
+  whole = whole < tiles ? whole : tiles;
   auto every = [](int kt) { return kt; };
   if (!(GENERAL && a.documents)) {
     // those first, then the ones that need a mask
-    if (tiles > 0) load(0, it);
-    int kt = 0;
+    int kt = split;
+    if (kt < tiles) load(kt, it);
     while (kt < whole) {
       const int next = arrive(kt, every);
       compute(kt, bool_constant<false>{}, bool_constant<false>{});
@@ -441,7 +448,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       int looked = -1;
       uint64_t open = 0, full = 0;
       // the first tile from ``kt`` on that rows see some of, all of (FULL), or not all of
-      auto find = [&](int kt, bool any, bool want_full) {
+      auto find = [&](int kt, bool want_full) {
         while (kt < tiles) {
           if (kt / SPAN != looked) {
             looked = kt / SPAN;
@@ -479,15 +486,15 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
               full |= (w >> 32) << (i * PER_WAVE);
             }
           }
-          const uint64_t left = (any ? open : want_full ? full : open & ~full) >> (kt % SPAN);
-          if (left) return kt + __builtin_ctzll(left);
-          kt = (looked + 1) * SPAN;
+          const uint64_t these = want_full ? full : open & ~full;
+          for (; kt < tiles && kt / SPAN == looked; kt += a.splits)
+            if ((these >> (kt % SPAN)) & 1) return kt;
         }
         return tiles;
       };
-      auto full_ones = [&](int kt) { return find(kt, false, true); };
-      auto other_ones = [&](int kt) { return find(kt, false, false); };
-      int kt = full_ones(0);
+      auto full_ones = [&](int kt) { return find(kt, true); };
+      auto other_ones = [&](int kt) { return find(kt, false); };
+      int kt = full_ones(split);
       if (kt < tiles) load(kt, it);
       while (kt < tiles) {
         const int next = arrive(kt, full_ones);
@@ -495,7 +502,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         turn();
         kt = next;
       }
-      kt = other_ones(0);
+      kt = other_ones(split);
       if (kt < tiles) load(kt, it);
       while (kt < tiles) {
         const int next = arrive(kt, other_ones);
@@ -520,8 +527,8 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
     m = -__builtin_inff();
     l = 0.0f;
-    if (tiles > 0) load(0, it);
-    for (int kt = 0; kt < tiles; ++kt) {
+    if (split < tiles) load(split, it);
+    for (int kt = split; kt < tiles; kt += a.splits) {
       arrive(kt, every);
       if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
       turn();
@@ -529,6 +536,19 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   }
   if (row >= rows) return;
   l = xor32<OpSum>(l);
+  if (a.splits > 1) {
+    float* const part = a.part + (((int64_t)split * a.batch * a.kv_heads + pair) * rows + row) * (a.dim + 4);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const int d = 32 * i + 8 * z + 4 * h;
+        if (d < a.dim)
+          *reinterpret_cast<float4v*>(part + d) = float4v{o[i][4 * z], o[i][4 * z + 1], o[i][4 * z + 2], o[i][4 * z + 3]};
+      }
+    if (h == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{m, l, 0.0f, 0.0f};
+    return;
+  }
   const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
   T* const out = reinterpret_cast<T*>(a.out) +
                  (((int64_t)b * a.queries + t) * a.kv_heads * a.group + head) * a.dim;
@@ -546,9 +566,25 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
 }
 
+// One workgroup for each (sequence, token, head).
+template <class T, int WAVES>
+__device__ __forceinline__ void attention_join(const AttentionArgs& a) {
+  const int heads = a.kv_heads * a.group, head = (int)(blockIdx.x % (uint32_t)heads);
+  const uint32_t w = blockIdx.x / (uint32_t)heads;
+  const int t = (int)(w % (uint32_t)a.queries), b = (int)(w / (uint32_t)a.queries);
+  const int64_t rows = (int64_t)a.queries * a.group;
+  const int64_t row = ((int64_t)b * a.kv_heads + head / a.group) * rows + (int64_t)t * a.group + head % a.group;
+  join_parts<WAVES>(a.part + row * (a.dim + 4), a.batch * a.kv_heads * rows * (a.dim + 4), a.splits, a.dim,
+             reinterpret_cast<T*>(a.out) + (((int64_t)b * a.queries + t) * heads + head) * a.dim);
+}
+
 }  // namespace mlc
 
 #define ATTENTION(NAME, T, DP, WAVES, DIRECT, GENERAL)                                            \
-  extern "C" __global__ void __launch_bounds__(64 * WAVES, 2) NAME(mlc::AttentionArgs a) {        \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, DP == 64 ? 3 : 2) NAME(mlc::AttentionArgs a) {\
     mlc::attention<T, DP, WAVES, DIRECT, GENERAL>(a);                                             \
+  }
+#define ATTENTION_JOIN(NAME, T, WAVES)                                                   \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::AttentionArgs a) {                  \
+    mlc::attention_join<T, WAVES>(a);                                                   \
   }

@@ -47,7 +47,7 @@ __device__ __forceinline__ int held(const CacheAttentionArgs& a, int b, int& sta
 }
 
 struct Item {
-  int b, nth, of, length, keys;  // the nth of a sequence's items, ``length`` keys each
+  int b, nth, of, keys;  // the nth of the items of a sequence of so many keys
 };
 
 // How the sequences' keys are cut: every wave finds it again from the lengths.
@@ -78,7 +78,6 @@ __device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want,
       found.b = b0 + at_lane;
       found.of = __shfl(n, at_lane, 64);
       found.keys = __shfl(keys, at_lane, 64);
-      found.length = c;
       first += __shfl(sum, at_lane, 64) - found.of;
       found.nth = want >= 0 ? want - first : 0;
       return true;
@@ -130,8 +129,9 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   int start, count;
   held(a, b, start, count);
   if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
-  const int lo_key = item.nth * item.length;
-  const int hi_key = lo_key + item.length < item.keys ? lo_key + item.length : item.keys;
+  // an item's waves take every so-manieth step of the keys: what is read at one time lies
+  // side by side, not a power of two apart
+  const int hi_key = item.keys;
 
   const int rows = a.tokens * a.group;
   v8 q[RT][2 * KP];
@@ -181,7 +181,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   const int krow = 8 * (c >> 2) + (c & 3);
   const bool v_mine = c * VB < a.dim;
 
-  for (int tb = lo_key + wave * TOK; tb < hi_key; tb += WAVES * TOK) {
+  for (int tb = (item.nth * WAVES + wave) * TOK; tb < hi_key; tb += item.of * WAVES * TOK) {
     uint4v kr[CH][2][KP];
     words<VW> vr[CH][8];
     const bool whole = tb + TOK <= hi_key;
@@ -389,8 +389,9 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   }
 }
 
-// One workgroup of 64 for each (sequence, token, head): its items' parts as one.
-template <class T> __device__ __forceinline__ void cache_attention_join(const CacheAttentionArgs& a) {
+// One workgroup for each (sequence, token, head): its items' parts as one.
+template <class T, int WAVES>
+__device__ __forceinline__ void cache_attention_join(const CacheAttentionArgs& a) {
   const int heads = a.kv_heads * a.group;
   const int head = (int)(blockIdx.x % (uint32_t)heads);
   const uint32_t w = blockIdx.x / (uint32_t)heads;
@@ -401,28 +402,8 @@ template <class T> __device__ __forceinline__ void cache_attention_join(const Ca
   const int hk = head / a.group, rows = a.tokens * a.group, row = t * a.group + head % a.group;
   const int64_t step = (int64_t)a.kv_heads * rows * (a.dim + 4);
   const float* const part = a.part + (((int64_t)first * a.kv_heads + hk) * rows + row) * (a.dim + 4);
-  float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < item.of; i += 64) top = __builtin_fmaxf(top, part[i * step + a.dim]);
-  top = group_reduce<64, OpMax>(top);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
-  float x[4] = {}, sum = 0.0f;
-  const int d = threadIdx.x * 4;
-  for (int i = 0; i < item.of; ++i) {
-    const float4v ml = *reinterpret_cast<const float4v*>(part + i * step + a.dim);
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    sum = __builtin_fmaf(ml.y, f, sum);
-    if (d < a.dim) {
-      const float4v v = *reinterpret_cast<const float4v*>(part + i * step + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
-    }
-  }
-  if (d >= a.dim) return;
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-  T v[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(x[e] * inverse);
-  store_n<8>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.tokens + t) * heads + head) * a.dim + d, v);
+  join_parts<WAVES>(part, step, item.of, a.dim,
+             reinterpret_cast<T*>(a.out) + (((int64_t)b * a.tokens + t) * heads + head) * a.dim);
 }
 
 }  // namespace mlc
@@ -431,7 +412,7 @@ template <class T> __device__ __forceinline__ void cache_attention_join(const Ca
   extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::CacheAttentionArgs a) {      \
     mlc::cache_attention<T, DP, RT, TOK, WAVES, GENERAL>(a);                                      \
   }
-#define CACHE_ATTENTION_JOIN(NAME, T)                                                             \
-  extern "C" __global__ void __launch_bounds__(64) NAME(mlc::CacheAttentionArgs a) {              \
-    mlc::cache_attention_join<T>(a);                                                              \
+#define CACHE_ATTENTION_JOIN(NAME, T, WAVES)                                             \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::CacheAttentionArgs a) {             \
+    mlc::cache_attention_join<T, WAVES>(a);                                             \
   }

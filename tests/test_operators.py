@@ -693,7 +693,7 @@ def test_every_kernel_a_plan_asks_for_is_built_beforehand():
     seen = set()
     for _ in range(3000):
         dtype, kv, group = random.choice((HALF, BF, FULL)), random.choice((1, 2, 8)), random.choice((1, 4, 16))
-        b, t = random.choice((1, 2, 40)), random.choice((1, 2, 5, 31, 200, 5000))
+        b, t = random.choice((1, 2, 40)), random.choice((1, 2, 3, 5, 31, 200, 5000))
         dim, block = random.choice((16, 64, 80, 96, 128, 256)), random.choice((32, 64, 128))
         q, k = dense(b, t, kv * group, dim, dtype=dtype), dense(b, t, kv, dim, dtype=dtype)
         cache = dense(b, kv, 64 * block, dim, dtype=E4M3)
