@@ -191,8 +191,10 @@ def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
         return Plan(())
     group = heads // kv_heads
     dp = _padded(dim, ATTENTION_DIMS)
+    # a tile's rows are addressed by 32 bits from its first one
     direct = (dp == dim and keys > 0 and k.aligned and v.aligned
-              and all(n % 8 == 0 and n < 1 << 24 for n in (*k.strides[:3], *v.strides[:3])))
+              and all(n % 8 == 0 for n in (*k.strides[:3], *v.strides[:3]))
+              and max(k.strides[1], v.strides[1]) < 1 << 24)
     rows, pairs = queries * group, batch * kv_heads
     waves, splits = attention_split(rows, pairs, _ceil(keys, 32 if dp == 256 else 64), dp)
     tiles = _ceil(rows, 32 * waves)

@@ -147,9 +147,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int lim_wg = last((end_row - 1) / a.group);
   const int lim_wave = wave_row < rows ? last((wave_row + 31 < rows ? wave_row + 31 : rows - 1) / a.group) : -1;
   // Tiles of keys before ``tiles`` are seen. A split takes every splits-th of them: those that
-  // are read at one time then lie side by side. (Splits of adjacent tiles lie a power of two
-  // apart and meet in few memory channels: one query, 16384 keys, 8 heads of 128, 64 splits
-  // 58 us; 16000 keys 20.)
+  // are read at one time then lie side by side.
   const int tiles = lim_wg < 0 ? 0 : lim_wg / KEYS + 1;
 
   v8 q[DP / 16];

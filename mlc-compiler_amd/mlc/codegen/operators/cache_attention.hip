@@ -130,7 +130,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   held(a, b, start, count);
   if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
   // an item's waves take every so-manieth step of the keys: what is read at one time lies
-  // side by side, not a power of two apart
+  // side by side
   const int hi_key = item.keys;
 
   const int rows = a.tokens * a.group;

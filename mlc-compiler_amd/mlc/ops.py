@@ -98,7 +98,7 @@ def _check_rotary(q, k, positions, frequencies, interleaved, magnitude) -> None:
     _same(q, {"k": k, "positions": positions, "frequencies": frequencies})
 
 
-def _check_attention(q, k, v, scale, causal, cap, slopes, documents, prefix) -> None:
+def _check_attention(q, k, v, slopes, documents, prefix, scale, causal, cap) -> None:
     _rows("q", q, _HALF)
     _rows("k", k, (q.dtype,))
     _rows("v", v, (q.dtype,))
@@ -173,8 +173,8 @@ def _check_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count) 
               "v": v, "start": start, **({"count": count} if count is not None else {})})
 
 
-def _check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, scale, cap,
-                           slopes) -> None:
+def _check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, slopes, scale,
+                           cap) -> None:
     _check_cache(k_cache, v_cache, k_scale, v_scale)
     batch, kv_heads, capacity, dim = k_cache.shape
     _rows("q", q, _HALF)
@@ -201,65 +201,65 @@ def _check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, 
 # direct calls
 # --------------------------------------------------------------------------
 
-#: (operator, shapes, strides, types, options) -> plan
-_plans: dict = {}
-#: plans kept: calls of ever new sizes start again
-_MOST_PLANS = 4096
+#: (operator, options, each operand's type, shape, strides, device and place within
+#: 16 bytes) -> the call's launches (``runtime.operators.Call``): nothing that
+#: depends on an address or a value
+_calls: dict = {}
+#: calls kept: with ever new sizes it starts again
+_MOST_CALLS = 4096
+
+_Tensor, _grad_enabled = torch.Tensor, torch.is_grad_enabled
+_is_compiling = torch.compiler.is_compiling
+_contiguous = torch.contiguous_format
 
 
-def _direct(*tensors) -> bool:
-    """Whether the operands are plain GPU tensors outside of any tracing. One
-    that asks for a gradient is refused."""
-    if torch.compiler.is_compiling():
-        return False
-    plain = True
-    for x in tensors:
+def _signed(op: str, operands: tuple, options: tuple):
+    """The signature of a call and its operands' addresses, or ``(None, None)`` where
+    they are not plain GPU tensors outside of any tracing. An operand that asks for a
+    gradient is refused."""
+    key, at = [op, options], []
+    grad = _grad_enabled()
+    if _is_compiling():
+        return None, None
+    for x in operands:
         if x is None:
+            key.append(None)
+            at.append(0)
             continue
-        if x.requires_grad and torch.is_grad_enabled():
+        if grad and x.requires_grad:
             raise OperatorError("an operand asks for a gradient, and the operators of mlc.ops are "
                                 "for inference: call them under torch.no_grad()")
-        plain = plain and type(x) is torch.Tensor and x.is_cuda
-    return plain
+        if type(x) is not _Tensor:
+            return None, None
+        device = x.get_device()
+        if device < 0:
+            return None, None
+        p = x.data_ptr()
+        at.append(p)
+        key += (x.dtype, x.shape, x.stride(), device, p & 15)
+    return tuple(key), at
 
 
-def _operand(x, at: int | None = None) -> Operand | None:
-    if x is None:
-        return None
-    return Operand(tuple(x.shape), x.stride(), x.dtype,
-                   aligned=(x.data_ptr() if at is None else at) % 16 == 0)
+def _operand(x, p: int) -> Operand | None:
+    return None if x is None else Operand(tuple(x.shape), x.stride(), x.dtype, aligned=p % 16 == 0)
 
 
-def _signature(*tensors):
-    return [None if x is None else (x.dtype, x.shape, x.stride(), x.device.index,
-                                    x.data_ptr() % 16) for x in tensors]
+def _call_of(key, op: str, operands: tuple, at: list, options: tuple):
+    """The launches of a call of a new signature, checked."""
+    from .runtime.operators import Call
 
-
-def _run(plan, device: torch.device, pointers: dict[str, int]) -> None:
-    from .runtime import operators
-
-    modules = operators.device_modules(device.index)
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _run(plan, device, pointers)
-    flags = any("error" in launch.pointers for launch in plan.launches)
-    if flags:
-        pointers["error"] = modules.error_word()
-        if modules.pending() and not torch.cuda.is_current_stream_capturing():
-            _raise(modules)
-    if plan.workspace:
-        space = torch.empty(plan.workspace, dtype=torch.uint8, device=device)
-        pointers["workspace"] = space.data_ptr()
-    modules.run(plan, pointers, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _raise(modules) -> None:
-    from .runtime.executor import ExecutionError
-    from .runtime.operators import INVALID
-
-    code = modules.pending()
-    modules.clear()
-    raise ExecutionError(INVALID.get(code, f"an operator flagged an invalid input ({code})"))
+    check, plan, names = _OPERATORS[op]
+    check(*operands, *options)
+    for name, x, p in zip(names, operands, at):
+        if name.endswith("cache") or name.endswith("_scale"):
+            _require(p % 16 == 0, f"{name}: not on 16 bytes")
+    device = operands[0].get_device()
+    made = plan(*[_operand(x, p) for x, p in zip(operands, at)], *options)
+    call = Call(made, names, device)
+    if len(_calls) >= _MOST_CALLS:
+        _calls.clear()
+    _calls[key] = call
+    return call
 
 
 def check_errors() -> None:
@@ -268,78 +268,45 @@ def check_errors() -> None:
     that can meet one raises, once the call that met it is done."""
     from .runtime import operators
 
-    for index, modules in list(operators._devices.items()):
-        torch.cuda.synchronize(index)
-        if modules.pending():
-            _raise(modules)
+    operators.check_errors()
 
 
-def _planned(op: str, tensors: dict, options: tuple, check, build):
-    """The plan of a call, checked the first time its signature comes."""
-    key = (op, options, tuple(_signature(*tensors.values())))
-    found = _plans.get(key)
-    if found is None:
-        check(*tensors.values(), *options)
-        first = next(iter(tensors.values()))
-        for name, x in tensors.items():
-            if name.endswith("cache") or name.endswith("_scale"):
-                _require(x.data_ptr() % 16 == 0, f"{name}: not on 16 bytes")
-        found = build({n: _operand(x) for n, x in tensors.items()}, *options)
-        if len(_plans) >= _MOST_PLANS:
-            _plans.clear()
-        _plans[key] = found
-    return found
+def _plan_attention(q, k, v, slopes, documents, prefix, scale, causal, cap):
+    return plans.plan_attention(q, k, v, slopes, documents, prefix,
+                                plans.score_scale(scale, q.shape[3]), causal, float(cap))
 
 
-def _pointers(tensors: dict) -> dict[str, int]:
-    return {n: x.data_ptr() for n, x in tensors.items() if x is not None}
+def _plan_cache_attention(q, kc, vc, ks, vs, start, count, slopes, scale, cap):
+    return plans.plan_cache_attention(q, kc, vc, ks, vs, start, count, slopes,
+                                      plans.score_scale(scale, q.shape[3]), float(cap))
 
 
-def _rotary_now(q, k, positions, frequencies, interleaved, magnitude):
-    tensors = {"q": q, "k": k, "positions": positions, "frequencies": frequencies}
-    plan = _planned("rotary", tensors, (interleaved, magnitude), _check_rotary,
-                    lambda t, *o: plans.plan_rotary(t["q"], t["k"], t["positions"],
-                                                    t["frequencies"], *o))
-    out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-           torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    _run(plan, q.device, {**_pointers(tensors), "out0": out[0].data_ptr(), "out1": out[1].data_ptr()})
-    return out
+_CACHE = ("k_cache", "v_cache", "k_scale", "v_scale")
+#: operator -> its check, its plan (operands, then options) and its operands' names
+_OPERATORS = {
+    "rotary": (_check_rotary, plans.plan_rotary, ("q", "k", "positions", "frequencies")),
+    "attention": (_check_attention, _plan_attention,
+                  ("q", "k", "v", "slopes", "documents", "prefix")),
+    "cache_append": (_check_cache_append, plans.plan_cache_append,
+                     (*_CACHE, "k", "v", "start", "count")),
+    "cache_attention": (_check_cache_attention, _plan_cache_attention,
+                        ("q", *_CACHE, "start", "count", "slopes")),
+}
 
 
-def _attention_now(q, k, v, scale, causal, cap, slopes, documents, prefix):
-    tensors = {"q": q, "k": k, "v": v, "slopes": slopes, "documents": documents, "prefix": prefix}
-
-    def check(q, k, v, slopes, documents, prefix, scale, causal, cap):
-        _check_attention(q, k, v, scale, causal, cap, slopes, documents, prefix)
-
-    plan = _planned("attention", tensors, (scale, causal, cap), check,
-                    lambda t, s, c, p: plans.plan_attention(*t.values(), _scale(s, q.shape[3]),
-                                                            c, _cap(p)))
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _run(plan, q.device, {**_pointers(tensors), "out0": out.data_ptr()})
-    return out
-
-
-def _cache_append_now(k_cache, v_cache, k_scale, v_scale, k, v, start, count):
-    tensors = {"k_cache": k_cache, "v_cache": v_cache, "k_scale": k_scale, "v_scale": v_scale,
-               "k": k, "v": v, "start": start, "count": count}
-    plan = _planned("cache_append", tensors, (), _check_cache_append,
-                    lambda t: plans.plan_cache_append(*t.values()))
-    _run(plan, k.device, _pointers(tensors))
-
-
-def _cache_attention_now(q, k_cache, v_cache, k_scale, v_scale, start, count, scale, cap, slopes):
-    tensors = {"q": q, "k_cache": k_cache, "v_cache": v_cache, "k_scale": k_scale,
-               "v_scale": v_scale, "start": start, "count": count, "slopes": slopes}
-
-    def check(q, kc, vc, ks, vs, start, count, slopes, scale, cap):
-        _check_cache_attention(q, kc, vc, ks, vs, start, count, scale, cap, slopes)
-
-    plan = _planned("cache_attention", tensors, (scale, cap), check,
-                    lambda t, s, p: plans.plan_cache_attention(*t.values(), _scale(s, q.shape[3]),
-                                                               _cap(p)))
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _run(plan, q.device, {**_pointers(tensors), "out0": out.data_ptr()})
+def _now(op: str, operands: tuple, options: tuple, like: tuple):
+    """The call, with results like those operands, or None where ``_signed`` is."""
+    key, at = _signed(op, operands, options)
+    if key is None:
+        return None
+    call = _calls.get(key) or _call_of(key, op, operands, at, options)
+    if not like:
+        call.run(at, None)
+        return ()
+    out = [torch.empty_like(x, memory_format=_contiguous) for x in like]
+    for x in out:
+        at.append(x.data_ptr())
+    call.run(at, out[0])
     return out
 
 
@@ -363,43 +330,46 @@ def _like(x):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _fake_rotary(q, k, positions, frequencies, interleaved, magnitude):
-    _check_rotary(q, k, positions, frequencies, interleaved, magnitude)
-    return _like(q), _like(k)
+def _implement(op: str, split, results: int) -> None:
+    """``mlc::op``: ``split`` puts the schema's arguments into operands and options,
+    results are like the first operands."""
+    check = _OPERATORS[op][0]
 
+    def gpu(*args):
+        operands, options = split(*args)
+        # what the dispatcher hands over may be a parameter or another subclass
+        plain = tuple(x if x is None or type(x) is _Tensor else x.detach().as_subclass(_Tensor)
+                      for x in operands)
+        with torch.no_grad():
+            out = _now(op, plain, options, plain[:results])
+        _require(out is not None, f"{op}: not on one GPU")
+        return tuple(out) if results > 1 else out[0] if results else None
 
-def _fake_attention(q, *rest):
-    _check_attention(q, *rest)
-    return _like(q)
+    def fake(*args):
+        operands, options = split(*args)
+        check(*operands, *options)
+        out = tuple(map(_like, operands[:results]))
+        return out if results > 1 else out[0] if results else None
 
-
-def _fake_cache_append(*args):
-    _check_cache_append(*args)
-
-
-def _fake_cache_attention(q, *rest):
-    _check_cache_attention(q, *rest)
-    return _like(q)
-
-
-def _refuse_host(check):
-    def refuse(*args):
+    def host(*args):
         from .runtime.executor import ExecutionError
 
-        check(*args)
+        operands, options = split(*args)
+        check(*operands, *options)
         raise ExecutionError("the operators of mlc.ops run on a ROCm GPU (torch device 'cuda'), "
                              "not on the CPU")
 
-    return refuse
+    _lib.impl(op, gpu, "CUDA")
+    _lib.impl(op, host, "CPU")
+    torch.library.register_fake(f"mlc::{op}", fake, lib=_lib)
 
 
-for _name, _now, _fake in (("rotary", _rotary_now, _fake_rotary),
-                           ("attention", _attention_now, _fake_attention),
-                           ("cache_append", _cache_append_now, _fake_cache_append),
-                           ("cache_attention", _cache_attention_now, _fake_cache_attention)):
-    _lib.impl(_name, _now, "CUDA")
-    _lib.impl(_name, _refuse_host(_fake), "CPU")
-    torch.library.register_fake(f"mlc::{_name}", _fake, lib=_lib)
+_implement("rotary", lambda q, k, p, f, i, m: ((q, k, p, f), (i, m)), 2)
+_implement("attention", lambda q, k, v, scale, causal, cap, slopes, documents, prefix:
+           ((q, k, v, slopes, documents, prefix), (scale, causal, cap)), 1)
+_implement("cache_append", lambda *args: (args, ()), 0)
+_implement("cache_attention", lambda q, kc, vc, ks, vs, start, count, scale, cap, slopes:
+           ((q, kc, vc, ks, vs, start, count, slopes), (scale, cap)), 1)
 
 
 # --------------------------------------------------------------------------
@@ -416,8 +386,9 @@ def rotary(q, k, positions, frequencies, *, interleaved: bool = False, magnitude
     are turned, the rest is copied. A pair is values ``(i, i + len(frequencies))``, or
     ``(2 i, 2 i + 1)`` if ``interleaved``. ``magnitude`` multiplies what is turned.
     """
-    if _direct(q, k, positions, frequencies):
-        return _rotary_now(q, k, positions, frequencies, interleaved, magnitude)
+    out = _now("rotary", (q, k, positions, frequencies), (interleaved, magnitude), (q, k))
+    if out is not None:
+        return out[0], out[1]
     return torch.ops.mlc.rotary(q, k, positions, frequencies, interleaved, magnitude)
 
 
@@ -471,8 +442,9 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, cap:
     A query that sees nothing gets zeros. What is not seen has no influence, NaN and
     infinities included.
     """
-    if _direct(q, k, v, slopes, documents, prefix):
-        return _attention_now(q, k, v, scale, causal, cap, slopes, documents, prefix)
+    out = _now("attention", (q, k, v, slopes, documents, prefix), (scale, causal, cap), (q,))
+    if out is not None:
+        return out[0]
     return torch.ops.mlc.attention(q, k, v, scale, causal, cap, slopes, documents, prefix)
 
 
@@ -492,8 +464,8 @@ def cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count=None) ->
     A sequence whose ``start`` and ``count`` do not lie within the cache is left alone,
     and ``ExecutionError`` is raised by a later call or :func:`check_errors`.
     """
-    if _direct(k_cache, v_cache, k_scale, v_scale, k, v, start, count):
-        return _cache_append_now(k_cache, v_cache, k_scale, v_scale, k, v, start, count)
+    if _now("cache_append", (k_cache, v_cache, k_scale, v_scale, k, v, start, count), (), ()) is not None:
+        return None
     return torch.ops.mlc.cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count)
 
 
@@ -506,9 +478,10 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count=None, *,
     ``count`` do not lie within the cache (an ``ExecutionError`` later). ``scale``, ``cap``
     and ``slopes`` are those of :func:`attention`.
     """
-    if _direct(q, k_cache, v_cache, k_scale, v_scale, start, count, slopes):
-        return _cache_attention_now(q, k_cache, v_cache, k_scale, v_scale, start, count, scale,
-                                    cap, slopes)
+    out = _now("cache_attention", (q, k_cache, v_cache, k_scale, v_scale, start, count, slopes),
+               (scale, cap), (q,))
+    if out is not None:
+        return out[0]
     return torch.ops.mlc.cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count,
                                          scale, cap, slopes)
 

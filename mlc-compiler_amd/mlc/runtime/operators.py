@@ -10,6 +10,7 @@ and calls captured into several graphs have memory of their own.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -77,14 +78,6 @@ class OperatorModules:
     def clear(self) -> None:
         native.check(self.lib.mlc_error_clear(self._ctx), "mlc_error_clear")
 
-    def run(self, plan: Plan, pointers: dict[str, int], stream: int) -> None:
-        for launch in plan.launches:
-            args = launch.arguments(pointers)
-            rc = self.lib.mlc_launch(self.function(launch), launch.grid, launch.block, 0, args,
-                                     len(args), stream)
-            if rc:
-                native.check(rc, f"mlc_launch({launch.symbol})")
-
     def close(self) -> None:
         for mod in self._modules:
             self.lib.mlc_module_unload(mod)
@@ -100,3 +93,71 @@ def device_modules(index: int) -> OperatorModules:
         with torch.cuda.device(index):
             found = _devices.setdefault(index, OperatorModules(index))
     return found
+
+
+class Call:
+    """The launches of one signature on one device: functions loaded, arguments laid
+    out but for the addresses, which ``run`` gets in the order of the operands and
+    results."""
+
+    def __init__(self, plan: Plan, operands: tuple, device: int) -> None:
+        self.modules = device_modules(device)
+        self.device, self.workspace = device, plan.workspace
+        self.flags = any("error" in x.pointers for x in plan.launches)
+        error = self.modules.error_word() if self.flags else 0
+        # where a launch's pointers are in ``at`` with the workspace and constants behind it
+        names = [*operands, *sorted({p for x in plan.launches for p in x.pointers
+                                     if p is not None and p.startswith("out")})]
+        self.tail = (0, error)
+        place = {n: i for i, n in enumerate((*names, "workspace", None, "error"))}
+        self.launches = []
+        with torch.cuda.device(device):
+            for x in plan.launches:
+                layout = struct.Struct(f"<{len(x.pointers)}Q{len(x.tail)}s")
+                self.launches.append((self.modules.function(x), x.grid, x.block, layout.pack,
+                                      tuple(place[p] for p in x.pointers), x.tail, layout.size))
+        self._launch = self.modules.lib.mlc_launch
+
+    def run(self, at: list, like) -> None:
+        """Launch on torch's current stream of the device. ``like``: a tensor on it."""
+        if _current_device() != self.device:
+            with torch.cuda.device(self.device):
+                return self.run(at, like)
+        if self.flags and self.modules.pending() and not torch.cuda.is_current_stream_capturing():
+            raise_pending(self.modules)
+        space = None
+        if self.workspace:
+            space = like.new_empty(self.workspace, dtype=torch.uint8)
+            at.append(space.data_ptr())
+        else:
+            at.append(0)
+        at += self.tail
+        stream = _current_stream(self.device)
+        for fn, grid, block, pack, place, tail, size in self.launches:
+            rc = self._launch(fn, grid, block, 0, pack(*[at[i] for i in place], tail), size, stream)
+            if rc:
+                native.check(rc, "mlc_launch")
+
+
+def raise_pending(modules: OperatorModules) -> None:
+    from .executor import ExecutionError
+
+    code = modules.pending()
+    modules.clear()
+    raise ExecutionError(INVALID.get(code, f"an operator flagged an invalid input ({code})"))
+
+
+def check_errors() -> None:
+    """Wait for every device that operators ran on and raise for an invalid input."""
+    for index, modules in list(_devices.items()):
+        torch.cuda.synchronize(index)
+        if modules.pending():
+            raise_pending(modules)
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _current_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
