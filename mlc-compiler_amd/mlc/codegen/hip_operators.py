@@ -258,6 +258,7 @@ def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_sc
 
 
 CACHED_DIMS = (64, 128, 256)
+SHORT_CACHE = 2048
 
 
 def cached_kernel(dtype, dp: int, tall: int, step: int, waves: int, general: bool) -> tuple[str, str]:
@@ -278,11 +279,14 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
     dp = _padded(dim, CACHED_DIMS)
     tall = 1 if rows <= 16 else 2 if rows <= 32 or dp == 256 else 4
     row_tiles = _ceil(rows, 16 * tall)
-    step, waves = 64 if block % 64 == 0 else 32, 4
-    # items enough for the device, none shorter than two steps of every wave
+    step = 64 if block % 64 == 0 else 32
+    # A workgroup's waves go through a short cache at once; a longer one is cut into items,
+    # as many as the device holds, none shorter than two steps of every wave.
+    short = capacity <= SHORT_CACHE
+    waves = 8 if short and batch * kv_heads * row_tiles < UNITS and dp < 256 else 4
     shortest = 2 * 64 * waves
-    most = _ceil(capacity, shortest)
-    items = max(1, min(4 * UNITS // (kv_heads * row_tiles), batch * most))
+    most = 1 if short else _ceil(capacity, shortest)
+    items = 0 if short else max(1, min(2 * UNITS // (kv_heads * row_tiles), batch * most))
     slots = min(items + batch, batch * most)
     general = bool(cap) or slopes is not None
     off = lambda x: x.offset if x is not None else 0  # noqa: E731
@@ -334,9 +338,9 @@ def all_kernels() -> list[tuple[str, str]]:
     for dtype in (torch.float16, torch.bfloat16):
         out += [("attention", attention_kernel(dtype, dp, w, direct, g)[0]) for dp in ATTENTION_DIMS
                 for w in (1, 2, 4) for direct in (False, True) for g in (False, True)]
-        out += [("cache_attention", cached_kernel(dtype, dp, tall, step, 4, g)[0])
+        out += [("cache_attention", cached_kernel(dtype, dp, tall, step, w, g)[0])
                 for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
-                for step in (32, 64) for g in (False, True)]
+                for w in (4, 8) if w < 8 or dp < 256 for step in (32, 64) for g in (False, True)]
         out += [(op, join_kernel(op, dtype, w)[0]) for op in ("attention", "cache_attention")
                 for w in (1, 4)]
     return out

@@ -32,7 +32,7 @@ struct CacheAttentionArgs {
   int64_t q_off, cache_off[2], scale_off[2], sl_off, start_off, count_off;  // bytes
   int64_t qb, qt, qh, sls, ss, sc;                                          // elements
   int32_t batch, tokens, kv_heads, group, dim, capacity, block_shift, row_tiles;
-  int32_t items, shortest;  // items wanted of all sequences; keys of the shortest one
+  int32_t items, shortest;  // items wanted of all sequences, 0: each is one; keys of the shortest
   float factor, cap;
 };
 
@@ -50,22 +50,43 @@ struct Item {
   int b, nth, of, keys;  // the nth of the items of a sequence of so many keys
 };
 
-// How the sequences' keys are cut: every wave finds it again from the lengths.
+// How the sequences' keys are cut: every wave finds it again from the lengths. Items are
+// ``length`` keys long at most, as few as are wanted of all sequences together.
 // ``want`` < 0: the first item of sequence -1 - want.
 __device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want, Item& found, int& first) {
   const int lane = threadIdx.x & 63;
   int start, count;
-  int64_t total = 0;
-  for (int b = lane; b < a.batch; b += 64) total += held(a, b, start, count);
-  total = group_reduce<64, OpSum, int64_t>(total);
-  int64_t length = (total + a.items - 1) / a.items;
-  length = (length + 63) / 64 * 64;
-  if (length > a.capacity) length = ((int64_t)a.capacity + 63) / 64 * 64;
-  const int c = length > a.shortest ? (int)length : a.shortest;
+  if (a.items == 0) {  // none is cut
+    found.b = want >= 0 ? want : -1 - want;
+    found.nth = first = 0;
+    found.of = 1;
+    found.keys = held(a, found.b, start, count);
+    return true;
+  }
+  auto cut = [](int keys, int length) { return keys == 0 ? 1 : (keys + length - 1) / length; };
+  int mine = lane < a.batch ? held(a, lane, start, count) : 0;  // of the first 64 sequences
+  auto keys_of = [&](int b) { return b < 64 ? mine : b < a.batch ? held(a, b, start, count) : 0; };
+  float total = 0.0f;  // exact, or near enough: all waves come to the same
+  for (int b0 = 0; b0 < a.batch; b0 += 64) total += (float)keys_of(b0 + lane);
+  total = group_reduce<64, OpSum>(total);
+  int length = a.shortest;
+  for (int i = 0; i < 3; ++i) {
+    // each sequence's last item is short: longer items until there are no more than wanted
+    float n = 0.0f;
+    if (i > 0) {
+      for (int b0 = 0; b0 < a.batch; b0 += 64)
+        if (b0 + lane < a.batch) n += (float)cut(keys_of(b0 + lane), length);
+      n = group_reduce<64, OpSum>(n);
+      if (n <= (float)a.items) break;
+    }
+    const float longer = i == 0 ? total / (float)a.items : (float)length * n / (float)a.items;
+    const int next = longer < (float)a.capacity ? ((int)longer + 64) / 64 * 64 : (a.capacity + 63) / 64 * 64;
+    length = next > length ? next : length;
+  }
   first = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int b = b0 + lane, keys = b < a.batch ? held(a, b, start, count) : 0;
-    const int n = b < a.batch ? (keys + c - 1) / c + (keys == 0) : 0;
+    const int b = b0 + lane, keys = keys_of(b);
+    const int n = b < a.batch ? cut(keys, length) : 0;
     int sum = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -179,35 +200,52 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
     for (int j = 0; j < VB; ++j) o[rt][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const int krow = 8 * (c >> 2) + (c & 3);
-  const bool v_mine = c * VB < a.dim;
-
-  for (int tb = (item.nth * WAVES + wave) * TOK; tb < hi_key; tb += item.of * WAVES * TOK) {
-    uint4v kr[CH][2][KP];
-    words<VW> vr[CH][8];
-    const bool whole = tb + TOK <= hi_key;
+  // What lies past the last key or past dim is read as the last key or the row's start:
+  // such scores are masked, such values meet zeros of Q or columns that nobody stores.
+  const int v_at = c * VB < a.dim ? c * VB : 0;
+  uint4v kr[CH][2][KP];
+  words<VW> vr[CH][8];
+  float kscale_next, vscale_next, kscale, vscale;
+  auto load_keys = [&](int tb) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        int key = tb + 32 * ch + krow + 4 * u;
+        key = key < hi_key ? key : hi_key - 1;
+        const uint8_t* const p = kc + (int64_t)key * a.dim;
 #pragma unroll
         for (int s = 0; s < KP; ++s) {
-          const int key = tb + 32 * ch + krow + 4 * u, d = 64 * s + 16 * g;
-          if (d < a.dim && (whole || key < hi_key))
-            kr[ch][u][s] = *reinterpret_cast<const uint4v*>(kc + (int64_t)key * a.dim + d);
-          else
-            kr[ch][u][s] = uint4v{0, 0, 0, 0};
+          const int d = 64 * s + 16 * g;
+          kr[ch][u][s] = *reinterpret_cast<const uint4v*>(p + (d < a.dim ? d : 0));
         }
+      }
+    kscale_next = ks[tb >> a.block_shift];
+  };
+  auto load_values = [&](int tb) {
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int key = tb + 32 * ch + 8 * g + i;
-        if (v_mine && (whole || key < hi_key))
-          vr[ch][i] = *reinterpret_cast<const words<VW>*>(vc + (int64_t)key * a.dim + c * VB);
-        else
-          vr[ch][i] = words<VW>{};
+        int key = tb + 32 * ch + 8 * g + i;
+        key = key < hi_key ? key : hi_key - 1;
+        vr[ch][i] = *reinterpret_cast<const words<VW>*>(vc + (int64_t)key * a.dim + v_at);
       }
-    const float kscale = ks[tb >> a.block_shift], vscale = vs[tb >> a.block_shift];
+    vscale_next = vs[tb >> a.block_shift];
+  };
+
+  // The next step's keys are asked for when this one's are in the products, the next
+  // values likewise: half of the registers' loads are always on their way.
+  const int step = item.of * WAVES * TOK;
+  int tb = (item.nth * WAVES + wave) * TOK;
+  if (tb < hi_key) {
+    load_keys(tb);
+    load_values(tb);
+  }
+  for (; tb < hi_key; tb += step) {
+    kscale = kscale_next;
+    vscale = vscale_next;
+    const int next = tb + step < hi_key ? tb + step : tb;  // past the end: once more, for nothing
     const bool masked = tb + TOK - 1 > lim_min;
 
     float4v s[RT][CH][2];
@@ -229,6 +267,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
             s[rt][ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[rt][i], s[rt][ch][u]);
           }
         }
+    load_keys(next);
     half8 p[RT][CH];
     float alpha[RT];
 #pragma unroll
@@ -329,6 +368,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
           }
         }
       }
+    load_values(next);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
