@@ -258,13 +258,16 @@ def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_sc
 
 
 CACHED_DIMS = (64, 128, 256)
-SHORT_CACHE = 2048
 
 
 def cached_kernel(dtype, dp: int, tall: int, step: int, waves: int, general: bool) -> tuple[str, str]:
     name = f"cache_attention_{SHORT[dtype]}_{dp}_{tall}_{step}_{waves}{'_general' if general else ''}"
     return (f"CACHE_ATTENTION({name}, {NAMES[dtype]}, {dp}, {tall}, {step}, {waves}, "
             f"{str(general).lower()})"), name
+
+
+def cached_tall(rows: int, dp: int) -> int:
+    return 1 if rows <= 16 else 2 if rows <= 32 or dp == 256 else 4
 
 
 def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale: Operand,
@@ -277,12 +280,12 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
     group, block = heads // kv_heads, capacity // k_scale.shape[2] if k_scale.shape[2] else 32
     rows = tokens * group
     dp = _padded(dim, CACHED_DIMS)
-    tall = 1 if rows <= 16 else 2 if rows <= 32 or dp == 256 else 4
+    tall = cached_tall(rows, dp)
     row_tiles = _ceil(rows, 16 * tall)
     step = 64 if block % 64 == 0 else 32
     # A workgroup's waves go through a short cache at once; a longer one is cut into items,
     # as many as the device holds, none shorter than two steps of every wave.
-    short = capacity <= SHORT_CACHE
+    short = capacity <= (4096 if batch * kv_heads * row_tiles >= 2 * UNITS else 1024)
     waves = 8 if short and batch * kv_heads * row_tiles < UNITS and dp < 256 else 4
     shortest = 2 * 64 * waves
     most = 1 if short else _ceil(capacity, shortest)
@@ -305,7 +308,7 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
     launches = [Launch(kernel, "cache_attention", name, grid, 64 * waves, pointers, tail)]
     workspace = 0
     if most > 1:  # a sequence may be cut
-        workspace = slots * kv_heads * rows * (dim + 4) * 4
+        workspace = _ceil(batch, 2) * 16 + slots * kv_heads * rows * (dim + 4) * 4
         launches.append(_join("cache_attention", q.dtype, min(most, slots), batch * tokens * heads,
                               pointers, tail))
     return Plan(tuple(launches), workspace)

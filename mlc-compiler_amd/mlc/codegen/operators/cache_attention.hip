@@ -27,7 +27,7 @@ struct CacheAttentionArgs {
   const void* start;
   const void* count;  // null: every token is real
   void* out;
-  float* part;  // [item][kv head][row][dim + 4]: O not normalised, its maximum and sum
+  float* part;  // {first item, items} of each sequence, then [item][kv head][row][dim + 4]
   int* error;
   int64_t q_off, cache_off[2], scale_off[2], sl_off, start_off, count_off;  // bytes
   int64_t qb, qt, qh, sls, ss, sc;                                          // elements
@@ -46,18 +46,22 @@ __device__ __forceinline__ int held(const CacheAttentionArgs& a, int b, int& sta
   return count > 0 ? start + count : 0;
 }
 
+typedef int int2v __attribute__((ext_vector_type(2)));
+
+// Where the parts begin: behind two words a sequence.
+__device__ __forceinline__ int64_t parts_at(const CacheAttentionArgs& a) { return ((int64_t)a.batch + 1) / 2 * 4; }
+
 struct Item {
   int b, nth, of, keys;  // the nth of the items of a sequence of so many keys
 };
 
 // How the sequences' keys are cut: every wave finds it again from the lengths. Items are
 // ``length`` keys long at most, as few as are wanted of all sequences together.
-// ``want`` < 0: the first item of sequence -1 - want.
 __device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want, Item& found, int& first) {
   const int lane = threadIdx.x & 63;
   int start, count;
   if (a.items == 0) {  // none is cut
-    found.b = want >= 0 ? want : -1 - want;
+    found.b = want;
     found.nth = first = 0;
     found.of = 1;
     found.keys = held(a, found.b, start, count);
@@ -93,14 +97,14 @@ __device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want,
       const int other = __shfl_up(sum, d, 64);
       sum += lane >= d ? other : 0;
     }
-    const uint64_t past = want >= 0 ? __ballot(first + sum > want) : __ballot(b == -1 - want);
+    const uint64_t past = __ballot(first + sum > want);
     if (past) {
       const int at_lane = __builtin_ctzll(past);
       found.b = b0 + at_lane;
       found.of = __shfl(n, at_lane, 64);
       found.keys = __shfl(keys, at_lane, 64);
       first += __shfl(sum, at_lane, 64) - found.of;
-      found.nth = want >= 0 ? want - first : 0;
+      found.nth = want - first;
       return true;
     }
     first += __shfl(sum, 63, 64);
@@ -150,6 +154,8 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   int start, count;
   held(a, b, start, count);
   if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
+  if (a.items > 0 && item.nth == 0 && rt0 == 0 && hk == 0 && threadIdx.x == 0)
+    reinterpret_cast<int2v*>(a.part)[b] = int2v{first, item.of};
   // an item's waves take every so-manieth step of the keys: what is read at one time lies
   // side by side
   const int hi_key = item.keys;
@@ -421,7 +427,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
         store_n<8>(reinterpret_cast<T*>(a.out) +
                    (((int64_t)b * a.tokens + t) * a.kv_heads * a.group + head) * a.dim + d, v);
       } else {
-        float* const part = a.part + (((int64_t)w * a.kv_heads + hk) * rows + row) * (a.dim + 4);
+        float* const part = a.part + parts_at(a) + (((int64_t)w * a.kv_heads + hk) * rows + row) * (a.dim + 4);
         *reinterpret_cast<float4v*>(part + d) = x;
         if (d == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{top, sum, 0.0f, 0.0f};
       }
@@ -436,13 +442,12 @@ __device__ __forceinline__ void cache_attention_join(const CacheAttentionArgs& a
   const int head = (int)(blockIdx.x % (uint32_t)heads);
   const uint32_t w = blockIdx.x / (uint32_t)heads;
   const int t = (int)(w % (uint32_t)a.tokens), b = (int)(w / (uint32_t)a.tokens);
-  Item item;
-  int first;
-  if (!find_item(a, -1 - b, item, first) || item.of == 1) return;
+  const int2v items = reinterpret_cast<const int2v*>(a.part)[b];
+  if (items.y == 1) return;  // whole, and done
   const int hk = head / a.group, rows = a.tokens * a.group, row = t * a.group + head % a.group;
   const int64_t step = (int64_t)a.kv_heads * rows * (a.dim + 4);
-  const float* const part = a.part + (((int64_t)first * a.kv_heads + hk) * rows + row) * (a.dim + 4);
-  join_parts<WAVES>(part, step, item.of, a.dim,
+  const float* const part = a.part + parts_at(a) + (((int64_t)items.x * a.kv_heads + hk) * rows + row) * (a.dim + 4);
+  join_parts<WAVES>(part, step, items.y, a.dim,
              reinterpret_cast<T*>(a.out) + (((int64_t)b * a.tokens + t) * heads + head) * a.dim);
 }
 

@@ -47,21 +47,26 @@ template <class T> __device__ __forceinline__ const T* at(const void* p, int64_t
 // apart, each dim values not normalised, then the reference of their exponentials in log2
 // units and the sum of their weights. For one workgroup of WAVES: groups of 16, 32 or 64
 // lanes (4 values a lane, dim <= 256) take parts in turn, four loads on their way at a
-// time, since latency is all that this costs, and are added up in LDS.
+// time, since latency is all that this costs, and meet in LDS.
 template <int WAVES, class T>
 __device__ __forceinline__ void join_parts(const float* part, int64_t step, int of, int dim, T* out) {
   constexpr int THREADS = 64 * WAVES;
-  __shared__ float tops[WAVES];
   __shared__ __attribute__((aligned(16))) float4v lx[THREADS];
-  __shared__ float ls[THREADS];
-  float top = -__builtin_inff();
-  for (int i = threadIdx.x; i < of; i += THREADS) top = __builtin_fmaxf(top, part[i * step + dim]);
-  top = row_reduce<THREADS, OpMax>(top, tops);
-  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  __shared__ float2v ls[THREADS];
   const int width = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, groups = THREADS / width;
   const int group = threadIdx.x / width, d = threadIdx.x % width * 4;
   float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-  float sum = 0.0f;
+  float sum = 0.0f, top = -__builtin_inff();
+  // (top, sum, x) and a part or another group's: to their common reference
+  auto meet = [&](float2v ml, float4v v) {
+    const float next = ml.x > top ? ml.x : top;
+    const float ref = next == -__builtin_inff() ? 0.0f : next;
+    const float f = __builtin_amdgcn_exp2f(top - ref), g = __builtin_amdgcn_exp2f(ml.x - ref);
+    top = next;
+    sum = __builtin_fmaf(ml.y, g, sum * f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], g, x[e] * f);
+  };
   for (int i0 = group; i0 < of; i0 += 4 * groups) {
     float4v v[4];
     float2v ml[4];
@@ -76,23 +81,13 @@ __device__ __forceinline__ void join_parts(const float* part, int64_t step, int 
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f = __builtin_amdgcn_exp2f(ml[j].x - ref);
-      sum = __builtin_fmaf(ml[j].y, f, sum);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[j][e], f, x[e]);
-    }
+    for (int j = 0; j < 4; ++j) meet(ml[j], v[j]);
   }
   lx[threadIdx.x] = x;
-  ls[threadIdx.x] = sum;
+  ls[threadIdx.x] = float2v{top, sum};
   __syncthreads();
   if (group > 0 || d >= dim) return;
-  for (int g = 1; g < groups; ++g) {
-    const float4v y = lx[threadIdx.x + g * width];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] += y[e];
-    sum += ls[threadIdx.x + g * width];
-  }
+  for (int g = 1; g < groups; ++g) meet(ls[threadIdx.x + g * width], lx[threadIdx.x + g * width]);
   const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
   T v[4];
 #pragma unroll
