@@ -154,10 +154,9 @@ def _factors(scale: float, cap: float) -> tuple[float, float]:
     return (scale / cap, cap * LOG2E) if cap else (scale * LOG2E, 0.0)
 
 
-def attention_kernel(dtype, dp: int, waves: int, direct: bool, general: bool) -> tuple[str, str]:
-    name = (f"attention_{SHORT[dtype]}_{dp}_w{waves}{'_direct' if direct else ''}"
-            f"{'_general' if general else ''}")
-    return (f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {waves}, {str(direct).lower()}, "
+def attention_kernel(dtype, dp: int, waves: int, source: str, general: bool) -> tuple[str, str]:
+    name = f"attention_{SHORT[dtype]}_{dp}_w{waves}_{source.lower()}{'_general' if general else ''}"
+    return (f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {waves}, {source}, "
             f"{str(general).lower()})"), name
 
 
@@ -174,49 +173,81 @@ def _join(op: str, dtype, parts: int, rows: int, pointers: tuple, tail: bytes) -
     return Launch(kernel, op, name, _grid(rows, 64 * waves, op), 64 * waves, pointers, tail)
 
 
-def attention_split(rows: int, pairs: int, key_tiles: int, dp: int) -> tuple[int, int]:
-    """Waves of a workgroup, each with 32 rows, and splits of the keys."""
+def attention_split(rows: int, pairs: int, key_tiles: int, tile_us: float, dim: int
+                    ) -> tuple[int, int]:
+    """Waves of a workgroup, each with 32 rows, and splits of the keys.
+
+    Splits fill the device where rows are few. What they cost is a second launch and
+    parts of O in fp32, written and read: 4 us and 8 bytes a value at 3 TB/s. What they
+    save is tiles of keys one behind the other, ``tile_us`` each."""
     waves = 4 if rows > 64 else 2 if rows > 32 else 1
     blocks = _ceil(rows, 32 * waves) * pairs
-    splits = max(1, min(2 * UNITS // blocks, key_tiles // 4)) if blocks < UNITS else 1
-    return waves, splits
+    values = rows * pairs * (dim + 4)
+
+    def cost(n: int) -> float:
+        return _ceil(key_tiles, n) * tile_us + (4 + n * values * 8 / 3e6 if n > 1 else 0)
+
+    return waves, min(range(1, max(1, min(2 * UNITS // blocks, key_tiles)) + 1), key=cost)
+
+
+def _strides(x: Operand | None, n: int) -> tuple:
+    return x.strides[:n] if x is not None else (0,) * n
+
+
+def _offset(x: Operand | None) -> int:
+    return x.offset if x is not None else 0
+
+
+def _attention(source: str, q: Operand, k: Operand, v: Operand, pairs: tuple, key_strides: tuple,
+               masks: tuple, cache: tuple, causal: bool, factors: tuple) -> Plan:
+    """Launches of ``attention.hip``. ``pairs``: kv_heads, keys; ``masks``: slopes, documents,
+    prefix; ``cache``: key and value scales, start, count and the tokens of a
+    scale, in logarithm."""
+    batch, queries, heads, dim = q.shape
+    kv_heads, keys = pairs
+    slopes, documents, prefix = masks
+    *scales, start, count, shift = cache
+    codes = source == "CODES"
+    dp, group = _padded(dim, CACHED_DIMS if codes else ATTENTION_DIMS), heads // kv_heads
+    rows, tiles_of_keys = queries * group, _ceil(keys, 32 if codes or dp == 256 else 64)
+    # measured: 1 us for 64 keys of 64 values, 1.8 of 128; twice that through registers
+    tile_us = (0.2 + dp / 80) * (0.5 if tiles_of_keys > _ceil(keys, 64) else 1) * (1 if source == "DIRECT" else 2)
+    waves, splits = attention_split(rows, batch * kv_heads, tiles_of_keys, tile_us, dim)
+    tiles = _ceil(rows, 32 * waves)
+    general = bool(factors[1]) or slopes is not None or documents is not None
+    operands = {"q": q, "k": k, "v": v, "slopes": slopes, "documents": documents, "prefix": prefix,
+                "k_scale": scales[0], "v_scale": scales[1], "start": start, "count": count}
+    names = {"k": "k_cache", "v": "v_cache"} if codes else {}
+    where = {n: names.get(n, n) if x is not None else None for n, x in operands.items()}
+    pointers = (*list(where.values())[:6], "out0", "workspace" if splits > 1 else None,
+                *list(where.values())[6:], "error" if codes else None)
+    tail = struct.pack("<10q15q10i2f", *map(_offset, operands.values()), *q.strides[:3],
+                       *key_strides, *_strides(slopes, 1), *_strides(documents, 2),
+                       *_strides(prefix, 1), *_strides(start, 1), *_strides(count, 1),
+                       batch, queries, keys, kv_heads, group, dim, causal, tiles, splits, shift,
+                       *factors)
+    kernel, name = attention_kernel(q.dtype, dp, waves, source, general)
+    grid = _grid(tiles * batch * kv_heads * splits, 64 * waves, "attention")
+    launch = Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail)
+    if splits == 1:
+        return Plan((launch,))
+    return Plan((launch, _join("attention", q.dtype, splits, batch * queries * heads, pointers, tail)),
+                splits * batch * kv_heads * rows * (dim + 4) * 4)
 
 
 def plan_attention(q: Operand, k: Operand, v: Operand, slopes: Operand | None,
                    documents: Operand | None, prefix: Operand | None, scale: float, causal: bool,
                    cap: float) -> Plan:
-    batch, queries, heads, dim = q.shape
-    keys, kv_heads = k.shape[1:3]
     if _numel(q) == 0:
         return Plan(())
-    group = heads // kv_heads
-    dp = _padded(dim, ATTENTION_DIMS)
+    keys, kv_heads = k.shape[1:3]
     # a tile's rows are addressed by 32 bits from its first one
-    direct = (dp == dim and keys > 0 and k.aligned and v.aligned
+    direct = (q.shape[3] in ATTENTION_DIMS and keys > 0 and k.aligned and v.aligned
               and all(n % 8 == 0 for n in (*k.strides[:3], *v.strides[:3]))
               and max(k.strides[1], v.strides[1]) < 1 << 24)
-    rows, pairs = queries * group, batch * kv_heads
-    waves, splits = attention_split(rows, pairs, _ceil(keys, 32 if dp == 256 else 64), dp)
-    tiles = _ceil(rows, 32 * waves)
-    general = bool(cap) or slopes is not None or documents is not None
-    some = lambda x, n: x.strides if x is not None else (0,) * n  # noqa: E731
-    off = lambda x: x.offset if x is not None else 0  # noqa: E731
-    tail = struct.pack("<6q13q10i2f", q.offset, k.offset, v.offset, off(slopes), off(documents),
-                       off(prefix), *q.strides[:3], *k.strides[:3], *v.strides[:3],
-                       *some(slopes, 1), *some(documents, 2), *some(prefix, 1),
-                       batch, queries, keys, kv_heads, group, dim, causal, tiles, splits, 0,
-                       *_factors(scale, cap))
-    kernel, name = attention_kernel(q.dtype, dp, waves, direct, general)
-    grid = _grid(tiles * pairs * splits, 64 * waves, "attention")
-    pointers = ("q", "k", "v", "slopes" if slopes is not None else None,
-                "documents" if documents is not None else None,
-                "prefix" if prefix is not None else None, "out0",
-                "workspace" if splits > 1 else None)
-    launch = Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail)
-    if splits == 1:
-        return Plan((launch,))
-    return Plan((launch, _join("attention", q.dtype, splits, batch * queries * heads, pointers, tail)),
-                splits * pairs * rows * (dim + 4) * 4)
+    return _attention("DIRECT" if direct else "COPIED", q, k, v, (kv_heads, keys),
+                      (*k.strides[:3], *v.strides[:3]), (slopes, documents, prefix),
+                      (None, None, None, None, 0), causal, _factors(scale, cap))
 
 
 # --------------------------------------------------------------------------
@@ -258,16 +289,13 @@ def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_sc
 
 
 CACHED_DIMS = (64, 128, 256)
+MANY_ROWS = 32
 
 
-def cached_kernel(dtype, dp: int, tall: int, step: int, waves: int, general: bool) -> tuple[str, str]:
-    name = f"cache_attention_{SHORT[dtype]}_{dp}_{tall}_{step}_{waves}{'_general' if general else ''}"
-    return (f"CACHE_ATTENTION({name}, {NAMES[dtype]}, {dp}, {tall}, {step}, {waves}, "
+def cached_kernel(dtype, dp: int, step: int, waves: int, general: bool) -> tuple[str, str]:
+    name = f"cache_attention_{SHORT[dtype]}_{dp}_{step}_{waves}{'_general' if general else ''}"
+    return (f"CACHE_ATTENTION({name}, {NAMES[dtype]}, {dp}, {step}, {waves}, "
             f"{str(general).lower()})"), name
-
-
-def cached_tall(rows: int, dp: int) -> int:
-    return 1 if rows <= 16 else 2 if rows <= 32 or dp == 256 else 4
 
 
 def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale: Operand,
@@ -279,9 +307,13 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
         return Plan(())
     group, block = heads // kv_heads, capacity // k_scale.shape[2] if k_scale.shape[2] else 32
     rows = tokens * group
+    if rows > MANY_ROWS:
+        strides = (kv_heads * capacity * dim, dim, capacity * dim)
+        return _attention("CODES", q, k_cache, v_cache, (kv_heads, capacity), strides * 2,
+                          (slopes, None, None), (k_scale, v_scale, start, count, block.bit_length() - 1),
+                          True, _factors(scale, cap))
     dp = _padded(dim, CACHED_DIMS)
-    tall = cached_tall(rows, dp)
-    row_tiles = _ceil(rows, 16 * tall)
+    row_tiles = _ceil(rows, 16)
     step = 64 if block % 64 == 0 else 32
     # A workgroup's waves go through a short cache at once; a longer one is cut into items,
     # as many as the device holds, none shorter than two steps of every wave.
@@ -299,7 +331,7 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
                        count.strides[0] if count is not None else 0, batch, tokens, kv_heads,
                        group, dim, capacity, block.bit_length() - 1, row_tiles, items, shortest,
                        *_factors(scale, cap))
-    kernel, name = cached_kernel(q.dtype, dp, tall, step, waves, general)
+    kernel, name = cached_kernel(q.dtype, dp, step, waves, general)
     pointers = ("q", "k_cache", "v_cache", "k_scale", "v_scale",
                 "slopes" if slopes is not None else None, "start",
                 "count" if count is not None else None, "out0",
@@ -339,11 +371,12 @@ def all_kernels() -> list[tuple[str, str]]:
         out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
                 for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
     for dtype in (torch.float16, torch.bfloat16):
-        out += [("attention", attention_kernel(dtype, dp, w, direct, g)[0]) for dp in ATTENTION_DIMS
-                for w in (1, 2, 4) for direct in (False, True) for g in (False, True)]
-        out += [("cache_attention", cached_kernel(dtype, dp, tall, step, w, g)[0])
-                for dp in CACHED_DIMS for tall in (1, 2, 4) if tall < 4 or dp < 256
-                for w in (4, 8) if w < 8 or dp < 256 for step in (32, 64) for g in (False, True)]
+        out += [("attention", attention_kernel(dtype, dp, w, source, g)[0]) for dp in ATTENTION_DIMS
+                for w in (1, 2, 4) for source in ("COPIED", "DIRECT", "CODES") for g in (False, True)
+                if source != "CODES" or (dp in CACHED_DIMS and 32 * w > MANY_ROWS)]
+        out += [("cache_attention", cached_kernel(dtype, dp, step, w, g)[0])
+                for dp in CACHED_DIMS for w in (4, 8) if w < 8 or dp < 256 for step in (32, 64)
+                for g in (False, True)]
         out += [(op, join_kernel(op, dtype, w)[0]) for op in ("attention", "cache_attention")
                 for w in (1, 4)]
     return out

@@ -27,17 +27,23 @@ struct AttentionArgs {
   const void* prefix;     // null: none
   void* out;
   float* part;  // where keys are split: [split][pair][row][dim + 4], see join_parts
+  const void* k_scale;  // and what follows: of an 8-bit cache
+  const void* v_scale;
+  const void* start;
+  const void* count;  // null: every token is real
+  int* error;
   int64_t q_off, k_off, v_off, s_off, d_off, p_off;      // bytes
-  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ss, db, dt, ps;  // elements
+  int64_t ks_off, vs_off, start_off, count_off;
+  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ss, db, dt, ps, start_s, count_s;  // elements
   int32_t batch, queries, keys, kv_heads, group, dim, causal, tiles;  // tiles of rows
-  int32_t splits, pad;  // of keys
+  int32_t splits, block_shift;  // of keys; tokens of a scale
   float scale, cap;  // scale times log2 e where cap is 0, else 1/cap of it and cap log2 e
 };
 
-// Keys of a tile: with heads of 256, rows of 64 scores would not fit the registers
-// beside O and Q, and O would move between vector and accumulation registers twice a
-// tile (2048 causal tokens, 4 x 8 heads: 136 us; 32 keys: see the table of sizes).
-template <int DP> constexpr int tile_keys = DP == 256 ? 32 : 64;
+// Keys of a tile: with heads of 256, rows of 64 scores would not fit the registers beside O
+// and Q, and O would move between vector and accumulation registers twice a tile (2048 causal
+// tokens, 4 x 8 heads of 256: 136 us; 32 keys 116). A tile of the cache has one scale.
+template <int DP, int SOURCE> constexpr int tile_keys = DP == 256 || SOURCE == 2 ? 32 : 64;
 
 template <class T> struct vec8;
 template <> struct vec8<f16> { typedef half8 type; static constexpr uint32_t exponent = 0x7c00u; };
@@ -78,6 +84,8 @@ template <uint32_t E> __device__ __forceinline__ bool drop_not_finite(uint4v& x)
   return found;
 }
 
+template <bool B, class X, class Y> struct choose { typedef X type; };
+template <class X, class Y> struct choose<false, X, Y> { typedef Y type; };
 template <bool B> struct bool_constant { static constexpr bool value = B; };
 
 // 16 bytes of a lane from ``g`` straight to LDS at ``lds`` + 16 * lane.
@@ -86,26 +94,36 @@ __device__ __forceinline__ void to_lds(const void* g, void* lds) {
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// DIRECT: rows of 16-byte aligned pieces, dim == DP: tiles go from memory to LDS without
-// passing registers, the next one while one is in use. Otherwise through registers, with
-// zeros past dim.
-template <class T, int DP, int WAVES, bool DIRECT, bool GENERAL>
+// SOURCE of keys and values:
+//  DIRECT: rows of 16-byte aligned pieces, dim == DP: tiles go from memory to LDS without
+//    passing registers, the next one while one is in use;
+//  COPIED: through registers, with zeros past dim;
+//  CODES: the 8-bit cache of cache_attention, for many rows: codes are widened on their way
+//    to LDS, K's in the queries' type and V's, with P, in fp16, both exact; a scale of K goes
+//    into the factor of its scores, one of V multiplies its keys' part of O.
+enum { COPIED, DIRECT, CODES };
+
+template <class T, int DP, int WAVES, int SOURCE, bool GENERAL>
 __device__ __forceinline__ void attention(const AttentionArgs& a) {
   typedef typename vec8<T>::type v8;
+  typedef typename choose<SOURCE == CODES, f16, T>::type PT;  // of P and V
+  typedef typename vec8<PT>::type p8;
+  constexpr bool IS_DIRECT = SOURCE == DIRECT, CACHE = SOURCE == CODES, DOCS = GENERAL && !CACHE;
   constexpr int PC = DP == 64 ? 8 : DP <= 128 ? 16 : 32;  // 16-byte slots of an LDS row
   constexpr int CH = DP / 8;                               // of which hold values
   constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
-  constexpr int BUFFERS = DIRECT ? 2 : 1;
-  constexpr int KEYS = tile_keys<DP>, U = KEYS / 32;
-  constexpr int N = KEYS * CH / THREADS;               // pieces of a tile for a thread
-  constexpr int NL = KEYS * PC / THREADS;              // slots of a tile for a thread
-  static_assert(KEYS * CH % THREADS == 0 && KEYS * PC % THREADS == 0, "staging");
+  constexpr int BUFFERS = 2;
+  constexpr int KEYS = tile_keys<DP, SOURCE>, U = KEYS / 32;
+  constexpr int EACH = CACHE ? 16 : 8, ROW = DP / EACH;    // values of a piece, pieces of a row
+  constexpr int N = (KEYS * ROW + THREADS - 1) / THREADS;  // pieces of a tile for a thread
+  constexpr int NL = KEYS * PC / THREADS;                  // slots of a tile for a thread
+  static_assert(!IS_DIRECT || KEYS * PC % THREADS == 0, "staging");
   constexpr int TILE = KEYS * PC * 16;                 // bytes of LDS, a power of two
   __shared__ __attribute__((aligned(BUFFERS * TILE))) char lds[2 * BUFFERS * TILE];  // keys, then values
-  __shared__ __attribute__((aligned(16))) int ldoc[GENERAL ? BUFFERS : 1][GENERAL ? WAVES : 1][64];
+  __shared__ __attribute__((aligned(16))) int ldoc[DOCS ? BUFFERS : 1][DOCS ? WAVES : 1][64];
   __shared__ uint64_t lbits[WAVES];
   __shared__ int lrange[3][WAVES];
-  __shared__ __attribute__((aligned(16))) T lp[WAVES][32][16];
+  __shared__ __attribute__((aligned(16))) PT lp[WAVES][32][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -125,12 +143,22 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int pair = unit / a.splits, split = unit % a.splits;
   const int b = pair / a.kv_heads, hk = pair % a.kv_heads;
 
-  const int shift = a.keys - a.queries;  // position of query 0
+  int keys = a.keys, shift = a.keys - a.queries;  // position of query 0
+  int real = a.queries;                            // queries that are not padding
+  if constexpr (CACHE) {
+    const int start = at<int32_t>(a.start, a.start_off)[b * a.start_s];
+    const int count = a.count ? at<int32_t>(a.count, a.count_off)[b * a.count_s] : a.queries;
+    const bool ok = start >= 0 && count >= 0 && count <= a.queries && (int64_t)start + count <= a.keys;
+    if (!ok && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
+    shift = start;
+    real = ok ? count : 0;
+    keys = real > 0 ? start + real : 0;
+  }
   const int prefix = a.prefix ? at<int32_t>(a.prefix, a.p_off)[b * a.ps] : 0;
   // last key that query ``t`` may see
   auto last = [&](int t) {
-    int lim = a.keys - 1;
-    if (a.causal) {
+    int lim = keys - 1;
+    if (CACHE || a.causal) {
       const int own = t + shift > prefix - 1 ? t + shift : prefix - 1;
       lim = own < lim ? own : lim;
     }
@@ -141,7 +169,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   const int r = row < rows ? row : rows - 1;  // rows past the end repeat the last, and are not stored
   const int t = r / a.group, head = hk * a.group + r % a.group;
   const int32_t* const doc = at<int32_t>(a.documents, a.d_off) + b * a.db;
-  const int mine = GENERAL && a.documents ? doc[(t + shift) * a.dt] : 0;
+  const int mine = DOCS && a.documents ? doc[(t + shift) * a.dt] : 0;
   const int lim = mine < 0 ? -1 : last(t);
   const int end_row = first_row + ROWS < rows ? first_row + ROWS : rows;
   const int lim_wg = last((end_row - 1) / a.group);
@@ -164,11 +192,15 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   float slope = 0.0f;
   if (GENERAL && a.slopes) slope = at<float>(a.slopes, a.s_off)[head * a.ss] * 0x1.715476p+0f;
 
-  const T* const kp = at<T>(a.k, a.k_off) + b * a.kb + hk * a.kh;
-  const T* const vp = at<T>(a.v, a.v_off) + b * a.vb + hk * a.vh;
+  typedef typename choose<CACHE, uint8_t, T>::type stored;
+  const stored* const kp = at<stored>(a.k, a.k_off) + b * a.kb + hk * a.kh;
+  const stored* const vp = at<stored>(a.v, a.v_off) + b * a.vb + hk * a.vh;
+  const int64_t scales_at = CACHE ? ((int64_t)pair * a.keys) >> a.block_shift : 0;
+  const float* const ks = at<float>(a.k_scale, a.ks_off) + scales_at;
+  const float* const vs = at<float>(a.v_scale, a.vs_off) + scales_at;
   // slot i = thread + n * THREADS of a tile is chunk (i % PC) ^ swizzle of row i / PC; rows of
   // one thread are STEP apart, and the swizzle comes again after 16 rows
-  constexpr int STEP = THREADS / PC, KINDS = STEP >= 16 ? 1 : 16 / STEP < NL ? 16 / STEP : NL;
+  constexpr int STEP = THREADS / PC, KINDS = STEP >= 16 || !IS_DIRECT ? 1 : 16 / STEP < NL ? 16 / STEP : NL;
   uint32_t kv[KINDS], vv[KINDS];
   auto chunk_of = [&](int kr) { return (slot<PC>(kr, threadIdx.x % PC) % PC) % CH; };
 #pragma unroll
@@ -177,13 +209,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     kv[i] = (kr * (uint32_t)a.kt + chunk * 8) * (uint32_t)sizeof(T);
     vv[i] = (kr * (uint32_t)a.vt + chunk * 8) * (uint32_t)sizeof(T);
   }
-  T rk[DIRECT ? 1 : N][8], rv[DIRECT ? 1 : N][8];
+  // 8 values of 16 bits, or 16 codes, a piece
+  uint4v rk[IS_DIRECT ? 1 : N], rv[IS_DIRECT ? 1 : N];
   int rdoc = 0;
   auto load = [&](int kt, int into) {
     const int base = kt * KEYS;
-    if constexpr (DIRECT) {
+    if constexpr (IS_DIRECT) {
       char* const to = lds + into * TILE + wave * 1024;
-      if (base + KEYS <= a.keys) {
+      if (base + KEYS <= keys) {
         const char* const kb = reinterpret_cast<const char*>(kp + base * a.kt);
         const char* const vb = reinterpret_cast<const char*>(vp + base * a.vt);
 #pragma unroll
@@ -194,7 +227,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       } else {  // past the last key the last one again
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-          const int kr = threadIdx.x / PC + n * STEP, key = base + kr < a.keys ? base + kr : a.keys - 1;
+          const int kr = threadIdx.x / PC + n * STEP, key = base + kr < keys ? base + kr : keys - 1;
           const int chunk = chunk_of(kr);
           to_lds(kp + key * a.kt + chunk * 8, to + n * THREADS * 16);
           to_lds(vp + key * a.vt + chunk * 8, to + BUFFERS * TILE + n * THREADS * 16);
@@ -203,21 +236,27 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int i = threadIdx.x + n * THREADS, key = base + i / CH, d = i % CH * 8;
-        if (key < a.keys && d < a.dim) {
-          load_n<2>(rk[n], kp + key * a.kt + d);
-          load_n<2>(rv[n], vp + key * a.vt + d);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) rk[n][j] = rv[n][j] = (T)0.0f;
+        const int i = threadIdx.x + n * THREADS, key = base + i / ROW, d = i % ROW * EACH;
+        rk[n] = rv[n] = uint4v{0, 0, 0, 0};
+        if (key < keys && d < a.dim && i < KEYS * ROW) {
+          if constexpr (CACHE) {
+            rk[n] = *reinterpret_cast<const uint4v*>(kp + key * a.kt + d);
+            rv[n] = *reinterpret_cast<const uint4v*>(vp + key * a.vt + d);
+          } else {
+            T x[8];
+            load_n<2>(x, kp + key * a.kt + d);
+            rk[n] = __builtin_bit_cast(uint4v, x);
+            load_n<2>(x, vp + key * a.vt + d);
+            rv[n] = __builtin_bit_cast(uint4v, x);
+          }
         }
       }
     }
-    if (GENERAL && a.documents) {
+    if (DOCS && a.documents) {
       // every wave its own copy, so that all have as many loads on their way; what lies
       // behind the last key is masked by its index
-      const int key = base + lane % KEYS < a.keys ? base + lane % KEYS : a.keys - 1;
-      if constexpr (DIRECT)
+      const int key = base + lane % KEYS < keys ? base + lane % KEYS : keys - 1;
+      if constexpr (IS_DIRECT)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(doc + key * a.dt),
                                          (__attribute__((address_space(3))) void*)ldoc[into][wave], 4, 0, 0);
       else
@@ -240,31 +279,65 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   uint32_t k_at = slot<PC>(token, h) * 16, v_at = slot<PC>(vk, vd >> 3) * 16 + (vd & 7) * 2;
   constexpr int PITCH = PC * 16;
 
-  int it = 0;  // the buffer of the tile in use
-  // waits for the tile that is on its way, and for this wave's reads of the one before,
-  // whose buffer is the next to be filled, and starts on the one after ``kt``; which it is
+  int it = 0;       // the buffer of the tile in use
+  int behind = 0;   // the tile that is on its way: to the other buffer, or to registers
+  // registers to buffer ``into``
+  auto store = [&](int into) {
+    uint4v* const lk = reinterpret_cast<uint4v*>(lds + into * TILE);
+    uint4v* const lv = reinterpret_cast<uint4v*>(lds + (BUFFERS + into) * TILE);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = threadIdx.x + n * THREADS, r0 = i / ROW, c0 = i % ROW;
+      if (KEYS * ROW % THREADS != 0 && i >= KEYS * ROW) continue;
+      if constexpr (CACHE) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t k0 = rk[n][2 * y], k1 = rk[n][2 * y + 1], v0 = rv[n][2 * y], v1 = rv[n][2 * y + 1];
+          lk[slot<PC>(r0, 2 * c0 + y)] = uint4v{codes<T>::widen(k0, 0), codes<T>::widen(k0, 1),
+                                                codes<T>::widen(k1, 0), codes<T>::widen(k1, 1)};
+          lv[slot<PC>(r0, 2 * c0 + y)] = uint4v{codes<PT>::widen(v0, 0), codes<PT>::widen(v0, 1),
+                                                codes<PT>::widen(v1, 0), codes<PT>::widen(v1, 1)};
+        }
+      } else {
+        lk[slot<PC>(r0, c0)] = rk[n];
+        lv[slot<PC>(r0, c0)] = rv[n];
+      }
+    }
+    if (DOCS && a.documents) ldoc[into][wave][lane] = rdoc;
+  };
+  // the first tile on its way
+  auto begin = [&](int kt, auto after) {
+    if (kt < tiles) load(kt, it);
+    behind = kt;
+    if constexpr (!IS_DIRECT) {
+      if (kt < tiles) {
+        store(it);
+        behind = after(kt + a.splits);
+        if (behind < tiles) load(behind, 0);
+      }
+    }
+    return kt;
+  };
+  // Waits for tile ``kt``, and for this wave's reads of the one before, whose buffer is the
+  // next to be filled, and starts on the tile after it; which that is.
   auto arrive = [&](int kt, auto after) {
-    int next;
-    if constexpr (DIRECT) {
+    if constexpr (IS_DIRECT) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" : : : "memory");
-      next = after(kt + a.splits);
+      const int next = after(kt + a.splits);
       if (next < tiles) load(next, it ^ 1);
+      return next;
     } else {
       __syncthreads();
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int i = threadIdx.x + n * THREADS, at_slot = slot<PC>(i / CH, i % CH);
-        reinterpret_cast<uint4v*>(lds)[at_slot] = __builtin_bit_cast(uint4v, rk[n]);
-        reinterpret_cast<uint4v*>(lds + TILE)[at_slot] = __builtin_bit_cast(uint4v, rv[n]);
+      const int next = behind;
+      if (next < tiles) {
+        store(it ^ 1);
+        behind = after(next + a.splits);
+        if (behind < tiles) load(behind, 0);
       }
-      if (GENERAL && a.documents) ldoc[0][wave][lane] = rdoc;
-      __syncthreads();
-      next = after(kt + a.splits);
-      if (next < tiles) load(next, 0);
+      return next;
     }
-    return next;
   };
   auto compute = [&](int kt, auto is_masked, auto is_safe) {
     constexpr bool MASKED = decltype(is_masked)::value, SAFE = decltype(is_safe)::value;
@@ -279,25 +352,28 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int i = 0; i < DP / 16; ++i)
         s[u] = mfma_32x32x16(*reinterpret_cast<const v8*>(lds + (k_at ^ (i << 5)) + u * 32 * PITCH), q[i], s[u]);
     }
-    float scale = a.scale;
+    float scale = a.scale, v_scale = 1.0f;
+    if constexpr (CACHE) {
+      scale *= ks[base >> a.block_shift];
+      v_scale = vs[base >> a.block_shift];
+    }
     if constexpr (GENERAL) {
       // in log2 units: the cap, then the bias
-      scale = 1.0f;
       if (a.cap != 0.0f) {
         // cap tanh y = cap - 2 cap / (e^2y + 1)
-        const float by = a.scale * (2.0f * 0x1.715476p+0f);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             s[u][j] = __builtin_fmaf(-2.0f * a.cap,
-                                     __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][j] * by) + 1.0f), a.cap);
+                                     __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][j] * (scale * (2.0f * 0x1.715476p+0f))) + 1.0f), a.cap);
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s[u][j] *= a.scale;
+          for (int j = 0; j < 16; ++j) s[u][j] *= scale;
       }
+      scale = 1.0f;
       if (a.slopes) {
         const float away = (float)(base + 8 * h - (t + shift));
 #pragma unroll
@@ -315,7 +391,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         for (int j = 0; j < 16; ++j) {
           const int k = 32 * u + 16 * (j >> 3) + (j & 7);
           bool seen = k <= own;
-          if (GENERAL && a.documents) seen = seen && ldoc[it][wave][k + 8 * h] == mine;
+          if (DOCS && a.documents) seen = seen && ldoc[it][wave][k + 8 * h] == mine;
           s[u][j] = seen ? s[u][j] : -__builtin_inff();
         }
     }
@@ -338,14 +414,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       m = next;
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m;
-    v8 p[2 * U];
+    p8 p[2 * U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], scale, -ref));
         l += e;
-        p[2 * u + (j >> 3)][j & 7] = (T)e;
+        p[2 * u + (j >> 3)][j & 7] = (PT)e;
       }
     auto values = [&](int i, int u) {
       const char* const at = lds + BUFFERS * TILE + u * 16 * PITCH;
@@ -354,33 +430,50 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     bool spoiled = false;
+    if constexpr (CACHE) {
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+      for (int i = 0; i < DP / 32; ++i) {
+        float16v add;
 #pragma unroll
-      for (int u = 0; u < 2 * U; ++u) {
-        uint4v w = __builtin_bit_cast(uint4v, values(i, u));
-        if constexpr (SAFE) spoiled |= drop_not_finite<vec8<T>::exponent>(w);
-        o[i] = mfma_32x32x16(__builtin_bit_cast(v8, w), p[u], o[i]);
+        for (int j = 0; j < 16; ++j) add[j] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint4v w = __builtin_bit_cast(uint4v, values(i, u));
+          if constexpr (SAFE) spoiled |= drop_not_finite<vec8<PT>::exponent>(w);
+          add = mfma_32x32x16(__builtin_bit_cast(p8, w), p[u], add);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = __builtin_fmaf(add[j], v_scale, o[i][j]);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+          uint4v w = __builtin_bit_cast(uint4v, values(i, u));
+          if constexpr (SAFE) spoiled |= drop_not_finite<vec8<PT>::exponent>(w);
+          o[i] = mfma_32x32x16(__builtin_bit_cast(p8, w), p[u], o[i]);
+        }
+    }
     if constexpr (SAFE) {
       if (__any(spoiled)) {
-        const T* const value = reinterpret_cast<const T*>(lds + (BUFFERS + it) * TILE);
+        const PT* const value = reinterpret_cast<const PT*>(lds + (BUFFERS + it) * TILE);
 #pragma unroll 1
         for (int u = 0; u < 2 * U; ++u) {
           // p by a constant index only: it stays in registers
-          const v8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2 * U - 2] : p[2 * U - 1];
-          *reinterpret_cast<v8*>(&lp[wave][c][8 * h]) = pu;
+          const p8 pu = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2 * U - 2] : p[2 * U - 1];
+          *reinterpret_cast<p8*>(&lp[wave][c][8 * h]) = pu;
           __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
           for (int j = 0; j < 16; ++j) {
-            const float x = element<T>::widen(lp[wave][c][j]);
+            const float x = element<PT>::widen(lp[wave][c][j]);
             const int k = 16 * u + j;
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
               for (int z = 0; z < 16; ++z) {
                 const int d = 32 * i + 8 * (z >> 2) + 4 * h + (z & 3);
-                const float y = element<T>::widen(value[slot<PC>(k, d >> 3) * 8 + (d & 7)]);
+                const float y = element<PT>::widen(value[slot<PC>(k, d >> 3) * 8 + (d & 7)]);
                 if (x != 0.0f && !(__builtin_fabsf(y) < __builtin_inff())) o[i][z] += x * y;
               }
           }
@@ -391,20 +484,17 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   };
 
   auto turn = [&] {  // to the other buffer
-    if constexpr (DIRECT) {
-      k_at ^= TILE;
-      v_at ^= TILE;
-      it ^= 1;
-    }
+    k_at ^= TILE;
+    v_at ^= TILE;
+    it ^= 1;
   };
   // tiles that every row sees whole
   int whole = (last(first_row / a.group) + 1) / KEYS;
   whole = whole < tiles ? whole : tiles;
   auto every = [](int kt) { return kt; };
-  if (!(GENERAL && a.documents)) {
+  if (!(DOCS && a.documents)) {
     // those first, then the ones that need a mask
-    int kt = split;
-    if (kt < tiles) load(kt, it);
+    int kt = begin(split, every);
     while (kt < whole) {
       const int next = arrive(kt, every);
       compute(kt, bool_constant<false>{}, bool_constant<false>{});
@@ -418,7 +508,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       kt = next;
     }
   }
-  if constexpr (GENERAL) {
+  if constexpr (DOCS) {
     if (a.documents) {
       // The documents of the workgroup's rows, least and largest, and whether a row has none.
       // A tile whose documents lie outside is left out, one that is of the rows' only
@@ -455,7 +545,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
             bool gap = false;  // a token of no document
             for (int j = 0; j < 8; ++j) {
               const int key = tile * KEYS + lane % LANES * 8 + j;
-              const int x = key < a.keys ? doc[key * a.dt] : -1;
+              const int x = key < keys ? doc[key * a.dt] : -1;
               gap |= x < 0;
               dl = x < 0 ? dl : least(dl, x);
               dh = largest(dh, x);
@@ -492,16 +582,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       };
       auto full_ones = [&](int kt) { return find(kt, true); };
       auto other_ones = [&](int kt) { return find(kt, false); };
-      int kt = full_ones(split);
-      if (kt < tiles) load(kt, it);
+      int kt = begin(full_ones(split), full_ones);
       while (kt < tiles) {
         const int next = arrive(kt, full_ones);
         compute(kt, bool_constant<false>{}, bool_constant<false>{});
         turn();
         kt = next;
       }
-      kt = other_ones(split);
-      if (kt < tiles) load(kt, it);
+      kt = begin(other_ones(split), other_ones);
       while (kt < tiles) {
         const int next = arrive(kt, other_ones);
         if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
@@ -525,7 +613,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
     m = -__builtin_inff();
     l = 0.0f;
-    if (split < tiles) load(split, it);
+    begin(split, every);
     for (int kt = split; kt < tiles; kt += a.splits) {
       arrive(kt, every);
       if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
@@ -534,6 +622,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   }
   if (row >= rows) return;
   l = xor32<OpSum>(l);
+  if (CACHE && t >= real) {  // padding
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    m = -__builtin_inff();
+    l = 0.0f;
+  }
   if (a.splits > 1) {
     float* const part = a.part + (((int64_t)split * a.batch * a.kv_heads + pair) * rows + row) * (a.dim + 4);
 #pragma unroll
@@ -578,9 +674,9 @@ __device__ __forceinline__ void attention_join(const AttentionArgs& a) {
 
 }  // namespace mlc
 
-#define ATTENTION(NAME, T, DP, WAVES, DIRECT, GENERAL)                                            \
+#define ATTENTION(NAME, T, DP, WAVES, SOURCE, GENERAL)                                            \
   extern "C" __global__ void __launch_bounds__(64 * WAVES, DP == 64 ? 3 : 2) NAME(mlc::AttentionArgs a) {\
-    mlc::attention<T, DP, WAVES, DIRECT, GENERAL>(a);                                             \
+    mlc::attention<T, DP, WAVES, mlc::SOURCE, GENERAL>(a);                                             \
   }
 #define ATTENTION_JOIN(NAME, T, WAVES)                                                   \
   extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::AttentionArgs a) {                  \

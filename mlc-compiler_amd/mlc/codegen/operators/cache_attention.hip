@@ -1,6 +1,6 @@
 // Attention of the newest tokens over the 8-bit cache: token i of a sequence stands
 // at position start + i and sees the keys up to its own. Rows are (token, head of
-// a group) pairs, 16 * RT to a workgroup, so keys and values are read once for all
+// a group) pairs, 16 to a workgroup, so keys and values are read once for all
 // heads that share them.
 //
 // Bound by memory where rows are few: the cache is read once, 2 (dim + 4 / block)
@@ -112,25 +112,9 @@ __device__ __forceinline__ bool find_item(const CacheAttentionArgs& a, int want,
   return false;
 }
 
-template <class T> struct codes;
-template <> struct codes<f16> {
-  typedef half8 v8;
-  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
-    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
-  }
-};
-template <> struct codes<__bf16> {
-  typedef bf16x8 v8;
-  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
-    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-  }
-};
-
 template <int W> struct words { uint32_t x[W]; };
 
-template <class T, int DP, int RT, int TOK, int WAVES, bool GENERAL>
+template <class T, int DP, int TOK, int WAVES, bool GENERAL>
 __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   typedef typename codes<T>::v8 v8;
   constexpr int KP = DP / 64;   // 16-byte pieces of a key's row per lane
@@ -145,7 +129,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   uint32_t w = blockIdx.x;
   const int hk = (int)(w % (uint32_t)a.kv_heads);
   w /= (uint32_t)a.kv_heads;
-  const int rt0 = (int)(w % (uint32_t)a.row_tiles);
+  const int row_tile = (int)(w % (uint32_t)a.row_tiles);
   w /= (uint32_t)a.row_tiles;
   Item item;
   int first;
@@ -154,36 +138,29 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   int start, count;
   held(a, b, start, count);
   if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
-  if (a.items > 0 && item.nth == 0 && rt0 == 0 && hk == 0 && threadIdx.x == 0)
+  if (a.items > 0 && item.nth == 0 && row_tile == 0 && hk == 0 && threadIdx.x == 0)
     reinterpret_cast<int2v*>(a.part)[b] = int2v{first, item.of};
   // an item's waves take every so-manieth step of the keys: what is read at one time lies
   // side by side
   const int hi_key = item.keys;
 
   const int rows = a.tokens * a.group;
-  v8 q[RT][2 * KP];
-  int lim[RT], pos[RT];
-  float slope[RT];
-  int lim_min = 0x7fffffff;
+  const int own = row_tile * 16 + c, r = own < rows ? own : rows - 1;
+  const int t = r / a.group, head = hk * a.group + r % a.group;
+  const int pos = start + t, lim = t < count ? pos : -1;
+  v8 q[2 * KP];
+  float slope = GENERAL && a.slopes ? at<float>(a.slopes, a.sl_off)[head * a.sls] * 0x1.715476p+0f : 0.0f;
+  const T* p = at<T>(a.q, a.q_off) + b * a.qb + t * a.qt + head * a.qh;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = (rt0 * RT + rt) * 16 + c, r = row < rows ? row : rows - 1;
-    const int t = r / a.group, head = hk * a.group + r % a.group;
-    pos[rt] = start + t;
-    lim[rt] = t < count ? start + t : -1;
-    lim_min = lim[rt] < lim_min ? lim[rt] : lim_min;
-    slope[rt] = GENERAL && a.slopes ? at<float>(a.slopes, a.sl_off)[head * a.sls] * 0x1.715476p+0f : 0.0f;
-    const T* p = at<T>(a.q, a.q_off) + b * a.qb + t * a.qt + head * a.qh;
+  for (int s = 0; s < 2 * KP; ++s) {
+    const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    T x[8] = {};
+    if (d < a.dim) load_n<2>(x, p + d);
 #pragma unroll
-    for (int s = 0; s < 2 * KP; ++s) {
-      const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-      T x[8] = {};
-      if (d < a.dim) load_n<2>(x, p + d);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[rt][s][i] = x[i];
-    }
+    for (int i = 0; i < 8; ++i) q[s][i] = x[i];
   }
   // the least of the rows' last keys: steps below it need no mask
+  int lim_min = lim;
   for (int d = 1; d < 16; d <<= 1) {
     const int other = __shfl_xor(lim_min, d, 64);
     lim_min = other < lim_min ? other : lim_min;
@@ -196,15 +173,10 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   const float* const ks = at<float>(a.scale[0], a.scale_off[0]) + (head_at >> a.block_shift);
   const float* const vs = at<float>(a.scale[1], a.scale_off[1]) + (head_at >> a.block_shift);
 
-  float m[RT], l[RT];
-  float4v o[RT][VB];
+  float m = -__builtin_inff(), l = 0.0f;
+  float4v o[VB];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -__builtin_inff();
-    l[rt] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VB; ++j) o[rt][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int j = 0; j < VB; ++j) o[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   const int krow = 8 * (c >> 2) + (c & 3);
   // What lies past the last key or past dim is read as the last key or the row's start:
   // such scores are masked, such values meet zeros of Q or columns that nobody stores.
@@ -254,7 +226,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
     const int next = tb + step < hi_key ? tb + step : tb;  // past the end: once more, for nothing
     const bool masked = tb + TOK - 1 > lim_min;
 
-    float4v s[RT][CH][2];
+    float4v s[CH][2];
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -267,52 +239,45 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
           k.y = codes<T>::widen(w0, 1);
           k.z = codes<T>::widen(w1, 0);
           k.w = codes<T>::widen(w1, 1);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            if (i == 0) s[rt][ch][u] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-            s[rt][ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[rt][i], s[rt][ch][u]);
-          }
+          if (i == 0) s[ch][u] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+          s[ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[i], s[ch][u]);
         }
     load_keys(next);
-    half8 p[RT][CH];
-    float alpha[RT];
+    half8 p[CH];
+    const float factor = a.factor * kscale;
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float factor = a.factor * kscale;
-      float top = -__builtin_inff();
+    for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x = s[rt][ch][e >> 2][e & 3] * factor;
-          const int key = tb + 32 * ch + 8 * g + e;
-          if constexpr (GENERAL) {
-            if (a.cap != 0.0f) {
-              // tanh y = 1 - 2 / (e^2y + 1)
-              const float z = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
-              x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(z + 1.0f);
-            }
-            if (a.slopes) x = __builtin_fmaf(-slope[rt], __builtin_fabsf((float)(key - pos[rt])), x);
+      for (int e = 0; e < 8; ++e) {
+        float x = s[ch][e >> 2][e & 3] * factor;
+        const int key = tb + 32 * ch + 8 * g + e;
+        if constexpr (GENERAL) {
+          if (a.cap != 0.0f) {
+            // tanh y = 1 - 2 / (e^2y + 1)
+            const float z = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
+            x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(z + 1.0f);
           }
-          if (masked) x = key <= lim[rt] ? x : -__builtin_inff();
-          s[rt][ch][e >> 2][e & 3] = x;
-          top = __builtin_fmaxf(top, x);
+          if (a.slopes) x = __builtin_fmaf(-slope, __builtin_fabsf((float)(key - pos)), x);
         }
-      top = xor32<OpMax>(xor16<OpMax>(top));
-      const float now = top > m[rt] ? top : m[rt];
-      const float ref = now == -__builtin_inff() ? 0.0f : now;
-      alpha[rt] = __builtin_amdgcn_exp2f(m[rt] - ref);
-      m[rt] = now;
-      l[rt] *= alpha[rt];
+        if (masked) x = key <= lim ? x : -__builtin_inff();
+        s[ch][e >> 2][e & 3] = x;
+        top = __builtin_fmaxf(top, x);
+      }
+    top = xor32<OpMax>(xor16<OpMax>(top));
+    const float now = top > m ? top : m;
+    const float ref = now == -__builtin_inff() ? 0.0f : now;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = now;
+    l *= alpha;
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
+    for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[rt][ch][e >> 2][e & 3] - ref);
-          l[rt] += x;
-          p[rt][ch][e] = (f16)x;
-        }
-    }
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(s[ch][e >> 2][e & 3] - ref);
+        l += x;
+        p[ch][e] = (f16)x;
+      }
     // a value that is NaN and that some row does not see would spoil the row: 0 * NaN
     bool spoiled = false;
     if (masked) {
@@ -328,7 +293,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
           }
       spoiled = __any(spoiled);
     }
-    float4v add[RT][VB];
+    float4v add[VB];
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -356,81 +321,72 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
             }
           }
           const int j = 4 * z + y;
+          if (ch == 0) add[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+          add[j] = mfma_16x16x32(v, p[ch], add[j]);
+          if (spoiled) {
+            // rows that see one of the NaN values get a NaN
+            half8 sees;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            if (ch == 0) add[rt][j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-            add[rt][j] = mfma_16x16x32(v, p[rt][ch], add[rt][j]);
-            if (spoiled) {
-              // rows that see one of the NaN values get a NaN
-              half8 sees;
+            for (int e = 0; e < 8; ++e)
+              sees[e] = tb + 32 * ch + 8 * g + e <= lim ? (f16)1.0f : (f16)0.0f;
+            const float4v hits = mfma_16x16x32(nan, sees, float4v{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                sees[e] = tb + 32 * ch + 8 * g + e <= lim[rt] ? (f16)1.0f : (f16)0.0f;
-              const float4v hits = mfma_16x16x32(nan, sees, float4v{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (hits[i] > 0.0f) add[rt][j][i] = __builtin_nanf("");
-            }
+            for (int i = 0; i < 4; ++i)
+              if (hits[i] > 0.0f) add[j][i] = __builtin_nanf("");
           }
         }
       }
     load_values(next);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int j = 0; j < VB; ++j)
 #pragma unroll
-      for (int j = 0; j < VB; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[rt][j][i] = __builtin_fmaf(add[rt][j][i], vscale, o[rt][j][i] * alpha[rt]);
+      for (int i = 0; i < 4; ++i)
+        o[j][i] = __builtin_fmaf(add[j][i], vscale, o[j][i] * alpha);
   }
 
   // the waves' rows together; thread (row of 16, 4 values) at a time
+  l = xor32<OpSum>(xor16<OpSum>(l));
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] = xor32<OpSum>(xor16<OpSum>(l[rt]));
-    if (rt > 0) __syncthreads();
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < VB; j += 4)
+      *reinterpret_cast<float4v*>(&lo[wave][c][VB * (4 * g + i) + j]) =
+          float4v{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
+  if (g == 0) {
+    lm[wave][c] = m;
+    ll[wave][c] = l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * (DP / 4); i += 64 * WAVES) {
+    const int y = i / (DP / 4), d = i % (DP / 4) * 4;
+    const int row = row_tile * 16 + y;
+    if (row >= rows || d >= a.dim) continue;
+    float top = lm[0][y];
 #pragma unroll
-      for (int j = 0; j < VB; j += 4)
-        *reinterpret_cast<float4v*>(&lo[wave][c][VB * (4 * g + i) + j]) =
-            float4v{o[rt][j][i], o[rt][j + 1][i], o[rt][j + 2][i], o[rt][j + 3][i]};
-    if (g == 0) {
-      lm[wave][c] = m[rt];
-      ll[wave][c] = l[rt];
+    for (int z = 1; z < WAVES; ++z) top = __builtin_fmaxf(top, lm[z][y]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    float4v x = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int z = 0; z < WAVES; ++z) {
+      const float f = __builtin_amdgcn_exp2f(lm[z][y] - ref);
+      sum = __builtin_fmaf(ll[z][y], f, sum);
+      const float4v v = *reinterpret_cast<const float4v*>(&lo[z][y][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (DP / 4); i += 64 * WAVES) {
-      const int y = i / (DP / 4), d = i % (DP / 4) * 4;
-      const int row = (rt0 * RT + rt) * 16 + y;
-      if (row >= rows || d >= a.dim) continue;
-      float top = lm[0][y];
+    if (item.of == 1) {
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int t = row / a.group, head = hk * a.group + row % a.group;
+      T v[4];
 #pragma unroll
-      for (int z = 1; z < WAVES; ++z) top = __builtin_fmaxf(top, lm[z][y]);
-      const float ref = top == -__builtin_inff() ? 0.0f : top;
-      float4v x = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-      float sum = 0.0f;
-#pragma unroll
-      for (int z = 0; z < WAVES; ++z) {
-        const float f = __builtin_amdgcn_exp2f(lm[z][y] - ref);
-        sum = __builtin_fmaf(ll[z][y], f, sum);
-        const float4v v = *reinterpret_cast<const float4v*>(&lo[z][y][d]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
-      }
-      if (item.of == 1) {
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int t = row / a.group, head = hk * a.group + row % a.group;
-        T v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(x[e] * inverse);
-        store_n<8>(reinterpret_cast<T*>(a.out) +
-                   (((int64_t)b * a.tokens + t) * a.kv_heads * a.group + head) * a.dim + d, v);
-      } else {
-        float* const part = a.part + parts_at(a) + (((int64_t)w * a.kv_heads + hk) * rows + row) * (a.dim + 4);
-        *reinterpret_cast<float4v*>(part + d) = x;
-        if (d == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{top, sum, 0.0f, 0.0f};
-      }
+      for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(x[e] * inverse);
+      store_n<8>(reinterpret_cast<T*>(a.out) +
+                 (((int64_t)b * a.tokens + t) * a.kv_heads * a.group + head) * a.dim + d, v);
+    } else {
+      float* const part = a.part + parts_at(a) + (((int64_t)w * a.kv_heads + hk) * rows + row) * (a.dim + 4);
+      *reinterpret_cast<float4v*>(part + d) = x;
+      if (d == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{top, sum, 0.0f, 0.0f};
     }
   }
 }
@@ -453,9 +409,9 @@ __device__ __forceinline__ void cache_attention_join(const CacheAttentionArgs& a
 
 }  // namespace mlc
 
-#define CACHE_ATTENTION(NAME, T, DP, RT, TOK, WAVES, GENERAL)                                     \
+#define CACHE_ATTENTION(NAME, T, DP, TOK, WAVES, GENERAL)                                         \
   extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::CacheAttentionArgs a) {      \
-    mlc::cache_attention<T, DP, RT, TOK, WAVES, GENERAL>(a);                                      \
+    mlc::cache_attention<T, DP, TOK, WAVES, GENERAL>(a);                                          \
   }
 #define CACHE_ATTENTION_JOIN(NAME, T, WAVES)                                             \
   extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::CacheAttentionArgs a) {             \

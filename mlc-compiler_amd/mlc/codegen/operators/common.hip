@@ -43,6 +43,23 @@ template <class T> __device__ __forceinline__ const T* at(const void* p, int64_t
   return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + bytes);
 }
 
+// Two e4m3 codes of a word, the low or the high pair, as two 16-bit values: exact.
+template <class T> struct codes;
+template <> struct codes<f16> {
+  typedef half8 v8;
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
+};
+template <> struct codes<__bf16> {
+  typedef bf16x8 v8;
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, int hi) {
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  }
+};
+
 // One row of O out of the parts that workgroups made of it: ``of`` of them, ``step`` floats
 // apart, each dim values not normalised, then the reference of their exponentials in log2
 // units and the sum of their weights. For one workgroup of WAVES: groups of 16, 32 or 64

@@ -691,13 +691,14 @@ def test_every_kernel_a_plan_asks_for_is_built_beforehand():
     known = {kernel for _, kernel in plans.all_kernels()}
     random.seed(1)
     seen = set()
-    for _ in range(3000):
+    for _ in range(6000):
         dtype, kv, group = random.choice((HALF, BF, FULL)), random.choice((1, 2, 8)), random.choice((1, 4, 16))
         b, t = random.choice((1, 2, 40)), random.choice((1, 2, 3, 5, 31, 200, 5000))
         dim, block = random.choice((16, 64, 80, 96, 128, 256)), random.choice((32, 64, 128))
         q, k = dense(b, t, kv * group, dim, dtype=dtype), dense(b, t, kv, dim, dtype=dtype)
-        cache = dense(b, kv, 64 * block, dim, dtype=E4M3)
-        scale, start = dense(b, kv, 64, dtype=FULL), dense(b, dtype=torch.int32)
+        blocks = random.choice((8, 64))
+        cache = dense(b, kv, blocks * block, dim, dtype=E4M3)
+        scale, start = dense(b, kv, blocks, dtype=FULL), dense(b, dtype=torch.int32)
         slopes = dense(kv * group, dtype=FULL) if random.random() < 0.5 else None
         found = [plans.plan_rotary(q, k, dense(t, dtype=torch.int32), dense(dim // 2, dtype=torch.float64),
                                    random.random() < 0.5, 1.0),
