@@ -289,7 +289,7 @@ def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_sc
 
 
 CACHED_DIMS = (64, 128, 256)
-MANY_ROWS = 32
+MANY_ROWS = 256
 
 
 def cached_kernel(dtype, dp: int, step: int, waves: int, general: bool) -> tuple[str, str]:

@@ -86,7 +86,6 @@ template <uint32_t E> __device__ __forceinline__ bool drop_not_finite(uint4v& x)
 
 template <bool B, class X, class Y> struct choose { typedef X type; };
 template <class X, class Y> struct choose<false, X, Y> { typedef Y type; };
-template <bool B> struct bool_constant { static constexpr bool value = B; };
 
 // 16 bytes of a lane from ``g`` straight to LDS at ``lds`` + 16 * lane.
 __device__ __forceinline__ void to_lds(const void* g, void* lds) {

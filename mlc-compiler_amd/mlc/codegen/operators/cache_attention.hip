@@ -138,11 +138,12 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   int start, count;
   held(a, b, start, count);
   if (count < 0 && threadIdx.x == 0) *a.error = INVALID_CACHE_RANGE;
-  if (a.items > 0 && item.nth == 0 && row_tile == 0 && hk == 0 && threadIdx.x == 0)
-    reinterpret_cast<int2v*>(a.part)[b] = int2v{first, item.of};
   // an item's waves take every so-manieth step of the keys: what is read at one time lies
   // side by side
-  const int hi_key = item.keys;
+  const int hi_key = __builtin_amdgcn_readfirstlane(item.keys);
+  const int nth = __builtin_amdgcn_readfirstlane(item.nth), of = __builtin_amdgcn_readfirstlane(item.of);
+  if (a.items > 0 && nth == 0 && row_tile == 0 && hk == 0 && threadIdx.x == 0)
+    reinterpret_cast<int2v*>(a.part)[b] = int2v{first, of};
 
   const int rows = a.tokens * a.group;
   const int own = row_tile * 16 + c, r = own < rows ? own : rows - 1;
@@ -180,168 +181,192 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   const int krow = 8 * (c >> 2) + (c & 3);
   // What lies past the last key or past dim is read as the last key or the row's start:
   // such scores are masked, such values meet zeros of Q or columns that nobody stores.
-  const int v_at = c * VB < a.dim ? c * VB : 0;
+  const uint32_t v_at = c * VB < a.dim ? c * VB : 0;
+  uint32_t k_at[KP];
+#pragma unroll
+  for (int s = 0; s < KP; ++s) k_at[s] = 64 * s + 16 * g < a.dim ? 64 * s + 16 * g : 0;
   uint4v kr[CH][2][KP];
   words<VW> vr[CH][8];
-  float kscale_next, vscale_next, kscale, vscale;
+  float kscale_next, vscale_next;
   auto load_keys = [&](int tb) {
+    const uint8_t* const base = kc + (int64_t)tb * a.dim;
+    auto rows_at = [&](auto place) {
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+      for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        int key = tb + 32 * ch + krow + 4 * u;
-        key = key < hi_key ? key : hi_key - 1;
-        const uint8_t* const p = kc + (int64_t)key * a.dim;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int s = 0; s < KP; ++s) {
-          const int d = 64 * s + 16 * g;
-          kr[ch][u][s] = *reinterpret_cast<const uint4v*>(p + (d < a.dim ? d : 0));
-        }
-      }
+          for (int s = 0; s < KP; ++s)
+            kr[ch][u][s] = *reinterpret_cast<const uint4v*>(place(32 * ch + 4 * u) + k_at[s]);
+    };
+    if (tb + TOK <= hi_key) {
+      const uint32_t own = krow * (uint32_t)a.dim;
+      rows_at([&](int row) { return base + row * a.dim + own; });
+    } else {
+      rows_at([&](int row) {
+        const int key = row + krow < hi_key - tb ? row + krow : hi_key - tb - 1;
+        return base + key * (uint32_t)a.dim;
+      });
+    }
     kscale_next = ks[tb >> a.block_shift];
   };
   auto load_values = [&](int tb) {
+    const uint8_t* const base = vc + (int64_t)tb * a.dim;
+    auto rows_at = [&](auto place) {
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+      for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int key = tb + 32 * ch + 8 * g + i;
-        key = key < hi_key ? key : hi_key - 1;
-        vr[ch][i] = *reinterpret_cast<const words<VW>*>(vc + (int64_t)key * a.dim + v_at);
-      }
+        for (int i = 0; i < 8; ++i) vr[ch][i] = *reinterpret_cast<const words<VW>*>(place(32 * ch + i) + v_at);
+    };
+    if (tb + TOK <= hi_key) {
+      const uint32_t own = 8 * g * (uint32_t)a.dim;
+      rows_at([&](int row) { return base + row * a.dim + own; });
+    } else {
+      rows_at([&](int row) {
+        const int key = row + 8 * g < hi_key - tb ? row + 8 * g : hi_key - tb - 1;
+        return base + key * (uint32_t)a.dim;
+      });
+    }
     vscale_next = vs[tb >> a.block_shift];
   };
 
   // The next step's keys are asked for when this one's are in the products, the next
   // values likewise: half of the registers' loads are always on their way.
-  const int step = item.of * WAVES * TOK;
-  int tb = (item.nth * WAVES + wave) * TOK;
-  if (tb < hi_key) {
-    load_keys(tb);
-    load_values(tb);
-  }
-  for (; tb < hi_key; tb += step) {
-    kscale = kscale_next;
-    vscale = vscale_next;
-    const int next = tb + step < hi_key ? tb + step : tb;  // past the end: once more, for nothing
-    const bool masked = tb + TOK - 1 > lim_min;
+  const int step = of * WAVES * TOK, begin = (nth * WAVES + wave) * TOK;
+  auto pass = [&](auto is_safe) {
+    constexpr bool SAFE = decltype(is_safe)::value;
+    if (begin < hi_key) {
+      load_keys(begin);
+      load_values(begin);
+    }
+    for (int tb = begin; tb < hi_key; tb += step) {
+      const float kscale = kscale_next, vscale = vscale_next;
+      const int next = tb + step < hi_key ? tb + step : tb;  // past the end: once more, for nothing
+      const bool masked = tb + TOK - 1 > lim_min;
 
-    float4v s[CH][2];
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 2 * KP; ++i) {
-          uint4v k;
-          const uint32_t w0 = kr[ch][u][i >> 1][(i & 1) * 2], w1 = kr[ch][u][i >> 1][(i & 1) * 2 + 1];
-          k.x = codes<T>::widen(w0, 0);
-          k.y = codes<T>::widen(w0, 1);
-          k.z = codes<T>::widen(w1, 0);
-          k.w = codes<T>::widen(w1, 1);
-          if (i == 0) s[ch][u] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-          s[ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[i], s[ch][u]);
-        }
-    load_keys(next);
-    half8 p[CH];
-    const float factor = a.factor * kscale;
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float x = s[ch][e >> 2][e & 3] * factor;
-        const int key = tb + 32 * ch + 8 * g + e;
-        if constexpr (GENERAL) {
-          if (a.cap != 0.0f) {
-            // tanh y = 1 - 2 / (e^2y + 1)
-            const float z = __builtin_amdgcn_exp2f(x * (2.0f * 0x1.715476p+0f));
-            x = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(z + 1.0f);
-          }
-          if (a.slopes) x = __builtin_fmaf(-slope, __builtin_fabsf((float)(key - pos)), x);
-        }
-        if (masked) x = key <= lim ? x : -__builtin_inff();
-        s[ch][e >> 2][e & 3] = x;
-        top = __builtin_fmaxf(top, x);
-      }
-    top = xor32<OpMax>(xor16<OpMax>(top));
-    const float now = top > m ? top : m;
-    const float ref = now == -__builtin_inff() ? 0.0f : now;
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = now;
-    l *= alpha;
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(s[ch][e >> 2][e & 3] - ref);
-        l += x;
-        p[ch][e] = (f16)x;
-      }
-    // a value that is NaN and that some row does not see would spoil the row: 0 * NaN
-    bool spoiled = false;
-    if (masked) {
+      float4v s[CH][2];
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int z = 0; z < VW; ++z) {
-            // a byte of 0x7f carries into its top bit when 1 is added to its low seven
-            const uint32_t x = (vr[ch][i].x[z] & 0x7f7f7f7fu) + 0x01010101u;
-            spoiled |= (x & 0x80808080u) != 0;
+          for (int i = 0; i < 2 * KP; ++i) {
+            uint4v k;
+            const uint32_t w0 = kr[ch][u][i >> 1][(i & 1) * 2], w1 = kr[ch][u][i >> 1][(i & 1) * 2 + 1];
+            k.x = codes<T>::widen(w0, 0);
+            k.y = codes<T>::widen(w0, 1);
+            k.z = codes<T>::widen(w1, 0);
+            k.w = codes<T>::widen(w1, 1);
+            if (i == 0) s[ch][u] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            s[ch][u] = mfma_16x16x32(__builtin_bit_cast(v8, k), q[i], s[ch][u]);
           }
-      spoiled = __any(spoiled);
-    }
-    float4v add[VB];
+      load_keys(next);
+      half8 p[CH];
+      const float factor = a.factor * kscale;
+      auto each = [&](auto of_score) {
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+        for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int z = 0; z < VW; ++z) {
-        uint32_t f[4][4];  // [byte][pair of tokens]
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t t0 = vr[ch][2 * i].x[z], t1 = vr[ch][2 * i + 1].x[z];
-          const uint32_t even = __builtin_amdgcn_perm(t1, t0, 0x05010400u);
-          const uint32_t odd = __builtin_amdgcn_perm(t1, t0, 0x07030602u);
-          f[0][i] = codes<f16>::widen(even, 0);
-          f[1][i] = codes<f16>::widen(even, 1);
-          f[2][i] = codes<f16>::widen(odd, 0);
-          f[3][i] = codes<f16>::widen(odd, 1);
-        }
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          half8 v = __builtin_bit_cast(half8, uint4v{f[y][0], f[y][1], f[y][2], f[y][3]});
-          half8 nan = {};
-          if (spoiled) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              nan[i] = v[i] != v[i] ? (f16)1.0f : (f16)0.0f;
-              v[i] = v[i] != v[i] ? (f16)0.0f : v[i];
-            }
-          }
-          const int j = 4 * z + y;
-          if (ch == 0) add[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-          add[j] = mfma_16x16x32(v, p[ch], add[j]);
-          if (spoiled) {
-            // rows that see one of the NaN values get a NaN
-            half8 sees;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              sees[e] = tb + 32 * ch + 8 * g + e <= lim ? (f16)1.0f : (f16)0.0f;
-            const float4v hits = mfma_16x16x32(nan, sees, float4v{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (hits[i] > 0.0f) add[j][i] = __builtin_nanf("");
-          }
-        }
+          for (int e = 0; e < 8; ++e)
+            s[ch][e >> 2][e & 3] = of_score(s[ch][e >> 2][e & 3], 32 * ch + e);
+      };
+      if (GENERAL && a.cap != 0.0f) {
+        // cap tanh y = cap - 2 cap / (e^2y + 1)
+        const float by = factor * (2.0f * 0x1.715476p+0f);
+        each([&](float x, int) {
+          return __builtin_fmaf(-2.0f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * by) + 1.0f), a.cap);
+        });
+      } else {
+        each([&](float x, int) { return x * factor; });
       }
-    load_values(next);
+      if (GENERAL && a.slopes) {
+        const float away = (float)(tb + 8 * g - pos);
+        each([&](float x, int k) { return __builtin_fmaf(-slope, __builtin_fabsf(away + (float)k), x); });
+      }
+      if (masked) {
+        const int left = lim - tb - 8 * g;
+        each([&](float x, int k) { return k <= left ? x : -__builtin_inff(); });
+      }
+      float top = s[0][0][0];
+      each([&](float x, int) {
+        top = __builtin_fmaxf(top, x);
+        return x;
+      });
+      top = xor32<OpMax>(xor16<OpMax>(top));
+      const float now = top > m ? top : m;
+      const float ref = now == -__builtin_inff() ? 0.0f : now;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      m = now;
+      l *= alpha;
 #pragma unroll
-    for (int j = 0; j < VB; ++j)
+      for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[j][i] = __builtin_fmaf(add[j][i], vscale, o[j][i] * alpha);
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(s[ch][e >> 2][e & 3] - ref);
+          l += x;
+          p[ch][e] = (f16)x;
+        }
+      float4v add[VB];
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int z = 0; z < VW; ++z) {
+          uint32_t f[4][4];  // [byte][pair of tokens]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t t0 = vr[ch][2 * i].x[z], t1 = vr[ch][2 * i + 1].x[z];
+            const uint32_t even = __builtin_amdgcn_perm(t1, t0, 0x05010400u);
+            const uint32_t odd = __builtin_amdgcn_perm(t1, t0, 0x07030602u);
+            f[0][i] = codes<f16>::widen(even, 0);
+            f[1][i] = codes<f16>::widen(even, 1);
+            f[2][i] = codes<f16>::widen(odd, 0);
+            f[3][i] = codes<f16>::widen(odd, 1);
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            half8 v = __builtin_bit_cast(half8, uint4v{f[y][0], f[y][1], f[y][2], f[y][3]});
+            const int j = 4 * z + y;
+            if (ch == 0) add[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (SAFE) {
+              // rows that see one of the values that are NaN get a NaN, others a zero of it
+              half8 nan, sees;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                nan[e] = v[e] != v[e] ? (f16)1.0f : (f16)0.0f;
+                v[e] = v[e] != v[e] ? (f16)0.0f : v[e];
+                sees[e] = tb + 32 * ch + 8 * g + e <= lim ? (f16)1.0f : (f16)0.0f;
+              }
+              const float4v hits = mfma_16x16x32(nan, sees, float4v{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (hits[i] > 0.0f) add[j][i] = __builtin_nanf("");
+            }
+            add[j] = mfma_16x16x32(v, p[ch], add[j]);
+          }
+        }
+      load_values(next);
+#pragma unroll
+      for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[j][i] = __builtin_fmaf(add[j][i], vscale, o[j][i] * alpha);
+    }
+
+  };
+  pass(bool_constant<false>{});
+  // 0 times a NaN of a key that a row does not see is NaN in the products. Where something
+  // came out not finite, the wave goes through its keys again with such values apart.
+  float check = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VB; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) check = __builtin_fmaf(o[j][i], 0.0f, check);
+  if (__any(check != 0.0f)) {
+    m = -__builtin_inff();
+    l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VB; ++j) o[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    pass(bool_constant<true>{});
   }
 
   // the waves' rows together; thread (row of 16, 4 values) at a time
@@ -375,7 +400,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
     }
-    if (item.of == 1) {
+    if (of == 1) {
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int t = row / a.group, head = hk * a.group + row % a.group;
       T v[4];

@@ -10,6 +10,8 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 // Codes that kernels leave in the invalid-input word.
 enum { INVALID_CACHE_RANGE = 2 };
 
+template <bool B> struct bool_constant { static constexpr bool value = B; };
+
 template <class T> struct element;
 template <> struct element<float> {
   static __device__ __forceinline__ float widen(float x) { return x; }
