@@ -289,7 +289,12 @@ def plan_cache_append(k_cache: Operand, v_cache: Operand, k_scale: Operand, v_sc
 
 
 CACHED_DIMS = (64, 128, 256)
-MANY_ROWS = 256
+#: products of scores and values from which on rows go through tiles of 128
+#: (``attention.hip``) and not of 16: keys are widened once for all of them, in more
+#: launches of work that is fixed. Tiles of 128 / 16, 8 key heads of 128: 4 x 128 rows over
+#: 2048 keys (1.1e9) 27 / 25 us, 4 x 512 (4.3e9) 46 / 58, 512 over 16384 (8.6e9) 75 / 102;
+#: 2 x 488 rows of 2 heads over 8192 (2.0e9) 40 / 36, over 16384 (4.1e9) 50 / 58.
+MANY_ROWS, MANY_PRODUCTS = 128, 3e9
 
 
 def cached_kernel(dtype, dp: int, step: int, waves: int, general: bool) -> tuple[str, str]:
@@ -307,7 +312,7 @@ def plan_cache_attention(q: Operand, k_cache: Operand, v_cache: Operand, k_scale
         return Plan(())
     group, block = heads // kv_heads, capacity // k_scale.shape[2] if k_scale.shape[2] else 32
     rows = tokens * group
-    if rows > MANY_ROWS:
+    if rows >= MANY_ROWS and batch * heads * tokens * capacity * dim > MANY_PRODUCTS:
         strides = (kv_heads * capacity * dim, dim, capacity * dim)
         return _attention("CODES", q, k_cache, v_cache, (kv_heads, capacity), strides * 2,
                           (slopes, None, None), (k_scale, v_scale, start, count, block.bit_length() - 1),
@@ -373,7 +378,7 @@ def all_kernels() -> list[tuple[str, str]]:
     for dtype in (torch.float16, torch.bfloat16):
         out += [("attention", attention_kernel(dtype, dp, w, source, g)[0]) for dp in ATTENTION_DIMS
                 for w in (1, 2, 4) for source in ("COPIED", "DIRECT", "CODES") for g in (False, True)
-                if source != "CODES" or (dp in CACHED_DIMS and 32 * w > MANY_ROWS)]
+                if source != "CODES" or (dp in CACHED_DIMS and w == 4)]
         out += [("cache_attention", cached_kernel(dtype, dp, step, w, g)[0])
                 for dp in CACHED_DIMS for w in (4, 8) if w < 8 or dp < 256 for step in (32, 64)
                 for g in (False, True)]
