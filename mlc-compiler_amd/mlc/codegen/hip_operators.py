@@ -100,7 +100,7 @@ def _numel(x: Operand) -> int:
 # rotary positions
 # --------------------------------------------------------------------------
 
-ROTARY_BLOCK, ROTARY_PAIRS = 256, 1024
+ROTARY_BLOCK, ROTARY_PAIRS, ROTARY_TOKENS = 256, 1024, 64
 
 
 def rotary_kernel(dtype, v: int, interleaved: bool) -> tuple[str, str]:
@@ -116,12 +116,15 @@ def plan_rotary(q: Operand, k: Operand, positions: Operand, frequencies: Operand
     tokens = batch * seq
     if tokens * (heads + kv_heads) * dim == 0:
         return Plan(())
-    pack = 16 // q.dtype.itemsize
     run = turned if interleaved else turned // 2
-    whole = all(n % pack == 0 for n in (dim, turned, run, *q.strides[:3], *k.strides[:3]))
-    v = pack if whole and q.aligned and k.aligned else 1
-    # enough workgroups first, then as many tokens of one as fill it
-    group = max(1, min(ROTARY_PAIRS // max(1, turned // 2), tokens // (4 * UNITS)))
+    v = 16 // q.dtype.itemsize if q.aligned and k.aligned else 1
+    while v > 1 and any(n % v for n in (dim, turned, run, *q.strides[:3], *k.strides[:3])):
+        v //= 2
+    # many workgroups first, so that some stream while others evaluate angles (4 x 4096 tokens,
+    # 40 heads of 128: 16 tokens a workgroup 81 us, 1 69), then as many tokens of one as fit;
+    # fewer than 2^20 rows of heads
+    group = max(1, min(ROTARY_PAIRS // max(1, turned // 2), ROTARY_TOKENS, tokens // (64 * UNITS),
+                       (1 << 20) // (heads + kv_heads)))
     blocks = min(_ceil(tokens, group), 1 << 22)
     pb, pt = (0, positions.strides[0]) if len(positions.shape) == 1 else positions.strides
     tail = struct.pack("<4q9q8ifi", q.offset, k.offset, positions.offset, frequencies.offset,
@@ -371,8 +374,8 @@ def all_kernels() -> list[tuple[str, str]]:
     """``(file, kernel)`` of everything that a plan can ask for."""
     out = []
     for dtype in (torch.float16, torch.bfloat16, torch.float32):
-        out += [("rotary", rotary_kernel(dtype, v, i)[0]) for v in (16 // dtype.itemsize, 1)
-                for i in (False, True)]
+        out += [("rotary", rotary_kernel(dtype, v, i)[0]) for v in (8, 4, 2, 1)
+                for i in (False, True) if v * dtype.itemsize <= 16]
         out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
                 for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
     for dtype in (torch.float16, torch.bfloat16):

@@ -101,6 +101,7 @@ class Call:
     results."""
 
     def __init__(self, plan: Plan, operands: tuple, device: int) -> None:
+        self.plan = plan
         self.modules = device_modules(device)
         self.device, self.workspace = device, plan.workspace
         self.flags = any("error" in x.pointers for x in plan.launches)

@@ -314,6 +314,60 @@ def test_cache_attention(dtype, batch, tokens, heads, kv, dim, capacity, block, 
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (HALF, BF))
+@pytest.mark.parametrize("batch,tokens,heads,kv,dim,capacity,block,start,count", [
+    (1, 64, 4, 2, 64, 512, 64, [300], None),
+    (2, 33, 8, 2, 128, 256, 32, [0, 223], [33, 20]),
+    (3, 40, 4, 1, 96, 128, 128, [0, 88, 5], [40, 40, 0]),
+    (1, 150, 1, 1, 256, 384, 64, [100], [149]),
+    (2, 20, 16, 2, 16, 96, 32, [76, 1], None),
+    (1, 128, 2, 2, 128, 4096, 64, [3900], None),
+])
+@pytest.mark.parametrize("options", ({}, {"cap": 4.0, "slopes": True, "scale": 0.2}), ids=("", "all"))
+def test_cache_attention_of_many_rows(monkeypatch, dtype, batch, tokens, heads, kv, dim, capacity, block,
+                                      start, count, options):
+    """By tiles of codes, which are for more products than a test has."""
+    from mlc.codegen import hip_operators
+
+    monkeypatch.setattr(hip_operators, "MANY_PRODUCTS", 0)
+    monkeypatch.setattr(hip_operators, "MANY_ROWS", 1)
+    ops._calls.clear()
+    try:
+        cache = filled(batch, kv, capacity, dim, block, seed=2)
+        q = normal(batch, tokens, heads, dim, dtype=dtype, seed=6)
+        options = dict(options)
+        if "slopes" in options:
+            options["slopes"] = torch.linspace(0, 0.3, heads, device="cuda")
+        start, count = ints(start), None if count is None else ints(count)
+        for at in (q, strided(q, "wide")):
+            ref.close(cache.attend(at, start, count, **options),
+                      *ref.cache_attention(q, *parts(cache), start, count, **options))
+        # NaN behind the last key, and at a key that the first rows do not see
+        codes = cache.values.view(torch.uint8)
+        end = int(start[0]) + (tokens if count is None else int(count[0]))
+        codes[0, :, end:] = 127
+        codes[0, 0, end - 1, 3] = 255
+        ref.close(cache.attend(q, start, count, **options),
+                  *ref.cache_attention(q, *parts(cache), start, count, **options))
+        assert any("attention_" in x.symbol and "codes" in x.symbol for c in ops._calls.values()
+                   for x in c.plan.launches)
+    finally:
+        ops._calls.clear()
+
+
+@gpu
+def test_cache_attention_of_a_piece_of_a_prompt():
+    """As many rows and keys as go through tiles of codes by themselves."""
+    cache = filled(1, 2, 16384, 128)
+    q, start = normal(1, 192, 8, 128, seed=1, dtype=BF), ints([16000])
+    got = cache.attend(q, start)
+    for t in (0, 100, 191):
+        one = ops.cache_attention(q[:, t:t + 1], *parts(cache), start + t)
+        ref.close(one, *ref.cache_attention(q[:, t:t + 1], *parts(cache), start + t))
+        ref.close(got[:, t:t + 1], *ref.cache_attention(q[:, t:t + 1], *parts(cache), start + t))
+
+
+@gpu
 def test_cache_attention_does_not_read_behind_a_sequence():
     """NaN behind the last key and, among several new tokens, at keys that only the
     later ones see."""
