@@ -46,8 +46,16 @@ struct AttentionArgs {
 template <int DP, int SOURCE> constexpr int tile_keys = DP == 256 || SOURCE == 2 ? 32 : 64;
 
 template <class T> struct vec8;
-template <> struct vec8<f16> { typedef half8 type; static constexpr uint32_t exponent = 0x7c00u; };
-template <> struct vec8<__bf16> { typedef bf16x8 type; static constexpr uint32_t exponent = 0x7f80u; };
+template <> struct vec8<f16> {
+  typedef half8 type;
+  static constexpr uint32_t exponent = 0x7c00u;
+  static constexpr float lift = 7.0f;  // see LIFT
+};
+template <> struct vec8<__bf16> {
+  typedef bf16x8 type;
+  static constexpr uint32_t exponent = 0x7f80u;
+  static constexpr float lift = -40.0f;
+};
 
 __device__ __forceinline__ float16v mfma_32x32x16(half8 a, half8 b, float16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -400,10 +408,13 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = __builtin_fmaxf(top, s[u][j]);
     top = xor32<OpMax>(top * scale);
-    // the reference of the exponentials follows the maximum in steps of at least 2^8:
-    // weights stay below 2^8 and O is seldom scaled
-    if (__any(top > m + 8.0f)) {
-      const float next = top > m ? top : m;
+    // The reference of the exponentials is not the maximum itself: O is scaled only when a
+    // maximum is 2^8 above the one that set it, and the largest weight is then 2^LIFT. In
+    // fp16 that keeps weights down to 2^-21 of it normal numbers, up to 2^15; bf16 has
+    // exponents to spare, and weights of 2^-40 leave fp32 room for any value it holds.
+    constexpr float LIFT = vec8<PT>::lift;
+    if (__any(top > m + (LIFT + 8.0f))) {
+      const float next = top - LIFT > m ? top - LIFT : m;
       const float alpha = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - next);
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)

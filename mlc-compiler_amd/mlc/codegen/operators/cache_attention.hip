@@ -11,7 +11,8 @@
 //  * S^T = K Q^T on 16x16x32 products; the order of K's rows makes lane (c, g) end
 //    with row c's scores of keys 8 g .. 8 g + 7 of every 32, the B operand of
 //  * O^T = V^T P^T, whose V^T operand is made of V's rows by byte permutes. P is
-//    fp16 whatever the queries are: e4m3 is exact in it and P is below 1.
+//    fp16 whatever the queries are: e4m3 is exact in it, and P, 2^14 where a score is the
+//    largest, is a normal number down to 2^-28 of that.
 //  * A key block's scales are powers of two outside the products: K's goes into the
 //    factor of its scores, V's multiplies the block's part of O.
 // The waves of a workgroup are joined in LDS, the items of a sequence by a second
@@ -295,14 +296,14 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
       top = xor32<OpMax>(xor16<OpMax>(top));
       const float now = top > m ? top : m;
       const float ref = now == -__builtin_inff() ? 0.0f : now;
-      const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      const float low = ref - 14.0f, alpha = __builtin_amdgcn_exp2f(m - ref);
       m = now;
       l *= alpha;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[ch][e >> 2][e & 3] - ref);
+          const float x = __builtin_amdgcn_exp2f(s[ch][e >> 2][e & 3] - low);
           l += x;
           p[ch][e] = (f16)x;
         }
