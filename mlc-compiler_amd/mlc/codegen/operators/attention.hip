@@ -50,11 +50,13 @@ template <> struct vec8<f16> {
   typedef half8 type;
   static constexpr uint32_t exponent = 0x7c00u;
   static constexpr float lift = 7.0f;  // see LIFT
+  static constexpr float least = 0x1p-24f;
 };
 template <> struct vec8<__bf16> {
   typedef bf16x8 type;
   static constexpr uint32_t exponent = 0x7f80u;
   static constexpr float lift = -40.0f;
+  static constexpr float least = 0x1p-126f;
 };
 
 __device__ __forceinline__ float16v mfma_32x32x16(half8 a, half8 b, float16v c) {
@@ -120,6 +122,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   constexpr int CH = DP / 8;                               // of which hold values
   constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
   constexpr int BUFFERS = 2;
+  constexpr float V_FACTOR = CACHE ? SCALE_ROOM : 1.0f;
   constexpr int KEYS = tile_keys<DP, SOURCE>, U = KEYS / 32;
   constexpr int EACH = CACHE ? 16 : 8, ROW = DP / EACH;    // values of a piece, pieces of a row
   constexpr int N = (KEYS * ROW + THREADS - 1) / THREADS;  // pieces of a tile for a thread
@@ -161,7 +164,8 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     real = ok ? count : 0;
     keys = real > 0 ? start + real : 0;
   }
-  const int prefix = a.prefix ? at<int32_t>(a.prefix, a.p_off)[b * a.ps] : 0;
+  int prefix = a.prefix ? at<int32_t>(a.prefix, a.p_off)[b * a.ps] : 0;
+  prefix = prefix < 0 ? 0 : prefix;
   // last key that query ``t`` may see
   auto last = [&](int t) {
     int lim = keys - 1;
@@ -362,7 +366,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     float scale = a.scale, v_scale = 1.0f;
     if constexpr (CACHE) {
       scale *= ks[base >> a.block_shift];
-      v_scale = vs[base >> a.block_shift];
+      v_scale = vs[base >> a.block_shift] * V_FACTOR;
+      // scales that are not finite, of keys that this row does not see
+      if (SAFE && base > lim) scale = 1.0f, v_scale = 0.0f;
     }
     if constexpr (GENERAL) {
       // in log2 units: the cap, then the bias
@@ -432,6 +438,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], scale, -ref));
         l += e;
         p[2 * u + (j >> 3)][j & 7] = (PT)e;
+        // a weight that is too small for its type still makes an infinity or a NaN count
+        if (SAFE && s[u][j] > -__builtin_inff() && e < vec8<PT>::least)
+          p[2 * u + (j >> 3)][j & 7] = (PT)vec8<PT>::least;
       }
     auto values = [&](int i, int u) {
       const char* const at = lds + BUFFERS * TILE + u * 16 * PITCH;
@@ -631,7 +640,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
   }
   if (row >= rows) return;
-  l = xor32<OpSum>(l);
+  l = xor32<OpSum>(l) * V_FACTOR;
   if (CACHE && t >= real) {  // padding
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)

@@ -241,7 +241,10 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
       load_values(begin);
     }
     for (int tb = begin; tb < hi_key; tb += step) {
-      const float kscale = kscale_next, vscale = vscale_next;
+      const float kscale = kscale_next;
+      float vscale = vscale_next * SCALE_ROOM;
+      // a scale that is not finite, of keys that this row does not see
+      if (SAFE && tb > lim) vscale = 0.0f;
       const int next = tb + step < hi_key ? tb + step : tb;  // past the end: once more, for nothing
       const bool masked = tb + TOK - 1 > lim_min;
 
@@ -371,7 +374,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
   }
 
   // the waves' rows together; thread (row of 16, 4 values) at a time
-  l = xor32<OpSum>(xor16<OpSum>(l));
+  l = xor32<OpSum>(xor16<OpSum>(l)) * SCALE_ROOM;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll

@@ -10,6 +10,11 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 // Codes that kernels leave in the invalid-input word.
 enum { INVALID_CACHE_RANGE = 2 };
 
+// The weights of values from the 8-bit cache are fp16, the largest 2^14 or 2^15, and a value
+// with its scale may be as large as fp32 holds: O and the sum of the weights are kept 2^-46
+// times themselves, so that O stays finite over 2^30 keys. Values below 2^-100 lose digits.
+constexpr float SCALE_ROOM = 0x1p-46f;
+
 template <bool B> struct bool_constant { static constexpr bool value = B; };
 
 template <class T> struct element;

@@ -308,6 +308,8 @@ class _Translation:
     def _opaque(self, fx, op, args, kwargs):
         """An op with no rule: it runs as one torch call, a fusion barrier,
         with result types taken from the exporter."""
+        if op.startswith("mlc."):
+            args = self._rows_together(fx.target, args)
         recorded = fx.meta.get("val")
         results = list(recorded) if isinstance(recorded, (list, tuple)) else [recorded]
         outputs = []
@@ -319,6 +321,22 @@ class _Translation:
         self._emit(op, args, kwargs, outputs, export_val=recorded, target=fx.target,
                    types_from_export=True, opaque=True)
         return self._single_or_list(outputs)
+
+    def _rows_together(self, target, args: list) -> list:
+        """Operands of an operator of ``mlc.ops`` with the rows of heads in one piece and a
+        cache whole, as its checks found the exporter's tensors: a value here may lie
+        otherwise in its buffer (results are contiguous, whatever torch makes them)."""
+        out = []
+        for a, v in zip(target._schema.arguments, args):
+            if isinstance(v, Value) and v.numel:
+                cache = a.name.endswith(("_cache", "_scale"))
+                if cache and v.layout.strides != Layout.contiguous(v.shape).strides:
+                    raise CaptureError(f"{target}: {a.name} is a view of a buffer that lies otherwise: "
+                                       "give the buffer itself")
+                if not cache and v.rank == 4 and v.shape[3] > 1 and v.layout.strides[3] != 1:
+                    v = self._contiguous_copy(v)
+            out.append(v)
+        return out
 
     def _in_place(self, fx) -> list:
         """An operator of ``mlc.ops`` that changes its operands: they have to be
@@ -345,6 +363,7 @@ class _Translation:
                 raise CaptureError(f"{target}: one buffer is given for two operands that change")
             args.append(base)
             changed.append(base)
+        args = self._rows_together(target, args)
         outputs = {id(v): Value(f"{fx.name}_{i}", v.buffer, v.layout) for i, v in enumerate(changed)}
         self._emit(str(target), args, {}, list(outputs.values()), target=target,
                    types_from_export=True, opaque=True, pin=True)

@@ -37,6 +37,8 @@ _FLOATS = (*_HALF, torch.float32)
 _INTS = (torch.int32, torch.int64)
 _E4M3 = torch.float8_e4m3fn
 _MAX = 2 ** 31 - 256
+#: and of keys: kernels look some tiles past the last one
+_MOST_KEYS = 2 ** 30
 
 
 # --------------------------------------------------------------------------
@@ -95,6 +97,7 @@ def _check_rotary(q, k, positions, frequencies, interleaved, magnitude) -> None:
              f"{frequencies.shape[0]} pairs do not fit a dim of {q.shape[3]}")
     _require(math.isfinite(magnitude), f"magnitude: a finite number expected, got {magnitude}")
     _require(q.shape[0] * q.shape[1] <= _MAX, "rotary: too many tokens for one call")
+    _require(q.shape[2] + k.shape[2] <= 1 << 20, "rotary: too many heads for one call")
     _same(q, {"k": k, "positions": positions, "frequencies": frequencies})
 
 
@@ -111,7 +114,7 @@ def _check_attention(q, k, v, slopes, documents, prefix, scale, causal, cap) -> 
              f"{heads} query heads are not a multiple of {kv_heads} key heads")
     _require(dim % 8 == 0 and dim <= plans.ATTENTION_DIMS[-1],
              f"dim {dim}: a multiple of 8 up to {plans.ATTENTION_DIMS[-1]} expected")
-    _require(keys <= _MAX and queries * (heads // kv_heads) <= _MAX,
+    _require(keys <= _MOST_KEYS and queries * (heads // kv_heads) <= _MAX,
              "attention: too many tokens for one call")
     _scale(scale, dim)
     _cap(cap)
@@ -147,7 +150,7 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale) -> None:
              f"a capacity of {capacity} in {blocks} blocks: blocks of 32, 64 or 128 tokens expected")
     _require(dim % 16 == 0 and 16 <= dim <= plans.CACHED_DIMS[-1],
              f"dim {dim}: a multiple of 16 up to {plans.CACHED_DIMS[-1]} expected")
-    _require(capacity <= _MAX, "the cache's capacity is too large")
+    _require(capacity <= _MOST_KEYS, "the cache's capacity is too large")
     for name, x, dtype in (("k_cache", k_cache, _E4M3), ("v_cache", v_cache, _E4M3),
                            ("k_scale", k_scale, torch.float32), ("v_scale", v_scale, torch.float32)):
         _require(x.dtype == dtype and x.is_contiguous(),
@@ -299,6 +302,8 @@ def _now(op: str, operands: tuple, options: tuple, like: tuple):
     key, at = _signed(op, operands, options)
     if key is None:
         return None
+    if op == "cache_append" and (at[0] == at[1] or at[2] == at[3]) and operands[0].numel():
+        raise OperatorError("cache_append: keys and values share a cache or its scales")
     call = _calls.get(key) or _call_of(key, op, operands, at, options)
     if not like:
         call.run(at, None)
@@ -386,6 +391,7 @@ def rotary(q, k, positions, frequencies, *, interleaved: bool = False, magnitude
     are turned, the rest is copied. A pair is values ``(i, i + len(frequencies))``, or
     ``(2 i, 2 i + 1)`` if ``interleaved``. ``magnitude`` multiplies what is turned.
     """
+    interleaved, magnitude = bool(interleaved), float(magnitude)
     out = _now("rotary", (q, k, positions, frequencies), (interleaved, magnitude), (q, k))
     if out is not None:
         return out[0], out[1]
@@ -442,6 +448,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, cap:
     A query that sees nothing gets zeros. What is not seen has no influence, NaN and
     infinities included.
     """
+    scale, causal, cap = None if scale is None else float(scale), bool(causal), float(cap)
     out = _now("attention", (q, k, v, slopes, documents, prefix), (scale, causal, cap), (q,))
     if out is not None:
         return out[0]
@@ -478,6 +485,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count=None, *,
     ``count`` do not lie within the cache (an ``ExecutionError`` later). ``scale``, ``cap``
     and ``slopes`` are those of :func:`attention`.
     """
+    scale, cap = None if scale is None else float(scale), float(cap)
     out = _now("cache_attention", (q, k_cache, v_cache, k_scale, v_scale, start, count, slopes),
                (scale, cap), (q,))
     if out is not None:
@@ -503,6 +511,14 @@ class KeyValueCache(torch.nn.Module):
             self.register_buffer(f"{name[:-1]}_scales",
                                  torch.ones(*shape[:2], capacity // block, device=device),
                                  persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        """Moves the buffers with the module but keeps their types: ``model.half()`` is for
+        weights."""
+        for name, x in self._buffers.items():
+            y = fn(x)
+            self._buffers[name] = y if y.dtype == x.dtype else x.to(y.device)
+        return self
 
     def append(self, k, v, start, count=None) -> None:
         cache_append(self.keys, self.values, self.key_scales, self.value_scales, k, v, start, count)

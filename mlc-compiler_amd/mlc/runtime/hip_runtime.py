@@ -59,6 +59,12 @@ class Bound:
     args: bytes
 
 
+class Launches(list):
+    """The ``Bound`` launches of one operator and the memory they share."""
+
+    workspace: torch.Tensor | None = None
+
+
 @dataclass
 class Range:
     """Entries ``[begin, end)`` of the native launch plan."""
@@ -107,8 +113,6 @@ class HipRuntime:
         self._plans: list[ctypes.c_void_p] = []
         #: native plan -> its launches, by entry
         self._launches: dict[int, list[Bound]] = {}
-        #: memory of operators that take several launches
-        self._workspaces: list[torch.Tensor] = []
         self._arena_tensor: torch.Tensor | None = None
         self._static_arena = bool(getattr(cfg, "static_arena", False))
         #: device address of the context's invalid-input word, if a kernel
@@ -162,7 +166,7 @@ class HipRuntime:
                      args)
 
     def bind_native_extern(self, k: ExternKernel, buffers: dict[str, torch.Tensor]
-                           ) -> "Bound | list[Bound] | None":
+                           ) -> "Bound | Launches | None":
         """An extern op this module implements natively (``aten.embedding``, the
         operators of ``mlc.ops``), resolved like a generated kernel; ``None``
         leaves it to the library."""
@@ -202,9 +206,9 @@ class HipRuntime:
         return Bound(k.name, self.functions[spec.symbol], spec.grid, spec.block, spec.lds_bytes,
                      struct.pack(f"<{len(ptrs)}Q", *ptrs))
 
-    def _bind_operator(self, k: ExternKernel, buffers: dict[str, torch.Tensor]) -> list[Bound]:
+    def _bind_operator(self, k: ExternKernel, buffers: dict[str, torch.Tensor]) -> Launches:
         """The launches of an operator of ``mlc.ops``. Memory they share is the
-        binding's own, held as long as the model."""
+        binding's own and lives as long."""
         names = [a.name for a in k.node.meta["target"]._schema.arguments]
         operands, pointers = {}, {}
         for name, v in zip(names, k.node.args):
@@ -224,11 +228,13 @@ class HipRuntime:
         plan = hip_operators.PLANS[k.node.op](**operands)
         if self._error_word is not None:
             pointers["error"] = self._error_word
+        bound = Launches()
         if plan.workspace:
-            self._workspaces.append(torch.empty(plan.workspace, dtype=torch.uint8, device=self.device))
-            pointers["workspace"] = self._workspaces[-1].data_ptr()
-        return [Bound(k.name, self._operators.function(x), x.grid, x.block, 0, x.arguments(pointers))
-                for x in plan.launches]
+            bound.workspace = torch.empty(plan.workspace, dtype=torch.uint8, device=self.device)
+            pointers["workspace"] = bound.workspace.data_ptr()
+        bound += [Bound(k.name, self._operators.function(x), x.grid, x.block, 0, x.arguments(pointers))
+                  for x in plan.launches]
+        return bound
 
     # -- invalid inputs ------------------------------------------------------------
     @property

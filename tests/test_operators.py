@@ -177,6 +177,28 @@ def test_attention_is_not_touched_by_what_it_does_not_see(dtype, dim):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (HALF, BF))
+@pytest.mark.parametrize("bad", (float("nan"), float("inf")))
+def test_a_key_of_hardly_any_weight_is_still_seen(dtype, bad):
+    """A weight of e^-100 is below what its type holds, and times infinity it is not zero."""
+    q, k, v = _heads(1, 40, 100, 1, 1, 64, dtype, seed=4)
+    k[0, 7], v[0, 7, 0, 5] = -1.0, bad
+    q.fill_(10.0)
+    k[0, 8:] = 0.25
+    got = ops.attention(q, k, v)
+    ref.close(got, *ref.attention(q, k, v))
+    assert not got[..., 5].isfinite().any() and got[..., 6:].isfinite().all()
+
+
+@gpu
+def test_prefixes_of_any_value():
+    q, k, v = _heads(4, 70, 70, 2, 1, 64, HALF, seed=4)
+    prefix = ints([-2 ** 31, 2 ** 31 - 1, -1, 1])
+    ref.close(ops.attention(q, k, v, causal=True, prefix=prefix),
+              *ref.attention(q, k, v, causal=True, prefix=prefix))
+
+
+@gpu
 def test_attention_over_a_long_row_and_its_last_tokens():
     q, k, v = _heads(1, 3, 5000, 4, 2, 64, HALF, seed=2)
     ref.close(ops.attention(q, k, v, causal=True), *ref.attention(q, k, v, causal=True))
@@ -391,6 +413,44 @@ def test_cache_attention_over_blocks_of_very_different_scales():
     ref.close(cache.attend(q, ints([400])), *ref.cache_attention(q, *parts(cache), ints([400])))
 
 
+@pytest.fixture(params=("rows", "tiles"))
+def way(request, monkeypatch):
+    """Both ways that rows go over the cache, whatever their number."""
+    from mlc.codegen import hip_operators
+
+    if request.param == "tiles":
+        monkeypatch.setattr(hip_operators, "MANY_PRODUCTS", 0)
+        monkeypatch.setattr(hip_operators, "MANY_ROWS", 1)
+    ops._calls.clear()
+    yield request.param
+    ops._calls.clear()
+
+
+@gpu
+@pytest.mark.parametrize("dim,capacity", [(64, 256), (128, 8192)])
+def test_cache_attention_of_the_largest_values(way, dim, capacity):
+    """As many keys of bf16's largest values as there are: the sum of weights and values
+    stays finite."""
+    cache = ops.KeyValueCache(1, 1, capacity, dim, device="cuda")
+    cache.keys.fill_(0.0)
+    cache.values.fill_(1.75)
+    cache.value_scales.fill_(2.0 ** 127)
+    q = normal(1, 3, 2, dim, dtype=BF)
+    ref.close(cache.attend(q, ints([capacity - 3])),
+              *ref.cache_attention(q, *parts(cache), ints([capacity - 3])))
+
+
+@gpu
+@pytest.mark.parametrize("bad", (float("nan"), float("inf")))
+def test_scales_of_blocks_that_a_row_does_not_see(way, bad):
+    cache = filled(1, 1, 256, 64)
+    cache.key_scales[0, 0, 2:], cache.value_scales[0, 0, 2:] = bad, bad
+    q, start = normal(1, 40, 2, 64), ints([100])  # 28 rows see two blocks, 12 a third
+    got = cache.attend(q, start)
+    assert got[:, 28:].isnan().all()
+    ref.close(got[:, :28], *ref.cache_attention(q[:, :28], *parts(cache), start))
+
+
 # --------------------------------------------------------------------------
 # streams, graphs, devices
 # --------------------------------------------------------------------------
@@ -592,6 +652,57 @@ def test_a_buffer_that_would_be_copied_is_refused():
         mlc.compile(m.cpu(), [t.cpu() for t in inputs], device="cuda")
 
 
+@gpu
+def test_operands_of_a_compiled_operator_that_lie_otherwise_are_copied():
+    """A pointwise result keeps a permuted order in torch and not in a compiled model, where
+    its rows of heads then lie apart."""
+
+    class Turned(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            f, _ = ops.rotary_frequencies(64, device="cuda")
+            self.register_buffer("f", f)
+
+        def forward(self, q, positions):
+            y = (q.permute(0, 3, 1, 2) * 2.0).permute(0, 2, 3, 1)  # [batch, tokens, heads, dim]
+            a, b = ops.rotary(y, y, positions, self.f)
+            return ops.attention(a, b, y, causal=True)
+
+    m, q = Turned(), normal(2, 9, 3, 64)
+    args = (q, torch.arange(9, device="cuda", dtype=torch.int32))
+    compiled = mlc.compile(m, args)
+    with torch.no_grad():
+        assert torch.equal(compiled(*args), m(*args))
+
+
+@gpu
+def test_unplanned_calls_leave_no_memory_behind():
+    class Step(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.cache = filled(1, 1, 8192, 64)
+
+        def forward(self, q, start):
+            return self.cache.attend(q, start) * 2.0
+
+    m, args = Step(), (normal(1, 1, 2, 64), ints([8000]))
+    compiled = mlc.compile(m, args, mlc.Config(memory_planning=False))
+    for _ in range(3):
+        compiled(*args)
+    held = torch.cuda.memory_allocated()
+    for _ in range(5):
+        compiled(*args)
+    assert torch.cuda.memory_allocated() == held
+
+
+@gpu
+def test_a_cache_given_for_both_keys_and_values_is_refused():
+    c = filled(1, 1, 64, 64)
+    k = normal(1, 1, 1, 64)
+    _refused(lambda: ops.cache_append(c.keys, c.keys, c.key_scales, c.value_scales, k, k, ints([0])), "share")
+    _refused(lambda: ops.cache_append(c.keys, c.values, c.key_scales, c.key_scales, k, k, ints([0])), "share")
+
+
 # --------------------------------------------------------------------------
 # what is refused
 # --------------------------------------------------------------------------
@@ -669,6 +780,24 @@ def test_what_the_cache_refuses():
     _refused(lambda: ops.KeyValueCache(1, 1, 64, 64, block=16), "capacity")
     odd = ops.KeyValueCache(1, 1, 64, 24)
     _refused(lambda: odd.attend(host(1, 1, 1, 24), start[:1]), "multiple of 16")
+
+
+def test_sizes_beyond_the_kernels_indexes_are_refused():
+    shape = lambda *s, dtype=HALF: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    _refused(lambda: ops.attention(shape(1, 1, 1, 8), *[shape(1, 2 ** 30 + 1, 1, 8)] * 2), "too many tokens")
+    _refused(lambda: ops.rotary(*[shape(1, 1, 2 ** 19 + 1, 2)] * 2, shape(1, dtype=torch.int32),
+                                shape(1, dtype=torch.float64)), "too many heads")
+    cache = ops.KeyValueCache(1, 1, 2 ** 30 + 64, 16, device="meta")
+    _refused(lambda: cache.attend(shape(1, 1, 1, 16), shape(1, dtype=torch.int32)), "too large")
+
+
+def test_a_cache_keeps_its_types_when_a_model_changes_its_own():
+    m = torch.nn.Sequential(torch.nn.Linear(4, 4))
+    m.cache = ops.KeyValueCache(1, 1, 64, 16)
+    m.half()
+    assert m[0].weight.dtype == HALF
+    assert m.cache.keys.dtype == E4M3 and m.cache.key_scales.dtype == FULL
+    assert m.to("meta").cache.values.device.type == "meta"
 
 
 def test_operands_that_ask_for_gradients_are_refused():
@@ -754,7 +883,8 @@ def test_every_kernel_a_plan_asks_for_is_built_beforehand():
         cache = dense(b, kv, blocks * block, dim, dtype=E4M3)
         scale, start = dense(b, kv, blocks, dtype=FULL), dense(b, dtype=torch.int32)
         slopes = dense(kv * group, dtype=FULL) if random.random() < 0.5 else None
-        found = [plans.plan_rotary(q, k, dense(t, dtype=torch.int32), dense(dim // 2, dtype=torch.float64),
+        pairs = dim // 2 - random.choice((0, 1, 2, 4))
+        found = [plans.plan_rotary(q, k, dense(t, dtype=torch.int32), dense(pairs, dtype=torch.float64),
                                    random.random() < 0.5, 1.0),
                  plans.plan_cache_append(cache, cache, scale, scale, k, k, start, None)]
         if dtype != FULL:
