@@ -223,8 +223,11 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   // 8 values of 16 bits, or 16 codes, a piece
   uint4v rk[IS_DIRECT ? 1 : N], rv[IS_DIRECT ? 1 : N];
   int rdoc = 0;
+  // with documents, a tile that needs a mask is its number and this
+  constexpr int MASK = 1 << 28;
+  auto place = [](int kt) { return DOCS ? kt & (MASK - 1) : kt; };
   auto load = [&](int kt, int into) {
-    const int base = kt * KEYS;
+    const int base = place(kt) * KEYS;
     if constexpr (IS_DIRECT) {
       char* const to = lds + into * TILE + wave * 1024;
       if (base + KEYS <= keys) {
@@ -316,15 +319,15 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
     if (DOCS && a.documents) ldoc[into][wave][lane] = rdoc;
   };
-  // the first tile on its way
+  // the first tile on its way; ``after`` says which follows one
   auto begin = [&](int kt, auto after) {
-    if (kt < tiles) load(kt, it);
+    if (place(kt) < tiles) load(kt, it);
     behind = kt;
     if constexpr (!IS_DIRECT) {
-      if (kt < tiles) {
+      if (place(kt) < tiles) {
         store(it);
-        behind = after(kt + a.splits);
-        if (behind < tiles) load(behind, 0);
+        behind = after(kt);
+        if (place(behind) < tiles) load(behind, 0);
       }
     }
     return kt;
@@ -336,23 +339,23 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" : : : "memory");
-      const int next = after(kt + a.splits);
-      if (next < tiles) load(next, it ^ 1);
+      const int next = after(kt);
+      if (place(next) < tiles) load(next, it ^ 1);
       return next;
     } else {
       __syncthreads();
       const int next = behind;
-      if (next < tiles) {
+      if (place(next) < tiles) {
         store(it ^ 1);
-        behind = after(next + a.splits);
-        if (behind < tiles) load(behind, 0);
+        behind = after(next);
+        if (place(behind) < tiles) load(behind, 0);
       }
       return next;
     }
   };
   auto compute = [&](int kt, auto is_masked, auto is_safe) {
     constexpr bool MASKED = decltype(is_masked)::value, SAFE = decltype(is_safe)::value;
-    const int base = kt * KEYS;
+    const int base = place(kt) * KEYS;
 
     float16v s[U];
 #pragma unroll
@@ -510,7 +513,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   // tiles that every row sees whole
   int whole = (last(first_row / a.group) + 1) / KEYS;
   whole = whole < tiles ? whole : tiles;
-  auto every = [](int kt) { return kt; };
+  auto every = [&](int kt) { return kt + a.splits; };
   if (!(DOCS && a.documents)) {
     // those first, then the ones that need a mask
     int kt = begin(split, every);
@@ -552,68 +555,68 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       lo = __builtin_amdgcn_readfirstlane(lo);
       hi = __builtin_amdgcn_readfirstlane(hi);
       const bool one = __builtin_amdgcn_readfirstlane(none) == 0 && lo == hi;
-      int looked = -1;
-      uint64_t open = 0, full = 0;
-      // the first tile from ``kt`` on that rows see some of, all of (FULL), or not all of
-      auto find = [&](int kt, bool want_full) {
-        while (kt < tiles) {
-          if (kt / SPAN != looked) {
-            looked = kt / SPAN;
-            const int tile = looked * SPAN + wave * PER_WAVE + lane / LANES;
-            int dl = 0x7fffffff, dh = -1;
-            bool gap = false;  // a token of no document
-            for (int j = 0; j < 8; ++j) {
-              const int key = tile * KEYS + lane % LANES * 8 + j;
-              const int x = key < keys ? doc[key * a.dt] : -1;
-              gap |= x < 0;
-              dl = x < 0 ? dl : least(dl, x);
-              dh = largest(dh, x);
-            }
-            int holes = gap;
-            for (int d = 1; d < LANES; d <<= 1) {
-              dl = least(dl, __shfl_xor(dl, d, 64));
-              dh = largest(dh, __shfl_xor(dh, d, 64));
-              holes |= __shfl_xor(holes, d, 64);
-            }
-            const bool first = lane % LANES == 0;
-            const uint64_t some = __ballot(first && dh >= lo && dl <= hi);
-            const uint64_t all = __ballot(first && one && !holes && dl == lo && dh == lo && tile < whole);
-            uint64_t bits = 0;
-            for (int i = 0; i < PER_WAVE; ++i) {
-              bits |= ((some >> (i * LANES)) & 1) << i;
-              bits |= ((all >> (i * LANES)) & 1) << (i + 32);
-            }
-            __syncthreads();  // everyone is done with the span before
-            if (lane == 0) lbits[wave] = bits;
-            __syncthreads();
-            open = full = 0;
-            for (int i = 0; i < WAVES; ++i) {
-              const uint64_t w = lbits[i];
-              open |= (w & 0xffffffffu) << (i * PER_WAVE);
-              full |= (w >> 32) << (i * PER_WAVE);
-            }
-          }
-          const uint64_t these = want_full ? full : open & ~full;
-          for (; kt < tiles && kt / SPAN == looked; kt += a.splits)
-            if ((these >> (kt % SPAN)) & 1) return kt;
+      for (int span = 0; span * SPAN < tiles; ++span) {
+        const int tile = span * SPAN + wave * PER_WAVE + lane / LANES;
+        int dl = 0x7fffffff, dh = -1;
+        bool gap = false;  // a token of no document
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = tile * KEYS + lane % LANES * 8 + j;
+          const int x = key < keys ? doc[key * a.dt] : -1;
+          gap |= x < 0;
+          dl = x < 0 ? dl : least(dl, x);
+          dh = largest(dh, x);
         }
-        return tiles;
-      };
-      auto full_ones = [&](int kt) { return find(kt, true); };
-      auto other_ones = [&](int kt) { return find(kt, false); };
-      int kt = begin(full_ones(split), full_ones);
-      while (kt < tiles) {
-        const int next = arrive(kt, full_ones);
-        compute(kt, bool_constant<false>{}, bool_constant<false>{});
-        turn();
-        kt = next;
-      }
-      kt = begin(other_ones(split), other_ones);
-      while (kt < tiles) {
-        const int next = arrive(kt, other_ones);
-        if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
-        turn();
-        kt = next;
+        int holes = gap;
+        for (int d = 1; d < LANES; d <<= 1) {
+          dl = least(dl, __shfl_xor(dl, d, 64));
+          dh = largest(dh, __shfl_xor(dh, d, 64));
+          holes |= __shfl_xor(holes, d, 64);
+        }
+        const bool first = lane % LANES == 0 && tile < tiles && tile % a.splits == split;
+        const uint64_t some = __ballot(first && dh >= lo && dl <= hi);
+        const uint64_t all = __ballot(first && one && !holes && dl == lo && dh == lo && tile < whole);
+        uint64_t bits = 0;
+        for (int i = 0; i < PER_WAVE; ++i) {
+          bits |= ((some >> (i * LANES)) & 1) << i;
+          bits |= ((all >> (i * LANES)) & 1) << (i + 32);
+        }
+        __syncthreads();  // everyone is done with the span before
+        if (lane == 0) lbits[wave] = bits;
+        __syncthreads();
+        // this split's tiles of the span that rows see some of, and all of
+        uint64_t open = 0, full = 0;
+        for (int i = 0; i < WAVES; ++i) {
+          const uint64_t w = lbits[i];
+          open |= (w & 0xffffffffu) << (i * PER_WAVE);
+          full |= (w >> 32) << (i * PER_WAVE);
+        }
+        auto uniform = [](uint64_t x) {
+          return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+        };
+        full = uniform(full);
+        open = uniform(open) & ~full;
+        // those that need no mask, then those that do
+        auto take = [&](uint64_t& from, int flag) {
+          const int at = __builtin_ctzll(from);
+          from &= from - 1;
+          return (span * SPAN + at) | flag;
+        };
+        auto after = [&](int) { return full ? take(full, 0) : open ? take(open, MASK) : tiles; };
+        int kt = begin(after(0), after);
+        while (kt < tiles) {
+          const int next = arrive(kt, after);
+          compute(kt, bool_constant<false>{}, bool_constant<false>{});
+          turn();
+          kt = next;
+        }
+        while (kt & MASK) {
+          const int next = arrive(kt, after);
+          if (place(kt) * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<false>{});
+          turn();
+          kt = next;
+        }
       }
     }
   }
