@@ -17,6 +17,12 @@
 //    factor of its scores, V's multiplies the block's part of O.
 // The waves of a workgroup are joined in LDS, the items of a sequence by a second
 // kernel (cache_attention_join).
+//
+// One token, 32 heads over 8 of 128, bf16: 32 sequences of up to 8192 keys 60 us, 5.1 TB/s,
+// one of 131072 48 us, 5.6 TB/s (a read reaches 6.2; the join is 4 us of each); 12 heads of
+// 64 over 1024 keys 7.0 us, the latency of one workgroup's steps. Many rows are bound by
+// the widening of codes, which every 16 rows do again: 2 x 61 tokens, 16 heads over 2, 4096
+// keys 24 us, where tiles of 128 rows (attention.hip) take 32.
 
 namespace mlc {
 
