@@ -71,13 +71,16 @@ def _same(first, others) -> None:
 
 def _scale(scale, dim: int) -> float:
     value = plans.score_scale(scale, dim)
-    _require(0.0 < value < math.inf, f"scale: a positive number expected, got {scale}")
+    _require(2.0 ** -100 <= value <= 2.0 ** 100, f"scale: a positive number between 2^-100 and 2^100 "
+             f"expected, got {scale}")
     return value
 
 
 def _cap(cap) -> float:
     value = float(cap)
-    _require(0.0 <= value < math.inf, f"cap: a positive number, or 0 for none, expected, got {cap}")
+    # a capped score is off by 2^-21 of the cap: at 1024 by what rounding its weight to fp16 is
+    _require(value == 0.0 or 2.0 ** -20 <= value <= 2.0 ** 10, "cap: a positive number between 2^-20 and "
+             f"1024, or 0 for none, expected, got {cap}")
     return value
 
 
@@ -95,7 +98,8 @@ def _check_rotary(q, k, positions, frequencies, interleaved, magnitude) -> None:
              f"{list(frequencies.shape)}")
     _require(2 * frequencies.shape[0] <= min(q.shape[3], 2 * plans.ROTARY_PAIRS),
              f"{frequencies.shape[0]} pairs do not fit a dim of {q.shape[3]}")
-    _require(math.isfinite(magnitude), f"magnitude: a finite number expected, got {magnitude}")
+    _require(abs(magnitude) <= torch.finfo(torch.float32).max,
+             f"magnitude: a finite fp32 number expected, got {magnitude}")
     _require(q.shape[0] * q.shape[1] <= _MAX, "rotary: too many tokens for one call")
     _require(q.shape[2] + k.shape[2] <= 1 << 20, "rotary: too many heads for one call")
     _same(q, {"k": k, "positions": positions, "frequencies": frequencies})
@@ -435,7 +439,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, cap:
     values ``[batch, keys, kv_heads, dim]`` in fp16 or bf16, ``dim`` a multiple of 8 up
     to 256.
 
-    A score is ``q . k * scale`` (``1 / sqrt(dim)``); with ``cap`` it becomes
+    A score is ``q . k * scale`` (``1 / sqrt(dim)``); with ``cap`` (up to 1024) it becomes
     ``cap * tanh(score / cap)``; with ``slopes`` (float32[heads]) ``slope * |i - j|`` is
     taken off for query position ``i`` and key position ``j``. Queries stand at the last
     positions of the keys: query ``t`` at ``t + keys - queries``. What it sees:

@@ -452,8 +452,78 @@ def test_scales_of_blocks_that_a_row_does_not_see(way, bad):
 
 
 # --------------------------------------------------------------------------
+# offsets past 32 bits
+# --------------------------------------------------------------------------
+
+@gpu
+def test_rotary_past_32_bits():
+    n = 2 ** 17 + 3  # times 128 heads of 128
+    q = torch.zeros(1, n, 128, 128, dtype=HALF, device="cuda")
+    q[0, -3:] = normal(3, 128, 128)
+    k = q[:, :, :1]
+    positions = torch.arange(n, device="cuda", dtype=torch.int32)
+    f, _ = ops.rotary_frequencies(128, device="cuda")
+    got = ops.rotary(q, k, positions, f)
+    want = ops.rotary(q[:, -3:], k[:, -3:], positions[-3:], f)
+    for x, y in zip(got, want):
+        assert torch.equal(x[:, -3:], y)
+
+
+@gpu
+@pytest.mark.parametrize("documents", (False, True))
+def test_attention_past_32_bits(documents):
+    """Keys of zeros, and the last ones so large that they alone have weight: the same as
+    over them alone."""
+    n, near = 2 ** 24 + 130, 100
+    k, v = (torch.zeros(1, n, 1, 128, dtype=BF, device="cuda") for _ in range(2))
+    q, k[:, -9:], v[:, -9:] = normal(1, 2, 2, 128, dtype=BF) + 8, normal(1, 9, 1, 128, dtype=BF) + 8, 1.0
+    v[0, -9:, 0] += normal(9, 128, dtype=BF)
+    ids = torch.zeros(1, n, dtype=torch.int32, device="cuda") if documents else None
+    got = ops.attention(q, k, v, causal=True, documents=ids)
+    ref.close(got, *ref.attention(q, k[:, -near:], v[:, -near:], causal=True))
+
+
+@gpu
+def test_the_cache_past_32_bits(way):
+    """The same where a sequence's codes, and a second sequence, begin past 2^31 bytes."""
+    capacity, dim = 2 ** 24 + 128, 128
+    long, short = (ops.KeyValueCache(2, 1, n, dim, device="cuda") for n in (capacity, 256))
+    k, v = (normal(2, 3, 1, dim, dtype=BF, seed=i) + 8 for i in range(2))
+    q, at = normal(2, 3, 2, dim, dtype=BF, seed=4) + 8, ints([125, 70])
+    far = at + (capacity - 128)
+    long.append(k, v, far)
+    short.append(k, v, at)
+    for x, y in zip(parts(long), parts(short)):
+        m = y.shape[2] // 2
+        assert torch.equal(x[:, :, -m:].view(torch.uint8), y[:, :, :m].view(torch.uint8))
+    ref.close(long.attend(q, far), *ref.cache_attention(q, *parts(short), at))
+    ops.check_errors()
+
+
+# --------------------------------------------------------------------------
 # streams, graphs, devices
 # --------------------------------------------------------------------------
+
+@gpu
+def test_calls_of_several_threads():
+    import concurrent.futures
+
+    cache = filled(2, 2, 8192, 64)
+
+    def calls(i):
+        q, start = normal(2, 1 + i % 2, 4, 64, seed=i), ints([8000 - i, 17 * i])
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            outs = [cache.attend(q, start) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return q, start, outs
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        results = list(pool.map(calls, range(8)))
+    for q, start, outs in results:
+        ref.close(outs[0], *ref.cache_attention(q, *parts(cache), start))
+        assert all(torch.equal(x, outs[0]) for x in outs)
+
 
 @gpu
 def test_operators_run_on_the_current_stream_with_memory_of_their_own():
@@ -726,7 +796,8 @@ def test_what_rotary_refuses():
                       ((q.transpose(2, 3), k.transpose(2, 3), p, f), "stride"),
                       ((q, k, p, f), "ROCm GPU")):
         _refused(lambda: ops.rotary(*args), why)
-    _refused(lambda: ops.rotary(q, k, p, f, magnitude=float("inf")), "magnitude")
+    for magnitude in (float("inf"), 1e300, float("nan")):
+        _refused(lambda: ops.rotary(q, k, p, f, magnitude=magnitude), "magnitude")
 
 
 def test_what_attention_refuses():
@@ -780,6 +851,16 @@ def test_what_the_cache_refuses():
     _refused(lambda: ops.KeyValueCache(1, 1, 64, 64, block=16), "capacity")
     odd = ops.KeyValueCache(1, 1, 64, 24)
     _refused(lambda: odd.attend(host(1, 1, 1, 24), start[:1]), "multiple of 16")
+
+
+@pytest.mark.parametrize("option,value", [("scale", 1e300), ("scale", 0.0), ("scale", -1.0), ("cap", 1e-300),
+                                          ("cap", 2000.0), ("cap", -1.0), ("cap", float("nan")),
+                                          ("scale", float("inf"))])
+def test_options_that_fp32_or_the_cap_do_not_hold_are_refused(option, value):
+    q = host(1, 1, 2, 64)
+    cache, start = ops.KeyValueCache(1, 2, 64, 64), torch.zeros(1, dtype=torch.int32)
+    _refused(lambda: ops.attention(q, q, q, **{option: value}), option)
+    _refused(lambda: cache.attend(q, start, **{option: value}), option)
 
 
 def test_sizes_beyond_the_kernels_indexes_are_refused():
