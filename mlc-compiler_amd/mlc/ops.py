@@ -28,6 +28,7 @@ import torch
 
 from .codegen import hip_operators as plans
 from .codegen.hip_operators import Operand, OperatorError
+from .runtime import native, operators
 
 __all__ = ["rotary", "rotary_frequencies", "attention", "cache_append", "cache_attention",
            "KeyValueCache", "check_errors", "OperatorError"]
@@ -208,73 +209,32 @@ def _check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, 
 # direct calls
 # --------------------------------------------------------------------------
 
-#: (operator, options, each operand's type, shape, strides, device and place within
-#: 16 bytes) -> the call's launches (``runtime.operators.Call``): nothing that
-#: depends on an address or a value
-_calls: dict = {}
-#: calls kept: with ever new sizes it starts again
-_MOST_CALLS = 4096
-
-_Tensor, _grad_enabled = torch.Tensor, torch.is_grad_enabled
+_plans = operators.Calls()
 _is_compiling = torch.compiler.is_compiling
-_contiguous = torch.contiguous_format
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _signed(op: str, operands: tuple, options: tuple):
-    """The signature of a call and its operands' addresses, or ``(None, None)`` where
-    they are not plain GPU tensors outside of any tracing. An operand that asks for a
-    gradient is refused."""
-    key, at = [op, options], []
-    grad = _grad_enabled()
-    if _is_compiling():
-        return None, None
-    for x in operands:
-        if x is None:
-            key.append(None)
-            at.append(0)
-            continue
-        if grad and x.requires_grad:
-            raise OperatorError("an operand asks for a gradient, and the operators of mlc.ops are "
-                                "for inference: call them under torch.no_grad()")
-        if type(x) is not _Tensor:
-            return None, None
-        device = x.get_device()
-        if device < 0:
-            return None, None
-        p = x.data_ptr()
-        at.append(p)
-        key += (x.dtype, x.shape, x.stride(), device, p & 15)
-    return tuple(key), at
+def _operand(x) -> Operand | None:
+    return None if x is None else Operand(tuple(x.shape), x.stride(), x.dtype,
+                                          aligned=x.data_ptr() % 16 == 0)
 
 
-def _operand(x, p: int) -> Operand | None:
-    return None if x is None else Operand(tuple(x.shape), x.stride(), x.dtype, aligned=p % 16 == 0)
-
-
-def _call_of(key, op: str, operands: tuple, at: list, options: tuple):
+def _add(signature: bytes, op: str, operands: tuple, options: tuple, results: int) -> None:
     """The launches of a call of a new signature, checked."""
-    from .runtime.operators import Call
-
     check, plan, names = _OPERATORS[op]
     check(*operands, *options)
-    for name, x, p in zip(names, operands, at):
+    for name, x in zip(names, operands):
         if name.endswith("cache") or name.endswith("_scale"):
-            _require(p % 16 == 0, f"{name}: not on 16 bytes")
-    device = operands[0].get_device()
-    made = plan(*[_operand(x, p) for x, p in zip(operands, at)], *options)
-    call = Call(made, names, device)
-    if len(_calls) >= _MOST_CALLS:
-        _calls.clear()
-    _calls[key] = call
-    return call
+            _require(x.data_ptr() % 16 == 0, f"{name}: not on 16 bytes")
+    made = plan(*map(_operand, operands), *options)
+    changed = len(_CACHE) if op == "cache_append" else 0
+    _plans.add(signature, made, names, changed, results, operands[0].get_device())
 
 
 def check_errors() -> None:
     """Wait for the device and raise ``ExecutionError`` if an operator called so far
     met an invalid ``start`` or ``count``. Without it the next call of an operator
     that can meet one raises, once the call that met it is done."""
-    from .runtime import operators
-
     operators.check_errors()
 
 
@@ -301,22 +261,35 @@ _OPERATORS = {
 }
 
 
-def _now(op: str, operands: tuple, options: tuple, like: tuple):
-    """The call, with results like those operands, or None where ``_signed`` is."""
-    key, at = _signed(op, operands, options)
-    if key is None:
+_NUMBERS = {op: i for i, op in enumerate(_OPERATORS)}
+
+
+def _now(op: str, operands: tuple, options: tuple, results: int) -> tuple | None:
+    """The call, with so many results like the first operands, or None where they are not
+    plain GPU tensors outside of any tracing. An operand that asks for a gradient is refused."""
+    if _is_compiling():
         return None
-    if op == "cache_append" and (at[0] == at[1] or at[2] == at[3]) and operands[0].numel():
-        raise OperatorError("cache_append: keys and values share a cache or its scales")
-    call = _calls.get(key) or _call_of(key, op, operands, at, options)
-    if not like:
-        call.run(at, None)
-        return ()
-    out = [torch.empty_like(x, memory_format=_contiguous) for x in like]
-    for x in out:
-        at.append(x.data_ptr())
-    call.run(at, out[0])
-    return out
+    run, poll = native.load_calls().call, True
+    while True:
+        out = run(_NUMBERS[op], operands, options, results, _stream_of, poll)
+        if out is None or type(out) is tuple:
+            return out
+        if out is False:
+            raise OperatorError("an operand asks for a gradient, and the operators of mlc.ops are "
+                                "for inference: call them under torch.no_grad()")
+        if out is True:
+            if not torch.cuda.is_current_stream_capturing():
+                operators.raise_pending(operators.device_modules(operands[0].get_device()))
+            poll = False
+        elif out is NotImplemented:
+            with torch.cuda.device(operands[0].get_device()):
+                return _now(op, operands, options, results)
+        elif out is Ellipsis:
+            raise OperatorError(f"{op}: keys and values share a cache or its scales")
+        elif type(out) is bytes:
+            _add(out, op, operands, options, results)
+        else:
+            native.check(out, f"a launch of {op}")
 
 
 # --------------------------------------------------------------------------
@@ -346,12 +319,14 @@ def _implement(op: str, split, results: int) -> None:
 
     def gpu(*args):
         operands, options = split(*args)
-        # what the dispatcher hands over may be a parameter or another subclass
-        plain = tuple(x if x is None or type(x) is _Tensor else x.detach().as_subclass(_Tensor)
-                      for x in operands)
+        # what the dispatcher hands over may be a subclass
+        plain = tuple(x if x is None or type(x) is torch.Tensor
+                      else x.detach().as_subclass(torch.Tensor) for x in operands)
         with torch.no_grad():
-            out = _now(op, plain, options, plain[:results])
-        _require(out is not None, f"{op}: not on one GPU")
+            out = _now(op, plain, options, results)
+        if out is None:
+            check(*operands, *options)
+        _require(out is not None, f"{op}: not plain tensors of one GPU")
         return tuple(out) if results > 1 else out[0] if results else None
 
     def fake(*args):
@@ -396,7 +371,7 @@ def rotary(q, k, positions, frequencies, *, interleaved: bool = False, magnitude
     ``(2 i, 2 i + 1)`` if ``interleaved``. ``magnitude`` multiplies what is turned.
     """
     interleaved, magnitude = bool(interleaved), float(magnitude)
-    out = _now("rotary", (q, k, positions, frequencies), (interleaved, magnitude), (q, k))
+    out = _now("rotary", (q, k, positions, frequencies), (interleaved, magnitude), 2)
     if out is not None:
         return out[0], out[1]
     return torch.ops.mlc.rotary(q, k, positions, frequencies, interleaved, magnitude)
@@ -453,7 +428,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, cap:
     infinities included.
     """
     scale, causal, cap = None if scale is None else float(scale), bool(causal), float(cap)
-    out = _now("attention", (q, k, v, slopes, documents, prefix), (scale, causal, cap), (q,))
+    out = _now("attention", (q, k, v, slopes, documents, prefix), (scale, causal, cap), 1)
     if out is not None:
         return out[0]
     return torch.ops.mlc.attention(q, k, v, scale, causal, cap, slopes, documents, prefix)
@@ -475,7 +450,7 @@ def cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count=None) ->
     A sequence whose ``start`` and ``count`` do not lie within the cache is left alone,
     and ``ExecutionError`` is raised by a later call or :func:`check_errors`.
     """
-    if _now("cache_append", (k_cache, v_cache, k_scale, v_scale, k, v, start, count), (), ()) is not None:
+    if _now("cache_append", (k_cache, v_cache, k_scale, v_scale, k, v, start, count), (), 0) is not None:
         return None
     return torch.ops.mlc.cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count)
 
@@ -491,7 +466,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count=None, *,
     """
     scale, cap = None if scale is None else float(scale), float(cap)
     out = _now("cache_attention", (q, k_cache, v_cache, k_scale, v_scale, start, count, slopes),
-               (scale, cap), (q,))
+               (scale, cap), 1)
     if out is not None:
         return out[0]
     return torch.ops.mlc.cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count,

@@ -4,6 +4,8 @@
   code-object modules, the arena slab, launch plans, hipGraph capture and
   replay, hipEvent timing), built from ``csrc/mlc_hip.cpp`` with ``hipcc`` and
   loaded with ``ctypes``.
+* ``_calls.so`` -- direct calls of the operators of ``mlc.ops`` as a CPython module
+  (``csrc/mlc_calls.cpp``), built with the host compiler against torch's headers.
 * gfx950 code objects of generated kernel modules, compiled with
   ``hipcc --genco`` and kept in a content-addressed cache, keyed by the
   source, the device template header, the compile flags and the compiler
@@ -24,6 +26,7 @@ import os
 import pathlib
 import shutil
 import subprocess
+import sysconfig
 import threading
 
 PKG = pathlib.Path(__file__).resolve().parents[1]          # .../mlc
@@ -33,6 +36,7 @@ CSRC = ROOT / "csrc"
 INCLUDE = REPO / "include"
 TEMPLATES = PKG / "codegen" / "templates"
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libmlc_hip.so"
+CALLS_PATH = LIB_PATH.with_name("_calls.so")
 
 ARCH = "gfx950"
 #: flags for every piece of HIP code built here. Packed-fp32 instructions are
@@ -87,6 +91,36 @@ def build_library(force: bool = True) -> pathlib.Path:
           str(src), "-o", str(tmp)])
     tmp.replace(LIB_PATH)
     return LIB_PATH
+
+
+def build_calls(force: bool = True) -> pathlib.Path:
+    """Compile ``_calls.so`` in-tree, for this interpreter and this torch."""
+    import torch
+
+    src = CSRC / "mlc_calls.cpp"
+    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime >= src.stat().st_mtime:
+        return CALLS_PATH
+    home = pathlib.Path(torch.__file__).parent
+    tmp = CALLS_PATH.with_name(CALLS_PATH.name + f".tmp{os.getpid()}")
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f"-I{home / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp),
+          f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"])
+    tmp.replace(CALLS_PATH)
+    return CALLS_PATH
+
+
+@functools.lru_cache(maxsize=None)
+def load_calls():
+    """The module of direct calls. Raises if it was not built."""
+    if not CALLS_PATH.exists():
+        raise NativeError(f"{CALLS_PATH} is missing: build it first (python -c "
+                          "'import __graft_entry__ as g; g.build()')")
+    import torch  # noqa: F401  (whose libraries it links)
+    from . import _calls
+
+    return _calls
 
 
 _c_int, _c_u32, _c_size, _vp = ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t, ctypes.c_void_p

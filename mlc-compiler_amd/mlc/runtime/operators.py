@@ -1,16 +1,16 @@
 """Direct calls of the operators of ``mlc.ops``: their code objects, loaded once a
-device, and their launches on torch's current stream of the operands' device.
+device, and the table of their launches.
 
 A call's plan follows from shapes, strides, types and options alone, so it is kept
-under them; addresses are put in at every call. Memory that a call's launches share
-is allocated for that call through torch, on its stream: calls on several streams
-and calls captured into several graphs have memory of their own.
+under them; ``_calls.call`` (``csrc/mlc_calls.cpp``) puts addresses in at every call and
+launches on torch's current stream. Memory that a call's launches share is allocated
+for that call through torch, on its stream: calls on several streams and calls captured
+into several graphs have memory of their own.
 """
 
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
@@ -60,6 +60,10 @@ class OperatorModules:
         self._functions[launch.symbol] = fn.value
         return fn.value
 
+    @property
+    def context(self) -> int:
+        return self._ctx.value
+
     def error_word(self) -> int:
         if self._error_word is None:
             word = ctypes.c_void_p()
@@ -95,49 +99,36 @@ def device_modules(index: int) -> OperatorModules:
     return found
 
 
-class Call:
-    """The launches of one signature on one device: functions loaded, arguments laid
-    out but for the addresses, which ``run`` gets in the order of the operands and
-    results."""
+#: calls kept: with ever new sizes it starts again
+MOST_CALLS = 4096
 
-    def __init__(self, plan: Plan, operands: tuple, device: int) -> None:
-        self.plan = plan
-        self.modules = device_modules(device)
-        self.device, self.workspace = device, plan.workspace
-        self.flags = any("error" in x.pointers for x in plan.launches)
-        error = self.modules.error_word() if self.flags else 0
-        # where a launch's pointers are in ``at`` with the workspace and constants behind it
-        names = [*operands, *sorted({p for x in plan.launches for p in x.pointers
-                                     if p is not None and p.startswith("out")})]
-        self.tail = (0, error)
-        place = {n: i for i, n in enumerate((*names, "workspace", None, "error"))}
-        self.launches = []
+
+class Calls(dict):
+    """Signature (bytes) -> the ``Plan`` of its calls, which ``_calls.call`` launches."""
+
+    def add(self, signature: bytes, plan: Plan, operands: tuple, changed: int, results: int,
+            device: int) -> None:
+        """``operands``: their names, of which the first ``changed`` change. Functions are
+        loaded, arguments laid out but for the addresses: of the operands, the results, the
+        shared memory, nothing and the invalid-input word."""
+        modules = device_modules(device)
+        flags = any("error" in x.pointers for x in plan.launches)
+        names = (*operands, *(f"out{i}" for i in range(results)), "workspace", None, "error")
+        place = {n: i for i, n in enumerate(names)}
         with torch.cuda.device(device):
-            for x in plan.launches:
-                layout = struct.Struct(f"<{len(x.pointers)}Q{len(x.tail)}s")
-                self.launches.append((self.modules.function(x), x.grid, x.block, layout.pack,
-                                      tuple(place[p] for p in x.pointers), x.tail, layout.size))
-        self._launch = self.modules.lib.mlc_launch
+            launches = tuple((modules.function(x), x.grid, x.block, bytes(place[p] for p in x.pointers),
+                              x.tail) for x in plan.launches)
+        address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+        if len(self) >= MOST_CALLS:
+            self.clear()
+        native.load_calls().add(signature, len(names), changed, address(modules.lib.mlc_launch), launches,
+                                plan.workspace, address(modules.lib.mlc_error_poll) if flags else 0,
+                                modules.context if flags else 0, modules.error_word() if flags else 0)
+        self[signature] = plan
 
-    def run(self, at: list, like) -> None:
-        """Launch on torch's current stream of the device. ``like``: a tensor on it."""
-        if _current_device() != self.device:
-            with torch.cuda.device(self.device):
-                return self.run(at, like)
-        if self.flags and self.modules.pending() and not torch.cuda.is_current_stream_capturing():
-            raise_pending(self.modules)
-        space = None
-        if self.workspace:
-            space = like.new_empty(self.workspace, dtype=torch.uint8)
-            at.append(space.data_ptr())
-        else:
-            at.append(0)
-        at += self.tail
-        stream = _current_stream(self.device)
-        for fn, grid, block, pack, place, tail, size in self.launches:
-            rc = self._launch(fn, grid, block, 0, pack(*[at[i] for i in place], tail), size, stream)
-            if rc:
-                native.check(rc, "mlc_launch")
+    def clear(self) -> None:
+        native.load_calls().clear()
+        super().clear()
 
 
 def raise_pending(modules: OperatorModules) -> None:
@@ -154,11 +145,3 @@ def check_errors() -> None:
         torch.cuda.synchronize(index)
         if modules.pending():
             raise_pending(modules)
-
-
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
-
-
-def _current_stream(device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device)

@@ -353,7 +353,7 @@ def test_cache_attention_of_many_rows(monkeypatch, dtype, batch, tokens, heads, 
 
     monkeypatch.setattr(hip_operators, "MANY_PRODUCTS", 0)
     monkeypatch.setattr(hip_operators, "MANY_ROWS", 1)
-    ops._calls.clear()
+    ops._plans.clear()
     try:
         cache = filled(batch, kv, capacity, dim, block, seed=2)
         q = normal(batch, tokens, heads, dim, dtype=dtype, seed=6)
@@ -371,10 +371,10 @@ def test_cache_attention_of_many_rows(monkeypatch, dtype, batch, tokens, heads, 
         codes[0, 0, end - 1, 3] = 255
         ref.close(cache.attend(q, start, count, **options),
                   *ref.cache_attention(q, *parts(cache), start, count, **options))
-        assert any("attention_" in x.symbol and "codes" in x.symbol for c in ops._calls.values()
-                   for x in c.plan.launches)
+        assert any("attention_" in x.symbol and "codes" in x.symbol for plan in ops._plans.values()
+                   for x in plan.launches)
     finally:
-        ops._calls.clear()
+        ops._plans.clear()
 
 
 @gpu
@@ -421,9 +421,9 @@ def way(request, monkeypatch):
     if request.param == "tiles":
         monkeypatch.setattr(hip_operators, "MANY_PRODUCTS", 0)
         monkeypatch.setattr(hip_operators, "MANY_ROWS", 1)
-    ops._calls.clear()
+    ops._plans.clear()
     yield request.param
-    ops._calls.clear()
+    ops._plans.clear()
 
 
 @gpu
@@ -503,6 +503,31 @@ def test_the_cache_past_32_bits(way):
 # --------------------------------------------------------------------------
 # streams, graphs, devices
 # --------------------------------------------------------------------------
+
+@gpu
+def test_operands_that_are_not_plain_tensors():
+    """Parameters are; a subclass goes through torch's dispatcher, where a mode sees the call,
+    and so does a batched tensor."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Subclass(torch.Tensor):
+        pass
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+    q, k, v = _heads(1, 5, 70, 2, 1, 64, HALF)
+    want = ops.attention(q, k, v)
+    assert torch.equal(ops.attention(q, torch.nn.Parameter(k, requires_grad=False), v), want)
+    assert torch.equal(ops.attention(q, k.as_subclass(Subclass), v), want)
+    with Log():
+        assert torch.equal(ops.attention(q, k, v), want)
+    assert "mlc.attention.default" in seen
+    assert torch.equal(torch.vmap(lambda x: ops.attention(x, k, v))(q[None])[0], want)
+
 
 @gpu
 def test_calls_of_several_threads():
@@ -879,6 +904,20 @@ def test_a_cache_keeps_its_types_when_a_model_changes_its_own():
     assert m[0].weight.dtype == HALF
     assert m.cache.keys.dtype == E4M3 and m.cache.key_scales.dtype == FULL
     assert m.to("meta").cache.values.device.type == "meta"
+
+
+def test_what_the_module_of_calls_refuses():
+    from mlc.runtime import native
+
+    calls, x = native.load_calls(), torch.ones(2)
+    for args in ((0, (3,), (), 1, None, True), (0, (), (), 0, None, True), (0, (x,), (), 2, None, True),
+                 (0, (x,) * 17, (), 1, None, True), (0, [x], (), 1, None, True), (0, (x,), ()), (0, (x, "k"), (), 1, None, 1)):
+        with pytest.raises(TypeError):
+            calls.call(*args)
+    assert calls.call(0, (x,), (), 1, None, True) is None
+    for launch in ((7, 1, 2, b"\x00\x05", b"tail"), (7, 1, 2, b"\x00", b"x" * 2000), (0, 1, 2, b"\x00", b"")):
+        with pytest.raises(ValueError, match="fit"):
+            calls.add(b"not a signature", 5, 0, 1, (launch,), 0, 0, 0, 0)
 
 
 def test_operands_that_ask_for_gradients_are_refused():
