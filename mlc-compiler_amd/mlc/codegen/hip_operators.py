@@ -157,10 +157,12 @@ def _factors(scale: float, cap: float) -> tuple[float, float]:
     return (scale / cap, cap * LOG2E) if cap else (scale * LOG2E, 0.0)
 
 
-def attention_kernel(dtype, dp: int, waves: int, source: str, general: bool) -> tuple[str, str]:
-    name = f"attention_{SHORT[dtype]}_{dp}_w{waves}_{source.lower()}{'_general' if general else ''}"
-    return (f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {waves}, {source}, "
-            f"{str(general).lower()})"), name
+def attention_kernel(dtype, dp: int, waves: int, source: str, scores: str, apart: bool
+                     ) -> tuple[str, str]:
+    name = (f"attention_{SHORT[dtype]}_{dp}_w{waves}_{source.lower()}"
+            f"_{scores.lower()}{'_apart' if apart else ''}")
+    return (f"ATTENTION({name}, {NAMES[dtype]}, {dp}, {waves}, {source}, {scores}, "
+            f"{str(apart).lower()})"), name
 
 
 def join_kernel(op: str, dtype, waves: int) -> tuple[str, str]:
@@ -176,21 +178,37 @@ def _join(op: str, dtype, parts: int, rows: int, pointers: tuple, tail: bytes) -
     return Launch(kernel, op, name, _grid(rows, 64 * waves, op), 64 * waves, pointers, tail)
 
 
-def attention_split(rows: int, pairs: int, key_tiles: int, tile_us: float, dim: int
-                    ) -> tuple[int, int]:
-    """Waves of a workgroup, each with 32 rows, and splits of the keys.
+def attention_split(rows: int, pairs: int, keys: int, dim: int, teams: tuple, apart: tuple | None
+                    ) -> tuple[bool, int, int]:
+    """Whether the waves of a workgroup take keys apart, how many waves it has, and splits
+    of the keys, by what the ways cost in us. ``teams`` and ``apart``: keys of a tile and the
+    time of one, and for the second the waves.
 
-    Splits fill the device where rows are few. What they cost is a second launch and
-    parts of O in fp32, written and read: 4 us and 8 bytes a value at 3 TB/s. What they
-    save is tiles of keys one behind the other, ``tile_us`` each."""
-    waves = 4 if rows > 64 else 2 if rows > 32 else 1
-    blocks = _ceil(rows, 32 * waves) * pairs
+    Waves that share tiles have 32 rows each, and two such workgroups fit a unit; waves
+    apart have the same 32 rows, a quarter of the tiles one behind the other, four times the
+    workgroups, and one fits a unit. 1000 tokens, 12 heads of 64: shared 19.3, apart 12.3; 3 x
+    1024, 4 heads of 128 with a bias 34.9, 24.0; 4096, 8 heads of 128 73, 85; 4 x 300, 32 heads
+    over 8 of 128 16, 32.
+
+    Splits fill the device where there are few workgroups. What they cost is a second
+    launch and parts of O in fp32, written and read: 4 us and 8 bytes a value at 3 TB/s."""
     values = rows * pairs * (dim + 4)
+    best = None
 
-    def cost(n: int) -> float:
-        return _ceil(key_tiles, n) * tile_us + (4 + n * values * 8 / 3e6 if n > 1 else 0)
+    def consider(is_apart: bool, waves: int, blocks: int, room: int, first: float, tiles: int, us: float):
+        nonlocal best
+        for n in range(1, max(1, min(room // blocks, tiles)) + 1):
+            cost = max(1.0, blocks * n / room) * (first + _ceil(tiles, n) * us)
+            cost += 4 + n * values * 8 / 3e6 if n > 1 else 0
+            if best is None or cost < best[0]:
+                best = cost, (is_apart, waves, n)
 
-    return waves, min(range(1, max(1, min(2 * UNITS // blocks, key_tiles)) + 1), key=cost)
+    waves = 4 if rows > 64 else 2 if rows > 32 else 1
+    consider(False, waves, _ceil(rows, 32 * waves) * pairs, 2 * UNITS, 5, _ceil(keys, teams[0]), teams[1])
+    if apart:
+        n, us, waves = apart
+        consider(True, waves, _ceil(rows, 32) * pairs, UNITS, 5.5, _ceil(keys, n * waves), us)
+    return best[1]
 
 
 def _strides(x: Operand | None, n: int) -> tuple:
@@ -212,12 +230,16 @@ def _attention(source: str, q: Operand, k: Operand, v: Operand, pairs: tuple, ke
     *scales, start, count, shift = cache
     codes = source == "CODES"
     dp, group = _padded(dim, CACHED_DIMS if codes else ATTENTION_DIMS), heads // kv_heads
-    rows, tiles_of_keys = queries * group, _ceil(keys, 32 if codes or dp == 256 else 64)
-    # measured: 1 us for 64 keys of 64 values, 1.8 of 128; twice that through registers
-    tile_us = (0.2 + dp / 80) * (0.5 if tiles_of_keys > _ceil(keys, 64) else 1) * (1 if source == "DIRECT" else 2)
-    waves, splits = attention_split(rows, batch * kv_heads, tiles_of_keys, tile_us, dim)
-    tiles = _ceil(rows, 32 * waves)
-    general = bool(factors[1]) or slopes is not None or documents is not None
+    rows = queries * group
+    # measured: 1 us for 64 keys of 64 values, 1.8 of 128; twice that through registers.
+    # Waves apart take 32 keys of more than 64 values at a time, in 0.6 of it.
+    us = (0.2 + dp / 80) * (1 if source == "DIRECT" else 2)
+    teams = (32, us / 2) if codes or dp == 256 else (64, us)
+    alone = (64, us, 4) if dp == 64 else (32, us * 0.6, 4) if dp < 256 else (32, us / 2, 2)
+    apart, waves, splits = attention_split(rows, batch * kv_heads, keys, dim, teams, None if codes else alone)
+    tiles = _ceil(rows, 32 if apart else 32 * waves)
+    scores = ("DOCUMENTS" if documents is not None else
+              "BIASED" if factors[1] or slopes is not None else "PLAIN")
     operands = {"q": q, "k": k, "v": v, "slopes": slopes, "documents": documents, "prefix": prefix,
                 "k_scale": scales[0], "v_scale": scales[1], "start": start, "count": count}
     names = {"k": "k_cache", "v": "v_cache"} if codes else {}
@@ -229,7 +251,7 @@ def _attention(source: str, q: Operand, k: Operand, v: Operand, pairs: tuple, ke
                        *_strides(prefix, 1), *_strides(start, 1), *_strides(count, 1),
                        batch, queries, keys, kv_heads, group, dim, causal, tiles, splits, shift,
                        *factors)
-    kernel, name = attention_kernel(q.dtype, dp, waves, source, general)
+    kernel, name = attention_kernel(q.dtype, dp, waves, source, scores, apart)
     grid = _grid(tiles * batch * kv_heads * splits, 64 * waves, "attention")
     launch = Launch(kernel, "attention", name, grid, 64 * waves, pointers, tail)
     if splits == 1:
@@ -379,9 +401,13 @@ def all_kernels() -> list[tuple[str, str]]:
         out += [("cache_append", append_kernel(dtype, a, n, w)[0]) for a in (16, dtype.itemsize)
                 for n, w in ((1, 1), (1, 4), (2, 4), (4, 4), (8, 4), (16, 4))]
     for dtype in (torch.float16, torch.bfloat16):
-        out += [("attention", attention_kernel(dtype, dp, w, source, g)[0]) for dp in ATTENTION_DIMS
-                for w in (1, 2, 4) for source in ("COPIED", "DIRECT", "CODES") for g in (False, True)
-                if source != "CODES" or (dp in CACHED_DIMS and w == 4)]
+        for source in ("COPIED", "DIRECT", "CODES"):
+            for scores in ("PLAIN", "BIASED", "DOCUMENTS")[:2 if source == "CODES" else 3]:
+                ways = [(dp, 4, False) for dp in CACHED_DIMS] if source == "CODES" else \
+                    [(dp, w, False) for dp in ATTENTION_DIMS for w in (1, 2, 4)] + \
+                    [(dp, 4 if dp < 256 else 2, True) for dp in ATTENTION_DIMS]
+                out += [("attention", attention_kernel(dtype, dp, w, source, scores, apart)[0])
+                        for dp, w, apart in ways]
         out += [("cache_attention", cached_kernel(dtype, dp, step, w, g)[0])
                 for dp in CACHED_DIMS for w in (4, 8) if w < 8 or dp < 256 for step in (32, 64)
                 for g in (False, True)]

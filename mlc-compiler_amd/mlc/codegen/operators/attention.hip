@@ -5,7 +5,8 @@
 // Rows are (token, head of a group) pairs: all heads that share keys and values
 // go through one workgroup, which so reads them once. A workgroup of 4 waves has
 // 128 rows, a wave 32 of them, one row in lanes c and c + 32. Keys pass in tiles
-// of 64 through LDS.
+// of 64 through LDS. Where there are few rows its waves have the same 32 instead, and a
+// quarter of the tiles each (APART).
 //  * S^T = K Q^T on 32x32x16 products: lane (c, h) ends with row c's scores. The
 //    rows of K are taken in the order that makes them tokens 16 i + 8 h .. + 7,
 //    the B operand of O^T = V^T P^T: probabilities never leave their lane.
@@ -15,9 +16,9 @@
 // Long rows are bound by the softmax's vector work beside the products, and by the clock,
 // which falls under them: 8192 tokens, 32 heads over 8 of 128, bf16, causal 552 us, 995
 // TFLOP/s, without a mask 1045 (a library's product of 8192^3 reaches 1214); a cap adds two
-// transcendentals to a score's one, 680 us, 805 TFLOP/s. Short ones are bound by a chain of
+// transcendentals to a score's one, 666 us, 825 TFLOP/s. Short ones are bound by a chain of
 // loads and products that few waves hide: 32 x 512 tokens, 12 heads of 64, fp16, causal 32
-// us, with a bias and prefixes 40 (19 to move the bytes); 128 tokens, 12 heads 6.6.
+// us, with a bias and prefixes 40 (19 to move the bytes); 128 tokens, 12 heads 5.6.
 //
 // Tried and slower: 8 waves a workgroup and 4 buffers (916 against 960 TFLOP/s then), the
 // scores of a tile before the softmax of the one before (registers spill), the sums as one
@@ -54,7 +55,9 @@ struct AttentionArgs {
 // Keys of a tile: with heads of 256, rows of 64 scores would not fit the registers beside O
 // and Q, and O would move between vector and accumulation registers twice a tile (2048 causal
 // tokens, 4 x 8 heads of 256: 136 us; 32 keys 116). A tile of the cache has one scale.
-template <int DP, int SOURCE> constexpr int tile_keys = DP == 256 || SOURCE == 2 ? 32 : 64;
+// Where waves take keys apart, four tiles of 32 rows of 128 values have room in LDS.
+template <int DP, int SOURCE, bool APART>
+constexpr int tile_keys = DP == 256 || SOURCE == 2 || (APART && DP > 64) ? 32 : 64;
 
 template <class T> struct vec8;
 template <> struct vec8<f16> {
@@ -123,24 +126,35 @@ __device__ __forceinline__ void to_lds(const void* g, void* lds) {
 //    into the factor of its scores, one of V multiplies its keys' part of O.
 enum { COPIED, DIRECT, CODES };
 
-template <class T, int DP, int WAVES, int SOURCE, bool GENERAL>
+// APART: the waves of a workgroup have the same 32 rows and take tiles of keys in turn, each
+// with LDS of its own and no barrier until their parts of O are joined there. Few workgroups
+// wait for a row's tiles one behind the other: 128 tokens, 12 heads of 64 5.6 us for 7.2 in
+// workgroups of 128 rows, 1000 tokens 12.3 for 19.3.
+// SCORES that are more than products: PLAIN none, BIASED a cap or a bias, DOCUMENTS both and
+// documents. Apart, since what a kernel does not use still takes its registers: 32 x 512 tokens,
+// 12 heads of 64 with a bias 45 us in a kernel that looks for documents too, 39 without.
+enum { PLAIN, BIASED, DOCUMENTS };
+template <class T, int DP, int WAVES, int SOURCE, int SCORES, bool APART>
 __device__ __forceinline__ void attention(const AttentionArgs& a) {
   typedef typename vec8<T>::type v8;
   typedef typename choose<SOURCE == CODES, f16, T>::type PT;  // of P and V
   typedef typename vec8<PT>::type p8;
-  constexpr bool IS_DIRECT = SOURCE == DIRECT, CACHE = SOURCE == CODES, DOCS = GENERAL && !CACHE;
+  constexpr bool IS_DIRECT = SOURCE == DIRECT, CACHE = SOURCE == CODES;
+  constexpr bool GENERAL = SCORES != PLAIN, DOCS = SCORES == DOCUMENTS;
   constexpr int PC = DP == 64 ? 8 : DP <= 128 ? 16 : 32;  // 16-byte slots of an LDS row
   constexpr int CH = DP / 8;                               // of which hold values
-  constexpr int THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+  constexpr int TEAMS = APART ? WAVES : 1, TEAM = WAVES / TEAMS;  // waves that share tiles of keys
+  constexpr int THREADS = 64 * TEAM, ROWS = 32 * TEAM;
   constexpr int BUFFERS = 2;
   constexpr float V_FACTOR = CACHE ? SCALE_ROOM : 1.0f;
-  constexpr int KEYS = tile_keys<DP, SOURCE>, U = KEYS / 32;
+  constexpr int KEYS = tile_keys<DP, SOURCE, APART>, U = KEYS / 32;
   constexpr int EACH = CACHE ? 16 : 8, ROW = DP / EACH;    // values of a piece, pieces of a row
   constexpr int N = (KEYS * ROW + THREADS - 1) / THREADS;  // pieces of a tile for a thread
   constexpr int NL = KEYS * PC / THREADS;                  // slots of a tile for a thread
   static_assert(!IS_DIRECT || KEYS * PC % THREADS == 0, "staging");
   constexpr int TILE = KEYS * PC * 16;                 // bytes of LDS, a power of two
-  __shared__ __attribute__((aligned(BUFFERS * TILE))) char lds[2 * BUFFERS * TILE];  // keys, then values
+  // keys, then values
+  __shared__ __attribute__((aligned(BUFFERS * TILE))) char all_lds[TEAMS][2 * BUFFERS * TILE];
   __shared__ __attribute__((aligned(16))) int ldoc[DOCS ? BUFFERS : 1][DOCS ? WAVES : 1][64];
   __shared__ uint64_t lbits[WAVES];
   __shared__ int lrange[3][WAVES];
@@ -148,6 +162,17 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 31, h = lane >> 5;
+  const int team = APART ? wave : 0, mate = APART ? 0 : wave;  // and which of its waves
+  const int thread = APART ? lane : (int)threadIdx.x;          // of the team
+  char* const lds = all_lds[team];
+  auto sync = [] {
+    if constexpr (APART) {
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
   const int rows = a.queries * a.group;
   // Workgroups go to the 8 XCDs in turn: a unit (batch, key head, split of the keys) stays on
   // one where there are enough of them, and long tiles come first
@@ -161,7 +186,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     unit = blockIdx.x % units;
     tile = a.tiles - 1 - blockIdx.x / units;
   }
-  const int pair = unit / a.splits, split = unit % a.splits;
+  const int pair = unit / a.splits, split = unit % a.splits * TEAMS + team, splits = a.splits * TEAMS;
   const int b = pair / a.kv_heads, hk = pair % a.kv_heads;
 
   int keys = a.keys, shift = a.keys - a.queries;  // position of query 0
@@ -186,7 +211,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
     return lim;
   };
-  const int first_row = tile * ROWS, wave_row = first_row + wave * 32;
+  const int first_row = tile * ROWS, wave_row = first_row + mate * 32;
   const int row = wave_row + c;
   const int r = row < rows ? row : rows - 1;  // rows past the end repeat the last, and are not stored
   const int t = r / a.group, head = hk * a.group + r % a.group;
@@ -224,10 +249,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   // one thread are STEP apart, and the swizzle comes again after 16 rows
   constexpr int STEP = THREADS / PC, KINDS = STEP >= 16 || !IS_DIRECT ? 1 : 16 / STEP < NL ? 16 / STEP : NL;
   uint32_t kv[KINDS], vv[KINDS];
-  auto chunk_of = [&](int kr) { return (slot<PC>(kr, threadIdx.x % PC) % PC) % CH; };
+  auto chunk_of = [&](int kr) { return (slot<PC>(kr, thread % PC) % PC) % CH; };
 #pragma unroll
   for (int i = 0; i < KINDS; ++i) {
-    const int kr = threadIdx.x / PC, chunk = chunk_of(kr + i * STEP);
+    const int kr = thread / PC, chunk = chunk_of(kr + i * STEP);
     kv[i] = (kr * (uint32_t)a.kt + chunk * 8) * (uint32_t)sizeof(T);
     vv[i] = (kr * (uint32_t)a.vt + chunk * 8) * (uint32_t)sizeof(T);
   }
@@ -240,7 +265,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   auto load = [&](int kt, int into) {
     const int base = place(kt) * KEYS;
     if constexpr (IS_DIRECT) {
-      char* const to = lds + into * TILE + wave * 1024;
+      char* const to = lds + into * TILE + mate * 1024;
       if (base + KEYS <= keys) {
         const char* const kb = reinterpret_cast<const char*>(kp + base * a.kt);
         const char* const vb = reinterpret_cast<const char*>(vp + base * a.vt);
@@ -252,7 +277,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       } else {  // past the last key the last one again
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-          const int kr = threadIdx.x / PC + n * STEP, key = base + kr < keys ? base + kr : keys - 1;
+          const int kr = thread / PC + n * STEP, key = base + kr < keys ? base + kr : keys - 1;
           const int chunk = chunk_of(kr);
           to_lds(kp + key * a.kt + chunk * 8, to + n * THREADS * 16);
           to_lds(vp + key * a.vt + chunk * 8, to + BUFFERS * TILE + n * THREADS * 16);
@@ -261,7 +286,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int i = threadIdx.x + n * THREADS, key = base + i / ROW, d = i % ROW * EACH;
+        const int i = thread + n * THREADS, key = base + i / ROW, d = i % ROW * EACH;
         rk[n] = rv[n] = uint4v{0, 0, 0, 0};
         if (key < keys && d < a.dim && i < KEYS * ROW) {
           if constexpr (CACHE) {
@@ -312,7 +337,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     uint4v* const lv = reinterpret_cast<uint4v*>(lds + (BUFFERS + into) * TILE);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int i = threadIdx.x + n * THREADS, r0 = i / ROW, c0 = i % ROW;
+      const int i = thread + n * THREADS, r0 = i / ROW, c0 = i % ROW;
       if (KEYS * ROW % THREADS != 0 && i >= KEYS * ROW) continue;
       if constexpr (CACHE) {
 #pragma unroll
@@ -348,13 +373,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   auto arrive = [&](int kt, auto after) {
     if constexpr (IS_DIRECT) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-      __builtin_amdgcn_s_barrier();
+      if constexpr (APART) __builtin_amdgcn_wave_barrier();
+      else __builtin_amdgcn_s_barrier();
       asm volatile("" : : : "memory");
       const int next = after(kt);
       if (place(next) < tiles) load(next, it ^ 1);
       return next;
     } else {
-      __syncthreads();
+      sync();
       const int next = behind;
       if (place(next) < tiles) {
         store(it ^ 1);
@@ -379,7 +405,8 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     }
     float scale = a.scale, v_scale = 1.0f;
     if constexpr (CACHE) {
-      scale *= ks[base >> a.block_shift];
+      const float k_scale = ks[base >> a.block_shift];
+      scale *= __builtin_fmaf(k_scale, 0.0f, k_scale);  // keys of infinity: NaN, not a mask's -infinity
       v_scale = vs[base >> a.block_shift] * V_FACTOR;
       // scales that are not finite, of keys that this row does not see
       if (SAFE && base > lim) scale = 1.0f, v_scale = 0.0f;
@@ -524,7 +551,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   // tiles that every row sees whole
   int whole = (last(first_row / a.group) + 1) / KEYS;
   whole = whole < tiles ? whole : tiles;
-  auto every = [&](int kt) { return kt + a.splits; };
+  auto every = [&](int kt) { return kt + splits; };
   if (!(DOCS && a.documents)) {
     // those first, then the ones that need a mask
     int kt = begin(split, every);
@@ -548,61 +575,78 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       // document needs no mask: tiles are looked through SPAN at a time, 8 keys a lane. 2 us
       // a span, before 2 us a tile without a mask and 3 with one: 3 x 2021 tokens, 16 heads
       // over 4 of 96, bf16, causal, 8 documents a row 39 us, 64 29 us, one 74 (63 without).
-      constexpr int LANES = KEYS / 8, PER_WAVE = 64 / LANES, SPAN = PER_WAVE * WAVES;
+      constexpr int LANES = APART ? 1 : KEYS / 8, PER_WAVE = 64 / LANES, SPAN = PER_WAVE * TEAM;
       static_assert(SPAN <= 64, "bits");
       auto least = [](int x, int y) { return x < y ? x : y; };
       auto largest = [](int x, int y) { return x > y ? x : y; };
+      // One or two tiles are not worth a look: all with a mask (9 tokens 10.7 us with it, 9.0).
+      const bool few = tiles <= 2 * splits && tiles <= SPAN;
       int lo = mine < 0 ? 0x7fffffff : mine, hi = mine, none = mine < 0;
-      for (int d = 1; d < 32; d <<= 1) {
-        lo = least(lo, __shfl_xor(lo, d, 64));
-        hi = largest(hi, __shfl_xor(hi, d, 64));
-        none |= __shfl_xor(none, d, 64);
+      if (!few) {
+        for (int d = 1; d < 32; d <<= 1) {
+          lo = least(lo, __shfl_xor(lo, d, 64));
+          hi = largest(hi, __shfl_xor(hi, d, 64));
+          none |= __shfl_xor(none, d, 64);
+        }
+        if constexpr (TEAM > 1) {
+          if (lane == 0) lrange[0][wave] = lo, lrange[1][wave] = hi, lrange[2][wave] = none;
+          sync();
+          for (int i = 0; i < TEAM; ++i) {
+            lo = least(lo, lrange[0][i]);
+            hi = largest(hi, lrange[1][i]);
+            none |= lrange[2][i];
+          }
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
       }
-      if (lane == 0) lrange[0][wave] = lo, lrange[1][wave] = hi, lrange[2][wave] = none;
-      __syncthreads();
-      for (int i = 0; i < WAVES; ++i) {
-        lo = least(lo, lrange[0][i]);
-        hi = largest(hi, lrange[1][i]);
-        none |= lrange[2][i];
-      }
-      lo = __builtin_amdgcn_readfirstlane(lo);
-      hi = __builtin_amdgcn_readfirstlane(hi);
       const bool one = __builtin_amdgcn_readfirstlane(none) == 0 && lo == hi;
       for (int span = 0; span * SPAN < tiles; ++span) {
-        const int tile = span * SPAN + wave * PER_WAVE + lane / LANES;
-        int dl = 0x7fffffff, dh = -1;
-        bool gap = false;  // a token of no document
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = tile * KEYS + lane % LANES * 8 + j;
-          const int x = key < keys ? doc[key * a.dt] : -1;
-          gap |= x < 0;
-          dl = x < 0 ? dl : least(dl, x);
-          dh = largest(dh, x);
-        }
-        int holes = gap;
-        for (int d = 1; d < LANES; d <<= 1) {
-          dl = least(dl, __shfl_xor(dl, d, 64));
-          dh = largest(dh, __shfl_xor(dh, d, 64));
-          holes |= __shfl_xor(holes, d, 64);
-        }
-        const bool first = lane % LANES == 0 && tile < tiles && tile % a.splits == split;
-        const uint64_t some = __ballot(first && dh >= lo && dl <= hi);
-        const uint64_t all = __ballot(first && one && !holes && dl == lo && dh == lo && tile < whole);
-        uint64_t bits = 0;
-        for (int i = 0; i < PER_WAVE; ++i) {
-          bits |= ((some >> (i * LANES)) & 1) << i;
-          bits |= ((all >> (i * LANES)) & 1) << (i + 32);
-        }
-        __syncthreads();  // everyone is done with the span before
-        if (lane == 0) lbits[wave] = bits;
-        __syncthreads();
         // this split's tiles of the span that rows see some of, and all of
         uint64_t open = 0, full = 0;
-        for (int i = 0; i < WAVES; ++i) {
-          const uint64_t w = lbits[i];
-          open |= (w & 0xffffffffu) << (i * PER_WAVE);
-          full |= (w >> 32) << (i * PER_WAVE);
+        if (few) {
+          for (int kt = split; kt < tiles; kt += splits) open |= 1ull << kt;
+        } else {
+          const int tile = span * SPAN + mate * PER_WAVE + lane / LANES;
+          int dl = 0x7fffffff, dh = -1;
+          bool gap = false;  // a token of no document
+#pragma unroll
+          for (int j = 0; j < KEYS / LANES; ++j) {
+            const int key = tile * KEYS + lane % LANES * (KEYS / LANES) + j;
+            const int x = key < keys ? doc[key * a.dt] : -1;
+            gap |= x < 0;
+            dl = x < 0 ? dl : least(dl, x);
+            dh = largest(dh, x);
+          }
+          int holes = gap;
+          for (int d = 1; d < LANES; d <<= 1) {
+            dl = least(dl, __shfl_xor(dl, d, 64));
+            dh = largest(dh, __shfl_xor(dh, d, 64));
+            holes |= __shfl_xor(holes, d, 64);
+          }
+          const bool first = lane % LANES == 0 && tile < tiles && tile % splits == split;
+          const uint64_t some = __ballot(first && dh >= lo && dl <= hi);
+          const uint64_t all = __ballot(first && one && !holes && dl == lo && dh == lo && tile < whole);
+          open = some;
+          full = all;
+          if constexpr (LANES > 1) {
+            uint64_t bits = 0;
+            for (int i = 0; i < PER_WAVE; ++i) {
+              bits |= ((some >> (i * LANES)) & 1) << i;
+              bits |= ((all >> (i * LANES)) & 1) << (i + 32);
+            }
+            open = full = 0;
+            if constexpr (TEAM > 1) {
+              sync();  // everyone is done with the span before
+              if (lane == 0) lbits[wave] = bits;
+              sync();
+            }
+            for (int i = 0; i < TEAM; ++i) {
+              const uint64_t w = TEAM > 1 ? lbits[i] : bits;
+              open |= (w & 0xffffffffu) << (i * PER_WAVE);
+              full |= (w >> 32) << (i * PER_WAVE);
+            }
+          }
         }
         auto uniform = [](uint64_t x) {
           return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
@@ -641,7 +685,7 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) check = __builtin_fmaf(o[i][j], 0.0f, check);
-  if (__syncthreads_or(check != 0.0f)) {
+  if (APART ? __any(check != 0.0f) : __syncthreads_or(check != 0.0f)) {
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -649,13 +693,12 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     m = -__builtin_inff();
     l = 0.0f;
     begin(split, every);
-    for (int kt = split; kt < tiles; kt += a.splits) {
+    for (int kt = split; kt < tiles; kt += splits) {
       arrive(kt, every);
       if (kt * KEYS <= lim_wave) compute(kt, bool_constant<true>{}, bool_constant<true>{});
       turn();
     }
   }
-  if (row >= rows) return;
   l = xor32<OpSum>(l) * V_FACTOR;
   if (CACHE && t >= real) {  // padding
 #pragma unroll
@@ -665,34 +708,67 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     m = -__builtin_inff();
     l = 0.0f;
   }
-  if (a.splits > 1) {
-    float* const part = a.part + (((int64_t)split * a.batch * a.kv_heads + pair) * rows + row) * (a.dim + 4);
+  // four values of a row: to the parts, or as they are
+  auto put = [&](int row, int d, float4v x, float m, float l) {
+    if (a.splits > 1) {
+      float* const part = a.part + (((int64_t)(unit % a.splits) * a.batch * a.kv_heads + pair) * rows + row) * (a.dim + 4);
+      *reinterpret_cast<float4v*>(part + d) = x;
+      if (d == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{m, l, 0.0f, 0.0f};
+      return;
+    }
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    const int t = row / a.group, head = hk * a.group + row % a.group;
+    T y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = element<T>::narrow(x[j] * inverse);
+    store_n<8>(reinterpret_cast<T*>(a.out) +
+               (((int64_t)b * a.queries + t) * a.kv_heads * a.group + head) * a.dim + d, y);
+  };
+  if constexpr (APART) {
+    // the waves' parts, each in its own LDS, whose tiles it is done with
+    constexpr int PITCH = DP + 4;
+    static_assert(32 * PITCH * 4 <= 2 * BUFFERS * TILE, "parts");
+    __shared__ float lm[WAVES][32], ll[WAVES][32];
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+    float* const mine = reinterpret_cast<float*>(lds) + c * PITCH;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        *reinterpret_cast<float4v*>(mine + 32 * i + 8 * z + 4 * h) =
+            float4v{o[i][4 * z], o[i][4 * z + 1], o[i][4 * z + 2], o[i][4 * z + 3]};
+    if (h == 0) lm[wave][c] = m, ll[wave][c] = l;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (DP / 4); i += 64 * WAVES) {
+      const int y = i / (DP / 4), d = i % (DP / 4) * 4;
+      if (first_row + y >= rows || d >= a.dim) continue;
+      float top = lm[0][y];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) top = __builtin_fmaxf(top, lm[w][y]);
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float4v x = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float f = __builtin_amdgcn_exp2f(lm[w][y] - ref);
+        sum = __builtin_fmaf(ll[w][y], f, sum);
+        const float4v v = *reinterpret_cast<const float4v*>(reinterpret_cast<const float*>(all_lds[w]) + y * PITCH + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(v[e], f, x[e]);
+      }
+      put(first_row + y, d, x, top, sum);
+    }
+  } else {
+    if (row >= rows) return;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const int d = 32 * i + 8 * z + 4 * h;
         if (d < a.dim)
-          *reinterpret_cast<float4v*>(part + d) = float4v{o[i][4 * z], o[i][4 * z + 1], o[i][4 * z + 2], o[i][4 * z + 3]};
+          put(row, d, float4v{o[i][4 * z], o[i][4 * z + 1], o[i][4 * z + 2], o[i][4 * z + 3]}, m, l);
       }
-    if (h == 0) *reinterpret_cast<float4v*>(part + a.dim) = float4v{m, l, 0.0f, 0.0f};
-    return;
   }
-  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-  T* const out = reinterpret_cast<T*>(a.out) +
-                 (((int64_t)b * a.queries + t) * a.kv_heads * a.group + head) * a.dim;
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int z = 0; z < 4; ++z) {
-      const int d = 32 * i + 8 * z + 4 * h;
-      if (d < a.dim) {
-        T x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = element<T>::narrow(o[i][4 * z + j] * inverse);
-        store_n<8>(out + d, x);
-      }
-    }
 }
 
 // One workgroup for each (sequence, token, head).
@@ -709,9 +785,10 @@ __device__ __forceinline__ void attention_join(const AttentionArgs& a) {
 
 }  // namespace mlc
 
-#define ATTENTION(NAME, T, DP, WAVES, SOURCE, GENERAL)                                            \
-  extern "C" __global__ void __launch_bounds__(64 * WAVES, DP == 64 ? 3 : 2) NAME(mlc::AttentionArgs a) {\
-    mlc::attention<T, DP, WAVES, mlc::SOURCE, GENERAL>(a);                                             \
+#define ATTENTION(NAME, T, DP, WAVES, SOURCE, SCORES, APART)                                      \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, DP == 64 && !APART ? 3 : 2)            \
+  NAME(mlc::AttentionArgs a) {                                                                    \
+    mlc::attention<T, DP, WAVES, mlc::SOURCE, mlc::SCORES, APART>(a);                             \
   }
 #define ATTENTION_JOIN(NAME, T, WAVES)                                                   \
   extern "C" __global__ void __launch_bounds__(64 * WAVES) NAME(mlc::AttentionArgs a) {                  \

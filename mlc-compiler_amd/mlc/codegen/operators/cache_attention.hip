@@ -247,7 +247,7 @@ __device__ __forceinline__ void cache_attention(const CacheAttentionArgs& a) {
       load_values(begin);
     }
     for (int tb = begin; tb < hi_key; tb += step) {
-      const float kscale = kscale_next;
+      const float kscale = __builtin_fmaf(kscale_next, 0.0f, kscale_next);  // infinity: NaN, not a mask's
       float vscale = vscale_next * SCALE_ROOM;
       // a scale that is not finite, of keys that this row does not see
       if (SAFE && tb > lim) vscale = 0.0f;

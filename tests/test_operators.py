@@ -156,6 +156,27 @@ def test_attention_masks_and_biases(dtype, tq, tk, dim, options):
 
 
 @gpu
+@pytest.mark.parametrize("batch,tq,tk,heads,kv,dim", [
+    (2, 1200, 1200, 2, 2, 64), (2, 700, 900, 4, 1, 128), (2, 600, 640, 2, 1, 256), (2, 2, 5000, 2, 1, 96),
+    (2, 500, 700, 1, 1, 80), (8, 300, 333, 24, 24, 64), (2, 260, 700, 32, 32, 128), (2, 700, 700, 16, 16, 80)])
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_over_documents_of_many_tiles(batch, tq, tk, heads, kv, dim, causal):
+    """In order, out of order with gaps, and few large ones with padding, where workgroups share
+    tiles of keys and where their waves take them apart."""
+    q, k, v = _heads(batch, tq, tk, heads, kv, dim, BF, seed=11)
+    g = torch.Generator().manual_seed(5)
+    at = torch.arange(tk)
+    ordered = at * 9 // tk
+    mixed = torch.randint(-1, 4, (tk // 50 + 1,), generator=g).repeat_interleave(50)[:tk]
+    padded = torch.where(at < tk * 7 // 8, at // (tk // 2), -1)
+    documents = torch.stack([(ordered, mixed, padded)[i % 3] for i in range(batch)]).to(torch.int32).cuda()
+    if batch == 2:
+        documents[0] = padded.to(torch.int32)
+    ref.close(ops.attention(q, k, v, documents=documents, causal=causal),
+              *ref.attention(q, k, v, documents=documents, causal=causal))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", (HALF, BF))
 @pytest.mark.parametrize("dim", (64, 128))
 def test_attention_is_not_touched_by_what_it_does_not_see(dtype, dim):
@@ -994,9 +1015,11 @@ def test_every_kernel_a_plan_asks_for_is_built_beforehand():
     known = {kernel for _, kernel in plans.all_kernels()}
     random.seed(1)
     seen = set()
-    for _ in range(6000):
+    for _ in range(100000):
+        if seen == known:
+            break
         dtype, kv, group = random.choice((HALF, BF, FULL)), random.choice((1, 2, 8)), random.choice((1, 4, 16))
-        b, t = random.choice((1, 2, 40)), random.choice((1, 2, 3, 5, 31, 200, 5000))
+        b, t = random.choice((1, 2, 40, 300)), random.choice((1, 2, 3, 5, 31, 50, 200, 5000))
         dim, block = random.choice((16, 64, 80, 96, 128, 256)), random.choice((32, 64, 128))
         q, k = dense(b, t, kv * group, dim, dtype=dtype), dense(b, t, kv, dim, dtype=dtype)
         blocks = random.choice((8, 64))
@@ -1008,7 +1031,9 @@ def test_every_kernel_a_plan_asks_for_is_built_beforehand():
                                    random.random() < 0.5, 1.0),
                  plans.plan_cache_append(cache, cache, scale, scale, k, k, start, None)]
         if dtype != FULL:
-            found += [plans.plan_attention(q, k, k, slopes, None, None, 0.1, True, 0.0),
+            documents = dense(b, t, dtype=torch.int32) if random.random() < 0.3 else None
+            keys = dense(b, t + random.choice((0, 10, 900)), kv, dim, dtype=dtype)
+            found += [plans.plan_attention(q, keys, keys, slopes, documents, None, 0.1, True, 0.0),
                       plans.plan_cache_attention(q, cache, cache, scale, scale, start, None, slopes, 0.1, 0.0)]
         seen |= {launch.kernel for p in found for launch in p.launches}
     assert seen <= known, seen - known
