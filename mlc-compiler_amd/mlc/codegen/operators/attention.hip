@@ -134,6 +134,13 @@ enum { COPIED, DIRECT, CODES };
 // documents. Apart, since what a kernel does not use still takes its registers: 32 x 512 tokens,
 // 12 heads of 64 with a bias 45 us in a kernel that looks for documents too, 39 without.
 enum { PLAIN, BIASED, DOCUMENTS };
+// Waves that a SIMD has to have registers for. More hide more, where nothing spills: with a
+// cap and documents, 6 x 999 tokens, 8 heads of 256 56 us for one and 66 for two, plain 2048
+// tokens of them 133 and 121; 8 x 512, 12 heads of 64 with documents 19.2 for two, 20.6 three.
+constexpr int waves_a_simd(int dp, int scores, bool apart) {
+  return dp == 256 && scores != PLAIN ? 1 : dp == 64 && scores != DOCUMENTS && !apart ? 3 : 2;
+}
+
 template <class T, int DP, int WAVES, int SOURCE, int SCORES, bool APART>
 __device__ __forceinline__ void attention(const AttentionArgs& a) {
   typedef typename vec8<T>::type v8;
@@ -786,7 +793,7 @@ __device__ __forceinline__ void attention_join(const AttentionArgs& a) {
 }  // namespace mlc
 
 #define ATTENTION(NAME, T, DP, WAVES, SOURCE, SCORES, APART)                                      \
-  extern "C" __global__ void __launch_bounds__(64 * WAVES, DP == 64 && !APART ? 3 : 2)            \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, mlc::waves_a_simd(DP, mlc::SCORES, APART)) \
   NAME(mlc::AttentionArgs a) {                                                                    \
     mlc::attention<T, DP, WAVES, mlc::SOURCE, mlc::SCORES, APART>(a);                             \
   }
