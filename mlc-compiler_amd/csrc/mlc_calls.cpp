@@ -144,7 +144,9 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (found == table().end()) return PyBytes_FromStringAndSize(key.data(), static_cast<Py_ssize_t>(key.size()));
   const std::shared_ptr<Entry> entry = found->second;
 
-  for (Py_ssize_t i = 0; i < entry->changed; ++i)
+  for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)
+    if (x[i] != nullptr) at[i] = reinterpret_cast<uint64_t>(x[i]->mutable_data_ptr());  // a lazy copy is made now
+  for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)
     for (Py_ssize_t j = 0; j < i; ++j)
       if (at[i] == at[j] && at[i] != 0) {
         Py_INCREF(Py_Ellipsis);
