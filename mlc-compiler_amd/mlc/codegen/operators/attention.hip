@@ -579,9 +579,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
     if (a.documents) {
       // The documents of the workgroup's rows, least and largest, and whether a row has none.
       // A tile whose documents lie outside is left out, one that is of the rows' only
-      // document needs no mask: tiles are looked through SPAN at a time, 8 keys a lane. 2 us
-      // a span, before 2 us a tile without a mask and 3 with one: 3 x 2021 tokens, 16 heads
-      // over 4 of 96, bf16, causal, 8 documents a row 39 us, 64 29 us, one 74 (63 without).
+      // document needs no mask: tiles are looked through SPAN at a time, 8 keys a lane, or, by
+      // a wave apart, a tile. That takes 2 us a span, a tile without a mask 2 and with one 3:
+      // 3 x 2021 tokens, 16 heads over 4 of 96, bf16, causal, 8 documents a row 39 us, 64 29
+      // us, one 74 (63 without).
       constexpr int LANES = APART ? 1 : KEYS / 8, PER_WAVE = 64 / LANES, SPAN = PER_WAVE * TEAM;
       static_assert(SPAN <= 64, "bits");
       auto least = [](int x, int y) { return x < y ? x : y; };
