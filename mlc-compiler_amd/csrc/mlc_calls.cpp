@@ -15,6 +15,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <cstdint>
@@ -32,10 +33,25 @@ using poll_fn = int (*)(void*, int32_t*);
 constexpr Py_ssize_t kMostOperands = 16, kMostResults = 2;
 constexpr size_t kMostBytes = 1024;  // of a launch's arguments
 
+// The flags of a call. kDispatched: torch's dispatcher has brought it, and whoever looks on
+// has seen it.
+enum { kPoll = 1, kDispatched = 2 };
+
 // tensors that stand for others
 constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched,
                                         c10::DispatchKey::Python, c10::DispatchKey::ZeroTensor});
+
+// and what is traced by: a direct call would leave the allocation of its result in a graph
+// in the operator's place
+constexpr c10::DispatchKeySet kTraced({c10::DispatchKey::Tracer, c10::DispatchKey::Functionalize,
+                                       c10::DispatchKey::Python, c10::DispatchKey::PreDispatch,
+                                       c10::DispatchKey::PythonDispatcher});
+
+bool is_traced() {
+  const auto keys = c10::impl::tls_local_dispatch_key_set();
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || (keys.included_ - keys.excluded_).has_any(kTraced);
+}
 
 struct Launch {
   void* fn;
@@ -63,17 +79,17 @@ template <class T> void put(std::string& key, T x) {
   key.append(reinterpret_cast<const char*>(&x), sizeof(x));
 }
 
-// call(operator, operands, options, results, stream_of, poll), with the current stream's
+// call(operator, operands, options, results, stream_of, flags), with the current stream's
 // address from stream_of(device):
 //   a tuple of results: done;  bytes: the signature, of which nothing is known yet;
-//   None: not plain tensors of one GPU, or a mode looks on;  False: an operand asks for a
-//   gradient;  True: an earlier call met an invalid input (where ``poll``);  NotImplemented:
-//   the device is not the current one;  Ellipsis: an operand that changes is given twice;
-//   an int: the launch's error.
+//   None: not plain tensors of one GPU, or someone looks on (but for kDispatched);  False: an
+//   operand asks for a gradient;  True: an earlier call met an invalid input (where kPoll);
+//   NotImplemented: the device is not the current one;  Ellipsis: an operand that changes is
+//   given twice;  an int: the launch's error.
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 6 || !PyTuple_Check(args[1]) || !PyTuple_Check(args[2])) {
-    PyErr_SetString(PyExc_TypeError, "call(operator, operands, options, results, stream_of, poll)");
+    PyErr_SetString(PyExc_TypeError, "call(operator, operands, options, results, stream_of, flags)");
     return nullptr;
   }
   const Py_ssize_t operands = PyTuple_GET_SIZE(args[1]), results = PyLong_AsSsize_t(args[3]);
@@ -81,12 +97,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "call: too many operands or results");
     return nullptr;
   }
-  const long op = PyLong_AsLong(args[0]);
+  const long op = PyLong_AsLong(args[0]), flags = PyLong_AsLong(args[5]);
   if (PyErr_Occurred()) return nullptr;
 
   const at::Tensor* x[kMostOperands];
   const bool grad = at::GradMode::is_enabled();
-  bool plain = !c10::impl::TorchDispatchModeTLS::any_modes_set();
+  bool plain = (flags & kDispatched) || !is_traced();
   int device = -1;
   for (Py_ssize_t i = 0; i < operands; ++i) {
     PyObject* const o = PyTuple_GET_ITEM(args[1], i);
@@ -152,7 +168,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_INCREF(Py_Ellipsis);
         return Py_Ellipsis;
       }
-  if (entry->poll != nullptr && PyObject_IsTrue(args[5])) {
+  if (entry->poll != nullptr && (flags & kPoll)) {
     int32_t word = 0;
     const int rc = entry->poll(entry->ctx, &word);
     if (rc != 0) return PyLong_FromLong(rc);

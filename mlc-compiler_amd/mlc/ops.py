@@ -22,6 +22,7 @@ sums are held in fp32, the angles of ``rotary`` in 64 bits.
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -264,14 +265,17 @@ _OPERATORS = {
 _NUMBERS = {op: i for i, op in enumerate(_OPERATORS)}
 
 
-def _now(op: str, operands: tuple, options: tuple, results: int) -> tuple | None:
+_POLL, _DISPATCHED = 1, 2
+
+
+def _now(op: str, operands: tuple, options: tuple, results: int, flags: int = _POLL) -> tuple | None:
     """The call, with so many results like the first operands, or None where they are not
     plain GPU tensors outside of any tracing. An operand that asks for a gradient is refused."""
     if _is_compiling():
         return None
-    run, poll = native.load_calls().call, True
+    run = native.load_calls().call
     while True:
-        out = run(_NUMBERS[op], operands, options, results, _stream_of, poll)
+        out = run(_NUMBERS[op], operands, options, results, _stream_of, flags)
         if out is None or type(out) is tuple:
             return out
         if out is False:
@@ -280,10 +284,10 @@ def _now(op: str, operands: tuple, options: tuple, results: int) -> tuple | None
         if out is True:
             if not torch.cuda.is_current_stream_capturing():
                 operators.raise_pending(operators.device_modules(operands[0].get_device()))
-            poll = False
+            flags &= ~_POLL
         elif out is NotImplemented:
             with torch.cuda.device(operands[0].get_device()):
-                return _now(op, operands, options, results)
+                return _now(op, operands, options, results, flags)
         elif out is Ellipsis:
             raise OperatorError(f"{op}: keys and values share a cache or its scales")
         elif type(out) is bytes:
@@ -312,18 +316,33 @@ def _like(x):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+@contextlib.contextmanager
+def _untraced():
+    """While torch.jit traces, sizes are tensors and what is done with them goes into its
+    graph: not below an operator, which is in it as a whole."""
+    state = torch._C._get_tracing_state()
+    if state is not None:
+        torch._C._set_tracing_state(None)
+    try:
+        yield
+    finally:
+        if state is not None:
+            torch._C._set_tracing_state(state)
+
+
 def _implement(op: str, split, results: int) -> None:
     """``mlc::op``: ``split`` puts the schema's arguments into operands and options,
     results are like the first operands."""
     check = _OPERATORS[op][0]
 
+    @_untraced()
     def gpu(*args):
         operands, options = split(*args)
         # what the dispatcher hands over may be a subclass
         plain = tuple(x if x is None or type(x) is torch.Tensor
                       else x.detach().as_subclass(torch.Tensor) for x in operands)
         with torch.no_grad():
-            out = _now(op, plain, options, results)
+            out = _now(op, plain, options, results, _POLL | _DISPATCHED)
         if out is None:
             check(*operands, *options)
         _require(out is not None, f"{op}: not plain tensors of one GPU")
@@ -335,6 +354,7 @@ def _implement(op: str, split, results: int) -> None:
         out = tuple(map(_like, operands[:results]))
         return out if results > 1 else out[0] if results else None
 
+    @_untraced()
     def host(*args):
         from .runtime.executor import ExecutionError
 

@@ -1,0 +1,35 @@
+"""Calls of ``mlc.ops`` that something else looks on or that hand it memory in unusual
+ways: tracing, modes, gradients of both directions, overlapping and lazily copied
+operands, many sequences of uneven lengths."""
+
+from __future__ import annotations
+
+import torch
+
+import operators_reference as ref
+from mlc import ops
+from test_operators import HALF, _heads, filled, gpu, ints, parts
+
+
+# --------------------------------------------------------------------------
+# what looks on
+# --------------------------------------------------------------------------
+
+@gpu
+def test_a_traced_call_is_the_operator():
+    """torch.jit's tracer sees the operator and not the allocation of its result."""
+    q, k, v = _heads(1, 5, 70, 2, 1, 64, HALF)
+    cache, start = filled(1, 1, 128, 64), ints([70])
+
+    def f(q, k, v):
+        cache.append(k[:, :5], v[:, :5], start)
+        return ops.attention(q, k, v, causal=True), cache.attend(q, start)
+
+    traced = torch.jit.trace(f, (q, k, v), check_trace=False)
+    kinds = [n.kind() for n in traced.graph.nodes()]
+    for name in ("cache_append", "attention", "cache_attention"):
+        assert f"mlc::{name}" in kinds, kinds
+    q, k, v = _heads(1, 5, 70, 2, 1, 64, HALF, seed=20)
+    got = traced(q, k, v)
+    ref.close(got[0], *ref.attention(q, k, v, causal=True))
+    ref.close(got[1], *ref.cache_attention(q, *parts(cache), start))
