@@ -10,8 +10,10 @@
 
 #define PY_SSIZE_T_CLEAN
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
@@ -51,6 +53,19 @@ constexpr c10::DispatchKeySet kTraced({c10::DispatchKey::Tracer, c10::DispatchKe
 bool is_traced() {
   const auto keys = c10::impl::tls_local_dispatch_key_set();
   return c10::impl::TorchDispatchModeTLS::any_modes_set() || (keys.included_ - keys.excluded_).has_any(kTraced);
+}
+
+// torch.utils._device.DeviceContext: a function mode that fills in factories' devices alone
+PyTypeObject* device_context = nullptr;
+
+// Whether a function mode (torch.overrides) wants to see calls.
+bool is_watched() {
+  if (!at::impl::torch_function_mode_enabled()) return false;
+  for (int64_t i = 0; i < at::impl::PythonTorchFunctionTLS::stack_len(); ++i) {
+    PyObject* const mode = at::impl::PythonTorchFunctionTLS::get_stack_at(i)->ptr(getPyInterpreter());
+    if (Py_TYPE(mode) != device_context) return true;
+  }
+  return false;
 }
 
 struct Launch {
@@ -102,7 +117,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
   const at::Tensor* x[kMostOperands];
   const bool grad = at::GradMode::is_enabled();
-  bool plain = (flags & kDispatched) || !is_traced();
+  bool plain = (flags & kDispatched) || !(is_traced() || is_watched());
   int device = -1;
   for (Py_ssize_t i = 0; i < operands; ++i) {
     PyObject* const o = PyTuple_GET_ITEM(args[1], i);
@@ -274,4 +289,12 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, kMethods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* const torch_device = PyImport_ImportModule("torch.utils._device");
+  if (torch_device == nullptr) return nullptr;
+  PyObject* const type = PyObject_GetAttrString(torch_device, "DeviceContext");  // kept
+  Py_DECREF(torch_device);
+  if (type == nullptr) return nullptr;
+  device_context = reinterpret_cast<PyTypeObject*>(type);
+  return PyModule_Create(&kModule);
+}

@@ -33,3 +33,25 @@ def test_a_traced_call_is_the_operator():
     got = traced(q, k, v)
     ref.close(got[0], *ref.attention(q, k, v, causal=True))
     ref.close(got[1], *ref.cache_attention(q, *parts(cache), start))
+
+
+@gpu
+def test_function_modes_see_the_operator():
+    from torch.overrides import TorchFunctionMode
+
+    class Log(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+    q, k, v = _heads(1, 5, 70, 2, 1, 64, HALF)
+    want = ops.attention(q, k, v)
+    with Log():
+        assert torch.equal(ops.attention(q, k, v), want)
+    assert any("mlc.attention" in x for x in seen), seen
+    with torch.device("cuda"):  # a mode too, for factories only
+        assert torch.equal(ops.attention(q, k, v), want)
+    traced = torch.jit.trace(lambda q: ops.attention(q, k, v), (q,), check_trace=False)
+    with Log():  # the traced operator, called below Python's modes
+        assert torch.equal(traced(q), want)
