@@ -15,6 +15,7 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/ops/empty.h>
+#include <ATen/record_function.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -22,6 +23,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <iterator>
 #include <memory>
 #include <string>
 #include <unordered_map>
@@ -38,6 +40,9 @@ constexpr size_t kMostBytes = 1024;  // of a launch's arguments
 // The flags of a call. kDispatched: torch's dispatcher has brought it, and whoever looks on
 // has seen it.
 enum { kPoll = 1, kDispatched = 2 };
+
+// by number, as mlc.ops gives it
+constexpr const char* kOperators[] = {"mlc::rotary", "mlc::attention", "mlc::cache_append", "mlc::cache_attention"};
 
 // tensors that stand for others
 constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
@@ -188,6 +193,13 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int rc = entry->poll(entry->ctx, &word);
     if (rc != 0) return PyLong_FromLong(rc);
     if (word != 0) Py_RETURN_TRUE;
+  }
+  std::vector<c10::IValue> inputs;  // outlives the record
+  at::RecordFunction record(at::RecordScope::FUNCTION);  // the dispatcher makes one of its own
+  if (record.isActive() && !(flags & kDispatched) && op >= 0 && op < static_cast<long>(std::size(kOperators))) {
+    if (record.needsInputs())
+      for (Py_ssize_t i = 0; i < operands; ++i) inputs.push_back(x[i] ? c10::IValue(*x[i]) : c10::IValue());
+    record.before(kOperators[op], &inputs);
   }
   PyObject* const index = PyLong_FromLong(device);
   if (index == nullptr) return nullptr;

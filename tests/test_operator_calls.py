@@ -55,3 +55,17 @@ def test_function_modes_see_the_operator():
     traced = torch.jit.trace(lambda q: ops.attention(q, k, v), (q,), check_trace=False)
     with Log():  # the traced operator, called below Python's modes
         assert torch.equal(traced(q), want)
+
+
+@gpu
+def test_the_profiler_records_each_call_once():
+    from torch.profiler import ProfilerActivity, profile
+
+    q, k, v = _heads(1, 5, 70, 2, 1, 64, HALF)
+    ops.attention(q, k, v)
+    with profile(activities=[ProfilerActivity.CPU], record_shapes=True) as p:
+        ops.attention(q, k, v)
+        torch.ops.mlc.attention(q, k, v, None, False, 0.0, None, None, None)
+    found = [e for e in p.events() if e.name == "mlc::attention"]
+    assert len(found) == 2, [e.name for e in p.events()]
+    assert found[0].input_shapes[:3] == [list(q.shape), list(k.shape), list(v.shape)]
