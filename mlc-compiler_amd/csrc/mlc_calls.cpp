@@ -16,6 +16,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/ops/empty.h>
 #include <ATen/record_function.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -121,7 +122,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
 
   const at::Tensor* x[kMostOperands];
-  const bool grad = at::GradMode::is_enabled();
+  // forward mode goes on where gradients are off, and ends in inference mode
+  const bool grad = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   bool plain = (flags & kDispatched) || !(is_traced() || is_watched());
   int device = -1;
   for (Py_ssize_t i = 0; i < operands; ++i) {
@@ -133,7 +135,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
       return nullptr;
     }
     x[i] = &THPVariable_Unpack(o);
-    if (grad && x[i]->requires_grad()) Py_RETURN_FALSE;
+    if ((grad && x[i]->requires_grad()) || (forward && x[i]->_fw_grad(0).defined())) Py_RETURN_FALSE;
     plain = plain && THPVariable_CheckExact(o) && x[i]->is_cuda() && x[i]->layout() == at::kStrided &&
             x[i]->has_storage() && !x[i]->is_neg() && !x[i]->is_conj() && !x[i]->key_set().has_any(kWrapped);
     if (plain) {

@@ -16,8 +16,8 @@ key head ``h // (heads // kv_heads)``.
 Called with GPU tensors, each launches this build's kernels on the current stream.
 Used in a module given to ``mlc.compile`` they become launches of the compiled
 schedule; ``cache_append`` then changes the module's own buffers. They are for
-inference: a tensor that asks for a gradient is refused. Softmax statistics and
-sums are held in fp32, the angles of ``rotary`` in 64 bits.
+inference: a tensor that asks for a gradient, backward or forward, is refused. Softmax
+statistics and sums are held in fp32, the angles of ``rotary`` in 64 bits.
 """
 
 from __future__ import annotations
@@ -280,7 +280,8 @@ def _now(op: str, operands: tuple, options: tuple, results: int, flags: int = _P
             return out
         if out is False:
             raise OperatorError("an operand asks for a gradient, and the operators of mlc.ops are "
-                                "for inference: call them under torch.no_grad()")
+                                "for inference: call them under torch.no_grad(), or, in forward mode, "
+                                "on the primal (torch.autograd.forward_ad.unpack_dual)")
         if out is True:
             if not torch.cuda.is_current_stream_capturing():
                 operators.raise_pending(operators.device_modules(operands[0].get_device()))

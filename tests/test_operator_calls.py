@@ -8,7 +8,7 @@ import torch
 
 import operators_reference as ref
 from mlc import ops
-from test_operators import HALF, _heads, filled, gpu, ints, parts
+from test_operators import HALF, _heads, _refused, filled, gpu, host, ints, parts
 
 
 # --------------------------------------------------------------------------
@@ -69,3 +69,20 @@ def test_the_profiler_records_each_call_once():
     found = [e for e in p.events() if e.name == "mlc::attention"]
     assert len(found) == 2, [e.name for e in p.events()]
     assert found[0].input_shapes[:3] == [list(q.shape), list(k.shape), list(v.shape)]
+
+# --------------------------------------------------------------------------
+# gradients
+# --------------------------------------------------------------------------
+
+def test_operands_with_a_forward_gradient_are_refused():
+    import torch.autograd.forward_ad as forward
+
+    q = host(1, 1, 2, 64)
+    with forward.dual_level():
+        dual = forward.make_dual(q, torch.ones_like(q))
+        with torch.no_grad():  # forward mode goes on there
+            _refused(lambda: ops.attention(dual, q, q), "gradient")
+        _refused(lambda: ops.attention(q, q, dual), "gradient")
+        with torch.inference_mode():  # and not there
+            _refused(lambda: ops.attention(dual, q, q), "ROCm GPU")
+    _refused(lambda: ops.attention(q, q, q), "ROCm GPU")
