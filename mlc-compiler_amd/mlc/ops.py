@@ -26,6 +26,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .codegen import hip_operators as plans
 from .codegen.hip_operators import Operand, OperatorError
@@ -266,6 +267,9 @@ _NUMBERS = {op: i for i, op in enumerate(_OPERATORS)}
 
 
 _POLL, _DISPATCHED = 1, 2
+_GRADIENT = ("an operand asks for a gradient, and the operators of mlc.ops are for inference: call "
+             "them under torch.no_grad(), or, in forward mode, on the primal "
+             "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def _now(op: str, operands: tuple, options: tuple, results: int, flags: int = _POLL) -> tuple | None:
@@ -279,9 +283,7 @@ def _now(op: str, operands: tuple, options: tuple, results: int, flags: int = _P
         if out is None or type(out) is tuple:
             return out
         if out is False:
-            raise OperatorError("an operand asks for a gradient, and the operators of mlc.ops are "
-                                "for inference: call them under torch.no_grad(), or, in forward mode, "
-                                "on the primal (torch.autograd.forward_ad.unpack_dual)")
+            raise OperatorError(_GRADIENT)
         if out is True:
             if not torch.cuda.is_current_stream_capturing():
                 operators.raise_pending(operators.device_modules(operands[0].get_device()))
@@ -317,6 +319,12 @@ def _like(x):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _asks_gradient(x) -> bool:
+    return isinstance(x, torch.Tensor) and (
+        (torch.is_grad_enabled() and x.requires_grad)
+        or (torch._C._is_fwd_grad_enabled() and unpack_dual(x).tangent is not None))
+
+
 @contextlib.contextmanager
 def _untraced():
     """While torch.jit traces, sizes are tensors and what is done with them goes into its
@@ -335,6 +343,13 @@ def _implement(op: str, split, results: int) -> None:
     """``mlc::op``: ``split`` puts the schema's arguments into operands and options,
     results are like the first operands."""
     check = _OPERATORS[op][0]
+
+    def autograd(keys, *args):
+        # a program that is exported is a graph, and refuses when it is run
+        if not torch.compiler.is_exporting() and any(map(_asks_gradient, args)):
+            raise OperatorError(_GRADIENT)
+        with torch._C._AutoDispatchBelowAutograd():
+            return overload.redispatch(keys & torch._C._after_autograd_keyset, *args)
 
     @_untraced()
     def gpu(*args):
@@ -364,6 +379,8 @@ def _implement(op: str, split, results: int) -> None:
         raise ExecutionError("the operators of mlc.ops run on a ROCm GPU (torch device 'cuda'), "
                              "not on the CPU")
 
+    overload = getattr(torch.ops.mlc, op).default
+    _lib.impl(op, autograd, "Autograd", with_keyset=True)
     _lib.impl(op, gpu, "CUDA")
     _lib.impl(op, host, "CPU")
     torch.library.register_fake(f"mlc::{op}", fake, lib=_lib)

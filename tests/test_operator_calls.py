@@ -4,6 +4,7 @@ operands, many sequences of uneven lengths."""
 
 from __future__ import annotations
 
+import pytest
 import torch
 
 import operators_reference as ref
@@ -86,3 +87,75 @@ def test_operands_with_a_forward_gradient_are_refused():
         with torch.inference_mode():  # and not there
             _refused(lambda: ops.attention(dual, q, q), "ROCm GPU")
     _refused(lambda: ops.attention(q, q, q), "ROCm GPU")
+
+
+def _dispatched(q, start, parts):
+    """A call of each operator through torch's dispatcher, by its name."""
+    f = torch.ones(32, dtype=torch.float64, device=q.device)
+    o = torch.ops.mlc
+    return {"rotary": lambda: o.rotary(q, q, start, f, False, 1.0),
+            "attention": lambda: o.attention(q, q, q, None, False, 0.0, None, None, None),
+            "cache_append": lambda: o.cache_append(*parts, q, q, start, None),
+            "cache_attention": lambda: o.cache_attention(q, *parts, start, None, None, 0.0, None)}
+
+
+@pytest.mark.parametrize("op", ("rotary", "attention", "cache_append", "cache_attention"))
+def test_the_dispatcher_refuses_operands_that_ask_for_gradients(op):
+    import torch.autograd.forward_ad as forward
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        cache = ops.KeyValueCache(1, 2, 64, 64, device="cuda")
+        q = torch.zeros(1, 1, 2, 64, dtype=HALF, device="cuda", requires_grad=True)
+        start = torch.zeros(1, dtype=torch.int32, device="cuda")
+        _refused(_dispatched(q, start, parts(cache))[op], "gradient")
+        with torch.no_grad():
+            _dispatched(q, start, parts(cache))[op]()
+        _dispatched(q.detach(), start, parts(cache))[op]()
+    q, start, cache = host(1, 1, 2, 64), torch.zeros(1, dtype=torch.int32), ops.KeyValueCache(1, 2, 64, 64)
+    with forward.dual_level():
+        dual = forward.make_dual(q, torch.ones_like(q))
+        with torch.no_grad():
+            _refused(_dispatched(dual, start, parts(cache))[op], "gradient")
+    _refused(_dispatched(q, start, parts(cache))[op], "ROCm GPU")
+
+
+def test_a_compiled_function_refuses_operands_that_ask_for_gradients():
+    w = torch.zeros(64, 64, dtype=HALF, requires_grad=True)
+    x = host(1, 3, 2, 64)
+    seen = []
+
+    def f(x):
+        return ops.attention(x @ w, x, x)
+
+    def backend(gm, example):
+        seen.append([str(n.target) for n in gm.graph.nodes])
+        return gm.forward
+
+    with pytest.raises(Exception, match="gradient"):
+        torch.compile(f, backend=backend, fullgraph=True)(x)
+    with torch.no_grad(), pytest.raises(Exception, match="ROCm GPU"):
+        torch.compile(f, backend=backend, fullgraph=True)(x)
+    assert any("mlc.attention" in n for n in seen[-1])
+
+
+def test_transforms_that_differentiate_are_refused():
+    q, t = host(1, 3, 2, 64), torch.ones(1, 3, 2, 64, dtype=HALF)
+    _refused(lambda: torch.func.grad(lambda x: ops.attention(x, q, q).sum())(q), "gradient")
+    _refused(lambda: torch.func.jvp(lambda x: ops.attention(x, q, q), (q,), (t,)), "gradient")
+
+
+def test_a_module_whose_weights_ask_for_gradients_is_exported():
+    """The program is a graph; who asks it for a gradient is refused then."""
+
+    class M(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.proj = torch.nn.Linear(64, 64).half()
+
+        def forward(self, x):
+            y = self.proj(x)
+            return ops.attention(y, y, y)
+
+    program = torch.export.export(M().eval(), (host(1, 3, 2, 64),))
+    assert any("mlc.attention" in str(n.target) for n in program.graph.nodes)
