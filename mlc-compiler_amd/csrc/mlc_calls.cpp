@@ -96,6 +96,16 @@ std::unordered_map<std::string, std::shared_ptr<Entry>>& table() {
   return *entries;
 }
 
+// Bytes from a tensor's first value to behind its last.
+uint64_t extent(const at::Tensor& x) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < x.dim(); ++i) {
+    if (x.size(i) == 0) return 0;
+    last += (x.size(i) - 1) * x.stride(i);
+  }
+  return static_cast<uint64_t>(last + 1) * x.element_size();
+}
+
 template <class T> void put(std::string& key, T x) {
   key.append(reinterpret_cast<const char*>(&x), sizeof(x));
 }
@@ -105,8 +115,8 @@ template <class T> void put(std::string& key, T x) {
 //   a tuple of results: done;  bytes: the signature, of which nothing is known yet;
 //   None: not plain tensors of one GPU, or someone looks on (but for kDispatched);  False: an
 //   operand asks for a gradient;  True: an earlier call met an invalid input (where kPoll);
-//   NotImplemented: the device is not the current one;  Ellipsis: an operand that changes is
-//   given twice;  an int: the launch's error.
+//   NotImplemented: the device is not the current one;  Ellipsis: an operand that changes
+//   lies in another's memory;  an int: the launch's error.
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 6 || !PyTuple_Check(args[1]) || !PyTuple_Check(args[2])) {
@@ -184,12 +194,16 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
   for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)
     if (x[i] != nullptr) at[i] = reinterpret_cast<uint64_t>(x[i]->mutable_data_ptr());  // a lazy copy is made now
-  for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)
-    for (Py_ssize_t j = 0; j < i; ++j)
-      if (at[i] == at[j] && at[i] != 0) {
-        Py_INCREF(Py_Ellipsis);
-        return Py_Ellipsis;
-      }
+  if (entry->changed > 0) {
+    uint64_t end[kMostOperands];
+    for (Py_ssize_t i = 0; i < operands; ++i) end[i] = x[i] != nullptr ? at[i] + extent(*x[i]) : 0;
+    for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)
+      for (Py_ssize_t j = 0; j < operands; ++j)
+        if (j != i && at[i] < end[j] && at[j] < end[i]) {
+          Py_INCREF(Py_Ellipsis);
+          return Py_Ellipsis;
+        }
+  }
   if (entry->poll != nullptr && (flags & kPoll)) {
     int32_t word = 0;
     const int rc = entry->poll(entry->ctx, &word);

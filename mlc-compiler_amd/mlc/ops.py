@@ -292,7 +292,8 @@ def _now(op: str, operands: tuple, options: tuple, results: int, flags: int = _P
             with torch.cuda.device(operands[0].get_device()):
                 return _now(op, operands, options, results, flags)
         elif out is Ellipsis:
-            raise OperatorError(f"{op}: keys and values share a cache or its scales")
+            raise OperatorError(f"{op}: keys and values share a cache or its scales, or another "
+                                "operand shares memory with them")
         elif type(out) is bytes:
             _add(out, op, operands, options, results)
         else:
@@ -485,8 +486,9 @@ def cache_append(k_cache, v_cache, k_scale, v_scale, k, v, start, count=None) ->
     are rounded to it. A block's first token starts its scale anew; tokens behind the
     last are not kept. NaN and infinities are stored as NaN.
 
-    A sequence whose ``start`` and ``count`` do not lie within the cache is left alone,
-    and ``ExecutionError`` is raised by a later call or :func:`check_errors`.
+    Operands that overlap the cache or its scales in memory are refused. A sequence whose
+    ``start`` and ``count`` do not lie within the cache is left alone, and
+    ``ExecutionError`` is raised by a later call or :func:`check_errors`.
     """
     if _now("cache_append", (k_cache, v_cache, k_scale, v_scale, k, v, start, count), (), 0) is not None:
         return None

@@ -9,7 +9,7 @@ import torch
 
 import operators_reference as ref
 from mlc import ops
-from test_operators import HALF, _heads, _refused, filled, gpu, host, ints, parts
+from test_operators import E4M3, FULL, HALF, _heads, _refused, filled, gpu, host, ints, normal, parts
 
 
 # --------------------------------------------------------------------------
@@ -159,3 +159,31 @@ def test_a_module_whose_weights_ask_for_gradients_is_exported():
 
     program = torch.export.export(M().eval(), (host(1, 3, 2, 64),))
     assert any("mlc.attention" in str(n.target) for n in program.graph.nodes)
+
+# --------------------------------------------------------------------------
+# memory
+# --------------------------------------------------------------------------
+
+def _pool():
+    codes = torch.zeros(3, 2, 64, 64, dtype=torch.uint8, device="cuda").view(E4M3)
+    return codes, torch.ones(3, 2, 4, device="cuda")
+
+
+@gpu
+def test_operands_that_lie_in_a_cache_that_changes_are_refused():
+    """In part, too: two caches or scales cut out of one pool, scales inside of keys."""
+    codes, scales = _pool()
+    apart, ones = torch.zeros_like(codes), torch.ones_like(scales)
+    scales, ones = scales[..., :2].contiguous(), ones[..., :2].contiguous()
+    k, start = normal(2, 1, 2, 64), ints([0, 0])
+    one = (codes[:2], apart[:2], scales[:2], ones[:2])
+    inside = codes[1:].view(torch.uint8).flatten()[:2 * 2 * 2 * 4].view(FULL).view(2, 2, 2)
+    inside.fill_(1.0)
+    for bad in ((codes[:2], codes[1:], scales[:2], ones[:2]), (*one[:2], scales[:2], scales[1:]),
+                (codes[:2], apart[:2], inside, ones[:2])):
+        _refused(lambda: ops.cache_append(*bad, k, k, start), "share")
+    rows = codes[:2].view(torch.uint8).flatten()[:2 * 2 * 64 * 2].view(HALF).view(2, 1, 2, 64)
+    _refused(lambda: ops.cache_append(*one, rows, k, start), "share")
+    _refused(lambda: ops.cache_append(*one, k, k, scales.flatten()[:2].view(torch.int32)), "share")
+    ops.cache_append(codes[:1], codes[1:2], scales[:1], scales[1:2], k[:1], k[:1], start[:1])  # side by side
+    ops.check_errors()
