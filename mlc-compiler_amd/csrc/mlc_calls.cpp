@@ -252,6 +252,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   Py_END_ALLOW_THREADS
   if (rc != 0) return PyLong_FromLong(rc);
+  for (Py_ssize_t i = 0; i < entry->changed && i < operands; ++i)  // autograd asks whether what it kept has changed
+    if (x[i] != nullptr && !x[i]->is_inference()) x[i]->unsafeGetTensorImpl()->bump_version();
   PyObject* const made = PyTuple_New(results);
   if (made == nullptr) return nullptr;
   for (Py_ssize_t i = 0; i < results; ++i) PyTuple_SET_ITEM(made, i, THPVariable_Wrap(std::move(out[i])));

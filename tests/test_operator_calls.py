@@ -187,3 +187,24 @@ def test_operands_that_lie_in_a_cache_that_changes_are_refused():
     _refused(lambda: ops.cache_append(*one, k, k, scales.flatten()[:2].view(torch.int32)), "share")
     ops.cache_append(codes[:1], codes[1:2], scales[:1], scales[1:2], k[:1], k[:1], start[:1])  # side by side
     ops.check_errors()
+
+
+@gpu
+def test_autograd_sees_that_a_cache_changed():
+    cache = filled(1, 1, 64, 64)
+    k, start = normal(1, 1, 1, 64), ints([3])
+    before = [x._version for x in parts(cache)]
+    cache.append(k, k, start)
+    assert all(x._version > b for x, b in zip(parts(cache), before))
+    w = torch.ones_like(cache.key_scales, requires_grad=True)
+    y = (w * cache.key_scales).sum()  # keeps the scales for its backward
+    cache.append(k, k, start)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    before = [x._version for x in parts(cache)]
+    cache.attend(normal(1, 1, 2, 64), start)
+    assert [x._version for x in parts(cache)] == before
+    with torch.inference_mode():  # which counts no versions
+        other = filled(1, 1, 64, 64)
+        other.append(k, k, start)
+    other.append(k, k, start)
