@@ -214,6 +214,8 @@ class _Buffers:
                 raise ExecutionError(
                     f"buffer {graph.param_origin[v.name]} is changed in place, and a copy of it would "
                     f"be: it has to be contiguous and on {model.device} before the model is compiled")
+        #: those of them that count versions, by which autograd sees a change
+        self.versioned = [t for n, t in self.params.items() if n in self.changed and not t.is_inference()]
         #: products of groups that run as one launch, which never stores them
         self.unstored = {schedule.kernels[i].outputs[0].buffer.name: schedule.kernels[i].outputs[0].buffer
                          for i in schedule.merged}
@@ -569,9 +571,14 @@ class CompiledModel:
         if fetch is not None:
             fetch()
 
+    def _count_versions(self) -> None:
+        if self._buffers.versioned:
+            torch.autograd.graph.increment_version(self._buffers.versioned)
+
     def forward(self, *inputs: torch.Tensor):
         """One uncaptured run."""
         self._check_inputs(inputs)
+        self._count_versions()
         plan = self.schedule.plan
         if plan is not None and plan.mode == "eager":
             table = self._buffers.per_call(inputs)
@@ -595,6 +602,7 @@ class CompiledModel:
             out = self.forward(*inputs)
         else:
             self._check_inputs(inputs)
+            self._count_versions()
             if self._runs is None:
                 self._resolve(self._buffers.resident(inputs))
             if self._direct:

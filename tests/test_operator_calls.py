@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import mlc
 import operators_reference as ref
 from mlc import ops
 from test_operators import E4M3, FULL, HALF, _heads, _refused, filled, gpu, host, ints, normal, parts
@@ -208,3 +209,26 @@ def test_autograd_sees_that_a_cache_changed():
         other = filled(1, 1, 64, 64)
         other.append(k, k, start)
     other.append(k, k, start)
+
+
+class _Step(torch.nn.Module):
+    def __init__(self, cache):
+        super().__init__()
+        self.cache = cache
+
+    def forward(self, k, start):
+        self.cache.append(k, k, start)
+        return self.cache.attend(k, start)
+
+
+@gpu
+@pytest.mark.parametrize("config", [{}, {"memory_planning": False}, {"cuda_graphs": False}],
+                         ids=("graph", "unplanned", "planned"))
+def test_autograd_sees_that_a_compiled_model_changed_its_cache(config):
+    m = _Step(filled(1, 2, 64, 64))
+    args = normal(1, 1, 2, 64), ints([3])
+    compiled = mlc.compile(m, args, mlc.Config(**config))
+    for _ in range(2):
+        before = [x._version for x in parts(m.cache)]
+        compiled(*args)
+        assert all(x._version > b for x, b in zip(parts(m.cache), before))
