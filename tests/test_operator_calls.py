@@ -4,13 +4,15 @@ operands, many sequences of uneven lengths."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import mlc
 import operators_reference as ref
 from mlc import ops
-from test_operators import E4M3, FULL, HALF, _heads, _refused, filled, gpu, host, ints, normal, parts
+from test_operators import BF, E4M3, FULL, HALF, _heads, _refused, filled, gpu, host, ints, normal, parts
 
 
 # --------------------------------------------------------------------------
@@ -232,3 +234,59 @@ def test_autograd_sees_that_a_compiled_model_changed_its_cache(config):
         before = [x._version for x in parts(m.cache)]
         compiled(*args)
         assert all(x._version > b for x, b in zip(parts(m.cache), before))
+
+# --------------------------------------------------------------------------
+# over the cache
+# --------------------------------------------------------------------------
+
+def _items(lengths, kv_heads, capacity, dim=64, block=64):
+    """How the kernel cuts sequences of these lengths, ``[first item, items]`` of each, from the
+    memory that its launches share."""
+    from mlc.codegen import hip_operators as plans
+    from mlc.runtime import native, operators
+
+    batch = len(lengths)
+    cache = ops.KeyValueCache(batch, kv_heads, capacity, dim, block=block, device="cuda")
+    q, start = normal(batch, 1, kv_heads, dim), ints([n - 1 for n in lengths])
+    operands = {"q": q, **dict(zip(("k_cache", "v_cache", "k_scale", "v_scale"), parts(cache))), "start": start}
+    plan = plans.plan_cache_attention(*map(ops._operand, operands.values()), None, None, 0.125, 0.0)
+    modules, launch, out = operators.device_modules(0), plan.launches[0], torch.empty_like(q)
+    space = torch.zeros(plan.workspace, dtype=torch.uint8, device="cuda")
+    at = {n: x.data_ptr() for n, x in operands.items()}
+    at.update(out0=out.data_ptr(), workspace=space.data_ptr(), error=modules.error_word())
+    args = launch.arguments(at)
+    native.check(modules.lib.mlc_launch(modules.function(launch), launch.grid, launch.block, 0, args, len(args),
+                                        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    torch.cuda.synchronize()
+    return space.view(torch.int32)[:2 * batch].view(batch, 2).tolist(), launch.grid // kv_heads
+
+
+@gpu
+@pytest.mark.parametrize("lengths", [
+    [819 + 117 * i for i in range(64)],          # as many sequences as items are wanted
+    [65536] + [200] * 255,                       # one that is long among many
+    [1] * 69 + [32768],
+    [8192] * 3 + [64] * 5,
+], ids=("even", "one", "tokens", "few"))
+def test_the_cache_is_cut_into_even_items_however_many_sequences(lengths):
+    """None is longer than two even shares, rounded up to whole steps of 64 keys."""
+    found, slots = _items(lengths, 8, max(lengths) + 63 & ~63)
+    at = 0
+    for first, n in found:  # one behind the other, and within the launch
+        assert first == at and n >= 1
+        at += n
+    assert at <= slots
+    even = max(sum(lengths) / 64, 512)
+    assert max(-(-n // of) for n, (_, of) in zip(lengths, found)) <= 2 * (even + 64)
+
+
+@gpu
+def test_cache_attention_of_many_sequences_of_uneven_lengths():
+    lengths = [1 + 37 * i for i in range(65)] + [1, 64, 65, 8192, 8191]
+    cache = filled(len(lengths), 8, 8192, 64)
+    q, start = normal(len(lengths), 1, 8, 64, dtype=BF), ints([n - 1 for n in lengths])
+    got = cache.attend(q, start)
+    some = [0, 30, 63, 64, 65, 66, 67, 68, 69]
+    held = [x[some] for x in (x.view(torch.uint8) for x in parts(cache))]
+    held = [x.view(y.dtype) for x, y in zip(held, parts(cache))]
+    ref.close(got[some], *ref.cache_attention(q[some], *held, start[some]))
