@@ -445,6 +445,14 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       }
     }
     if constexpr (MASKED) {
+      if constexpr (CACHE) {
+        // before the mask: the scale of a key block may be zero, and a mask's -infinity times it NaN
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[u][j] *= scale;
+        scale = 1.0f;
+      }
       const int own = lim - base - 8 * h;
 #pragma unroll
       for (int u = 0; u < U; ++u)

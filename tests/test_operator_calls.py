@@ -290,3 +290,30 @@ def test_cache_attention_of_many_sequences_of_uneven_lengths():
     held = [x[some] for x in (x.view(torch.uint8) for x in parts(cache))]
     held = [x.view(y.dtype) for x, y in zip(held, parts(cache))]
     ref.close(got[some], *ref.cache_attention(q[some], *held, start[some]))
+
+
+@pytest.fixture(params=("rows", "tiles"))
+def way(request, monkeypatch):
+    """Both ways that rows go over the cache, whatever their number."""
+    from mlc.codegen import hip_operators
+
+    if request.param == "tiles":
+        monkeypatch.setattr(hip_operators, "MANY_PRODUCTS", 0)
+        monkeypatch.setattr(hip_operators, "MANY_ROWS", 1)
+    ops._plans.clear()
+    yield request.param
+    ops._plans.clear()
+
+
+@gpu
+@pytest.mark.parametrize("options", ({}, {"scale": 2.0 ** -60}, {"cap": 5.0}), ids=("", "scale", "cap"))
+def test_blocks_of_zero_scale_behind_a_row_and_under_it(way, options):
+    """A mask's -infinity is not multiplied by a factor of zero: a scale of zero, or one of
+    2^-126 (of a block of zeros) times a small ``scale``."""
+    cache = filled(2, 1, 256, 64)
+    cache.key_scales[0, 0, 1:3] = torch.tensor([0.0, 2.0 ** -126])
+    cache.key_scales[1, 0] = 2.0 ** -126
+    q, start = normal(2, 70, 2, 64, dtype=BF), ints([90, 186])
+    got = cache.attend(q, start, **options)
+    assert got.isfinite().all()
+    ref.close(got, *ref.cache_attention(q, *parts(cache), start, **options))
