@@ -46,6 +46,13 @@ class Operand:
     aligned: bool = True
 
 
+def require_aligned(operands: dict) -> None:
+    """Caches and their scales lie on 16 bytes: kernels take their rows in such pieces."""
+    for name, x in operands.items():
+        if name.endswith(("_cache", "_scale")) and not x.aligned:
+            raise OperatorError(f"{name}: not on 16 bytes")
+
+
 @dataclass(frozen=True)
 class Launch:
     """One kernel launch: ``pointers`` names what its leading arguments point

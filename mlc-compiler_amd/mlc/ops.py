@@ -225,10 +225,9 @@ def _add(signature: bytes, op: str, operands: tuple, options: tuple, results: in
     """The launches of a call of a new signature, checked."""
     check, plan, names = _OPERATORS[op]
     check(*operands, *options)
-    for name, x in zip(names, operands):
-        if name.endswith("cache") or name.endswith("_scale"):
-            _require(x.data_ptr() % 16 == 0, f"{name}: not on 16 bytes")
-    made = plan(*map(_operand, operands), *options)
+    seen = tuple(map(_operand, operands))
+    plans.require_aligned(dict(zip(names, seen)))
+    made = plan(*seen, *options)
     changed = len(_CACHE) if op == "cache_append" else 0
     _plans.add(signature, made, names, changed, results, operands[0].get_device())
 

@@ -225,6 +225,7 @@ class HipRuntime:
                                                    (t.data_ptr() + offset) % 16 == 0)
         for i, v in enumerate(k.outputs):
             pointers[f"out{i}"] = buffers[v.buffer.name].data_ptr()
+        hip_operators.require_aligned(operands)
         plan = hip_operators.PLANS[k.node.op](**operands)
         if self._error_word is not None:
             pointers["error"] = self._error_word

@@ -235,6 +235,21 @@ def test_autograd_sees_that_a_compiled_model_changed_its_cache(config):
         compiled(*args)
         assert all(x._version > b for x, b in zip(parts(m.cache), before))
 
+
+@gpu
+@pytest.mark.parametrize("name", ("keys", "value_scales"))
+def test_a_compiled_model_refuses_a_cache_off_16_bytes(name):
+    cache = filled(1, 2, 128, 64)
+    x = cache._buffers[name]
+    raw = torch.zeros(x.numel() * x.element_size() + 16, dtype=torch.uint8, device="cuda")
+    at = raw[4:4 + x.numel() * x.element_size()].view(x.dtype if x.dtype == E4M3 else FULL).view(x.shape)
+    at.copy_(x)
+    cache._buffers[name] = at
+    args = normal(1, 1, 2, 64), ints([0])
+    _refused(lambda: cache.append(args[0], args[0], args[1]), "16 bytes")
+    with pytest.raises(ops.OperatorError, match="16 bytes"):
+        mlc.compile(_Step(cache), args)(*args)
+
 # --------------------------------------------------------------------------
 # over the cache
 # --------------------------------------------------------------------------
