@@ -371,7 +371,8 @@ class _Translation:
 
     def _check_changes(self) -> None:
         """A buffer's old contents cannot be read beside the new ones: nothing
-        orders such a reader before the change."""
+        orders such a reader before the change. So what a pass reads of a buffer
+        it reads after its last change."""
         readers: dict[int, list[Node]] = self.graph.use_map()
         windows: dict[int, list[Value]] = {}
         for node in self.graph.nodes:
@@ -388,10 +389,17 @@ class _Translation:
                 while seen:
                     at = seen.pop()
                     seen += windows.get(id(at), [])
-                    if any(n is not node for n in readers.get(id(at), [])) or any(
-                            at is o for o in self.graph.outputs):
-                        raise CaptureError(f"{v.name} is read by another operator beside "
-                                           f"{node.op}, which changes it: read it after the change")
+                    others = [n for n in readers.get(id(at), []) if n is not node]
+                    returned = any(at is o for o in self.graph.outputs)
+                    if not others and not returned:
+                        continue
+                    by = others[0].op if others else "the module's result"
+                    if v.producer is not None and v.producer.meta.get("pin"):
+                        raise CaptureError(f"{v.name} is changed once more after {by} read it: {node.op} "
+                                           "may change a buffer again only where nothing has read it "
+                                           "in between. Compile one step and call it twice")
+                    raise CaptureError(f"{v.name} is read by another operator beside {node.op}, which "
+                                       f"changes it ({by}): read it after the change")
 
     def _view(self, fx, op, args, kwargs) -> Value:
         """A restride of the source's buffer. When the requested view needs

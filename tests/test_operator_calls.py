@@ -332,3 +332,24 @@ def test_blocks_of_zero_scale_behind_a_row_and_under_it(way, options):
     got = cache.attend(q, start, **options)
     assert got.isfinite().all()
     ref.close(got, *ref.cache_attention(q, *parts(cache), start, **options))
+
+# --------------------------------------------------------------------------
+# in compiled models
+# --------------------------------------------------------------------------
+
+def test_a_cache_changed_again_after_it_was_read_is_refused_by_its_reason():
+    from mlc.ir.capture import CaptureError, capture
+
+    class Twice(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.cache = ops.KeyValueCache(2, 2, 128, 64)
+
+        def forward(self, k, start):
+            self.cache.append(k, k, start)
+            a = self.cache.attend(k, start)
+            self.cache.append(a, a, start + 1)
+            return self.cache.attend(a, start + 1)
+
+    with pytest.raises(CaptureError, match="changed once more after mlc.cache_attention.default read it"):
+        capture(Twice(), (host(2, 1, 2, 64), torch.zeros(2, dtype=torch.int32)))
