@@ -39,6 +39,7 @@ GPU.
 
 from __future__ import annotations
 
+import collections
 from dataclasses import dataclass
 from typing import Any, Sequence
 
@@ -214,6 +215,10 @@ class _Buffers:
                 raise ExecutionError(
                     f"buffer {graph.param_origin[v.name]} is changed in place, and a copy of it would "
                     f"be: it has to be contiguous and on {model.device} before the model is compiled")
+        #: those of them that a pass changes more than once, so that a second pass need not leave
+        #: what one does (``cache_append`` rounds codes again where a scale grows)
+        writes = collections.Counter(v.buffer.name for k in schedule.kernels for v in k.writes())
+        self.changed_again = [self.params[n] for n in self.changed if writes[n] > 1]
         #: those of them that count versions, by which autograd sees a change
         self.versioned = [t for n, t in self.params.items() if n in self.changed and not t.is_inference()]
         #: products of groups that run as one launch, which never stores them
@@ -629,15 +634,20 @@ class CompiledModel:
         """Three warm-up runs on a side stream (modules loaded, library
         workspaces allocated), then one run captured into the context's
         hipGraph. Capture must allocate nothing: every library call writes a
-        pre-bound slice, and an allocation is reported with its culprits."""
+        pre-bound slice, and an allocation is reported with its culprits. What
+        the warm-up runs leave in buffers that a pass changes is what one leaves,
+        or taken back."""
         self._check_inputs(inputs)
         table = self._buffers.resident(inputs)
         self._resolve(table)
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
+            kept = [t.clone() for t in self._buffers.changed_again]
             for _ in range(3):
                 self.run_kernels(table)
+            for t, was in zip(self._buffers.changed_again, kept):
+                t.copy_(was)
             side.synchronize()
             before = _alloc_count(self.device)
             self._module.capture_begin(side.cuda_stream)

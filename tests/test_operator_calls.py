@@ -337,6 +337,32 @@ def test_blocks_of_zero_scale_behind_a_row_and_under_it(way, options):
 # in compiled models
 # --------------------------------------------------------------------------
 
+@gpu
+def test_many_appends_of_one_pass_round_as_direct_calls():
+    """Token by token into one block, each larger than those before, so that the scale grows and
+    codes are rounded again and again: a first call that makes a graph runs once for its caller."""
+
+    class Appends(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.cache = filled(2, 2, 64, 64)
+
+        def forward(self, k, start):
+            for i in range(k.shape[1]):
+                self.cache.append(k[:, i:i + 1], k[:, i:i + 1], start + i)
+            return self.cache.attend(k[:, :1], start)
+
+    m, other = Appends(), Appends()
+    k = normal(2, 20, 2, 64, spread=2.0 ** -5) * torch.arange(20, device="cuda").exp2()[:, None, None].sqrt()
+    k = (k * normal(2, 20, 2, 64, dtype=FULL, seed=3, spread=5.0).exp2()).half()
+    compiled = mlc.compile(m, (k, ints([1, 7])))
+    for start in ([1, 7], [21, 30]):
+        compiled(k, ints(start))
+        other(k, ints(start))
+        for x, y in zip(parts(m.cache), parts(other.cache)):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 def test_a_cache_changed_again_after_it_was_read_is_refused_by_its_reason():
     from mlc.ir.capture import CaptureError, capture
 
