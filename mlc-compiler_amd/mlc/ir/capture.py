@@ -110,11 +110,30 @@ def _in_eval_mode(model: torch.nn.Module):
         model.train(restore)
 
 
+def _shared_buffers(model: torch.nn.Module) -> tuple[str, str] | None:
+    """Two names of buffers that share memory."""
+    seen: dict[int, str] = {}
+    for name, x in model.named_buffers(remove_duplicate=False):
+        if x is None or not x.numel():
+            continue
+        other = seen.setdefault(x.untyped_storage().data_ptr(), name)
+        if other != name:
+            return other, name
+    return None
+
+
 def _export(model: torch.nn.Module, example: tuple, extra: Sequence[str]):
     with _in_eval_mode(model), torch.no_grad(), warnings.catch_warnings():
         warnings.simplefilter("ignore")
-        program = export(model, example)
-        return program.run_decompositions(_decomposition_table(extra))
+        try:
+            return export(model, example).run_decompositions(_decomposition_table(extra))
+        except AssertionError as e:  # what the exporter makes of a change seen under two names
+            shared = _shared_buffers(model)
+            if shared is None:
+                raise
+            raise CaptureError(f"{shared[0]} and {shared[1]} share memory, and a buffer that changes "
+                               "may have one name only: keep a cache that several modules use in one "
+                               "of them and hand it to the others' calls") from e
 
 
 def capture(model: torch.nn.Module, example_inputs: tuple, *, name: str | None = None,

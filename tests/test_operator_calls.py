@@ -379,3 +379,29 @@ def test_a_cache_changed_again_after_it_was_read_is_refused_by_its_reason():
 
     with pytest.raises(CaptureError, match="changed once more after mlc.cache_attention.default read it"):
         capture(Twice(), (host(2, 1, 2, 64), torch.zeros(2, dtype=torch.int32)))
+
+
+def test_a_cache_under_several_names_is_refused_by_its_reason():
+    from mlc.ir.capture import CaptureError, capture
+
+    class Layer(torch.nn.Module):
+        def __init__(self, cache, fills):
+            super().__init__()
+            self.cache, self.fills = cache, fills
+
+        def forward(self, k, start):
+            if self.fills:
+                self.cache.append(k, k, start)
+            return self.cache.attend(k, start)
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            cache = ops.KeyValueCache(2, 2, 128, 64)
+            self.one, self.two = Layer(cache, True), Layer(cache, False)
+
+        def forward(self, k, start):
+            return self.two(self.one(k, start), start)
+
+    with pytest.raises(CaptureError, match="one.cache.keys and two.cache.keys share memory"):
+        capture(Model(), (host(2, 1, 2, 64), torch.zeros(2, dtype=torch.int32)))
