@@ -240,11 +240,14 @@ class _Buffers:
         return table
 
     def per_call(self, inputs: Sequence[torch.Tensor]) -> dict[str, torch.Tensor]:
-        """Eager mode: the caller's inputs used in place, intermediates come
-        and go with the alloc/free plan."""
+        """Eager mode: the caller's inputs used in place, but for one in memory
+        that the pass changes; intermediates come and go with the alloc/free plan."""
         table = self._base()
+        changed = [_span(self.params[n]) for n in self.changed]
         for v, t in zip(self.model.graph.inputs, inputs):
-            table[v.buffer.name] = t.to(self.model.device).contiguous().reshape(-1)
+            t = t.to(self.model.device).contiguous().reshape(-1)
+            lo, hi = _span(t)
+            table[v.buffer.name] = t.clone() if any(lo < b and a < hi for a, b in changed) else t
         return table
 
     def resident(self, inputs: Sequence[torch.Tensor]) -> dict[str, torch.Tensor]:
@@ -303,6 +306,11 @@ class _Buffers:
 # --------------------------------------------------------------------------
 # the model
 # --------------------------------------------------------------------------
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """Where a contiguous tensor begins and ends."""
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
 
 def _address(t: torch.Tensor, own: torch.Tensor) -> int:
     """Where a kernel may read the caller's ``t`` in the place of the input
@@ -442,8 +450,7 @@ class CompiledModel:
             mine = {id(t) for t in (*self._buffers.inputs,
                                     *(t for n, t in self.params.items() if n not in changed))}
             held = [t for t in table.values() if id(t) not in mine]
-            self._own = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                         for t in (*held, *([self._arena] if self._arena is not None else []))]
+            self._own = [_span(t) for t in (*held, *([self._arena] if self._arena is not None else []))]
             self._direct = True
 
     def _launch_directly(self) -> bool:
@@ -545,8 +552,7 @@ class CompiledModel:
         """Address ranges of the inputs' buffers that outputs are views of."""
         if self._shown is None:
             outputs = {v.buffer.name for v in self.graph.outputs}
-            self._shown = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                           for v, t in zip(self.graph.inputs, self._buffers.inputs)
+            self._shown = [_span(t) for v, t in zip(self.graph.inputs, self._buffers.inputs)
                            if v.buffer.name in outputs]
         return self._shown
 

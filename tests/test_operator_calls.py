@@ -250,6 +250,25 @@ def test_a_compiled_model_refuses_a_cache_off_16_bytes(name):
     with pytest.raises(ops.OperatorError, match="16 bytes"):
         mlc.compile(_Step(cache), args)(*args)
 
+
+@gpu
+def test_an_input_that_lies_in_a_cache_that_changes_is_read_as_it_was():
+    """By a compiled model whose inputs are read in place."""
+
+    class M(_Step):
+        def forward(self, k, start, x):
+            y = super().forward(k, start)
+            return y, x * 2.0 + y[..., :2].reshape(1, 2, 2).float() * 0.0  # behind the change
+
+    m = M(filled(1, 2, 128, 64))
+    k, start = normal(1, 1, 2, 64), ints([0])
+    for config in ({}, {"memory_planning": False, "cuda_graphs": False}, {"cuda_graphs": False}):
+        compiled = mlc.compile(m, (k, start, m.cache.key_scales.clone()), mlc.Config(**config))
+        for i in range(2):
+            m.cache.key_scales.fill_(2.0 ** (20 + i))  # the append starts it anew
+            want = m.cache.key_scales * 2.0
+            assert torch.equal(compiled(k, start, m.cache.key_scales)[1], want)
+
 # --------------------------------------------------------------------------
 # over the cache
 # --------------------------------------------------------------------------
