@@ -252,6 +252,22 @@ def test_a_compiled_model_refuses_a_cache_off_16_bytes(name):
 
 
 @gpu
+def test_a_lazy_copy_of_a_cache_is_changed_and_its_source_is_not():
+    cache = filled(1, 2, 128, 64)
+    copy = [torch._lazy_clone(x) for x in parts(cache)]
+    kept = [x.clone().view(torch.uint8) for x in parts(cache)]
+    k, start = normal(1, 3, 2, 64, spread=50.0), ints([62])
+    wants = [ref.cache_append(c, s, k, start) for c, s in ((cache.keys, cache.key_scales),
+                                                           (cache.values, cache.value_scales))]
+    ops.cache_append(*copy, k, k, start)
+    for (codes, scales), c, s in zip(wants, copy[:2], copy[2:]):
+        assert torch.equal(c.view(torch.uint8).cpu(), torch.from_numpy(codes))
+        assert torch.equal(s.double().cpu(), torch.from_numpy(scales))
+    for x, y in zip(parts(cache), kept):
+        assert torch.equal(x.view(torch.uint8), y)
+
+
+@gpu
 def test_an_input_that_lies_in_a_cache_that_changes_is_read_as_it_was():
     """By a compiled model whose inputs are read in place."""
 
@@ -355,6 +371,38 @@ def test_blocks_of_zero_scale_behind_a_row_and_under_it(way, options):
 # --------------------------------------------------------------------------
 # in compiled models
 # --------------------------------------------------------------------------
+
+@gpu
+def test_many_layers_over_caches_of_their_own_are_the_direct_calls_to_the_bit():
+    """Every attention over a cache is used, so all of them are in the graph, replayed
+    between other work."""
+
+    class Layers(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.caches = torch.nn.ModuleList(filled(2, 2, 2048, 64, seed=i) for i in range(12))
+            f, _ = ops.rotary_frequencies(64, device="cuda")
+            self.register_buffer("f", f)
+
+        def forward(self, q, k, start):
+            for cache in self.caches:
+                q, b = ops.rotary(q, k, start.unsqueeze(1), self.f)
+                cache.append(b, k, start)
+                q = cache.attend(q, start)
+            return q
+
+    m, other = Layers(), Layers()
+    q, k = normal(2, 1, 4, 64, dtype=BF), normal(2, 1, 2, 64, dtype=BF, seed=1)
+    compiled = mlc.compile(m, (q, k, ints([0, 0])))
+    assert sum("mlc.cache_attention" in x.summary() for x in compiled.schedule) == 12
+    for i, at in enumerate(([5, 1999], [6, 2000], [2047, 0])):
+        got = compiled(q * (1 + i), k, ints(at)).clone()
+        assert torch.equal(got, other(q * (1 + i), k, ints(at)))
+        for a, b in zip(m.caches, other.caches):
+            for x, y in zip(parts(a), parts(b)):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    compiled.check_errors()
+
 
 @gpu
 def test_many_appends_of_one_pass_round_as_direct_calls():
