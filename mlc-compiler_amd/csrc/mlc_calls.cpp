@@ -26,6 +26,7 @@
 #include <cstring>
 #include <iterator>
 #include <memory>
+#include <optional>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -211,11 +212,14 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (word != 0) Py_RETURN_TRUE;
   }
   std::vector<c10::IValue> inputs;  // outlives the record
-  at::RecordFunction record(at::RecordScope::FUNCTION);  // the dispatcher makes one of its own
-  if (record.isActive() && !(flags & kDispatched) && op >= 0 && op < static_cast<long>(std::size(kOperators))) {
-    if (record.needsInputs())
+  std::optional<at::RecordFunction> record;
+  if (auto callbacks = at::getStepCallbacksUnlessEmpty(at::RecordScope::FUNCTION);
+      callbacks.has_value() && !(flags & kDispatched) &&  // the dispatcher makes a record of its own
+      op >= 0 && op < static_cast<long>(std::size(kOperators))) {
+    record.emplace(std::move(*callbacks));
+    if (record->needsInputs())
       for (Py_ssize_t i = 0; i < operands; ++i) inputs.push_back(x[i] ? c10::IValue(*x[i]) : c10::IValue());
-    record.before(kOperators[op], &inputs);
+    record->before(kOperators[op], &inputs);
   }
   PyObject* const index = PyLong_FromLong(device);
   if (index == nullptr) return nullptr;
