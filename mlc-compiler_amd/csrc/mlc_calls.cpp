@@ -5,6 +5,9 @@
 // rest. One token's operators are bound by the host: a call with four to eight operands
 // takes 4-6 us, of which a launch is 2.3 and a result 1; the same in Python took 8-10.
 //
+// Where something looks on (a tracer, a mode, a transform) a call is handed back, to go through
+// torch's dispatcher; a profiler gets a record from here.
+//
 // Nothing is kept by an operand's address or identity. The table is used under the
 // interpreter's lock, which launches are made without.
 

@@ -193,9 +193,17 @@ def attention_split(rows: int, pairs: int, keys: int, dim: int, teams: tuple, ap
 
     Waves that share tiles have 32 rows each, and two such workgroups fit a unit; waves
     apart have the same 32 rows, a quarter of the tiles one behind the other, four times the
-    workgroups, and one fits a unit. 1000 tokens, 12 heads of 64: shared 19.3, apart 12.3; 3 x
-    1024, 4 heads of 128 with a bias 34.9, 24.0; 4096, 8 heads of 128 73, 85; 4 x 300, 32 heads
-    over 8 of 128 16, 32.
+    workgroups, and one fits a unit. Causal, bf16: 1000 tokens, 12 heads of 64 shared 18.6, apart
+    11.2; 3 x 1024, 4 heads of 128 28.5, 17.4; 4096, 8 heads of 128 69, 83; 4 x 300, 32 heads over
+    8 of 128 15, 31.
+
+    All keys are priced for every row. A causal mask leaves out half of both ways' tiles, and
+    without one the same ways are faster (18.5, 16.5; 29.9, 26.6; 93, 142; 19, 39). How much
+    documents and prefixes leave out is known on the device alone; with documents: 4096 tokens, 8
+    heads of 128, 8 documents 38, 64 and one 78, 137; 3 x 2021, 16 heads over 4 of 96, 8 documents
+    41, 129; 4 x 1000, 16 heads of 64, 8 documents 18, 74; 6 x 999, 8 heads of 256, 5 documents 64,
+    118; 300, 4 heads of 128, 2 documents 13.1, 11.9; 1000, 12 heads of 64, 4 documents 20.4, 20.5:
+    what the rule takes is within 5 % of the better one in all of them.
 
     Splits fill the device where there are few workgroups. What they cost is a second
     launch and parts of O in fp32, written and read: 4 us and 8 bytes a value at 3 TB/s."""
@@ -324,8 +332,8 @@ CACHED_DIMS = (64, 128, 256)
 #: products of scores and values from which on rows go through tiles of 128
 #: (``attention.hip``) and not of 16: keys are widened once for all of them, in more
 #: launches of work that is fixed. Tiles of 128 / 16, 8 key heads of 128: 4 x 128 rows over
-#: 2048 keys (1.1e9) 27 / 25 us, 4 x 512 (4.3e9) 46 / 58, 512 over 16384 (8.6e9) 75 / 102;
-#: 2 x 488 rows of 2 heads over 8192 (2.0e9) 40 / 36, over 16384 (4.1e9) 50 / 58.
+#: 2048 keys (1.1e9) 25 / 22 us, 4 x 512 (4.3e9) 39 / 53, 512 over 16384 (8.6e9) 61 / 97;
+#: 2 x 488 rows of 2 heads over 8192 (2.0e9) 34 / 35, over 16384 (4.1e9) 41 / 55.
 MANY_ROWS, MANY_PRODUCTS = 128, 3e9
 
 

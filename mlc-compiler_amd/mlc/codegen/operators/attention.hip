@@ -14,11 +14,14 @@
 //  * The softmax is online: a running maximum, the sum and O scaled when it grows.
 //
 // Long rows are bound by the softmax's vector work beside the products, and by the clock,
-// which falls under them: 8192 tokens, 32 heads over 8 of 128, bf16, causal 552 us, 995
-// TFLOP/s, without a mask 1045 (a library's product of 8192^3 reaches 1214); a cap adds two
-// transcendentals to a score's one, 666 us, 825 TFLOP/s. Short ones are bound by a chain of
-// loads and products that few waves hide: 32 x 512 tokens, 12 heads of 64, fp16, causal 32
-// us, with a bias and prefixes 40 (19 to move the bytes); 128 tokens, 12 heads 5.6.
+// which falls under them and differs from card to card: 8192 tokens, 32 heads over 8 of 128,
+// bf16, causal 550 to 570 us, 970 TFLOP/s, without a mask 1100 us, 1000 TFLOP/s (a library's
+// product of 8192^3 reaches 1214); a cap adds two transcendentals to a score's one, 660 to 715
+// us, 800 TFLOP/s. Short ones are bound by a chain of loads and products that few waves hide:
+// 32 x 512 tokens, 12 heads of 64, fp16, causal 34 us, with a bias and prefixes 38 to 40 (19 to
+// move the bytes), vector units 55 % and matrix units 15 % of the time busy; 128 tokens, 12 heads
+// 5.3. 4 x 2048 tokens, 8 heads of 256, causal 107 us for 57 of products: tiles of 32 keys, each
+// behind a wait and a barrier, two waves a SIMD.
 //
 // Tried and slower: 8 waves a workgroup and 4 buffers (916 against 960 TFLOP/s then), the
 // scores of a tile before the softmax of the one before (registers spill), the sums as one
@@ -486,6 +489,10 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       m = next;
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m;
+    // Weights are rounded to 16 bits, as a product of 16-bit values takes them; the sum is of what
+    // they were. Against 64 bits results are so off by 2.0e-3 to 2.2e-3 (bf16, root of the mean
+    // square) and 2.2e-4 to 2.4e-4 (fp16), where the result's own rounding makes 1.6e-3 and
+    // 2.0e-4. With the sum of the rounded weights 1.9e-3 to 2.1e-3, in 2 to 7 % more time.
     p8 p[2 * U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -589,8 +596,9 @@ __device__ __forceinline__ void attention(const AttentionArgs& a) {
       // A tile whose documents lie outside is left out, one that is of the rows' only
       // document needs no mask: tiles are looked through SPAN at a time, 8 keys a lane, or, by
       // a wave apart, a tile. That takes 2 us a span, a tile without a mask 2 and with one 3:
-      // 3 x 2021 tokens, 16 heads over 4 of 96, bf16, causal, 8 documents a row 39 us, 64 29
-      // us, one 74 (63 without).
+      // 3 x 2021 tokens, 16 heads over 4 of 96, bf16, causal, 8 documents a row 39 to 45 us, 64
+      // 29 us, one 67 to 75 (55 to 63 without). Latency bounds it: vector units are 25 %, matrix
+      // units 6 % of the time busy.
       constexpr int LANES = APART ? 1 : KEYS / 8, PER_WAVE = 64 / LANES, SPAN = PER_WAVE * TEAM;
       static_assert(SPAN <= 64, "bits");
       auto least = [](int x, int y) { return x < y ? x : y; };

@@ -18,11 +18,15 @@
 // The waves of a workgroup are joined in LDS, the items of a sequence by a second
 // kernel (cache_attention_join).
 //
-// One token, 32 heads over 8 of 128, bf16: 32 sequences of up to 8192 keys 60 us, 5.1 TB/s,
-// one of 131072 48 us, 5.6 TB/s (a read reaches 6.2; the join is 4 us of each); 12 heads of
-// 64 over 1024 keys 7.0 us, the latency of one workgroup's steps. Many rows are bound by
-// the widening of codes, which every 16 rows do again: 2 x 61 tokens, 16 heads over 2, 4096
-// keys 24 us, where tiles of 128 rows (attention.hip) take 32.
+// One token, 32 heads over 8 of 128, bf16: 32 sequences of up to 8192 keys 63 to 67 us a call,
+// 4.6 TB/s, one of 131072 55 to 57 us, 4.8 TB/s (a read reaches 6.2; the join is 4 us of each);
+// over the same cache again and again, some of it in the last-level cache, 57 and 48 us. 12 heads
+// of 64 over 1024 keys 6.3 us, the latency of one workgroup's steps. Tens of rows are bound by
+// latency too: 2 x 61 tokens, 16 heads over 2, 4096 keys 24 us for 3.2 of products, with vector
+// units a third and matrix units 6 % of the time busy. A wave has two steps between looking for
+// its item, the first loads and the join in LDS, and a second launch follows; the last step's
+// loads are made once more for nothing; every 16 rows widen the codes again. Tiles of 128 rows
+// (attention.hip) widen them once and take 28.
 
 namespace mlc {
 

@@ -463,7 +463,8 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, cap:
       of a negative document sees nothing and is seen by none.
 
     A query that sees nothing gets zeros. What is not seen has no influence, NaN and
-    infinities included.
+    infinities included. Softmax weights are rounded to the type of ``q`` before they meet
+    the values; a capped score is off by up to 2^-21 of the cap, whatever its size.
     """
     scale, causal, cap = None if scale is None else float(scale), bool(causal), float(cap)
     out = _now("attention", (q, k, v, slopes, documents, prefix), (scale, causal, cap), 1)
