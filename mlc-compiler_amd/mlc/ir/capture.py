@@ -114,7 +114,7 @@ def _shared_buffers(model: torch.nn.Module) -> tuple[str, str] | None:
     """Two names of buffers that share memory."""
     seen: dict[int, str] = {}
     for name, x in model.named_buffers(remove_duplicate=False):
-        if x is None or not x.numel():
+        if x is None or not x.numel() or x.is_meta:
             continue
         other = seen.setdefault(x.untyped_storage().data_ptr(), name)
         if other != name:
