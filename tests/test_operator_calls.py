@@ -62,6 +62,32 @@ def test_function_modes_see_the_operator():
 
 
 @gpu
+def test_functions_that_torch_compiles_or_records_call_the_operators():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    a, b = filled(1, 2, 128, 64), filled(1, 2, 128, 64)
+    f, _ = ops.rotary_frequencies(64, device="cuda")
+    q, k, start = normal(1, 1, 4, 64), normal(1, 1, 2, 64, seed=1), ints([5])
+
+    def step(cache, q, k, start):
+        q, k = ops.rotary(q, k, start, f)
+        cache.append(k, k, start)
+        return cache.attend(q, start) * 2.0, ops.attention(q, k, k)
+
+    with torch.no_grad():
+        compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+        for i in range(2):
+            for x, y in zip(compiled(a, q, k, start + i), step(b, q, k, start + i)):
+                assert torch.equal(x, y)
+            for x, y in zip(parts(a), parts(b)):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    for pre in (False, True):
+        recorded = make_fx(lambda q, k: ops.attention(q, k, k), pre_dispatch=pre)(q, k)
+        assert "mlc.attention.default" in [str(n.target) for n in recorded.graph.nodes]
+        assert torch.equal(recorded(q, k), ops.attention(q, k, k))
+
+
+@gpu
 def test_the_profiler_records_each_call_once():
     from torch.profiler import ProfilerActivity, profile
 
