@@ -12,6 +12,7 @@
 // interpreter's lock, which launches are made without.
 
 #define PY_SSIZE_T_CLEAN
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,7 +40,7 @@ namespace {
 using launch_fn = int (*)(void*, uint32_t, uint32_t, uint32_t, const void*, size_t, void*);
 using poll_fn = int (*)(void*, int32_t*);
 
-constexpr Py_ssize_t kMostOperands = 16, kMostResults = 2;
+constexpr Py_ssize_t kMostOperands = 16, kMostResults = 3;
 constexpr size_t kMostBytes = 1024;  // of a launch's arguments
 
 // The flags of a call. kDispatched: torch's dispatcher has brought it, and whoever looks on
@@ -47,7 +48,10 @@ constexpr size_t kMostBytes = 1024;  // of a launch's arguments
 enum { kPoll = 1, kDispatched = 2 };
 
 // by number, as mlc.ops gives it
-constexpr const char* kOperators[] = {"mlc::rotary", "mlc::attention", "mlc::cache_append", "mlc::cache_attention"};
+constexpr const char* kOperators[] = {
+    "mlc::rotary",         "mlc::attention",    "mlc::cache_append",       "mlc::cache_attention",
+    "mlc::rms_norm",       "mlc::add_rms_norm", "mlc::rms_norm_quantized", "mlc::add_rms_norm_quantized",
+    "mlc::quantize",       "mlc::scaled_product", "mlc::sample"};
 
 // tensors that stand for others
 constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
@@ -85,6 +89,11 @@ struct Launch {
   std::string tail;             // and what follows them
 };
 
+struct Result {
+  at::ScalarType type;
+  std::vector<int64_t> sizes;
+};
+
 struct Entry {
   launch_fn launch;
   std::vector<Launch> launches;
@@ -93,6 +102,7 @@ struct Entry {
   poll_fn poll;        // null: cannot meet an invalid input
   void* ctx;
   uint64_t error;
+  std::vector<Result> results;  // empty: like the first operands
 };
 
 std::unordered_map<std::string, std::shared_ptr<Entry>>& table() {
@@ -233,8 +243,14 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_DECREF(current);
   if (PyErr_Occurred()) return nullptr;
   at::Tensor out[kMostResults], space;
+  if (!entry->results.empty() && static_cast<size_t>(results) != entry->results.size()) {
+    PyErr_SetString(PyExc_TypeError, "call: another number of results than the operator has");
+    return nullptr;
+  }
   for (Py_ssize_t i = 0; i < results; ++i) {
-    out[i] = at::empty(x[i]->sizes(), x[i]->options(), at::MemoryFormat::Contiguous);
+    out[i] = entry->results.empty()
+                 ? at::empty(x[i]->sizes(), x[i]->options(), at::MemoryFormat::Contiguous)
+                 : at::empty(entry->results[i].sizes, x[0]->options().dtype(entry->results[i].type));
     at[operands + i] = reinterpret_cast<uint64_t>(out[i].const_data_ptr());
   }
   uint64_t* const rest = at + operands + results;
@@ -268,8 +284,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// add(signature, addresses, changed, launch, launches, workspace, poll, ctx, error): launches are
-// (function, grid, block, places, tail) with places below ``addresses``.
+// add(signature, addresses, changed, launch, launches, workspace, poll, ctx, error, results = ()): launches
+// are (function, grid, block, places, tail) with places below ``addresses``; results (type, sizes).
 PyObject* add(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   const char* key;
@@ -277,9 +293,9 @@ PyObject* add(PyObject*, PyObject* args) {
   int addresses, changed;
   unsigned long long launch, poll, ctx, error;
   long long workspace;
-  PyObject* launches;
-  if (!PyArg_ParseTuple(args, "y#iiKO!LKKK", &key, &key_size, &addresses, &changed, &launch, &PyTuple_Type, &launches,
-                        &workspace, &poll, &ctx, &error))
+  PyObject *launches, *results = nullptr;
+  if (!PyArg_ParseTuple(args, "y#iiKO!LKKK|O!", &key, &key_size, &addresses, &changed, &launch, &PyTuple_Type,
+                        &launches, &workspace, &poll, &ctx, &error, &PyTuple_Type, &results))
     return nullptr;
   auto entry = std::make_shared<Entry>();
   entry->launch = reinterpret_cast<launch_fn>(launch);
@@ -306,6 +322,20 @@ PyObject* add(PyObject*, PyObject* args) {
       return nullptr;
     }
     entry->launches.push_back(std::move(l));
+  }
+  for (Py_ssize_t i = 0; results != nullptr && i < PyTuple_GET_SIZE(results); ++i) {
+    PyObject *type, *sizes;
+    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(results, i), "OO!", &type, &PyTuple_Type, &sizes)) return nullptr;
+    if (!THPDtype_Check(type) || i >= kMostResults) {
+      PyErr_SetString(PyExc_TypeError, "add: up to three results, (type, sizes)");
+      return nullptr;
+    }
+    Result r{reinterpret_cast<THPDtype*>(type)->scalar_type, {}};
+    for (Py_ssize_t j = 0; j < PyTuple_GET_SIZE(sizes); ++j) {
+      r.sizes.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(sizes, j)));
+      if (PyErr_Occurred()) return nullptr;
+    }
+    entry->results.push_back(std::move(r));
   }
   table()[std::string(key, static_cast<size_t>(key_size))] = std::move(entry);
   Py_RETURN_NONE;

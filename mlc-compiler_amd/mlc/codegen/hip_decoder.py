@@ -1,0 +1,264 @@
+"""Launches of the operators of ``mlc.ops`` that stand around a decoder's attention: norms
+and rows in 8 bits, products of scaled 8-bit values, the choice of a token.
+
+Like those of ``hip_operators`` their plans follow from sizes, types and alignment alone and
+serve direct calls and compiled models. Results have shapes and types of their own, which a
+plan carries.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from .hip_operators import (NAMES, SHORT, UNITS, Launch, Operand, OperatorError, Plan, _ceil, _grid,
+                            _numel, _offset)
+
+E4M3 = torch.float8_e4m3fn
+#: values that share a scale
+BLOCK = 128
+#: types of a product's result, by the number that stands for one among a call's options
+RESULTS = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def blocks_of(dim: int) -> int:
+    return _ceil(dim, BLOCK)
+
+
+def _rows(x: Operand | None) -> tuple[int, int, tuple]:
+    """Rows of the last dimension, how many of them follow each other with the second stride, and
+    the strides of both. What a dimension of one says of its stride means nothing."""
+    if x is None:
+        return 0, 1, (0, 0)
+    strides = tuple(s if n > 1 else 0 for s, n in zip(x.strides[:-1], x.shape[:-1]))
+    if len(x.shape) == 3:
+        return x.shape[0] * x.shape[1], max(1, x.shape[1]), strides
+    return x.shape[0], max(1, x.shape[0]), (0, *strides)
+
+
+def _in_packs(x: Operand | None, n: int) -> bool:
+    """Whether rows begin on 16 bytes, as packs of ``n`` values do."""
+    return x is None or (x.aligned and all(s % n == 0 for s in _rows(x)[2]))
+
+
+# --------------------------------------------------------------------------
+# rows
+# --------------------------------------------------------------------------
+
+#: values of a row in registers at most
+MOST_DIM = 1 << 15
+#: (waves of a row, packs of 8 values of a lane), shortest rows first
+NORM_SHAPES = ((1, 1), (1, 2), (1, 4), (4, 2), (4, 4), (16, 2), (16, 4))
+QUANTIZE_THREADS, QUANTIZE_PACKS = 256, 2
+
+
+def norm_kernel(dtype, align: int, waves: int, n: int, eight: bool) -> tuple[str, str]:
+    name = f"rms_norm_{SHORT[dtype]}_a{align}_w{waves}_n{n}{'_e4m3' if eight else ''}"
+    return f"RMS_NORM({name}, {NAMES[dtype]}, {align}, {waves}, {n}, {str(eight).lower()})", name
+
+
+def quantize_kernel(dtype, align: int, gated: bool) -> tuple[str, str]:
+    name = f"quantize_{SHORT[dtype]}_a{align}{'_gated' if gated else ''}"
+    return f"QUANTIZE({name}, {NAMES[dtype]}, {align}, {str(gated).lower()})", name
+
+
+def eight_bits(x) -> tuple:
+    """Shapes and types of the codes and scales of rows like ``x``."""
+    return ((tuple(x.shape), E4M3), ((*x.shape[:-1], blocks_of(x.shape[-1])), torch.float32))
+
+
+def norm_results(x, residual, quantized: bool) -> tuple:
+    made = eight_bits(x) if quantized else ((tuple(x.shape), x.dtype),)
+    return (*made, (tuple(x.shape), x.dtype)) if residual is not None else made
+
+
+def _row_args(x: Operand, other: Operand | None, weight: Operand | None, eps: float) -> bytes:
+    rows, seq, strides = _rows(x)
+    return struct.pack("<3q4q4id", x.offset, _offset(other), _offset(weight), *strides,
+                       *_rows(other)[2], rows, seq, x.shape[-1], weight is not None
+                       and weight.dtype == torch.float32, eps)
+
+
+def plan_norm(x: Operand, weight: Operand, residual: Operand | None, eps: float, quantized: bool) -> Plan:
+    results = norm_results(x, residual, quantized)
+    rows, _, _ = _rows(x)
+    dim = x.shape[-1]
+    if rows * dim == 0:
+        return Plan((), results=results)
+    align = 16 if dim % 8 == 0 and _in_packs(x, 8) and _in_packs(residual, 8) else x.dtype.itemsize
+    waves, n = next((w, n) for w, n in NORM_SHAPES if 512 * w * n >= dim)
+    kernel, name = norm_kernel(x.dtype, align, waves, n, quantized)
+    grid = _grid(_ceil(rows, 4) if waves == 1 else rows, max(256, 64 * waves), "rms_norm")
+    pointers = ("x", "residual" if residual is not None else None, "weight", "out0",
+                "out1" if quantized else None,
+                f"out{len(results) - 1}" if residual is not None else None)
+    return Plan((Launch(kernel, "rows", name, grid, max(256, 64 * waves), pointers,
+                        _row_args(x, residual, weight, eps)),), results=results)
+
+
+def plan_quantize(x: Operand, gate: Operand | None) -> Plan:
+    results = eight_bits(x)
+    rows, _, _ = _rows(x)
+    if _numel(x) == 0:
+        return Plan((), results=results)
+    align = 16 if _in_packs(x, 8) and _in_packs(gate, 8) else x.dtype.itemsize
+    kernel, name = quantize_kernel(x.dtype, align, gate is not None)
+    packs = rows * blocks_of(x.shape[-1]) * (BLOCK // 8)
+    grid = _grid(_ceil(packs, QUANTIZE_THREADS * QUANTIZE_PACKS), QUANTIZE_THREADS, "quantize")
+    return Plan((Launch(kernel, "rows", name, grid, QUANTIZE_THREADS,
+                        ("x", "gate" if gate is not None else None, None, "out0", "out1", None),
+                        _row_args(x, gate, None, 0.0)),), results=results)
+
+
+# --------------------------------------------------------------------------
+# products
+# --------------------------------------------------------------------------
+
+#: rows that a workgroup of few rows takes at most, and its waves
+FEW_ROWS, FEW_WAVES = 64, 8
+#: tiles of many rows: rows of both operands, waves along both, blocks in LDS
+TILES = ((256, 256, 4, 2, 2),)
+JOIN_THREADS = 256
+
+
+def few_kernel(dtype, tiles: int) -> tuple[str, str]:
+    name = f"scaled_product_rows_{SHORT[dtype]}_m{tiles}"
+    return f"SCALED_PRODUCT_ROWS({name}, {NAMES[dtype]}, {tiles}, {FEW_WAVES})", name
+
+
+def tiles_kernel(dtype, tile: tuple) -> tuple[str, str]:
+    name = f"scaled_product_tiles_{SHORT[dtype]}_{'_'.join(map(str, tile))}"
+    return f"SCALED_PRODUCT_TILES({name}, {NAMES[dtype]}, {', '.join(map(str, tile))})", name
+
+
+def product_join_kernel(dtype) -> tuple[str, str]:
+    name = f"scaled_product_join_{SHORT[dtype]}"
+    return f"SCALED_PRODUCT_JOIN({name}, {NAMES[dtype]})", name
+
+
+def product_results(a, b, dtype) -> tuple:
+    return (((*a.shape[:-1], b.shape[0]), dtype),)
+
+
+def require_pieces(**operands) -> None:
+    """Rows of codes are taken in pieces of 16 bytes."""
+    for name, x in operands.items():
+        if _numel(x) and not _in_packs(x, 16):
+            raise OperatorError(f"{name}: rows of codes that lie on 16 bytes expected")
+
+
+def _reach(x: Operand, strides: tuple) -> int:
+    """Bytes from the first of the rows to the last."""
+    shape = x.shape[:-1] if len(x.shape) == 3 else (1, x.shape[0])
+    return sum((n - 1) * s for n, s in zip(shape, strides)) * x.dtype.itemsize
+
+
+def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, bias: Operand | None,
+                 dtype: torch.dtype) -> Plan:
+    results = product_results(a, b, dtype)
+    require_pieces(a=a, b=b)
+    rows, seq, strides = _rows(a)
+    n, k = b.shape
+    if rows * n == 0:
+        return Plan((), results=results)
+    blocks = blocks_of(k)
+    splits, row_tiles = 1, 1
+    scale_strides = _rows(a_scales)[2]
+    regular = all(s[0] == s[1] * seq for s in (strides, scale_strides)) or rows == seq
+    if regular:
+        seq = rows
+    pointers = ["a", "a_scales", "b", "b_scales", "bias" if bias is not None else None, "out0", None]
+    few = rows <= FEW_ROWS
+    if few:
+        kernel, name = few_kernel(dtype, next(t for t in (1, 2, 4) if 16 * t >= rows))
+        grid, threads = _ceil(n, 16), 64 * FEW_WAVES
+    else:
+        tile = TILES[0]
+        reach = max(max(tile[:2]) * max(strides[1], b.strides[0], 4 * scale_strides[1]) if regular else
+                    max(_reach(a, strides), _reach(a_scales, scale_strides), max(tile[:2]) * b.strides[0]),
+                    4 * a_scales.strides[-1] * blocks) + k
+        if reach >= 1 << 31:
+            raise OperatorError("scaled_product: rows that lie too far apart: make them contiguous")
+        row_tiles, tiles = _ceil(rows, tile[0]), _ceil(rows, tile[0]) * _ceil(n, tile[1])
+        splits = max(1, min(UNITS // tiles, blocks // 4))
+        kernel, name = tiles_kernel(dtype, tile)
+        grid, threads = tiles * splits, 64 * tile[2] * tile[3]
+        if splits > 1:
+            pointers[-1] = "workspace"
+    tail = struct.pack("<5q8q8i", a.offset, a_scales.offset, b.offset, b_scales.offset, _offset(bias),
+                       *strides, *scale_strides, a_scales.strides[-1], b.strides[0],
+                       *b_scales.strides, rows, seq, n, k, splits, row_tiles,
+                       bias is not None and bias.dtype == torch.float32, regular)
+    launches = [Launch(kernel, "scaled_product", name, _grid(grid, threads, "scaled_product"), threads,
+                       tuple(pointers), tail)]
+    if splits > 1:
+        kernel, name = product_join_kernel(dtype)
+        launches.append(Launch(kernel, "scaled_product", name,
+                               _grid(_ceil(rows * n, JOIN_THREADS), JOIN_THREADS, "scaled_product"),
+                               JOIN_THREADS, tuple(pointers), tail))
+    return Plan(tuple(launches), splits * rows * n * 4 if splits > 1 else 0, results=results)
+
+
+# --------------------------------------------------------------------------
+# the choice of a token
+# --------------------------------------------------------------------------
+
+#: sums of weights, whole numbers up to 2^40 each, stay below 2^63
+MOST_TOKENS = 1 << 22
+SAMPLE_THREADS = 1024
+
+
+def sample_kernel(dtype) -> tuple[str, str]:
+    name = f"sample_{SHORT[dtype]}"
+    return f"SAMPLE({name}, {NAMES[dtype]})", name
+
+
+def sample_results(logits) -> tuple:
+    return (((logits.shape[0],), torch.int64),)
+
+
+def plan_sample(logits: Operand, uniform: Operand, temperature: Operand | None, top_k: Operand | None,
+                top_p: Operand | None, min_p: Operand | None) -> Plan:
+    results = sample_results(logits)
+    batch, size = logits.shape
+    if batch == 0:
+        return Plan((), results=results)
+    options = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    rows = (uniform, *options.values())
+    tail = struct.pack("<6q6q2i", logits.offset, *map(_offset, rows), logits.strides[0],
+                       *(x.strides[0] if x is not None else 0 for x in rows), batch, size)
+    kernel, name = sample_kernel(logits.dtype)
+    pointers = ("logits", "uniform", *(n if x is not None else None for n, x in options.items()),
+                "out0", "error")
+    return Plan((Launch(kernel, "sample", name, _grid(batch, SAMPLE_THREADS, "sample"), SAMPLE_THREADS,
+                        pointers, tail),), results=results)
+
+
+#: operators of a captured graph -> the plan of their operands, by their names in the schema
+PLANS = {
+    "mlc.rms_norm.default": lambda x, weight, eps: plan_norm(x, weight, None, eps, False),
+    "mlc.add_rms_norm.default": lambda x, weight, residual, eps: plan_norm(x, weight, residual, eps, False),
+    "mlc.rms_norm_quantized.default": lambda x, weight, eps: plan_norm(x, weight, None, eps, True),
+    "mlc.add_rms_norm_quantized.default": lambda x, weight, residual, eps:
+        plan_norm(x, weight, residual, eps, True),
+    "mlc.quantize.default": plan_quantize,
+    "mlc.scaled_product.default": plan_product,
+    "mlc.sample.default": plan_sample,
+}
+#: those that can meet an invalid input
+FLAGGING = ("mlc.sample.default",)
+
+
+def all_kernels() -> list[tuple[str, str]]:
+    """``(file, kernel)`` of everything that a plan can ask for."""
+    out = []
+    for dtype in RESULTS:
+        aligns = sorted({16, dtype.itemsize})
+        for w, n in NORM_SHAPES:
+            out += [("rows", norm_kernel(dtype, a, w, n, e)[0]) for a in aligns for e in (False, True)]
+        out += [("rows", quantize_kernel(dtype, a, g)[0]) for a in aligns for g in (False, True)]
+        out += [("scaled_product", few_kernel(dtype, t)[0]) for t in (1, 2, 4)]
+        out += [*(("scaled_product", tiles_kernel(dtype, t)[0]) for t in TILES),
+                ("scaled_product", product_join_kernel(dtype)[0]), ("sample", sample_kernel(dtype)[0])]
+    return out

@@ -76,6 +76,8 @@ class Plan:
     launches: tuple
     #: bytes of memory that the launches share and nobody reads afterwards
     workspace: int = 0
+    #: (shape, type) of each result; empty: results are like the first operands
+    results: tuple = ()
 
 
 @functools.lru_cache(maxsize=None)

@@ -72,6 +72,8 @@ _ADDMM = "aten.addmm.default"
 _UNBIND = "aten.unbind.int"
 _SPLIT_BY_CHUNK = "aten.split.Tensor"
 _SPLIT_BY_SIZES = "aten.split_with_sizes.default"
+#: operands of ``mlc.ops`` other than heads whose rows lie in one piece
+_LINES = ("x", "residual", "gate", "weight", "a", "b", "bias", "logits")
 #: how the exporter writes an op that changes its operands
 _IN_PLACE = "auto_functionalized_v2"
 
@@ -352,7 +354,8 @@ class _Translation:
                 if cache and v.layout.strides != Layout.contiguous(v.shape).strides:
                     raise CaptureError(f"{target}: {a.name} is a view of a buffer that lies otherwise: "
                                        "give the buffer itself")
-                if not cache and v.rank == 4 and v.shape[3] > 1 and v.layout.strides[3] != 1:
+                if not cache and (v.rank == 4 or a.name in _LINES) and v.shape[-1] > 1 \
+                        and v.layout.strides[-1] != 1:
                     v = self._contiguous_copy(v)
             out.append(v)
         return out

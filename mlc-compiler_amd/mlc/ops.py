@@ -1,6 +1,7 @@
 """Operators of decoders, as functions on GPU tensors: positions turned into
 queries and keys, attention whose masks are made from indices, a cache of keys and
-values in 8 bits and the attention over it.
+values in 8 bits and the attention over it; norms, linear layers in 8 bits, and the
+choice of a token.
 
     q, k = mlc.ops.rotary(q, k, positions, frequencies)
     out = mlc.ops.attention(q, k, v, causal=True)            # a prompt
@@ -8,7 +9,11 @@ values in 8 bits and the attention over it.
     cache.append(k, v, start)                                # then, token by token
     out = cache.attend(q, start)
 
-Tensors are token-major, ``[batch, tokens, heads, dim]``, as a linear layer's output
+    codes, scales, x = mlc.ops.rms_norm(x, weight, residual, quantized=True)
+    y = mlc.ops.scaled_product(codes, scales, *mlc.ops.quantize_weight(w))
+    tokens = mlc.ops.sample(logits, uniform, temperature=t, top_p=p)
+
+In attention and the cache tensors are token-major, ``[batch, tokens, heads, dim]``, as a linear layer's output
 is viewed, with any strides whose last is 1; results are contiguous. ``heads`` of the
 queries is a multiple of ``kv_heads`` of keys and values: query head ``h`` reads
 key head ``h // (heads // kv_heads)``.
@@ -28,12 +33,14 @@ import math
 import torch
 from torch.autograd.forward_ad import unpack_dual
 
+from .codegen import hip_decoder as decoder
 from .codegen import hip_operators as plans
 from .codegen.hip_operators import Operand, OperatorError
 from .runtime import native, operators
 
 __all__ = ["rotary", "rotary_frequencies", "attention", "cache_append", "cache_attention",
-           "KeyValueCache", "check_errors", "OperatorError"]
+           "KeyValueCache", "rms_norm", "quantize", "quantize_weight", "scaled_product", "ScaledLinear",
+           "sample", "check_errors", "OperatorError"]
 
 _HALF = (torch.float16, torch.bfloat16)
 _FLOATS = (*_HALF, torch.float32)
@@ -207,6 +214,88 @@ def _check_cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count, 
     _same(q, others)
 
 
+def _lines(name: str, x, dtypes, most: int) -> None:
+    _require(x.dim() in (2, 3), f"{name}: [rows, dim] or [batch, tokens, dim] expected, got {tuple(x.shape)}")
+    _require(x.dtype in dtypes, f"{name}: one of {[str(d) for d in dtypes]} expected, got {x.dtype}")
+    _require(1 <= x.shape[-1] <= most, f"{name}: a dim of 1 to {most} expected, got {x.shape[-1]}")
+    _require(x.shape[-1] == 1 or x.stride(-1) == 1, f"{name}: the last dimension's stride is "
+             f"{x.stride(-1)}, and 1 is expected")
+    _require(math.prod(x.shape[:-1]) <= _MAX, f"{name}: too many rows for one call")
+
+
+def _like_lines(name: str, x, first, of: str) -> None:
+    _require(x.shape == first.shape and x.dtype == first.dtype,
+             f"{name} {x.dtype}{list(x.shape)} and {of} {first.dtype}{list(first.shape)} differ")
+    _require(x.shape[-1] == 1 or x.stride(-1) == 1, f"{name}: the last dimension's stride is "
+             f"{x.stride(-1)}, and 1 is expected")
+
+
+def _pieces(name: str, x) -> None:
+    _require(x.shape[-1] % 16 == 0, f"{name}: a dim that is a multiple of 16 expected, got {x.shape[-1]}")
+
+
+def _check_norm(x, weight, residual, eps, quantized) -> None:
+    _lines("x", x, _FLOATS, decoder.MOST_DIM)
+    if quantized:
+        _pieces("x", x)
+    _require(tuple(weight.shape) == (x.shape[-1],) and weight.dtype in (x.dtype, torch.float32)
+             and weight.is_contiguous(), f"weight: contiguous {x.dtype}[{x.shape[-1]}] or float32 expected, "
+             f"got {weight.dtype}{list(weight.shape)} with strides {weight.stride()}")
+    _require(0.0 < eps <= torch.finfo(torch.float32).max, f"eps: a positive number expected, got {eps}")
+    others = {"weight": weight}
+    if residual is not None:
+        _like_lines("residual", residual, x, "x")
+        others["residual"] = residual
+    _same(x, others)
+
+
+def _check_quantize(x, gate) -> None:
+    _lines("x", x, _FLOATS, 1 << 24)
+    _pieces("x", x)
+    if gate is not None:
+        _like_lines("gate", gate, x, "x")
+        _same(x, {"gate": gate})
+
+
+def _result_number(dtype) -> int:
+    _require(dtype in decoder.RESULTS, f"dtype: one of {[str(d) for d in decoder.RESULTS]} expected, "
+             f"got {dtype}")
+    return decoder.RESULTS.index(dtype)
+
+
+def _check_product(a, a_scales, b, b_scales, bias, number) -> None:
+    dtype = decoder.RESULTS[int(number)]
+    _lines("a", a, (_E4M3,), 1 << 24)
+    _lines("b", b, (_E4M3,), 1 << 24)
+    _require(b.dim() == 2 and b.shape[1] == a.shape[-1],
+             f"b {tuple(b.shape)}: [outputs, {a.shape[-1]}] expected")
+    _pieces("a", a)
+    blocks, outputs = decoder.blocks_of(a.shape[-1]), decoder.blocks_of(b.shape[0])
+    for name, x, shape in (("a_scales", a_scales, (*a.shape[:-1], blocks)), ("b_scales", b_scales, (outputs, blocks))):
+        _require(tuple(x.shape) == tuple(shape) and x.dtype == torch.float32,
+                 f"{name}: float32{list(shape)} expected, got {x.dtype}{list(x.shape)}")
+    for name, x in (("a", a), ("b", b)):
+        _require(all(s % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape) if n > 1),
+                 f"{name}: rows of codes that lie on 16 bytes expected, got strides {x.stride()}")
+    others = {"a_scales": a_scales, "b": b, "b_scales": b_scales}
+    if bias is not None:
+        _require(tuple(bias.shape) == (b.shape[0],) and bias.dtype in (dtype, torch.float32)
+                 and bias.is_contiguous(), f"bias: contiguous {dtype}[{b.shape[0]}] or float32 expected, "
+                 f"got {bias.dtype}{list(bias.shape)} with strides {bias.stride()}")
+        others["bias"] = bias
+    _same(a, others)
+
+
+def _check_sample(logits, uniform, temperature, top_k, top_p, min_p) -> None:
+    _require(logits.dim() == 2, f"logits: [batch, tokens] expected, got {tuple(logits.shape)}")
+    _lines("logits", logits, _FLOATS, decoder.MOST_TOKENS)
+    others = {"uniform": uniform, "temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    others = {name: x for name, x in others.items() if x is not None}
+    for name, x in others.items():
+        _vector(name, x, torch.int32 if name == "top_k" else torch.float32, logits.shape[0])
+    _same(logits, others)
+
+
 # --------------------------------------------------------------------------
 # direct calls
 # --------------------------------------------------------------------------
@@ -262,6 +351,34 @@ _OPERATORS = {
 }
 
 
+def _norm_of(residual: bool, quantized: bool) -> tuple:
+    """The check, plan and operands' names of one of the four norms."""
+    def with_options(f):
+        if residual:
+            return lambda x, weight, other, eps: f(x, weight, other, eps, quantized)
+        return lambda x, weight, eps: f(x, weight, None, eps, quantized)
+
+    return (with_options(_check_norm), with_options(decoder.plan_norm),
+            ("x", "weight", "residual")[:3 if residual else 2])
+
+
+def _plan_product(a, a_scales, b, b_scales, bias, number):
+    return decoder.plan_product(a, a_scales, b, b_scales, bias, decoder.RESULTS[int(number)])
+
+
+#: (with a residual, in 8 bits) -> the norm's name
+_NORMS = {(False, False): "rms_norm", (True, False): "add_rms_norm",
+          (False, True): "rms_norm_quantized", (True, True): "add_rms_norm_quantized"}
+# in the order of the names that _calls.call knows
+_OPERATORS |= {name: _norm_of(*kind) for kind, name in _NORMS.items()}
+_OPERATORS |= {
+    "quantize": (_check_quantize, decoder.plan_quantize, ("x", "gate")),
+    "scaled_product": (_check_product, _plan_product, ("a", "a_scales", "b", "b_scales", "bias")),
+    "sample": (_check_sample, decoder.plan_sample,
+               ("logits", "uniform", "temperature", "top_k", "top_p", "min_p")),
+}
+
+
 _NUMBERS = {op: i for i, op in enumerate(_OPERATORS)}
 
 
@@ -313,6 +430,16 @@ _lib.define("cache_append(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_s
 _lib.define("cache_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, "
             "Tensor v_scale, Tensor start, Tensor? count, float? scale, float cap, "
             "Tensor? slopes) -> Tensor")
+_lib.define("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor")
+_lib.define("add_rms_norm(Tensor x, Tensor weight, Tensor residual, float eps) -> (Tensor, Tensor)")
+_lib.define("rms_norm_quantized(Tensor x, Tensor weight, float eps) -> (Tensor, Tensor)")
+_lib.define("add_rms_norm_quantized(Tensor x, Tensor weight, Tensor residual, float eps) -> "
+            "(Tensor, Tensor, Tensor)")
+_lib.define("quantize(Tensor x, Tensor? gate) -> (Tensor, Tensor)")
+_lib.define("scaled_product(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? bias, "
+            "ScalarType dtype) -> Tensor")
+_lib.define("sample(Tensor logits, Tensor uniform, Tensor? temperature, Tensor? top_k, Tensor? top_p, "
+            "Tensor? min_p) -> Tensor")
 
 
 def _like(x):
@@ -339,9 +466,9 @@ def _untraced():
             torch._C._set_tracing_state(state)
 
 
-def _implement(op: str, split, results: int) -> None:
+def _implement(op: str, split, results: int, made=None) -> None:
     """``mlc::op``: ``split`` puts the schema's arguments into operands and options,
-    results are like the first operands."""
+    results are like the first operands, or of the shapes and types that ``made`` gives."""
     check = _OPERATORS[op][0]
 
     def autograd(keys, *args):
@@ -367,7 +494,11 @@ def _implement(op: str, split, results: int) -> None:
     def fake(*args):
         operands, options = split(*args)
         check(*operands, *options)
-        out = tuple(map(_like, operands[:results]))
+        if made is None:
+            out = tuple(map(_like, operands[:results]))
+        else:
+            out = tuple(torch.empty(shape, dtype=dtype, device=operands[0].device)
+                        for shape, dtype in made(*operands, *options))
         return out if results > 1 else out[0] if results else None
 
     @_untraced()
@@ -392,6 +523,19 @@ _implement("attention", lambda q, k, v, scale, causal, cap, slopes, documents, p
 _implement("cache_append", lambda *args: (args, ()), 0)
 _implement("cache_attention", lambda q, kc, vc, ks, vs, start, count, scale, cap, slopes:
            ((q, kc, vc, ks, vs, start, count, slopes), (scale, cap)), 1)
+_implement("rms_norm", lambda x, w, eps: ((x, w), (eps,)), 1)
+_implement("add_rms_norm", lambda x, w, r, eps: ((x, w, r), (eps,)), 2,
+           lambda x, w, r, eps: decoder.norm_results(x, r, False))
+_implement("rms_norm_quantized", lambda x, w, eps: ((x, w), (eps,)), 2,
+           lambda x, w, eps: decoder.norm_results(x, None, True))
+_implement("add_rms_norm_quantized", lambda x, w, r, eps: ((x, w, r), (eps,)), 3,
+           lambda x, w, r, eps: decoder.norm_results(x, r, True))
+_implement("quantize", lambda *args: (args, ()), 2, lambda x, gate: decoder.eight_bits(x))
+_implement("scaled_product", lambda a, a_scales, b, b_scales, bias, dtype:
+           ((a, a_scales, b, b_scales, bias), (_result_number(dtype),)), 1,
+           lambda a, a_scales, b, b_scales, bias, number:
+           decoder.product_results(a, b, decoder.RESULTS[number]))
+_implement("sample", lambda *args: (args, ()), 1, lambda logits, *_: decoder.sample_results(logits))
 
 
 # --------------------------------------------------------------------------
@@ -513,7 +657,149 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, start, count=None, *,
                                          scale, cap, slopes)
 
 
-class KeyValueCache(torch.nn.Module):
+def rms_norm(x, weight, residual=None, *, eps: float = 1e-6, quantized: bool = False):
+    """``h / sqrt(mean(h^2) + eps) * weight`` for rows ``h`` of ``x [rows, dim]`` or
+    ``[batch, tokens, dim]`` (fp16, bf16 or fp32, ``dim`` up to 32768), with ``weight``
+    ``[dim]`` in the type of ``x`` or float32. With ``residual``, of the shape and type of
+    ``x``, ``h = x + residual``, and the sum, rounded to that type, comes back behind the
+    norm; the norm itself is taken of the sum as it is before that.
+
+    Returns the norm in the type of ``x``, or with ``quantized`` (``dim`` a multiple of 16)
+    its codes and scales as :func:`quantize` gives them: ``y``, ``(y, sum)``, ``(codes,
+    scales)`` or ``(codes, scales, sum)``. Sums of squares are held in 64 bits.
+    """
+    op = _NORMS[residual is not None, bool(quantized)]
+    operands, eps = (x, weight) if residual is None else (x, weight, residual), float(eps)
+    results = 1 + bool(quantized) + (residual is not None)
+    out = _now(op, operands, (eps,), results)
+    if out is None:
+        return getattr(torch.ops.mlc, op)(*operands, eps)
+    return out if results > 1 else out[0]
+
+
+def quantize(x, gate=None):
+    """``(codes, scales)`` of rows ``x [rows, dim]`` or ``[batch, tokens, dim]`` (fp16, bf16 or
+    fp32, ``dim`` a multiple of 16), or of ``x * gate / (1 + e^-gate)`` with ``gate`` of the
+    same shape and type.
+
+    A scale, ``float32 [..., ceil(dim / 128)]``, is that of 128 neighbouring values of a
+    row: their largest finite magnitude divided by 448, and 2^-126 or more. A code,
+    ``float8_e4m3fn``, is a value divided by its scale; infinities and NaN become NaN.
+    """
+    out = _now("quantize", (x, gate), (), 2)
+    return out if out is not None else torch.ops.mlc.quantize(x, gate)
+
+
+def quantize_weight(weight):
+    """``(codes, scales)`` of a weight ``[outputs, inputs]``, for :func:`scaled_product`: a scale
+    for each 128 x 128 values, as :func:`quantize` has them for 128. Once, in torch, on the weight's
+    device."""
+    _require(weight.dim() == 2 and weight.is_floating_point(),
+             f"weight: floating [outputs, inputs] expected, got {weight.dtype}{list(weight.shape)}")
+    n, k = weight.shape
+    _require(k % 16 == 0 and k > 0, f"weight: a multiple of 16 inputs expected, got {k}")
+    rows, blocks = decoder.blocks_of(n), decoder.blocks_of(k)
+    with torch.no_grad():
+        whole = torch.zeros(rows * decoder.BLOCK, blocks * decoder.BLOCK, device=weight.device)
+        whole[:n, :k] = weight
+        tiles = whole.view(rows, decoder.BLOCK, blocks, decoder.BLOCK)
+        top = torch.where(tiles.isfinite(), tiles.abs(), 0.0).amax(dim=(1, 3))
+        scales = (top / 448.0).clamp(min=2.0 ** -126)
+        tiles /= scales[:, None, :, None]
+        whole = torch.where(whole.isfinite(), whole, float("nan"))[:n, :k]
+        return whole.contiguous().to(_E4M3), scales
+
+
+def scaled_product(a, a_scales, b, b_scales, bias=None, *, dtype=torch.bfloat16):
+    """Rows of codes ``a [rows, k]`` or ``[batch, tokens, k]`` times a weight of codes ``b
+    [outputs, k]``, both ``float8_e4m3fn`` with ``k`` a multiple of 16 and rows on 16 bytes:
+
+        out[m, n] = sum_j a[m, j] * a_scales[m, j / 128] * b[n, j] * b_scales[n / 128, j / 128] + bias[n]
+
+    Scales are float32, ``[..., ceil(k / 128)]`` (:func:`quantize`) and ``[ceil(outputs / 128),
+    ceil(k / 128)]`` (:func:`quantize_weight`), of any value; ``bias [outputs]`` is in ``dtype`` or
+    float32. The result is ``dtype``: float16, bfloat16 or float32. Sums are held in fp32.
+    """
+    number = _result_number(dtype)
+    out = _now("scaled_product", (a, a_scales, b, b_scales, bias), (number,), 1)
+    if out is not None:
+        return out[0]
+    return torch.ops.mlc.scaled_product(a, a_scales, b, b_scales, bias, dtype)
+
+
+def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token, ``int64 [batch]``, of each row of ``logits [batch, tokens]`` (fp16, bf16 or
+    fp32) from the random numbers ``uniform`` (float32[batch], 0 or more and below 1).
+
+    A token's weight is ``e^((logit - largest) / temperature)`` (float32[batch]; 0, or less than
+    2^-100, takes the likeliest token, the first of several; without it 1). In the order of
+    falling logits, and of indexes where they are equal, kept are
+
+    * ``top_k`` (int32[batch]): the first so many; all where it is not positive;
+    * ``top_p`` (float32[batch]): of those the ones in front of which less than ``top_p`` of
+      their weight lies, the first always;
+    * ``min_p`` (float32[batch]): of those the ones of ``min_p`` times the largest weight or more.
+
+    The token is the first, by index, up to which more than ``uniform`` of the kept weight lies.
+    Weights count in steps of 2^-40 of the largest. Logits of -infinity are never taken; a row of
+    nothing else gets -1. So does a row with NaN or +infinity among its logits, a random number
+    outside its range, or an option that is NaN, negative or, for ``top_p`` and ``min_p``, above 1,
+    for the temperature above 2^100: ``ExecutionError`` is raised by a later call or :func:`check_errors`.
+    """
+    out = _now("sample", (logits, uniform, temperature, top_k, top_p, min_p), (), 1)
+    if out is not None:
+        return out[0]
+    return torch.ops.mlc.sample(logits, uniform, temperature, top_k, top_p, min_p)
+
+
+class _KeepsTypes(torch.nn.Module):
+    def _apply(self, fn, recurse=True):
+        """Moves the buffers with the module but keeps their types: ``model.half()`` is for
+        weights."""
+        for name, x in self._buffers.items():
+            if x is not None:
+                y = fn(x)
+                self._buffers[name] = y if y.dtype == x.dtype else x.to(y.device)
+        return self
+
+
+class ScaledLinear(_KeepsTypes):
+    """A linear layer whose weight is held in 8 bits (:func:`scaled_product`), as buffers of a
+    module. Called with rows it brings them into 8 bits itself; called with codes and scales
+    (of :func:`rms_norm` or :func:`quantize`) it takes those."""
+
+    def __init__(self, inputs: int, outputs: int, *, bias: bool = False, dtype=torch.bfloat16,
+                 device=None) -> None:
+        super().__init__()
+        _require(inputs > 0 and inputs % 16 == 0, f"a multiple of 16 inputs expected, got {inputs}")
+        _result_number(dtype)
+        self.inputs, self.outputs, self.dtype = inputs, outputs, dtype
+        self.register_buffer("codes", torch.zeros(outputs, inputs, dtype=torch.uint8, device=device)
+                             .view(_E4M3))
+        self.register_buffer("scales", torch.ones(decoder.blocks_of(outputs), decoder.blocks_of(inputs),
+                                                  device=device))
+        self.register_buffer("bias", torch.zeros(outputs, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, dtype=None) -> "ScaledLinear":
+        """``linear`` in 8 bits, with results in ``dtype`` (that of its weight)."""
+        w = linear.weight
+        made = cls(w.shape[1], w.shape[0], bias=linear.bias is not None, dtype=dtype or w.dtype,
+                   device=w.device)
+        codes, scales = quantize_weight(w.detach())
+        made.codes.copy_(codes)
+        made.scales.copy_(scales)
+        if linear.bias is not None:
+            made.bias.copy_(linear.bias.detach())
+        return made
+
+    def forward(self, x, scales=None):
+        if scales is None:
+            x, scales = quantize(x)
+        return scaled_product(x, scales, self.codes, self.scales, self.bias, dtype=self.dtype)
+
+
+class KeyValueCache(_KeepsTypes):
     """Keys and values of ``batch`` sequences of up to ``capacity`` tokens in 8 bits, as
     buffers of a module (:func:`cache_append`, :func:`cache_attention`)."""
 
@@ -530,14 +816,6 @@ class KeyValueCache(torch.nn.Module):
             self.register_buffer(f"{name[:-1]}_scales",
                                  torch.ones(*shape[:2], capacity // block, device=device),
                                  persistent=False)
-
-    def _apply(self, fn, recurse=True):
-        """Moves the buffers with the module but keeps their types: ``model.half()`` is for
-        weights."""
-        for name, x in self._buffers.items():
-            y = fn(x)
-            self._buffers[name] = y if y.dtype == x.dtype else x.to(y.device)
-        return self
 
     def append(self, k, v, start, count=None) -> None:
         cache_append(self.keys, self.values, self.key_scales, self.value_scales, k, v, start, count)

@@ -33,7 +33,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ..codegen import hip_operators
+from ..codegen import hip_decoder, hip_operators
 from ..codegen.hip_backend import LaunchSpec, build_module, build_products
 from ..config import Config
 from ..ir.graph import Value
@@ -45,6 +45,10 @@ _CAPSULE_NAME = b"dltensor"
 _PyCapsule_New = ctypes.pythonapi.PyCapsule_New
 _PyCapsule_New.restype = ctypes.py_object
 _PyCapsule_New.argtypes = [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p]
+
+#: operators of ``mlc.ops`` in a captured graph -> their plans, and those that can meet an invalid input
+PLANS = {**hip_operators.PLANS, **hip_decoder.PLANS}
+FLAGGING = (*hip_operators.FLAGGING, *hip_decoder.FLAGGING)
 
 
 @dataclass
@@ -121,7 +125,7 @@ class HipRuntime:
         #: the kernels of ``mlc.ops`` that the schedule calls, in this context
         self._operators = OperatorModules(self.index, self._ctx)
         if any(spec.meta.get("error_word") for spec in self.launch_table.values()) or any(
-                isinstance(k, ExternKernel) and k.node.op in hip_operators.FLAGGING
+                isinstance(k, ExternKernel) and k.node.op in FLAGGING
                 for k in schedule.kernels):
             word = ctypes.c_void_p()
             native.check(self.lib.mlc_error_word(self._ctx, ctypes.byref(word)), "mlc_error_word")
@@ -170,7 +174,7 @@ class HipRuntime:
         """An extern op this module implements natively (``aten.embedding``, the
         operators of ``mlc.ops``), resolved like a generated kernel; ``None``
         leaves it to the library."""
-        if k.node.op in hip_operators.PLANS:
+        if k.node.op in PLANS:
             return self._bind_operator(k, buffers)
         return self._bind_extern(k, self.launch_table.get(k.name), buffers)
 
@@ -226,7 +230,7 @@ class HipRuntime:
         for i, v in enumerate(k.outputs):
             pointers[f"out{i}"] = buffers[v.buffer.name].data_ptr()
         hip_operators.require_aligned(operands)
-        plan = hip_operators.PLANS[k.node.op](**operands)
+        plan = PLANS[k.node.op](**operands)
         if self._error_word is not None:
             pointers["error"] = self._error_word
         bound = Launches()

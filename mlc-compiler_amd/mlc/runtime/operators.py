@@ -22,7 +22,9 @@ from . import native
 INVALID = {1: ("an embedding id was outside its table (torch raises IndexError for such an "
                "id); the rows it addressed were written as zeros"),
            2: ("start and count of a sequence lay outside its cache, or count above the new "
-               "tokens: nothing was written for it, and its attention is zeros")}
+               "tokens: nothing was written for it, and its attention is zeros"),
+           3: ("a row of sample had NaN or +infinity among its logits, or a random number or an option "
+               "outside its range: its token is -1")}
 
 
 class OperatorModules:
@@ -123,7 +125,8 @@ class Calls(dict):
             self.clear()
         native.load_calls().add(signature, len(names), changed, address(modules.lib.mlc_launch), launches,
                                 plan.workspace, address(modules.lib.mlc_error_poll) if flags else 0,
-                                modules.context if flags else 0, modules.error_word() if flags else 0)
+                                modules.context if flags else 0, modules.error_word() if flags else 0,
+                                tuple((dtype, shape) for shape, dtype in plan.results))
         self[signature] = plan
 
     def clear(self) -> None:

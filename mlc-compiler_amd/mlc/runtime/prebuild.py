@@ -70,10 +70,11 @@ def prebuild_operators(verbose: bool = True) -> None:
     import concurrent.futures
     import os
 
-    from ..codegen import hip_operators
+    from ..codegen import hip_decoder, hip_operators
 
     t0 = time.time()
-    texts = [hip_operators.source(file, kernel) for file, kernel in hip_operators.all_kernels()]
+    texts = [hip_operators.source(file, kernel)
+             for file, kernel in hip_operators.all_kernels() + hip_decoder.all_kernels()]
     with concurrent.futures.ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
         list(pool.map(native.compile_code_object, texts))
     if verbose:
