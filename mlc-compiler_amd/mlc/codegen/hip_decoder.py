@@ -117,8 +117,8 @@ def plan_quantize(x: Operand, gate: Operand | None) -> Plan:
 
 #: rows that a workgroup of few rows takes at most, and its waves
 FEW_ROWS, FEW_WAVES = 64, 8
-#: tiles of many rows: rows of both operands, waves along both, blocks in LDS
-TILES = ((256, 256, 4, 2, 2),)
+#: tiles of many rows: rows of both operands, waves along both
+TILES = ((256, 256, 4, 2), (128, 128, 2, 2))
 JOIN_THREADS = 256
 
 
@@ -174,7 +174,7 @@ def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, b
         kernel, name = few_kernel(dtype, next(t for t in (1, 2, 4) if 16 * t >= rows))
         grid, threads = _ceil(n, 16), 64 * FEW_WAVES
     else:
-        tile = TILES[0]
+        tile = TILES[-1] if dtype == torch.float32 else TILES[0]
         reach = max(max(tile[:2]) * max(strides[1], b.strides[0], 4 * scale_strides[1]) if regular else
                     max(_reach(a, strides), _reach(a_scales, scale_strides), max(tile[:2]) * b.strides[0]),
                     4 * a_scales.strides[-1] * blocks) + k
@@ -259,6 +259,7 @@ def all_kernels() -> list[tuple[str, str]]:
             out += [("rows", norm_kernel(dtype, a, w, n, e)[0]) for a in aligns for e in (False, True)]
         out += [("rows", quantize_kernel(dtype, a, g)[0]) for a in aligns for g in (False, True)]
         out += [("scaled_product", few_kernel(dtype, t)[0]) for t in (1, 2, 4)]
-        out += [*(("scaled_product", tiles_kernel(dtype, t)[0]) for t in TILES),
+        out += [*(("scaled_product", tiles_kernel(dtype, t)[0])
+                  for t in (TILES[-1:] if dtype == torch.float32 else TILES)),
                 ("scaled_product", product_join_kernel(dtype)[0]), ("sample", sample_kernel(dtype)[0])]
     return out

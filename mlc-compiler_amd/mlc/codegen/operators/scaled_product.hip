@@ -75,6 +75,17 @@ __device__ __forceinline__ Codes<true> operand(const uint8_t* p, int g, int left
   return Codes<true>(lo, hi);
 }
 
+// The first ``count`` of N values, or all.
+template <int A, int N, class T> __device__ __forceinline__ void store_some(T* p, const T (&x)[N], int count) {
+  if (count >= N) {
+    store_n<A>(p, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < count) p[e] = x[e];
+  }
+}
+
 template <class T> __device__ __forceinline__ float bias_of(const ScaledProductArgs& a, int n) {
   return a.wide_bias ? at<float>(a.bias, a.c_off)[n] : element<T>::widen(at<T>(a.bias, a.c_off)[n]);
 }
@@ -129,36 +140,43 @@ __device__ __forceinline__ void scaled_product_rows(const ScaledProductArgs& a) 
   }
 }
 
-// Many rows: tiles of BM rows of a and BN of the weight, WM x WN waves. Blocks of both pass
-// through LDS, STAGES - 1 of them on their way while one is in use. A row is 8 pieces of 16 bytes, piece
-// c of row r in slot c ^ (r / 2 % 8): the same piece of 16 rows lies in 64 distinct banks.
+// Many rows: tiles of BM rows of a and BN of the weight, WM x WN waves. Two blocks of both are in LDS
+// or on their way there. A row is 8 pieces of 16 bytes, piece c of row r in slot c ^ (r / 2 % 8): the
+// same piece of 16 rows lies in 64 distinct banks.
+//
+// A wave keeps its rows of a in registers for a block and takes the weight's 16 by 16; each such row
+// of products begins when the one before is added. The weight's rows come in LB parts, each
+// with a barrier of its own: what has been read is free, and is asked for again for the block after
+// the next, nearly two blocks ahead (one ahead, with a barrier a block, 8192 rows, 12288 -> 4096 take 405 us and
+// with these 350). No branch lies between the rows: additions would be moved behind it, and their products
+// would not fit the registers.
+//
 // A buffer's offsets of 32 bits reach a tile of rows with one stride from its first, and others from
 // the tensor's; what lies past the last row or value has an offset past the buffer's end, and is zeros.
 constexpr uint32_t OUTSIDE = 0x80000000u;
 
-template <class T, int BM, int BN, int WM, int WN, int STAGES>
+template <class T, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void scaled_product_tiles(const ScaledProductArgs& a) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS, STEP = THREADS / 8;
-  constexpr int TILE = (BM + BN) * 128, STAGE = TILE + BM * 4;
-  static_assert(STEP % 16 == 0 && LA >= 1 && LB >= 1 && BN / WN <= 128 && BM % 64 == 0, "staging");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
+  constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS, STEP = THREADS / 8;  // loads, and rows of one
+  constexpr int R = TN / LB;                                                       // rows of products of a part
+  constexpr int STAGE = (BM + BN) * 128, GROUP = 8, SCALES = BM * GROUP * 4;       // scales of 8 blocks
+  static_assert(LA >= 1 && LB >= 2 && R * LB == TN && R * 16 * WN == STEP && BN / WN <= 128, "staging");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE + 2 * SCALES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int col_tiles = (a.n + BN - 1) / BN;
-  // neighbouring workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles
   int w = blockIdx.x;
   const int split = w % a.splits;
   w /= a.splits;
   const int all = a.row_tiles * col_tiles;
-  {
+  {  // neighbouring workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles
     const int per = all / 8, more = all % 8, x = w % 8, y = w / 8;
     w = x * per + (x < more ? x : more) + y;
   }
-  // in bands of 8 row tiles
   int mt, nt;
-  {
+  {  // in bands of 8 row tiles
     constexpr int BAND = 8;
     const int band = w / (BAND * col_tiles), first = band * BAND;
     const int high = a.row_tiles - first < BAND ? a.row_tiles - first : BAND;
@@ -170,8 +188,8 @@ __device__ __forceinline__ void scaled_product_tiles(const ScaledProductArgs& a)
   const int wm = wave % WM, wn = wave / WM;
   const int blocks = (a.k + 127) / 128;
   const int begin = (int)((int64_t)blocks * split / a.splits), end = (int)((int64_t)blocks * (split + 1) / a.splits);
+  const int steps = end - begin;
 
-  const int own = threadIdx.x / 8, chunk = (threadIdx.x & 7) ^ (own >> 1 & 7);
   const int base = a.regular ? m0 : 0;
   auto offset = [&](int m, int64_t batch, int64_t token) {
     m += m0 - base;
@@ -180,127 +198,201 @@ __device__ __forceinline__ void scaled_product_tiles(const ScaledProductArgs& a)
   const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at<uint8_t>(a.a, a.a_off) + base * a.at), 0, OUTSIDE, 0x27000);
   const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at<uint8_t>(a.b, a.b_off) + n0 * a.br), 0, OUTSIDE, 0x27000);
   const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(at<float>(a.a_scales, a.as_off) + base * a.ast), 0, OUTSIDE, 0x27000);
+  const int own = threadIdx.x / 8, chunk = (threadIdx.x & 7) ^ (own >> 1 & 7);
   uint32_t va[LA], vb[LB];
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
     const int m = own + i * STEP;
-    va[i] = m0 + m < a.rows ? offset(m, a.ab, a.at) : OUTSIDE;
+    va[i] = m0 + m < a.rows ? offset(m, a.ab, a.at) + 16 * chunk : OUTSIDE;
   }
 #pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    const int n = own + i * STEP;
-    vb[i] = n0 + n < a.n ? n * (uint32_t)a.br : OUTSIDE;
+  for (int i = 0; i < LB; ++i) {  // a part has R * 16 rows of each column of waves
+    const int n = own / (R * 16) * (TN * 16) + i * R * 16 + own % (R * 16);
+    vb[i] = n0 + n < a.n ? n * (uint32_t)a.br + 16 * chunk : OUTSIDE;
   }
-  const int sr = (wave * 64 + lane) % BM;
-  const uint32_t vs = m0 + sr < a.rows ? offset(sr, a.asb, a.ast) * 4 : OUTSIDE;
-  const int nb = (n0 + wn * (BN / WN)) / 128;
-  const float* const bs = at<float>(a.b_scales, a.bs_off) + (nb < (a.n + 127) / 128 ? nb : 0) * a.bsr;
-  // the weight's scales of 64 steps, one a lane: a load in every step would wait for the tiles on
-  // their way (a vector's) or for the reads of LDS (a scalar's)
-  float held = 0.0f;
-
-  auto load = [&](int i, int into) __attribute__((always_inline)) {
-    const uint32_t piece = 128 * i + 16 * chunk < a.k ? 16 * chunk : OUTSIDE;
-    uint8_t* const to = lds + into * STAGE + wave * 1024;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  auto past = [&](int i) { return i < end && 128 * i + 16 * chunk < a.k ? 0u : OUTSIDE; };
+  auto load_a = [&](int i) __attribute__((always_inline)) {
+    uint8_t* const to = lds + (i - begin & 1) * STAGE + wave * 1024;
 #pragma unroll
     for (int l = 0; l < LA; ++l)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(to + l * THREADS * 16), 16, va[l] | piece, i * 128, 0, 0);
-#pragma unroll
-    for (int l = 0; l < LB; ++l)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(to + BM * 128 + l * THREADS * 16), 16, vb[l] | piece, i * 128, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + into * STAGE + TILE + wave * 64 % BM * 4), 4, vs, i * (int)a.ass * 4, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(to + l * THREADS * 16), 16, va[l] | past(i), i * 128, 0, 0);
   };
-  float4v sum[TN][TM] = {};
+  auto load_b = [&](int i, int l) __attribute__((always_inline)) {
+    uint8_t* const to = lds + (i - begin & 1) * STAGE + wave * 1024 + BM * 128;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(to + l * THREADS * 16), 16, vb[l] | past(i), i * 128, 0, 0);
+  };
+  // Scales of a's rows for 8 blocks: row by row they lie far apart, and a load for each block would
+  // take as many requests as the codes. In pieces of 4 where no piece crosses a row's end.
+  const bool fours = a.ass == 1 && (blocks - begin & 3) == 0;
+  auto load_scales = [&](int i) __attribute__((always_inline)) {
+    uint8_t* const to = lds + 2 * STAGE + (i - begin & GROUP ? SCALES : 0);
+#pragma unroll
+    for (int at_row = wave * 32; at_row < BM; at_row += WAVES * 32) {  // 1024 bytes at a time
+      if (fours) {
+        const int m = at_row + lane / 2, block = i + lane % 2 * 4;
+        const uint32_t v = m0 + m < a.rows && block < blocks ? offset(m, a.asb, a.ast) * 4 + block * 4 : OUTSIDE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + at_row * GROUP * 4), 16, v, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = at_row + q * 8 + lane / 8, block = i + lane % 8;
+          const uint32_t v = m0 + m < a.rows && block < blocks ? (offset(m, a.asb, a.ast) + block * (uint32_t)a.ass) * 4 : OUTSIDE;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (at_row + q * 8) * GROUP * 4), 4, v, 0, 0, 0);
+        }
+      }
+    }
+  };
+  // the weight's scales of 64 blocks, one a lane
+  const int nb = (n0 + wn * (BN / WN)) / 128;
+  const float* const bs = at<float>(a.b_scales, a.bs_off) + (nb < (a.n + 127) / 128 ? nb : 0) * a.bsr;
+  float held = 0.0f;
+
+  float4v sum[TN][TM] = {}, p[TM] = {};
   const int swizzle = r >> 1 & 7;
-  const uint32_t a_at = (wm * TM * 16 + r) * 128, b_at = BM * 128 + (wn * TN * 16 + r) * 128;
-  const uint32_t lo = (g ^ swizzle) * 16, hi = ((4 + g) ^ swizzle) * 16, s_at = TILE + (wm * TM * 16 + r) * 4;
-  auto compute = [&](int i, int stage) __attribute__((always_inline)) {
-    const uint8_t* const from = lds + stage * STAGE;
-    auto read = [&](uint32_t row) __attribute__((always_inline)) {
-      return Codes<EXACT>(*reinterpret_cast<const int4v*>(from + row + lo), *reinterpret_cast<const int4v*>(from + row + hi));
-    };
-    const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), (i - begin) & 63));
-    Codes<EXACT> x[TM], y = read(b_at), z;
+  const uint32_t lo = (g ^ swizzle) * 16, hi = ((4 + g) ^ swizzle) * 16;
+  const uint32_t a_at = (wm * TM * 16 + r) * 128, b_at = BM * 128 + (wn * R * 16 + r) * 128;
+  auto read = [&](const uint8_t* from) __attribute__((always_inline)) {
+    return Codes<EXACT>(*reinterpret_cast<const int4v*>(from + lo), *reinterpret_cast<const int4v*>(from + hi));
+  };
+  auto part_of = [&](int l) { return b_at + (l / R * STEP + l % R * 16) * 128; };
+  // Part s of step i is there for everyone, and what lies in front of it has been read: its place
+  // is filled again. Loads end in order; the counts are of those that were asked for later.
+  auto arrive = [&](int i, int s) __attribute__((always_inline)) {
+    if (s < 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(LA + 2 * LB - 2) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(2 * LA + 2 * LB - 2) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    if (s == 0) {
+      load_b(i + 1, LB - 1);
+    } else {
+      if (s == 1) load_a(i + 2);
+      load_b(i + 2, s - 1);
+    }
+  };
+  load_scales(begin);
+  load_a(begin);
+#pragma unroll
+  for (int l = 0; l < LB; ++l) load_b(begin, l);
+  load_a(begin + 1);
+#pragma unroll
+  for (int l = 0; l < LB - 1; ++l) load_b(begin + 1, l);
+  arrive(begin, 0);
+  Codes<EXACT> x[TM], y, z;
+#pragma unroll
+  for (int j = 0; j < TM; ++j) x[j] = read(lds + a_at + j * 2048);
+  y = read(lds + part_of(0));
+  float before[TM] = {};  // the scales of the step before
+  for (int i = 0; i < steps; ++i) {
+    if (i % GROUP == 0) load_scales(begin + i + GROUP);
+    if (i % 64 == 0) {
+      held = bs[(begin + i + lane < end ? begin + i + lane : end - 1) * a.bss];
+      asm volatile("" : "+v"(held));  // waits here, and in no other step
+    }
+    const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), i % 64));
+    const uint8_t* const from = lds + (i & 1) * STAGE;
+    const uint8_t* const next = lds + (~i & 1) * STAGE;
+    const float* const scales = reinterpret_cast<const float*>(lds + 2 * STAGE + (i & GROUP ? SCALES : 0)) + i % GROUP;
     float s[TM];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      s[j] = *reinterpret_cast<const float*>(from + s_at + j * 64) * by;
-      x[j] = read(a_at + j * 2048);
-    }
-    float4v p[2][TM];
+    for (int j = 0; j < TM; ++j) s[j] = scales[((wm * TM + j) * 16 + r) * GROUP] * by;
 #pragma unroll
-    for (int l = 0; l <= TN; ++l) {
-      if (l + 1 < TN) z = read(b_at + (l + 1) * 2048);
+    for (int l = 0; l < TN; ++l) {
+      if (l % R < R - 1) {
+        z = read(from + part_of(l + 1));
+      } else if (l + 1 < TN) {
+        arrive(begin + i, l / R + 1);
+        z = read(from + part_of(l + 1));
+      } else {
+        arrive(begin + i + 1, 0);
+        z = read(next + part_of(0));
+      }
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        if (l < TN) p[l & 1][j] = dots(y, x[j]);
-        if (l > 0)
+        const float by_row = l > 0 ? s[j] : before[j];
+        float4v& to = sum[l > 0 ? l - 1 : TN - 1][j];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum[l - 1][j][e] = __builtin_fmaf(p[l - 1 & 1][j][e], s[j], sum[l - 1][j][e]);
+        for (int e = 0; e < 4; ++e) to[e] = __builtin_fmaf(p[j][e], by_row, to[e]);
+        p[j] = dots(y, x[j]);
+        if (l + 1 == TN) x[j] = read(next + a_at + j * 2048);  // as this step's goes
       }
       y = z;
-      // a product, then the four additions of one before, whose result is there by then
-      if (!EXACT && l > 0 && l < TN) {
+      if (!EXACT && l > 0 && l + 1 < TN) {
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // no reads further ahead: registers
     }
-  };
-  constexpr int LOADS = LA + LB + 1;
-  const int steps = end - begin;
 #pragma unroll
-  for (int p = 0; p < STAGES - 1; ++p)
-    if (p < steps) load(begin + p, p);
-  int stage = 0;
-  for (int i = 0; i < steps; ++i) {
-    if ((i & 63) == 0) held = bs[(begin + i + lane < end ? begin + i + lane : end - 1) * a.bss];
-    // all but the loads of the steps after this one
-    if (STAGES > 2 && i + STAGES - 1 <= steps)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(LOADS * (STAGES - 2)) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" : : : "memory");
-    if (i + STAGES - 1 < steps) load(begin + i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    compute(begin + i, stage);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    for (int j = 0; j < TM; ++j) before[j] = s[j];
   }
 #pragma unroll
-  for (int l = 0; l < TN; ++l)
+  for (int j = 0; j < TM; ++j)
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const int m = m0 + (wm * TM + j) * 16 + r, n = n0 + (wn * TN + l) * 16 + 4 * g;
-      if (m >= a.rows) continue;
-      if (a.splits > 1) {
-        float* const part = a.part + ((int64_t)split * a.rows + m) * a.n + n;
-        if (n + 4 <= a.n) {
-          const float y[4] = {sum[l][j][0], sum[l][j][1], sum[l][j][2], sum[l][j][3]};
-          store_n<4>(part, y);
-        } else {
+    for (int e = 0; e < 4; ++e) sum[TN - 1][j][e] = __builtin_fmaf(p[j][e], before[j], sum[TN - 1][j][e]);
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // the zeros behind the last step are in LDS too
+  const int first_m = m0 + wm * TM * 16, first_n = n0 + wn * TN * 16;
+  auto bias_from = [&](int n, float (&add)[4]) __attribute__((always_inline)) {
+    if (a.bias) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.n) part[e] = sum[l][j][e];
-        }
-      } else {
-        T* const out = reinterpret_cast<T*>(a.out) + (int64_t)m * a.n + n;
-        T y[4];
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.n) add[e] = bias_of<T>(a, n + e);
+    }
+  };
+  if (EXACT || a.splits > 1) {  // four fp32 values are a piece
+    const bool parts = a.splits > 1;
+    float* const out = parts ? a.part + (int64_t)split * a.rows * a.n : reinterpret_cast<float*>(a.out);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = element<T>::narrow(sum[l][j][e] + (a.bias && n + e < a.n ? bias_of<T>(a, n + e) : 0.0f));
-        if (n + 4 <= a.n) {
-          store_n<(int)sizeof(T)>(out, y);
-        } else {
+    for (int l = 0; l < TN; ++l) {
+      const int n = first_n + l * 16 + 4 * g;
+      float add[4] = {};
+      if (!parts) bias_from(n, add);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.n) out[e] = y[e];
-        }
+      for (int j = 0; j < TM; ++j) {
+        const int m = first_m + j * 16 + r;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = sum[l][j][e] + add[e];
+        if (m < a.rows) store_some<4>(out + (int64_t)m * a.n + n, v, a.n - n);
       }
     }
+    return;
+  }
+  // A wave's results go through LDS, so that rows are written in 16-byte pieces side by side: lanes
+  // hold four values of 16 rows, and stores of 8 bytes took 24 us a tile of 256 x 256. Pieces
+  // of a row are xor-ed with its number, as the tiles'.
+  constexpr int SIZE = sizeof(T), PIECES = TN * SIZE, EACH = 16 / SIZE;
+  static_assert(EXACT || WAVES * TM * 16 * PIECES * 16 <= 2 * STAGE, "results in LDS");
+  __syncthreads();
+  uint8_t* const own_lds = lds + wave * (TM * 16 * PIECES * 16);
+  auto slot = [&](int row, int piece) __attribute__((always_inline)) {
+    return (row * PIECES + (piece ^ (PIECES >= 16 ? row & 15 : PIECES == 8 ? row >> 1 & 7 : row >> 2 & 3))) * 16;
+  };
+#pragma unroll
+  for (int l = 0; l < TN; ++l) {
+    float add[4] = {};
+    bias_from(first_n + l * 16 + 4 * g, add);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      T v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = element<T>::narrow(sum[l][j][e] + add[e]);
+      const int at_byte = (l * 16 + 4 * g) * SIZE;
+      store_n<4 * SIZE>(reinterpret_cast<T*>(own_lds + slot(j * 16 + r, at_byte / 16) + at_byte % 16), v);
+    }
+  }
+  // a wave's own part of LDS: its writes are in order before its reads
+#pragma unroll
+  for (int i = lane; i < TM * 16 * PIECES; i += 64) {
+    const int row = i / PIECES, piece = i % PIECES, m = first_m + row, n = first_n + piece * EACH;
+    T v[EACH];
+    load_n<16>(v, reinterpret_cast<const T*>(own_lds + slot(row, piece)));
+    if (m < a.rows) store_some<SIZE>(reinterpret_cast<T*>(a.out) + (int64_t)m * a.n + n, v, a.n - n);
+  }
 }
 
 // The sum of the parts that splits of the blocks have left.
@@ -316,9 +408,9 @@ template <class T> __device__ __forceinline__ void scaled_product_join(const Sca
 
 }  // namespace mlc
 
-#define SCALED_PRODUCT_TILES(NAME, T, BM, BN, WM, WN, STAGES)                                  \
+#define SCALED_PRODUCT_TILES(NAME, T, BM, BN, WM, WN)                                          \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN) NAME(mlc::ScaledProductArgs a) {  \
-    mlc::scaled_product_tiles<T, BM, BN, WM, WN, STAGES>(a);                                   \
+    mlc::scaled_product_tiles<T, BM, BN, WM, WN>(a);                                           \
   }
 #define SCALED_PRODUCT_JOIN(NAME, T)                                                                \
   extern "C" __global__ void __launch_bounds__(mlc::JOIN_BLOCK) NAME(mlc::ScaledProductArgs a) {    \
