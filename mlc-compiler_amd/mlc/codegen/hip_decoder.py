@@ -115,16 +115,48 @@ def plan_quantize(x: Operand, gate: Operand | None) -> Plan:
 # products
 # --------------------------------------------------------------------------
 
-#: rows that a workgroup of few rows takes at most, and its waves
-FEW_ROWS, FEW_WAVES = 64, 8
-#: tiles of many rows: rows of both operands, waves along both
-TILES = ((256, 256, 4, 2), (128, 128, 2, 2))
+#: Rows and columns up to which a workgroup reads all of a beside 16 rows of the weight, in 8 waves with
+#: 4 blocks each: 1 row, 4096 -> 6144 8.6 us and in tiles 10.8, 4 rows, 4096 -> 4096 6.5 and 9.9; 16 rows,
+#: 4096 -> 16384 21.3 and 13.8.
+FEW_ROWS, FEW_COLUMNS, FEW_BLOCKS, FEW_WAVES = 8, 16384, 4, 8
+#: Tiles of many rows by the product's instructions, exact or not (rows of both operands, waves along both):
+#: workgroups that a unit holds, and in us what one takes beside its steps, a step of one alone and of each of
+#: many. Measured over 768 to 12288 inputs, 128 to 8192 rows and 2304 to 24576 outputs.
+TILES = {False: {(256, 256, 4, 2): (1, 8.5, 1.7, 1.7), (128, 128, 2, 2): (2, 3.5, 0.75, 0.59),
+                 (64, 64, 2, 2): (4, 2.5, 0.31, 0.21), (32, 64, 2, 2): (4, 2.5, 0.28, 0.155)},
+         True: {(128, 128, 2, 2): (2, 3.5, 1.25, 1.05), (64, 64, 2, 2): (4, 2.5, 0.46, 0.36),
+                (32, 64, 2, 2): (4, 2.5, 0.38, 0.22)}}
 JOIN_THREADS = 256
 
 
-def few_kernel(dtype, tiles: int) -> tuple[str, str]:
-    name = f"scaled_product_rows_{SHORT[dtype]}_m{tiles}"
-    return f"SCALED_PRODUCT_ROWS({name}, {NAMES[dtype]}, {tiles}, {FEW_WAVES})", name
+def is_exact(rows: int, n: int, dtype: torch.dtype) -> bool:
+    """Whether products are taken of widened codes: where that costs nothing, or fp32 results show it."""
+    return dtype == torch.float32 or (rows <= FEW_ROWS and n <= FEW_COLUMNS)
+
+
+def choose_tile(rows: int, n: int, blocks: int, dtype: torch.dtype) -> tuple[tuple, int]:
+    """The tile, and splits of the sum, that cost least. A unit's workgroups share it, so a step takes
+    as many times its work as there are, but not less than alone. Splits cost a second launch
+    and parts in fp32, written and read: 4 us and 8 bytes a value at 3 TB/s."""
+    best = None
+    for tile, (room, first, alone, each) in TILES[dtype == torch.float32].items():
+        tiles = _ceil(rows, tile[0]) * _ceil(n, tile[1])
+        for splits in range(1, max(1, min(blocks // 2, 2 * UNITS // tiles)) + 1):
+            steps = _ceil(blocks, splits)
+            full, rest = divmod(tiles * splits, UNITS * room)
+            cost = full * (first + steps * max(alone, room * each))
+            if rest:
+                cost += first + steps * max(alone, _ceil(rest, UNITS) * each)
+            if splits > 1:
+                cost += 4 + splits * rows * n * 8 / 3e6
+            if best is None or cost < best[0]:
+                best = cost, (tile, splits)
+    return best[1]
+
+
+def few_kernel(dtype) -> tuple[str, str]:
+    name = f"scaled_product_rows_{SHORT[dtype]}"
+    return f"SCALED_PRODUCT_ROWS({name}, {NAMES[dtype]}, {FEW_BLOCKS}, {FEW_WAVES})", name
 
 
 def tiles_kernel(dtype, tile: tuple) -> tuple[str, str]:
@@ -169,21 +201,19 @@ def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, b
     if regular:
         seq = rows
     pointers = ["a", "a_scales", "b", "b_scales", "bias" if bias is not None else None, "out0", None]
-    few = rows <= FEW_ROWS
-    if few:
-        kernel, name = few_kernel(dtype, next(t for t in (1, 2, 4) if 16 * t >= rows))
+    if rows <= FEW_ROWS and n <= FEW_COLUMNS:
+        kernel, name = few_kernel(dtype)
         grid, threads = _ceil(n, 16), 64 * FEW_WAVES
     else:
-        tile = TILES[-1] if dtype == torch.float32 else TILES[0]
+        tile, splits = choose_tile(rows, n, blocks, dtype)
         reach = max(max(tile[:2]) * max(strides[1], b.strides[0], 4 * scale_strides[1]) if regular else
                     max(_reach(a, strides), _reach(a_scales, scale_strides), max(tile[:2]) * b.strides[0]),
                     4 * a_scales.strides[-1] * blocks) + k
         if reach >= 1 << 31:
             raise OperatorError("scaled_product: rows that lie too far apart: make them contiguous")
-        row_tiles, tiles = _ceil(rows, tile[0]), _ceil(rows, tile[0]) * _ceil(n, tile[1])
-        splits = max(1, min(UNITS // tiles, blocks // 4))
+        row_tiles = _ceil(rows, tile[0])
         kernel, name = tiles_kernel(dtype, tile)
-        grid, threads = tiles * splits, 64 * tile[2] * tile[3]
+        grid, threads = row_tiles * _ceil(n, tile[1]) * splits, 64 * tile[2] * tile[3]
         if splits > 1:
             pointers[-1] = "workspace"
     tail = struct.pack("<5q8q8i", a.offset, a_scales.offset, b.offset, b_scales.offset, _offset(bias),
@@ -258,8 +288,7 @@ def all_kernels() -> list[tuple[str, str]]:
         for w, n in NORM_SHAPES:
             out += [("rows", norm_kernel(dtype, a, w, n, e)[0]) for a in aligns for e in (False, True)]
         out += [("rows", quantize_kernel(dtype, a, g)[0]) for a in aligns for g in (False, True)]
-        out += [("scaled_product", few_kernel(dtype, t)[0]) for t in (1, 2, 4)]
-        out += [*(("scaled_product", tiles_kernel(dtype, t)[0])
-                  for t in (TILES[-1:] if dtype == torch.float32 else TILES)),
-                ("scaled_product", product_join_kernel(dtype)[0]), ("sample", sample_kernel(dtype)[0])]
+        out += [("scaled_product", few_kernel(dtype)[0]), ("scaled_product", product_join_kernel(dtype)[0]),
+                ("sample", sample_kernel(dtype)[0])]
+        out += [("scaled_product", tiles_kernel(dtype, t)[0]) for t in TILES[dtype == torch.float32]]
     return out

@@ -9,7 +9,7 @@ import math
 import numpy as np
 import torch
 
-from mlc.codegen.hip_decoder import FEW_ROWS
+from mlc.codegen.hip_decoder import is_exact
 from operators_reference import F, LEAST, U
 
 E4M3 = torch.float8_e4m3fn
@@ -106,7 +106,7 @@ def product(a, a_scales, b, b_scales, bias=None):
 
 def check_product(got, want, bound, groups, dtype):
     assert got.dtype == dtype and got.is_contiguous() and got.shape == want.shape
-    if dtype != torch.float32 and math.prod(want.shape[:-1]) > FEW_ROWS:
+    if not is_exact(math.prod(want.shape[:-1]), want.shape[-1], dtype):
         bound = bound + groups
     bound = bound * (1 + U[dtype]) + U[dtype] * want.abs() + LEAST[dtype]
     off = (_host(got) - want).abs()
