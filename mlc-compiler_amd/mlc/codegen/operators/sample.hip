@@ -9,14 +9,17 @@
 // ``uniform`` of the kept weight lies.
 //
 // Sums are of whole numbers of 2^-40, so they are exact whatever their order: results do not depend
-// on how a row is divided or on the order of atomics.
+// on the order of atomics.
 //
-// A workgroup has a row, which its caches hold after the first pass, for the largest logit, the
-// only one that memory bounds. A pass over 131072 tokens on one unit then costs 0.85 us for each
-// instruction of a token. So what can be kept is gathered first where a bound for it is at
-// hand (the top_k-th of the threads' own largest, or min_p) and fits a list: sorted in LDS, it
-// says everything. Otherwise borders come from a histogram of distances to the largest, whose
-// border bin fits the list, and the token from the kept weight of ever smaller segments.
+// A workgroup has a row. Only its first pass, for the largest logit, is bound by memory; then caches hold the
+// row, and each instruction of a token takes 0.85 us in 131072 of them, on one unit. What runs once is
+// bound by its own way from memory, 64 bytes of code at a time. So loops are short and passes few:
+//  * What can be kept is gathered where a bound for it is at hand (the top_k-th of the threads' own
+//    largest, or min_p) and fits a list: sorted, it says everything.
+//  * Else tokens are counted by their distance to the largest, which says in which bins the borders
+//    are. The tokens of those are gathered, the weight in front of them is summed up, exactly.
+//  * The token comes from the kept weight of ever smaller segments of the row.
+//  * Where a list is too short (equal logits), borders are found digit by digit.
 
 namespace mlc {
 
@@ -38,8 +41,8 @@ struct SampleArgs {
 
 typedef unsigned long long u64;
 constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / 64, SAMPLE_BINS = 2048;
-constexpr int SAMPLE_LIST = 1024;                                          // a thread for each
-constexpr int SAMPLE_FEW = 512;                                            // top_k whose tokens are gathered
+constexpr int SAMPLE_LIST = 1024, SAMPLE_EACH = 512;  // tokens that are sorted, a thread for each, and gathered by a wave
+constexpr int SAMPLE_FEW = 512;                          // top_k whose tokens are gathered
 constexpr float LEAST_TEMPERATURE = 0x1p-100f, MOST_TEMPERATURE = 0x1p100f;  // below the least the likeliest token
 
 // A number that orders as floats do, -0 as 0, and back.
@@ -52,13 +55,17 @@ __device__ __forceinline__ float of_order(uint32_t k) {
 }
 
 struct SampleLds {
-  u64 bins[SAMPLE_BINS];  // and a list's weights
-  u64 list[SAMPLE_LIST], sorted[SAMPLE_LIST];
+  alignas(16) char tail[32];  // the row's last pack
+  union {
+    u64 bins[SAMPLE_BINS];  // and a list's weights
+    uint32_t counts[2 * SAMPLE_BINS];
+  };
+  u64 gathered[SAMPLE_WAVES][SAMPLE_EACH], list[SAMPLE_LIST], sorted[SAMPLE_LIST];
   u64 sums[SAMPLE_WAVES];
   u64 found[2];
   float tops[SAMPLE_WAVES];
   uint32_t least[SAMPLE_WAVES];
-  int count, digits[6];
+  int counts_of[SAMPLE_WAVES], digits[6];
 };
 
 // The sum of x over the workgroup; ``below``: of the threads before this one.
@@ -87,12 +94,16 @@ __device__ __forceinline__ u64 sum_over_threads(u64 x, SampleLds& l, u64& below)
 __device__ __forceinline__ u64 sort_list(int n, SampleLds& l) {
   const int tid = threadIdx.x;
   constexpr u64 LAST = ~(u64)0;
-  if (n <= 256) {  // by counting the ones below
+  if (n <= 256) {  // by counting the ones below, 16 at a time
+    if (tid >= n && tid < n + 15) l.list[tid] = LAST;
     __syncthreads();
     if (tid < n) {
       const u64 own = l.list[tid];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += l.list[i] < own;
+      for (int i = 0; i < n; i += 16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) rank += l.list[i + j] < own;
+      }
       l.sorted[rank] = own;
     }
     __syncthreads();
@@ -131,7 +142,8 @@ struct Weigh {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi, d * lo));
   }
 };
-// In units of 2^-40, rounded; up to 8.
+// In units of 2^-40, rounded: a whole number, as which a double adds them exactly up to 2^53.
+__device__ __forceinline__ double whole(float w) { return __builtin_fma((double)w, 0x1p40, 0x1p52) - 0x1p52; }
 __device__ __forceinline__ u64 units(float w) {
   return __builtin_bit_cast(u64, __builtin_fma((double)w, 0x1p40, 0x1p52)) & 0xfffffffffffffull;
 }
@@ -144,7 +156,7 @@ struct Border {
 };
 
 template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
-  __shared__ SampleLds l;
+  __shared__ __attribute__((aligned(16))) SampleLds l;
   const int b = blockIdx.x, tid = threadIdx.x, size = a.size;
   const T* const row = at<T>(a.logits, a.l_off) + b * a.lb;
   const float uniform = at<float>(a.uniform, a.u_off)[b * a.us];
@@ -152,48 +164,58 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   int top_k = a.top_k ? at<int32_t>(a.top_k, a.k_off)[b * a.ks] : 0;
   const float top_p = a.top_p ? at<float>(a.top_p, a.p_off)[b * a.ps] : 1.0f;
   const float min_p = a.min_p ? at<float>(a.min_p, a.m_off)[b * a.ms] : 0.0f;
+  constexpr float NONE = -__builtin_inff();
 
-  // f(8 logits, index of the first) of the tokens of this thread from lo up to hi, which is a
-  // multiple of 8 from lo or the row's end; -infinity past that. Four packs are on their way at a time.
+  // the row's last pack, with -infinity behind its end
+  T* const tail = reinterpret_cast<T*>(l.tail);
+  if (tid < 8) tail[tid] = size / 8 * 8 + tid < size ? row[size / 8 * 8 + tid] : element<T>::narrow(NONE);
+  __syncthreads();
+  // f(8 logits, index of the first) of the packs of this thread from lo up to hi, a multiple of 8 from
+  // lo or the row's end. One pack is on its way while one is in use.
   auto over = [&](int lo, int hi, int thread, int threads, auto f) __attribute__((always_inline)) {
-    for (int i = lo + thread * 8; i < hi; i += threads * 32) {
-      T x[4][8];
+    auto load = [&](int i, T (&x)[8]) __attribute__((always_inline)) {
+      if (i + 8 <= size) load_n<(int)sizeof(T)>(x, row + i);
+      else load_n<16>(x, tail);
+    };
+    int i = lo + thread * 8;
+    T next[8];
+    if (i < hi) load(i, next);
+#pragma unroll 1
+    for (; i < hi; i += threads * 8) {
+      float x[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int at = i + u * threads * 8;
-        if (at + 8 <= size && at < hi) load_n<(int)sizeof(T)>(x[u], row + at);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int at = i + u * threads * 8;
-        if (at >= hi) break;
-        float y[8];
-        if (at + 8 <= size) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = element<T>::widen(x[u][j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = at + j < size ? element<T>::widen(row[at + j]) : -__builtin_inff();
-        }
-        f(y, at);
-      }
+      for (int j = 0; j < 8; ++j) x[j] = element<T>::widen(next[j]);
+      if (i + threads * 8 < hi) load(i + threads * 8, next);
+      f(x, i);
     }
   };
 
-  float own_top = -__builtin_inff();
-  over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int) __attribute__((always_inline)) {
+  float own_top = NONE;
+#pragma unroll 1
+  for (int i = tid * 8; i < size; i += SAMPLE_THREADS * 32) {  // four packs on their way: from memory
+    T x[4][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) own_top = __builtin_elementwise_maximum(own_top, x[j]);
-  });
+    for (int u = 0; u < 4; ++u) {
+      const int at = i + u * SAMPLE_THREADS * 8;
+      if (at + 8 <= size) load_n<(int)sizeof(T)>(x[u], row + at);
+      else load_n<16>(x[u], tail);  // again and again, past the end
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) own_top = __builtin_elementwise_maximum(own_top, element<T>::widen(x[u][j]));
+  }
   float top = own_top;
+#pragma unroll
   for (int by = 1; by < 64; by *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, by));
   if ((tid & 63) == 0) l.tops[tid >> 6] = top;
-  if (tid == 0) l.count = 0;
   __syncthreads();
-  for (int w = 0; w < SAMPLE_WAVES; ++w) top = __builtin_elementwise_maximum(top, l.tops[w]);
+  top = l.tops[tid & (SAMPLE_WAVES - 1)];
+#pragma unroll
+  for (int by = 1; by < SAMPLE_WAVES; by *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, by));
   const bool fine = uniform >= 0.0f && uniform < 1.0f && temperature >= 0.0f && temperature <= MOST_TEMPERATURE &&
                     top_p >= 0.0f && top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f && top < __builtin_inff();
-  if (!fine || top == -__builtin_inff()) {
+  if (!fine || top == NONE) {
     if (tid == 0) {
       a.out[b] = -1;
       if (!fine) *a.error = INVALID_SAMPLE;
@@ -219,71 +241,80 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   }
   const Weigh weigh(top, temperature);
   if (top_k <= 0 || top_k >= size) top_k = 0;
-  float least = -__builtin_inff();  // the least logit of min_p's weight or more
-  if (min_p > 0.0f) {
-    const double x = (double)top + (double)temperature * log((double)min_p);
-    least = (float)x;
-    if ((double)least < x)  // the next float
-      least = least == 0.0f ? 0x1p-149f : __builtin_bit_cast(float, __builtin_bit_cast(int, least) + (least > 0.0f ? 1 : -1));
-  }
+  // logits below this have less than min_p's weight; which of the others have is for their weight to say
+  const float least = min_p > 0.0f ? top + (__builtin_amdgcn_logf(min_p) - 0.01f) / weigh.hi : NONE;
 
   auto clear_bins = [&] {
     __syncthreads();
-    for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) l.bins[i] = 0;
+    l.bins[tid] = l.bins[tid + SAMPLE_THREADS] = 0;
     __syncthreads();
   };
-  // The bin up to which the bins' sum reaches ``want``, and the sum in front of it
-  auto find_bin = [&](u64 want, u64& before) {
-    const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+  // Numbers that rise along the order. Each wave gathers its own, without atomics: ``held`` says how
+  // many it has, which may be more than fit.
+  const int wave = tid >> 6;
+  auto x_of = [](u64 key) { return of_order(~(uint32_t)(key >> 32)); };
+  int held = 0;
+  auto put = [&](bool in, float x, int i) __attribute__((always_inline)) {
+    const u64 mask = __ballot(in);
+    if (mask == 0) return;
+    const int at = held + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (in && at < SAMPLE_EACH) l.gathered[wave][at] = (u64)~order_of(x) << 32 | (uint32_t)i;
+    held += __popcll(mask);
+  };
+  // How many all waves have, and those of them that f says in one list, or more than fit it.
+  auto collect = [&](auto f) __attribute__((always_inline)) {
+    const bool fits = held <= SAMPLE_EACH;
+    int own = 0;
+    __syncthreads();  // gathered, and the list has been read
+    if (fits)
+#pragma unroll 1
+      for (int i = tid & 63; i < held; i += 64) own += f(l.gathered[wave][i]);
     u64 below;
-    sum_over_threads(first + second, l, below);
-    if (below < want && below + first >= want) {
-      l.found[0] = 2 * tid;
-      l.found[1] = below;
-    } else if (below + first < want && below + first + second >= want) {
-      l.found[0] = 2 * tid + 1;
-      l.found[1] = below + first;
-    }
+    const int n = (int)sum_over_threads(fits ? own : SAMPLE_LIST + 1, l, below);
+    int at = (int)below;
+    if (n <= SAMPLE_LIST)
+#pragma unroll 1
+      for (int i = tid & 63; i < held; i += 64) {
+        const u64 key = l.gathered[wave][i];
+        if (f(key)) l.list[at++] = key;
+      }
     __syncthreads();
-    before = l.found[1];
-    return (int)l.found[0];
+    return n;
   };
-  // the distance to the largest in 1 / per
-  auto bin_of = [&](float x, float per) __attribute__((always_inline)) {
-    return (int)__builtin_fminf((top - x) * per, (float)(SAMPLE_BINS - 1));
-  };
-  // Numbers that rise along the order, of the tokens that f says, into the list; how many there are,
-  // which may be more than fit.
+  auto any_of = [](u64) { return true; };
   auto gather = [&](auto f) __attribute__((always_inline)) {
+    held = 0;
     over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
       bool any = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) any |= f(x[j], i + j);
-      if (any) {
+      if (__any(any)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (f(x[j], i + j) && i + j < size) {
-            const int at = atomicAdd(&l.count, 1);
-            if (at < SAMPLE_LIST) l.list[at] = (u64)~order_of(x[j]) << 32 | (uint32_t)(i + j);
-          }
+        for (int j = 0; j < 8; ++j) put(f(x[j], i + j) && i + j < size, x[j], i + j);
       }
     });
-    __syncthreads();
-    const int n = l.count;
-    __syncthreads();
-    if (tid == 0) l.count = 0;
-    return n;
+    held = __builtin_amdgcn_readfirstlane(held);  // the first lane has seen every pack of the wave's
+    return collect(any_of);
+  };
+  // what of ``all`` lies in front of the token that is drawn
+  auto target_of = [](double part, u64 all) {
+    const u64 target = (u64)(part * (double)all);
+    return target < all ? target : all - 1;
   };
 
   bool gathers = size <= SAMPLE_LIST;
-  float from = -__builtin_inff();
+  float from = NONE;
   if (!gathers && top_k && top_k <= SAMPLE_FEW) {
-    // as many threads as top_k have a token at or above the bin's end
+    // as many threads as top_k have a token at or above the end of the bin, a 64th, of their top_k-th
     clear_bins();
-    atomicAdd(&l.bins[bin_of(own_top, 64.0f)], (u64)1);
+    atomicAdd(&l.bins[(int)__builtin_fminf((top - own_top) * 64.0f, (float)(SAMPLE_BINS - 1))], (u64)1);
     __syncthreads();
-    u64 before;
-    const int bin = find_bin(top_k, before);
+    const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+    u64 below;
+    sum_over_threads(first + second, l, below);
+    if (below < (u64)top_k && below + first + second >= (u64)top_k) l.digits[0] = 2 * tid + 1;
+    __syncthreads();
+    const int bin = l.digits[0];
     gathers = bin < SAMPLE_BINS - 1;
     from = top - (float)(bin + 2) * 0x1p-6f;  // one more for roundings
   }
@@ -295,129 +326,305 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
     const int n = gather([&](float x, int) __attribute__((always_inline)) { return x >= from; });
     if (n <= SAMPLE_LIST) {
       const u64 key = sort_list(n, l);
-      const float x = of_order(~(uint32_t)(key >> 32));
       const bool in = tid < n && (top_k == 0 || tid < top_k);
-      u64 w = in ? units(weigh(x)) : 0, below, all = sum_over_threads(w, l, below);
-      const bool kept = in && x >= least && (tid == 0 || top_p >= 1.0f || (double)below < (double)top_p * (double)all);
-      // and once more by their indexes
-      u64 rank;
-      const int m = (int)sum_over_threads(kept, l, rank);  // the first m
+      const float own = in ? weigh(x_of(key)) : 0.0f;
+      u64 w = units(own), below, all = sum_over_threads(w, l, below);
+      const bool kept = in && (tid == 0 || (own >= min_p && (top_p >= 1.0f || (double)below < (double)top_p * (double)all)));
+      // and by their indexes: the first m
+      u64 unused;
+      const int m = (int)sum_over_threads(kept, l, unused);
+      w = tid < m ? w : 0;
+      if (m <= 256) {  // the weight of the kept ones in front, 8 at a time
+        if (tid < m + 7) {
+          l.list[tid] = tid < m ? (uint32_t)key : ~(u64)0;
+          l.bins[tid] = w;
+        }
+        const u64 target = target_of(uniform, sum_over_threads(w, l, unused));
+        below = 0;
+        if (tid < m)
+          for (int i = 0; i < m; i += 8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) below += l.list[i + j] < (uint32_t)key ? l.bins[i + j] : 0;
+          }
+        if (below <= target && target < below + w) a.out[b] = (uint32_t)key;
+        return;
+      }
       if (tid < m) {
         l.bins[tid] = w;
         l.list[tid] = key << 32 | tid;
       }
       const u64 again = sort_list(m, l);
       w = tid < m ? l.bins[(int)(again & (SAMPLE_LIST - 1))] : 0;
-      all = sum_over_threads(w, l, below);
-      const double wanted = (double)uniform * (double)all;  // below all: uniform is below 1
-      if (w && (double)below <= wanted && (double)(below + w) > wanted) a.out[b] = (int64_t)(again >> 32);
+      const u64 target = target_of(uniform, sum_over_threads(w, l, below));
+      if (below <= target && target < below + w) a.out[b] = (int64_t)(again >> 32);
       return;
     }
   }
 
   // Border of the first tokens, among those in front of ``before``, whose ``mass`` reaches ``want``, a number
-  // or, where that is 0, ``share`` of all. By the distance's bin, and by the list, or
-  // where that is too short by 11, 11 and 10 bits of the logit, 11 and 11 of the index.
-  auto find = [&](const Border& before, u64 want, double share, float per, auto mass) __attribute__((always_inline)) {
+  // or, where that is 0, ``share`` of all: by 11, 11 and 10 bits of the logit, 11 and 11 of the index.
+  auto find = [&](const Border& before, u64 want, double share, auto mass) __attribute__((always_inline)) {
     auto digit = [&](int level, float x, int i) __attribute__((always_inline)) -> int {
-      if (level == 0) return bin_of(x, per);
       const uint32_t k = ~order_of(x);
-      return level == 1 ? (int)(k >> 21) : level == 2 ? (int)(k >> 10 & 2047) : level == 3 ? (int)(k & 1023)
-             : level == 4 ? i >> 11 : i & 2047;
+      return level == 0 ? (int)(k >> 21) : level == 1 ? (int)(k >> 10 & 2047) : level == 2 ? (int)(k & 1023)
+             : level == 3 ? i >> 11 : i & 2047;
     };
 #pragma unroll 1
-    for (int level = 0; level < 6; ++level) {
+    for (int level = 0; level < 5; ++level) {
       clear_bins();
       over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           bool in = before.keeps(x[j], i + j) && i + j < size;
-          if (level > 0)
-            for (int n = 0; n < level; ++n) in = in && digit(n, x[j], i + j) == l.digits[n];
+          for (int n = 0; n < level; ++n) in = in && digit(n, x[j], i + j) == l.digits[n];
           if (in) atomicAdd(&l.bins[digit(level, x[j], i + j)], mass(x[j]));
         }
       });
       __syncthreads();
+      const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+      u64 below;
+      const u64 all = sum_over_threads(first + second, l, below);
       if (want == 0) {
-        u64 below;
-        const double part = share * (double)sum_over_threads(l.bins[2 * tid] + l.bins[2 * tid + 1], l, below);
-        want = (u64)__builtin_ceil(part);
+        want = (u64)__builtin_ceil(share * (double)all);
         want = want ? want : 1;
       }
-      u64 front;
-      const int bin = find_bin(want, front);
-      if (tid == 0) l.digits[level] = bin;
-      want -= front;
-      if (level == 0) {
-        const int n = gather([&](float x, int i) __attribute__((always_inline)) { return bin_of(x, per) == bin && before.keeps(x, i); });
-        if (n <= SAMPLE_LIST) {
-          const u64 key = sort_list(n, l);
-          const u64 w = tid < n ? mass(of_order(~(uint32_t)(key >> 32))) : 0;
-          u64 below;
-          sum_over_threads(w, l, below);
-          if (below < want && below + w >= want) l.found[0] = key;
-          __syncthreads();
-          const u64 last = l.found[0];
-          return Border{of_order(~(uint32_t)(last >> 32)), (int)(uint32_t)last};
-        }
+      if (below < want && below + first + second >= want) {
+        l.digits[level] = 2 * tid + (below + first < want);
+        l.found[1] = below + first < want ? below + first : below;
       }
+      __syncthreads();
+      want -= l.found[1];
+      __syncthreads();
     }
-    __syncthreads();
-    return Border{of_order(~((uint32_t)l.digits[1] << 21 | (uint32_t)l.digits[2] << 10 | (uint32_t)l.digits[3])),
-                  l.digits[4] << 11 | l.digits[5]};
+    return Border{of_order(~((uint32_t)l.digits[0] << 21 | (uint32_t)l.digits[1] << 10 | (uint32_t)l.digits[2])),
+                  l.digits[3] << 11 | l.digits[4]};
   };
 
-  Border kept = {-__builtin_inff(), 0x7fffffff};
-  if (top_k) kept = find(kept, top_k, 0.0, 64.0f, [](float) { return (u64)1; });
-  if (top_p < 1.0f)
-    kept = find(kept, 0, (double)top_p, 64.0f * weigh.hi, [&](float x) __attribute__((always_inline)) { return units(weigh(x)); });
-  if (least > kept.x) kept = Border{least, 0x7fffffff};
+  // Segments of the row: a sixteenth each for the 16 waves, and of the one that the token is in again,
+  // until a wave sees all of it at once. ``part``: of a segment's kept weight what lies in front of the token.
+  auto segment = [](int length) { return ((length + SAMPLE_WAVES - 1) / SAMPLE_WAVES + 511) / 512 * 512; };
+  int lo = 0, hi = size, each = segment(size);
+  double part = uniform;
+  auto enter = [&](u64 own) __attribute__((always_inline)) {  // each lane's kept weight of its wave's segment
+#pragma unroll
+    for (int by = 1; by < 64; by *= 2) own += __shfl_xor(own, by);
+    __syncthreads();
+    if ((tid & 63) == 0) l.sums[wave] = own;
+    __syncthreads();
+    u64 before = 0, all = 0;
+    for (int w = 0; w < SAMPLE_WAVES; ++w) {
+      const u64 x = l.sums[w];
+      before += w < wave ? x : 0;
+      all += x;
+    }
+    const u64 target = target_of(part, all);
+    if ((tid & 63) == 0 && before <= target && target < before + own) {
+      l.digits[0] = wave;
+      const double rest = (part * (double)all - (double)before) / (double)own;
+      l.found[0] = __builtin_bit_cast(u64, __builtin_fmin(__builtin_fmax(rest, 0.0), 0x1.fffffffffffffp-1));
+    }
+    __syncthreads();
+    lo += l.digits[0] * each;
+    hi = lo + each < hi ? lo + each : hi;
+    part = __builtin_bit_cast(double, l.found[0]);
+    each = segment(hi - lo);
+    __syncthreads();
+  };
 
-  // Segments of the row: a sixteenth each for the 16 waves, and of the one that the token is in
-  // again, until a wave sees all of it at once. The kept weight of a pack is its weights' sum in fp32.
-  int lo = 0, hi = size;
-  u64 target = 0;
-  double wanted = -1.0;
+  Border kept = {NONE, 0x7fffffff};
+  if (top_k || top_p < 1.0f) {
+    // tokens in each 128th of a power of two of the weight
+    const float per = 128.0f * weigh.hi;
+    constexpr int COUNTS = 2 * SAMPLE_BINS, EACH = COUNTS / SAMPLE_THREADS;
+    auto count_of = [&](float x) __attribute__((always_inline)) { return (int)__builtin_fminf((top - x) * per, (float)(COUNTS - 1)); };
+    clear_bins();
+    over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) atomicAdd(&l.counts[count_of(x[j])], 1u);  // past the row's end in the last bin
+    });
+    __syncthreads();
+    if (top_k) {
+      u64 own = 0, below;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) own += l.counts[tid * EACH + j];
+      sum_over_threads(own, l, below);
+      if (below < (u64)top_k && below + own >= (u64)top_k) {
+        int bin = tid * EACH;
+        while (below + l.counts[bin] < (u64)top_k) below += l.counts[bin++];
+        l.digits[0] = bin;
+        l.found[1] = below;
+      }
+      __syncthreads();
+      const int bin = l.digits[0];
+      const u64 more = top_k - l.found[1];  // of the bin
+      const int n = gather([&](float x, int) __attribute__((always_inline)) { return count_of(x) == bin; });
+      if (n <= SAMPLE_LIST) {
+        const u64 key = sort_list(n, l);
+        if ((u64)tid + 1 == more) l.found[0] = key;
+        __syncthreads();
+        kept = Border{x_of(l.found[0]), (int)(uint32_t)l.found[0]};
+        // and are the only ones that count for top_p
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+          if (tid * EACH + j >= bin) l.counts[tid * EACH + j] = tid * EACH + j == bin ? (uint32_t)more : 0;
+      } else {
+        kept = find(kept, top_k, 0.0, [](float) { return (u64)1; });
+        if (top_p < 1.0f) {
+          clear_bins();
+          over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (kept.keeps(x[j], i + j)) atomicAdd(&l.counts[count_of(x[j])], 1u);
+          });
+        }
+      }
+      __syncthreads();
+    }
+    if (top_p < 1.0f) {
+      // If all bins' tokens had the most weight that their bin allows, up to where would the border be, and if
+      // they had the least, RATIO of it (nothing in the last bin)? It lies where the one is large
+      // enough for the other's share, or before. A little apart, for roundings.
+      constexpr double RATIO = 0x1.fcp-1;  // below 2^(-1/128 - 1/512)
+      const Border before = kept;
+      u64 most[EACH], own = 0, below;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int bin = tid * EACH + j;
+        most[j] = l.counts[bin] * units(__builtin_amdgcn_exp2f((float)bin * -0x1p-7f + 0x1p-10f));
+        own += most[j];
+      }
+      if (tid == 0) l.digits[0] = l.digits[1] = COUNTS - 1;
+      if (tid == SAMPLE_THREADS - 1) l.found[0] = most[EACH - 1];
+      const u64 all_most = sum_over_threads(own, l, below);
+      const double early = (double)top_p * RATIO * (double)(all_most - l.found[0]), late = (double)top_p * (double)all_most;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const u64 up_to = below + most[j];
+        if (most[j] && (double)up_to >= early && (double)below <= early) atomicMin(&l.digits[0], tid * EACH + j);
+        if (most[j] && RATIO * (double)up_to > late && RATIO * (double)below <= late) atomicMin(&l.digits[1], tid * EACH + j);
+        below = up_to;
+      }
+      __syncthreads();
+      // logits above ``high`` are in front of the first of those bins, below ``low`` behind the last
+      const int first_bin = l.digits[0], last_bin = l.digits[1];
+      const float high = first_bin == 0 ? __builtin_inff() : top - ((float)first_bin - 0.25f) / per;
+      const float low = last_bin == COUNTS - 1 ? NONE : top - ((float)last_bin + 1.25f) / per;
+      const bool some = top_k != 0;
+      double all_own = 0.0, front_own = 0.0;
+      held = 0;
+      const int start = wave * each, end = start + each < size ? start + each : size;
+      over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
+        float sum = 0.0f, front = 0.0f;
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float w = weigh(x[j]);
+          if (some) w = before.keeps(x[j], i + j) ? w : 0.0f;
+          sum += w;
+          front += x[j] > high ? w : 0.0f;
+          any |= x[j] <= high && x[j] >= low;
+        }
+        all_own += whole(sum);
+        front_own += whole(front);
+        if (__any(any)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            put(x[j] <= high && x[j] >= low && i + j < size && before.keeps(x[j], i + j), x[j], i + j);
+        }
+      });
+      held = __builtin_amdgcn_readfirstlane(held);
+      u64 unused;
+      const u64 all = sum_over_threads((u64)all_own, l, unused), in_front = sum_over_threads((u64)front_own, l, unused);
+      const double share = __builtin_ceil((double)top_p * (double)all);
+      u64 want = share < 1.0 ? 1 : (u64)share;
+      bool done = false;
+      if (want > in_front && !__syncthreads_or(held > SAMPLE_EACH)) {
+        want -= in_front;
+        // into fine bins of the window, of which one is then sorted
+        const float wide = (float)SAMPLE_BINS / (float)(last_bin - first_bin + 2);
+        auto fine_bin = [&](u64 key) {
+          return (int)__builtin_fminf(__builtin_fmaxf(((top - x_of(key)) * per - ((float)first_bin - 0.5f)) * wide, 0.0f), (float)(SAMPLE_BINS - 1));
+        };
+        clear_bins();
+#pragma unroll 1
+        for (int i = tid & 63; i < held; i += 64) {
+          const u64 key = l.gathered[wave][i];
+          atomicAdd(&l.bins[fine_bin(key)], units(weigh(x_of(key))));
+        }
+        if (tid == 0) l.found[0] = ~(u64)0;
+        __syncthreads();
+        const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+        u64 below;
+        sum_over_threads(first + second, l, below);
+        if (below < want && below + first + second >= want) {
+          l.digits[0] = 2 * tid + (below + first < want);
+          l.found[0] = below + first < want ? below + first : below;
+        }
+        __syncthreads();
+        if (l.found[0] != ~(u64)0) {
+          const int bin = l.digits[0];
+          want -= l.found[0];
+          const int m = collect([&](u64 key) { return fine_bin(key) == bin; });
+          if (m <= SAMPLE_LIST) {
+            const u64 key = sort_list(m, l);
+            const u64 w = tid < m ? units(weigh(x_of(key))) : 0;
+            sum_over_threads(w, l, below);
+            if (below < want && below + w >= want) l.found[0] = key;
+            __syncthreads();
+            const u64 last = l.found[0];
+            kept = Border{x_of(last), (int)(uint32_t)last};
+            done = true;
+            if (weigh(kept.x) >= min_p) {
+              // each wave's segment: what lies in front of the window, and what is kept of it
+#pragma unroll 1
+              for (int i = tid & 63; i < held; i += 64) {
+                const u64 key = l.gathered[wave][i];
+                if (key <= last) front_own += whole(weigh(x_of(key)));
+              }
+              enter((u64)front_own);
+            }
+          }
+        }
+      }
+      if (!done) kept = find(before, 0, (double)top_p, [&](float x) __attribute__((always_inline)) { return units(weigh(x)); });
+    }
+  }
+
+  // The kept weight of a pack is its weights' sum in fp32.
+  const float least_weight = min_p;
+  const float above = kept.x == NONE ? NONE : of_order(order_of(kept.x) + 1);  // the next logit
   for (;;) {
-    const int each = ((hi - lo + SAMPLE_WAVES - 1) / SAMPLE_WAVES + 511) / 512 * 512;
-    const int wave = tid >> 6, start = lo + wave * each, end = start + each < hi ? start + each : hi;
-    u64 own = 0;
+    const int start = lo + wave * each, end = start + each < hi ? start + each : hi;
+    auto weight_of = [&](float x, int i) __attribute__((always_inline)) {
+      const float w = weigh(x);
+      return x >= (i <= kept.last ? kept.x : above) && w >= least_weight ? w : 0.0f;
+    };
+    double own = 0.0;
     over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += kept.keeps(x[j], i + j) ? weigh(x[j]) : 0.0f;
-      own += units(sum);
+      for (int j = 0; j < 8; ++j) sum += weight_of(x[j], i + j);
+      own += whole(sum);
     });
+    if (each > 512) {
+      enter((u64)own);
+      continue;
+    }
+    // a lane has one pack
     u64 below;
-    const u64 all = sum_over_threads(own, l, below);
-    if (wanted < 0.0) wanted = (double)uniform * (double)all;
-    if (each <= 512) {  // a lane has one pack
-      const u64 first = target + below;
-      if (own && (double)first <= wanted && (double)(first + own) > wanted) {
+    const u64 all = sum_over_threads((u64)own, l, below), target = target_of(part, all);
+    if (below <= target && target < below + (u64)own)
+      over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
         float sum = 0.0f;
         int token = -1;
-        over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sum += kept.keeps(x[j], i + j) ? weigh(x[j]) : 0.0f;
-            if (token < 0 && (double)(first + units(sum)) > wanted) token = i + j;
-          }
-        });
+        for (int j = 0; j < 8; ++j) {
+          sum += weight_of(x[j], i + j);
+          if (token < 0 && below + units(sum) > target) token = i + j;
+        }
         a.out[b] = token;
-      }
-      return;
-    }
-    u64 front = target;
-    for (int w = 0; w < wave; ++w) front += l.sums[w];
-    if ((tid & 63) == 0 && (double)front <= wanted && (double)(front + l.sums[wave]) > wanted) {
-      l.found[0] = wave;
-      l.found[1] = front;
-    }
-    __syncthreads();
-    lo += (int)l.found[0] * each;
-    hi = lo + each < hi ? lo + each : hi;
-    target = l.found[1];
-    __syncthreads();
+      });
+    return;
   }
 }
 
