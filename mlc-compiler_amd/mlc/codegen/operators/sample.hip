@@ -40,7 +40,7 @@ struct SampleArgs {
 };
 
 typedef unsigned long long u64;
-constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / 64, SAMPLE_BINS = 2048;
+constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / 64, SAMPLE_BINS = 2048, SAMPLE_COUNTS = 16384;
 constexpr int SAMPLE_LIST = 1024, SAMPLE_EACH = 512;  // tokens that are sorted, a thread for each, and gathered by a wave
 constexpr int SAMPLE_FEW = 512;                          // top_k whose tokens are gathered
 constexpr float LEAST_TEMPERATURE = 0x1p-100f, MOST_TEMPERATURE = 0x1p100f;  // below the least the likeliest token
@@ -58,7 +58,7 @@ struct SampleLds {
   alignas(16) char tail[32];  // the row's last pack
   union {
     u64 bins[SAMPLE_BINS];  // and a list's weights
-    uint32_t counts[2 * SAMPLE_BINS];
+    uint32_t counts[SAMPLE_COUNTS];
   };
   u64 gathered[SAMPLE_WAVES][SAMPLE_EACH], list[SAMPLE_LIST], sorted[SAMPLE_LIST];
   u64 sums[SAMPLE_WAVES];
@@ -68,14 +68,22 @@ struct SampleLds {
   int counts_of[SAMPLE_WAVES], digits[6];
 };
 
+// x of a lane below this one by DPP, 0 where there is none.
+template <int CONTROL, int ROWS> __device__ __forceinline__ u64 moved(u64 x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CONTROL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CONTROL, ROWS, 0xf, false);
+  return (u64)hi << 32 | lo;
+}
+
 // The sum of x over the workgroup; ``below``: of the threads before this one.
 __device__ __forceinline__ u64 sum_over_threads(u64 x, SampleLds& l, u64& below) {
   u64 run = x;
-#pragma unroll
-  for (int by = 1; by < 64; by *= 2) {
-    const u64 y = __shfl_up(run, by);
-    if ((threadIdx.x & 63) >= by) run += y;
-  }
+  run += moved<0x111, 0xf>(run);  // by 1, 2, 4 and 8 lanes of 16, then the last of 16 and of 32
+  run += moved<0x112, 0xf>(run);
+  run += moved<0x114, 0xf>(run);
+  run += moved<0x118, 0xf>(run);
+  run += moved<0x142, 0xa>(run);
+  run += moved<0x143, 0xc>(run);
   __syncthreads();  // sums of the time before have been read
   if ((threadIdx.x & 63) == 63) l.sums[threadIdx.x >> 6] = run;
   __syncthreads();
@@ -205,14 +213,10 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) own_top = __builtin_elementwise_maximum(own_top, element<T>::widen(x[u][j]));
   }
-  float top = own_top;
-#pragma unroll
-  for (int by = 1; by < 64; by *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, by));
+  float top = group_reduce<64, OpMax>(own_top);  // NaN where there is one
   if ((tid & 63) == 0) l.tops[tid >> 6] = top;
   __syncthreads();
-  top = l.tops[tid & (SAMPLE_WAVES - 1)];
-#pragma unroll
-  for (int by = 1; by < SAMPLE_WAVES; by *= 2) top = __builtin_elementwise_maximum(top, __shfl_xor(top, by));
+  top = group_reduce<SAMPLE_WAVES, OpMax>(l.tops[tid & (SAMPLE_WAVES - 1)]);
   const bool fine = uniform >= 0.0f && uniform < 1.0f && temperature >= 0.0f && temperature <= MOST_TEMPERATURE &&
                     top_p >= 0.0f && top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f && top < __builtin_inff();
   if (!fine || top == NONE) {
@@ -323,7 +327,24 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
     from = least > from ? least : from;
   }
   if (gathers) {
-    const int n = gather([&](float x, int) __attribute__((always_inline)) { return x >= from; });
+    int n;
+    if (__syncthreads_count(own_top >= from) <= 256) {
+      // few threads have one: their waves look through their packs, a token a lane
+      held = 0;
+      for (u64 some = __ballot(own_top >= from); some; some &= some - 1) {
+        const int first = (tid - (tid & 63) + __builtin_ctzll(some)) * 8;
+#pragma unroll 1
+        for (int e = tid & 63; e < (size - first + SAMPLE_THREADS * 8 - 1) / (SAMPLE_THREADS * 8) * 8; e += 64) {
+          const int i = first + e / 8 * (SAMPLE_THREADS * 8) + e % 8;
+          const float x = i < size ? element<T>::widen(row[i]) : NONE;
+          put(i < size && x >= from, x, i);
+        }
+        held = __builtin_amdgcn_readfirstlane(held);
+      }
+      n = collect(any_of);
+    } else {
+      n = gather([&](float x, int) __attribute__((always_inline)) { return x >= from; });
+    }
     if (n <= SAMPLE_LIST) {
       const u64 key = sort_list(n, l);
       const bool in = tid < n && (top_k == 0 || tid < top_k);
@@ -332,7 +353,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
       const bool kept = in && (tid == 0 || (own >= min_p && (top_p >= 1.0f || (double)below < (double)top_p * (double)all)));
       // and by their indexes: the first m
       u64 unused;
-      const int m = (int)sum_over_threads(kept, l, unused);
+      const int m = __syncthreads_count(kept);
       w = tid < m ? w : 0;
       if (m <= 256) {  // the weight of the kept ones in front, 8 at a time
         if (tid < m + 7) {
@@ -433,11 +454,17 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
 
   Border kept = {NONE, 0x7fffffff};
   if (top_k || top_p < 1.0f) {
-    // tokens in each 128th of a power of two of the weight
-    const float per = 128.0f * weigh.hi;
-    constexpr int COUNTS = 2 * SAMPLE_BINS, EACH = COUNTS / SAMPLE_THREADS;
+    // tokens in each 512th of a power of two of the weight
+    const float per = 512.0f * weigh.hi;
+    constexpr int COUNTS = SAMPLE_COUNTS, EACH = COUNTS / SAMPLE_THREADS;
     auto count_of = [&](float x) __attribute__((always_inline)) { return (int)__builtin_fminf((top - x) * per, (float)(COUNTS - 1)); };
-    clear_bins();
+    auto clear_counts = [&] {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < EACH; j += 4) *reinterpret_cast<uint4v*>(&l.counts[j * SAMPLE_THREADS + tid * 4]) = uint4v{0, 0, 0, 0};
+      __syncthreads();
+    };
+    clear_counts();
     over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) atomicAdd(&l.counts[count_of(x[j])], 1u);  // past the row's end in the last bin
@@ -445,7 +472,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
     __syncthreads();
     if (top_k) {
       u64 own = 0, below;
-#pragma unroll
+#pragma unroll 4
       for (int j = 0; j < EACH; ++j) own += l.counts[tid * EACH + j];
       sum_over_threads(own, l, below);
       if (below < (u64)top_k && below + own >= (u64)top_k) {
@@ -464,13 +491,13 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
         __syncthreads();
         kept = Border{x_of(l.found[0]), (int)(uint32_t)l.found[0]};
         // and are the only ones that count for top_p
-#pragma unroll
+#pragma unroll 4
         for (int j = 0; j < EACH; ++j)
           if (tid * EACH + j >= bin) l.counts[tid * EACH + j] = tid * EACH + j == bin ? (uint32_t)more : 0;
       } else {
         kept = find(kept, top_k, 0.0, [](float) { return (u64)1; });
         if (top_p < 1.0f) {
-          clear_bins();
+          clear_counts();
           over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -484,26 +511,26 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
       // If all bins' tokens had the most weight that their bin allows, up to where would the border be, and if
       // they had the least, RATIO of it (nothing in the last bin)? It lies where the one is large
       // enough for the other's share, or before. A little apart, for roundings.
-      constexpr double RATIO = 0x1.fcp-1;  // below 2^(-1/128 - 1/512)
+      constexpr double RATIO = 0x1.ffp-1;  // below 2^(-1/512 - 1/2048)
       const Border before = kept;
-      u64 most[EACH], own = 0, below;
-#pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        const int bin = tid * EACH + j;
-        most[j] = l.counts[bin] * units(__builtin_amdgcn_exp2f((float)bin * -0x1p-7f + 0x1p-10f));
-        own += most[j];
-      }
+      auto most_of = [&](int bin) __attribute__((always_inline)) {
+        return l.counts[bin] * units(__builtin_amdgcn_exp2f((float)bin * -0x1p-9f + 0x1p-12f));
+      };
+      u64 own = 0, below;
+#pragma unroll 4
+      for (int j = 0; j < EACH; ++j) own += most_of(tid * EACH + j);
       if (tid == 0) l.digits[0] = l.digits[1] = COUNTS - 1;
-      if (tid == SAMPLE_THREADS - 1) l.found[0] = most[EACH - 1];
+      if (tid == SAMPLE_THREADS - 1) l.found[0] = most_of(COUNTS - 1);
       const u64 all_most = sum_over_threads(own, l, below);
       const double early = (double)top_p * RATIO * (double)(all_most - l.found[0]), late = (double)top_p * (double)all_most;
-#pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        const u64 up_to = below + most[j];
-        if (most[j] && (double)up_to >= early && (double)below <= early) atomicMin(&l.digits[0], tid * EACH + j);
-        if (most[j] && RATIO * (double)up_to > late && RATIO * (double)below <= late) atomicMin(&l.digits[1], tid * EACH + j);
-        below = up_to;
-      }
+      if (own && ((double)(below + own) >= early && (double)below <= early) | (RATIO * (double)(below + own) > late && RATIO * (double)below <= late))
+#pragma unroll 1
+        for (int bin = tid * EACH; bin < (tid + 1) * EACH; ++bin) {
+          const u64 most = most_of(bin), up_to = below + most;
+          if (most && (double)up_to >= early && (double)below <= early) atomicMin(&l.digits[0], bin);
+          if (most && RATIO * (double)up_to > late && RATIO * (double)below <= late) atomicMin(&l.digits[1], bin);
+          below = up_to;
+        }
       __syncthreads();
       // logits above ``high`` are in front of the first of those bins, below ``low`` behind the last
       const int first_bin = l.digits[0], last_bin = l.digits[1];
@@ -592,6 +619,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
 
   // The kept weight of a pack is its weights' sum in fp32.
   const float least_weight = min_p;
+  const bool plain = kept.x == NONE && min_p == 0.0f;
   const float above = kept.x == NONE ? NONE : of_order(order_of(kept.x) + 1);  // the next logit
   for (;;) {
     const int start = lo + wave * each, end = start + each < hi ? start + each : hi;
@@ -600,12 +628,20 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
       return x >= (i <= kept.last ? kept.x : above) && w >= least_weight ? w : 0.0f;
     };
     double own = 0.0;
-    over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
-      float sum = 0.0f;
+    if (plain)
+      over(start, end, tid & 63, 64, [&](const float (&x)[8], int) __attribute__((always_inline)) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += weight_of(x[j], i + j);
-      own += whole(sum);
-    });
+        for (int j = 0; j < 8; ++j) sum += weigh(x[j]);
+        own += whole(sum);
+      });
+    else
+      over(start, end, tid & 63, 64, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += weight_of(x[j], i + j);
+        own += whole(sum);
+      });
     if (each > 512) {
       enter((u64)own);
       continue;
