@@ -31,10 +31,9 @@ def _rows(x: Operand | None) -> tuple[int, int, tuple]:
     the strides of both. What a dimension of one says of its stride means nothing."""
     if x is None:
         return 0, 1, (0, 0)
-    strides = tuple(s if n > 1 else 0 for s, n in zip(x.strides[:-1], x.shape[:-1]))
-    if len(x.shape) == 3:
-        return x.shape[0] * x.shape[1], max(1, x.shape[1]), strides
-    return x.shape[0], max(1, x.shape[0]), (0, *strides)
+    if len(x.shape) == 3 and x.shape[1] != 1:
+        return x.shape[0] * x.shape[1], max(1, x.shape[1]), (x.strides[0] if x.shape[0] > 1 else 0, x.strides[1])
+    return x.shape[0], max(1, x.shape[0]), (0, x.strides[0] if x.shape[0] > 1 else 0)
 
 
 def _in_packs(x: Operand | None, n: int) -> bool:
@@ -75,9 +74,9 @@ def norm_results(x, residual, quantized: bool) -> tuple:
 
 def _row_args(x: Operand, other: Operand | None, weight: Operand | None, eps: float) -> bytes:
     rows, seq, strides = _rows(x)
-    return struct.pack("<3q4q4id", x.offset, _offset(other), _offset(weight), *strides,
+    return struct.pack("<3q4q4i2d", x.offset, _offset(other), _offset(weight), *strides,
                        *_rows(other)[2], rows, seq, x.shape[-1], weight is not None
-                       and weight.dtype == torch.float32, eps)
+                       and weight.dtype == torch.float32, eps, 1.0 / x.shape[-1])
 
 
 def plan_norm(x: Operand, weight: Operand, residual: Operand | None, eps: float, quantized: bool) -> Plan:

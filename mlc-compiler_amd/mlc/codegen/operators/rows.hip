@@ -5,9 +5,12 @@
 //   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight
 //   scale = max(amax / 448, 2^-126) of a block's finite values;  code = e4m3(y / scale)
 //
-// Sums, the root and y are taken in 64 bits, whose additions and products cost what fp32's do
-// here: squares of any fp32 value fit, and y is rounded to fp32 once. Infinities and NaN become
-// codes of NaN and do not count for a scale.
+// Memory bounds both: a row is read once into registers, so that nothing is read again, and all of
+// its loads, the weight's too, are on their way before the first is used. What else is to be watched are the
+// instructions for each value: a wave's double takes one and its conversions take more.
+// fp32's sums, root, y and quotients are taken in 64 bits, and y is rounded once; 16-bit values'
+// in fp32, but for the sums of eight squares, whose range is any value's.
+// Infinities and NaN become codes of NaN and do not count for a scale.
 
 namespace mlc {
 
@@ -21,13 +24,26 @@ struct RowsArgs {
   int64_t x_off, o_off, w_off;  // bytes
   int64_t xb, xt, ob, ot;       // elements
   int32_t rows, seq, dim, wide_weight;
-  double eps;
+  double eps, part;  // part: 1 / dim
 };
 
+// x of a lane below this one by DPP, 0 where there is none.
+template <int CONTROL, int ROWS> __device__ __forceinline__ double lower(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CONTROL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CONTROL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double add_over_wave(double x) {
-#pragma unroll
-  for (int by = 1; by < 64; by *= 2) x += __shfl_xor(x, by);
-  return x;
+  x += lower<0x111, 0xf>(x);  // by 1, 2, 4 and 8 lanes of 16, then the last of 16 and of 32
+  x += lower<0x112, 0xf>(x);
+  x += lower<0x114, 0xf>(x);
+  x += lower<0x118, 0xf>(x);
+  x += lower<0x142, 0xa>(x);
+  x += lower<0x143, 0xc>(x);
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, 63), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 // Four values to e4m3, to nearest even; NaN becomes its NaN.
@@ -36,28 +52,54 @@ __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// What y is: of T's digits, or rounded to fp32 from more, or that of fp32 values.
+enum { GIVEN, ROUNDED, FULL };
+
 // The codes of a block of 128 values, 8 in each of 16 neighbouring lanes, of which the first
 // writes the scale. Lanes past the row's end have zeros and ``in`` false.
+//
+// Values that are given have quotients in the middle of two codes, which go to the even one, so these have to
+// be exact. y * 448 and the middle times the largest are whole numbers of 14 and 16 bits where y has 11: the
+// quotient is in the middle or at least 2^-16 beside it. So one in fp32, off by 2^-22, is rounded to 18
+// digits, which puts it there or leaves it on its side. Of fp32 values it is taken in 64 bits.
+template <int KIND>
 __device__ __forceinline__ void store_block(const float (&y)[8], bool in, uint8_t* codes, float* scale_at,
                                             bool first) {
   float top = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float m = __builtin_fabsf(y[j]);
-    top = m < __builtin_inff() ? __builtin_fmaxf(top, m) : top;
-  }
+  for (int j = 0; j < 8; ++j) top = __builtin_elementwise_maximum(top, __builtin_fabsf(y[j]));
   top = group_reduce<16, OpMax>(top);
-  const float scale = __builtin_fmaxf(top / 448.0f, 0x1p-126f);
-  // In 64 bits a quotient in the middle of two codes is there exactly, and goes to the even one:
-  // among 16-bit values, whose largest has few digits too, many are.
-  const double by = __builtin_fmin(448.0 / (double)top, 0x1p126);
-  float q[8];
+  const bool finite = top < __builtin_inff();
+  if (!finite) {
+    top = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)  // infinity is a NaN
-    q[j] = __builtin_fabsf(y[j]) < __builtin_inff() ? (float)((double)y[j] * by) : __builtin_nanf("");
+    for (int j = 0; j < 8; ++j) {
+      const float m = __builtin_fabsf(y[j]);
+      top = m < __builtin_inff() ? __builtin_fmaxf(top, m) : top;
+    }
+    top = group_reduce<16, OpMax>(top);
+  }
+  float q[8];
+  if constexpr (KIND == FULL) {
+    const double by = __builtin_fmin(448.0 / (double)top, 0x1p126);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = (float)((double)y[j] * by);
+  } else {
+    // 448 / top, whose reciprocal is a normal number: two roundings and the reciprocal's unit of a quotient
+    const float by = __builtin_fminf(1.75f * __builtin_amdgcn_rcpf(top * 0x1p-8f), 0x1p126f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      q[j] = y[j] * by;
+      if constexpr (KIND == GIVEN) q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
+    }
+  }
+  if (!finite) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __builtin_fabsf(y[j]) < __builtin_inff() ? q[j] : __builtin_nanf("");
+  }
   if (in) {
     *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
-    if (first) *scale_at = scale;
+    if (first) *scale_at = __builtin_fmaxf(top * (1.0f / 448.0f), 0x1p-126f);
   }
 }
 
@@ -94,7 +136,7 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   const int64_t b = row / a.seq, t = row % a.seq;
   const T* const x = at<T>(a.x, a.x_off) + b * a.xb + t * a.xt;
   const T* const r = at<T>(a.other, a.o_off) + b * a.ob + t * a.ot;
-  T v[N][8], u[N][8];
+  T v[N][8] = {}, u[N][8] = {};
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int d = (lane + n * LANES) * 8;
@@ -107,16 +149,18 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   double sum = 0.0;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const int d = (lane + n * LANES) * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f = 0.0f;
-      if (d + j < dim) {
-        f = element<T>::widen(v[n][j]);
-        if (a.other) f += element<T>::widen(u[n][j]);
-      }
-      h[n][j] = f;
-      sum = __builtin_fma((double)f, (double)f, sum);
+    for (int j = 0; j < 8; ++j) h[n][j] = element<T>::widen(v[n][j]) + element<T>::widen(u[n][j]);
+    float eight = 0.0f;
+    if constexpr (sizeof(T) < 4) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) eight = __builtin_fmaf(h[n][j], h[n][j], eight);
+    }
+    if (sizeof(T) < 4 && eight > 0x1p-80f && eight < 0x1p100f) {
+      sum += (double)eight;
+    } else {  // fp32, zeros, or squares that leave its range
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)h[n][j], (double)h[n][j], sum);
     }
   }
   if (a.sum) {
@@ -125,6 +169,20 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
       const int d = (lane + n * LANES) * 8;
       if (d < dim) store_pack_of<A>(reinterpret_cast<T*>(a.sum) + row * dim, h[n], d, dim);
     }
+  }
+  T z[N][8] = {};
+  float wide[N][8] = {};
+  auto load_weight = [&](int n) {
+    const int d = (lane + n * LANES) * 8;
+    if (d < dim) {
+      if (sizeof(T) < 4 && a.wide_weight) load_pack_of<4>(wide[n], at<float>(a.weight, a.w_off), d, dim);
+      else load_pack_of<(int)sizeof(T)>(z[n], at<T>(a.weight, a.w_off), d, dim);
+    }
+  };
+  constexpr bool EARLY = WAVES * N < 64;  // or there are no registers for it
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) load_weight(n);
   }
   sum = add_over_wave(sum);
   if constexpr (WAVES > 1) {
@@ -135,36 +193,42 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += parts[w];
   }
-  const double by = 1.0 / __builtin_sqrt(sum / (double)dim + a.eps);
+  const double mean = __builtin_fma(sum, a.part, a.eps);
+  auto weight = [&](int n, int j) { return sizeof(T) < 4 && a.wide_weight ? wide[n][j] : element<T>::widen(z[n][j]); };
+  if constexpr (sizeof(T) < 4) {
+    // a power of two near the root goes into h, so that the reciprocal is a normal number whatever the root
+    const int power = __builtin_amdgcn_frexp_exp(mean) >> 1;
+    const float by = __builtin_amdgcn_rsqf((float)__builtin_amdgcn_ldexp(mean, -2 * power));
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!EARLY) load_weight(n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[n][j] = __builtin_amdgcn_ldexpf(h[n][j], -power) * by * weight(n, j);
+    }
+  } else {
+    const double by = 1.0 / __builtin_sqrt(mean);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!EARLY) load_weight(n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[n][j] = (float)((double)h[n][j] * by * (double)weight(n, j));
+    }
+  }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int d = (lane + n * LANES) * 8;
-    const bool in = d < dim;
-    float w[8] = {}, y[8];
-    if (in) {
-      if (a.wide_weight) {
-        load_pack_of<4>(w, at<float>(a.weight, a.w_off), d, dim);
-      } else {
-        T z[8] = {};
-        load_pack_of<(int)sizeof(T)>(z, at<T>(a.weight, a.w_off), d, dim);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = element<T>::widen(z[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (float)((double)h[n][j] * by * (double)w[j]);
     if constexpr (EIGHT) {
-      store_block(y, in, reinterpret_cast<uint8_t*>(a.out) + row * dim + d,
-                  a.scales + row * ((dim + 127) / 128) + d / 128, lane % 16 == 0);
-    } else if (in) {
-      store_pack_of<A>(reinterpret_cast<T*>(a.out) + row * dim, y, d, dim);
+      store_block<sizeof(T) < 4 ? ROUNDED : FULL>(h[n], d < dim, reinterpret_cast<uint8_t*>(a.out) + row * dim + d,
+                                                  a.scales + row * ((dim + 127) / 128) + d / 128, lane % 16 == 0);
+    } else if (d < dim) {
+      store_pack_of<A>(reinterpret_cast<T*>(a.out) + row * dim, h[n], d, dim);
     }
   }
 }
 
 // g / (1 + e^-g). e^-g is 2^h with h the rounded product, corrected by what the rounding left
 // (as exp_nonpos does); where it is infinite the quotient is a zero, as in fp32's own formula.
-__device__ __forceinline__ float silu(float g) {
+__device__ __forceinline__ float silu_of_full(float g) {
   const float x = __builtin_fmaxf(-g, -104.0f), h = x * 0x1.715476p+0f;
   float r = __builtin_fmaf(-h, 0x1.62e430p-1f, x);
   r = __builtin_fmaf(-h, -0x1.05c610p-29f, r);
@@ -176,25 +240,48 @@ __device__ __forceinline__ float silu(float g) {
   return g * f * (s < __builtin_inff() ? __builtin_fmaf(n, q, q) : q);
 }
 
+// For 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is: g / (1 + t^2), and g
+// times t^2 of that below zero. The exponent's rounding is |g| / 2 times 2^-24 of t, so up to
+// |g| times that of the result.
+__device__ __forceinline__ float silu(float g) {
+  const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0x1.715476p-1f), f = g < 0.0f ? t : 1.0f;
+  return g * f * (f * __builtin_amdgcn_rcpf(__builtin_fmaf(t, t, 1.0f)));
+}
+
 constexpr int QUANTIZE_BLOCK = 256, QUANTIZE_PACKS = 2;  // of 8 values, for each thread
 
 template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(const RowsArgs& a) {
   constexpr int N = QUANTIZE_PACKS;
   const uint32_t blocks = (a.dim + 127) / 128, packs = blocks * 16;
   const uint64_t first = (uint64_t)blockIdx.x * (QUANTIZE_BLOCK * N);
-  const uint32_t row0 = (uint32_t)(first / packs), rest = (uint32_t)(first % packs);
-  T v[N][8], u[N][8];
+  uint32_t row0, rest;  // divided in 64 bits only where that is needed
+  if (first >> 32) {
+    row0 = (uint32_t)(first / packs);
+    rest = (uint32_t)(first % packs);
+  } else {
+    row0 = (uint32_t)first / packs;
+    rest = (uint32_t)first % packs;
+  }
+  const uint32_t b0 = row0 / (uint32_t)a.seq, t0 = row0 % (uint32_t)a.seq;
+  const float share = __builtin_amdgcn_rcpf((float)packs);
+  T v[N][8] = {}, u[N][8] = {};
   uint32_t rows[N], ds[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const uint32_t i = rest + threadIdx.x + n * QUANTIZE_BLOCK;
-    const uint32_t row = row0 + i / packs, d = i % packs * 8;
-    rows[n] = row;
-    ds[n] = d;
-    if (row < (uint32_t)a.rows && d < (uint32_t)a.dim) {
-      const int64_t b = row / (uint32_t)a.seq, t = row % (uint32_t)a.seq;
-      load_n<A>(v[n], at<T>(a.x, a.x_off) + b * a.xb + t * a.xt + d);
-      if constexpr (GATED) load_n<A>(u[n], at<T>(a.other, a.o_off) + b * a.ob + t * a.ot + d);
+    uint32_t more = (uint32_t)((float)i * share);  // i / packs, or one beside it
+    more -= more * packs > i;
+    more += (more + 1) * packs <= i;
+    rows[n] = row0 + more;
+    ds[n] = (i - more * packs) * 8;
+    if (rows[n] < (uint32_t)a.rows && ds[n] < (uint32_t)a.dim) {
+      uint32_t b = b0, t = t0 + more;
+      if (t >= (uint32_t)a.seq) {
+        b += t / (uint32_t)a.seq;
+        t %= (uint32_t)a.seq;
+      }
+      load_n<A>(v[n], at<T>(a.x, a.x_off) + (int64_t)b * a.xb + (int64_t)t * a.xt + ds[n]);
+      if constexpr (GATED) load_n<A>(u[n], at<T>(a.other, a.o_off) + (int64_t)b * a.ob + (int64_t)t * a.ot + ds[n]);
     }
   }
 #pragma unroll
@@ -203,11 +290,13 @@ template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(c
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      y[j] = in ? element<T>::widen(v[n][j]) : 0.0f;
-      if constexpr (GATED) y[j] *= silu(in ? element<T>::widen(u[n][j]) : 0.0f);
+      y[j] = element<T>::widen(v[n][j]);
+      if constexpr (GATED && sizeof(T) < 4) y[j] *= silu(element<T>::widen(u[n][j]));
+      if constexpr (GATED && sizeof(T) == 4) y[j] *= silu_of_full(element<T>::widen(u[n][j]));
     }
-    store_block(y, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
-                a.scales + (int64_t)rows[n] * blocks + ds[n] / 128, threadIdx.x % 16 == 0);
+    store_block<sizeof(T) == 4 ? FULL : GATED ? ROUNDED : GIVEN>(
+        y, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
+        a.scales + (int64_t)rows[n] * blocks + ds[n] / 128, threadIdx.x % 16 == 0);
   }
 }
 

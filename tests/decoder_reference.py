@@ -70,13 +70,17 @@ def check_eight(codes, scales, y, slack):
 
 
 def quantized(x, gate=None):
-    """What :func:`check_eight` takes: the sigmoid by exponential (2 F, and the correction's 2),
-    sum, reciprocal (2) and three products is within 12 F."""
-    y = _host(x)
+    """What :func:`check_eight` takes. fp32: the sigmoid by exponential (2 F, and the correction's 2),
+    sum, reciprocal (2) and three products is within 12 F. 16-bit values': e^(-|g| / 2), twice, has an
+    exponent that is 0.6 |g| F off, by the product's rounding and its factor's 0.22 F, and a unit of 2 F; with a sum,
+    a reciprocal and four products that is within (16 + 1.25 |g|) F, until |g| = 175 leaves nothing."""
+    y, slack = _host(x), 12 * F
     if gate is not None:
         g = _host(gate)
         y = y * (g * torch.special.expit(g))
-    return y, 12 * F
+        if gate.dtype != torch.float32:
+            slack = (16 + 1.25 * g.abs().clamp(max=175).nan_to_num().max().item()) * F if g.numel() else 0.0
+    return y, slack
 
 
 def product(a, a_scales, b, b_scales, bias=None):
