@@ -129,7 +129,8 @@ template <int A, class T> __device__ __forceinline__ void store_pack_of(T* p, co
 // One row in WAVES waves, N packs of 8 values for each lane.
 template <class T, int A, int WAVES, int N, bool EIGHT>
 __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
-  constexpr int LANES = 64 * WAVES, ROWS = WAVES < 4 ? 4 / WAVES : 1;
+  static_assert(WAVES == 1 || WAVES >= 4, "the grid is made for 4 rows or one");
+  constexpr int LANES = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
   const int lane = threadIdx.x % LANES, dim = a.dim;
   const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
   if (WAVES == 1 && row >= a.rows) return;  // a whole wave, and no barrier follows
