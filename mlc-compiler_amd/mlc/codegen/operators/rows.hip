@@ -227,18 +227,16 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   }
 }
 
-// g / (1 + e^-g). e^-g is 2^h with h the rounded product, corrected by what the rounding left
-// (as exp_nonpos does); where it is infinite the quotient is a zero, as in fp32's own formula.
-__device__ __forceinline__ float silu_of_full(float g) {
-  const float x = __builtin_fmaxf(-g, -104.0f), h = x * 0x1.715476p+0f;
+// 1 / (1 + e^-g) for fp32's values, off by what the hardware's 2^h is for |h| up to 1/2: h is the rounded product
+// without its whole part, and corrected by what the rounding left (as exp_nonpos does).
+__device__ __forceinline__ double sigmoid_of_full(float g) {
+  const float x = __builtin_fminf(__builtin_fmaxf(-g, -104.0f), 690.0f), h = x * 0x1.715476p+0f;
   float r = __builtin_fmaf(-h, 0x1.62e430p-1f, x);
   r = __builtin_fmaf(-h, -0x1.05c610p-29f, r);
-  const float e = __builtin_amdgcn_exp2f(h);
-  const float s = 1.0f + (e < __builtin_inff() ? __builtin_fmaf(e, r, e) : e);
-  const float f = s > 0x1p64f ? 0x1p-64f : 1.0f;  // no reciprocal below the normal numbers
-  const float z = s * f, q = __builtin_amdgcn_rcpf(z);
-  const float n = __builtin_fmaf(-z, q, 1.0f);  // one step of Newton's; z may be infinite
-  return g * f * (s < __builtin_inff() ? __builtin_fmaf(n, q, q) : q);
+  const float n = __builtin_rintf(h);
+  const double e = (double)__builtin_amdgcn_exp2f(h - n);
+  const double z = 1.0 + __builtin_amdgcn_ldexp(__builtin_fma(e, (double)r, e), (int)n), q = __builtin_amdgcn_rcp(z);
+  return __builtin_fma(__builtin_fma(-z, q, 1.0), q, q);  // one step of Newton's
 }
 
 // For 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is: g / (1 + t^2), and g
@@ -293,7 +291,10 @@ template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(c
     for (int j = 0; j < 8; ++j) {
       y[j] = element<T>::widen(v[n][j]);
       if constexpr (GATED && sizeof(T) < 4) y[j] *= silu(element<T>::widen(u[n][j]));
-      if constexpr (GATED && sizeof(T) == 4) y[j] *= silu_of_full(element<T>::widen(u[n][j]));
+      if constexpr (GATED && sizeof(T) == 4) {
+        const float gate = element<T>::widen(u[n][j]);
+        y[j] = (float)((double)y[j] * (double)gate * sigmoid_of_full(gate));
+      }
     }
     store_block<sizeof(T) == 4 ? FULL : GATED ? ROUNDED : GIVEN>(
         y, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
