@@ -51,6 +51,15 @@ PLANS = {**hip_operators.PLANS, **hip_decoder.PLANS}
 FLAGGING = (*hip_operators.FLAGGING, *hip_decoder.FLAGGING)
 
 
+#: runtimes that nobody holds any longer and that are still to be closed
+_late: list[HipRuntime] = []
+
+
+def close_late() -> None:
+    while _late:
+        _late.pop().close()
+
+
 @dataclass
 class Bound:
     """One generated kernel resolved against the buffer table."""
@@ -95,6 +104,8 @@ class HipRuntime:
         self.device = device
         self.index = device.index if device.index is not None else torch.cuda.current_device()
         self.lib = native.load_library()
+        if not torch.cuda.is_current_stream_capturing():
+            close_late()
         self.module = build_module(schedule, cfg)
         #: the generated HIP module text (``TritonRuntime.source``)
         self.source: str = self.module.source
@@ -447,6 +458,11 @@ class HipRuntime:
 
     def __del__(self) -> None:
         try:
+            # collected while a graph is captured, which freeing memory or a module would end
+            if torch.cuda.is_current_stream_capturing():
+                _late.append(self)
+                return
             self.close()
+            close_late()
         except Exception:
             pass

@@ -4,6 +4,7 @@ kernels go wrong."""
 
 from __future__ import annotations
 
+import gc
 import math
 
 import pytest
@@ -12,6 +13,7 @@ import torch
 import decoder_reference as ref
 import mlc
 from mlc import ops
+from mlc.runtime import hip_runtime
 from mlc.runtime.executor import ExecutionError
 from operators_reference import F
 
@@ -502,6 +504,41 @@ def test_steps_captured_into_graphs_and_replayed_in_turn():
             for x, y in zip(out, want):
                 assert torch.equal(x, y)
     ops.check_errors()
+
+
+@gpu
+def test_a_compiled_step_that_is_collected_while_a_graph_is_captured():
+    model, args = Step().cuda(), step_inputs(tokens=3)
+    compiled = mlc.compile(model, args)
+    compiled(*args)
+    want = model(*args)
+    g = torch.cuda.CUDAGraph()
+    gc.collect()
+    with torch.cuda.graph(g):
+        del compiled
+        gc.collect()
+        got = model(*args)
+    assert hip_runtime._late
+    g.replay()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    again = mlc.compile(model, args)
+    assert not hip_runtime._late and torch.equal(again(*args)[0], want[0])
+
+
+def test_runtimes_that_are_collected_late(monkeypatch):
+    closed, capturing = [], [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(hip_runtime.HipRuntime, "close", lambda self: closed.append(self.name))
+    for name in ("first", "second"):
+        r = hip_runtime.HipRuntime.__new__(hip_runtime.HipRuntime)
+        r.name = name
+        del r
+        assert closed == []
+    capturing[0] = False
+    r = hip_runtime.HipRuntime.__new__(hip_runtime.HipRuntime)
+    r.name = "third"
+    del r
+    assert sorted(closed) == ["first", "second", "third"] and not hip_runtime._late
 
 
 @gpu
