@@ -263,7 +263,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   // Of each lane the tokens from i on that ``bits`` names, as indexes first.
   auto put = [&](uint32_t bits, int i) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
+    for (u64 mask = __ballot(bits != 0); mask && held <= SAMPLE_EACH; mask = __ballot(bits != 0)) {
       const int at = held + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
       if (bits && at < SAMPLE_EACH) l.gathered[wave][at] = (uint32_t)(i + __builtin_ctz(bits));
       bits &= bits - 1;
@@ -427,40 +427,47 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   // Border of the first tokens, among those in front of ``before``, whose ``mass`` reaches ``want``, a number
   // or, where that is 0, ``share`` of all: by 11, 11 and 10 bits of the logit, 11 and 11 of the index.
   auto find = [&](const Border& before, u64 want, double share, auto mass) __attribute__((always_inline)) {
-    auto digit = [&](int level, float x, int i) __attribute__((always_inline)) -> int {
-      const uint32_t k = ~order_of(x);
-      return level == 0 ? (int)(k >> 21) : level == 1 ? (int)(k >> 10 & 2047) : level == 2 ? (int)(k & 1023)
-             : level == 3 ? i >> 11 : i & 2047;
-    };
+    uint32_t k = 0, i = 0;  // what is known of the border's logit and index, and which bits that are
+    uint32_t k_mask = 0, i_mask = 0;
 #pragma unroll 1
     for (int level = 0; level < 5; ++level) {
+      const bool of_index = level > 2;
+      const int shift = level == 0 ? 21 : level == 1 ? 10 : level == 3 ? 11 : 0;
+      const uint32_t digits = level == 2 ? 1023 : 2047;
       clear_bins();
-      over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int i) __attribute__((always_inline)) {
+      over(0, size, tid, SAMPLE_THREADS, [&](const float (&x)[8], int first) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          bool in = before.keeps(x[j], i + j) && i + j < size;
-          for (int n = 0; n < level; ++n) in = in && digit(n, x[j], i + j) == l.digits[n];
-          if (in) atomicAdd(&l.bins[digit(level, x[j], i + j)], mass(x[j]));
+          const uint32_t at = first + j, key = ~order_of(x[j]);
+          const bool in = ((((key ^ k) & k_mask) | ((at ^ i) & i_mask)) == 0) & (at < (uint32_t)size) & before.keeps(x[j], at);
+          const u64 some = __ballot(in);
+          if (some == 0) continue;
+          // equal logits, the reason to be here, at once: atomics on one word go one after the other
+          const int digit = ((of_index ? at : key) >> shift) & digits, lane = __builtin_ctzll(some);
+          const bool same = in & (key == (uint32_t)__builtin_amdgcn_readlane(key, lane)) & (digit == __builtin_amdgcn_readlane(digit, lane));
+          const int n = __popcll(__ballot(same));
+          if (in & (!same | ((tid & 63) == lane))) atomicAdd(&l.bins[digit], mass(x[j]) * (same ? n : 1));
         }
       });
       __syncthreads();
-      const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+      const u64 one = l.bins[2 * tid], two = l.bins[2 * tid + 1];
       u64 below;
-      const u64 all = sum_over_threads(first + second, l, below);
+      const u64 all = sum_over_threads(one + two, l, below);
       if (want == 0) {
         want = (u64)__builtin_ceil(share * (double)all);
         want = want ? want : 1;
       }
-      if (below < want && below + first + second >= want) {
-        l.digits[level] = 2 * tid + (below + first < want);
-        l.found[1] = below + first < want ? below + first : below;
+      if (below < want && below + one + two >= want) {
+        l.digits[0] = 2 * tid + (below + one < want);
+        l.found[1] = below + one < want ? below + one : below;
       }
       __syncthreads();
       want -= l.found[1];
+      (of_index ? i : k) |= (uint32_t)l.digits[0] << shift;
+      (of_index ? i_mask : k_mask) |= digits << shift;
       __syncthreads();
     }
-    return Border{of_order(~((uint32_t)l.digits[0] << 21 | (uint32_t)l.digits[1] << 10 | (uint32_t)l.digits[2])),
-                  l.digits[3] << 11 | l.digits[4]};
+    return Border{of_order(~k), (int)i};
   };
 
   // Segments of the row: a sixteenth each for the 16 waves, and of the one that the token is in again,
@@ -534,8 +541,10 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
       __syncthreads();
       const int bin = l.digits[0];
       const u64 more = top_k - l.found[1];  // of the bin
-      const int n = gather([&](float x, int) __attribute__((always_inline)) { return count_of(x) == bin; });
-      if (n <= SAMPLE_LIST) {
+      const int n = gather([&](float x, int) __attribute__((always_inline)) { return (count_of(x) == bin) & (x > NONE); });
+      if (n <= SAMPLE_LIST && (u64)n < more) {
+        // all that has a weight is kept
+      } else if (n <= SAMPLE_LIST) {
         const u64 key = sort_list(n, l);
         if ((u64)tid + 1 == more) l.found[0] = key;
         __syncthreads();
