@@ -13,16 +13,16 @@ choice of a token.
     y = mlc.ops.scaled_product(codes, scales, *mlc.ops.quantize_weight(w))
     tokens = mlc.ops.sample(logits, uniform, temperature=t, top_p=p)
 
-In attention and the cache tensors are token-major, ``[batch, tokens, heads, dim]``, as a linear layer's output
-is viewed, with any strides whose last is 1; results are contiguous. ``heads`` of the
-queries is a multiple of ``kv_heads`` of keys and values: query head ``h`` reads
+In attention and the cache tensors are token-major, ``[batch, tokens, heads, dim]``, as a
+linear layer's output is viewed, rows elsewhere ``[rows, dim]`` or ``[batch, tokens, dim]``, with
+any strides whose last is 1; results are contiguous. ``heads`` of the queries is a multiple of ``kv_heads`` of keys and values: query head ``h`` reads
 key head ``h // (heads // kv_heads)``.
 
 Called with GPU tensors, each launches this build's kernels on the current stream.
 Used in a module given to ``mlc.compile`` they become launches of the compiled
 schedule; ``cache_append`` then changes the module's own buffers. They are for
 inference: a tensor that asks for a gradient, backward or forward, is refused. Softmax
-statistics and sums are held in fp32, the angles of ``rotary`` in 64 bits.
+statistics and sums are held in fp32, the angles of ``rotary`` and the sums of ``sample`` in 64 bits.
 """
 
 from __future__ import annotations
@@ -666,7 +666,8 @@ def rms_norm(x, weight, residual=None, *, eps: float = 1e-6, quantized: bool = F
 
     Returns the norm in the type of ``x``, or with ``quantized`` (``dim`` a multiple of 16)
     its codes and scales as :func:`quantize` gives them: ``y``, ``(y, sum)``, ``(codes,
-    scales)`` or ``(codes, scales, sum)``. Sums of squares are held in 64 bits.
+    scales)`` or ``(codes, scales, sum)``. Sums of squares are held in 64 bits, the squares of
+    eight neighbouring 16-bit values in fp32.
     """
     op = _NORMS[residual is not None, bool(quantized)]
     operands, eps = (x, weight) if residual is None else (x, weight, residual), float(eps)
