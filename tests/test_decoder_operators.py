@@ -306,13 +306,15 @@ def test_tokens_that_are_equal_go_by_their_index():
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("kind", ("steps", "masked", "far", "cliff", "one"))
-def test_borders_in_rows_unlike_a_models(dtype, kind):
-    """Few different logits, few that are not masked, all but one far below the largest, some so and some near,
-    and one alone: with fewer tokens than top_k asks for, lists too short for what lies at a border, or nothing there."""
+@pytest.mark.parametrize("kind", ("even", "steps", "masked", "far", "cliff", "one"))
+def test_borders_in_rows_of_many_kinds(dtype, kind):
+    """As a model's, few different logits, few that are not masked, all but one far below the largest, some so and
+    some near, and one alone: with fewer tokens than top_k asks for, lists too short for what lies at a border, or nothing there."""
     size = 60000
     x = normal(4, size, dtype=dtype, spread=1.0)
-    if kind == "steps":
+    if kind == "even":
+        x *= 2.5
+    elif kind == "steps":
         x = (x * 4).round() / 4
     elif kind == "masked":
         x[x < 2.5] = -INF
@@ -323,8 +325,8 @@ def test_borders_in_rows_unlike_a_models(dtype, kind):
     else:
         x[:] = -INF
         x[:, 59999] = -3.0
-    uniform = torch.tensor([0.02, 0.5, 0.93, 0.999], device="cuda")
-    for given in ({"top_k": 60}, {"top_k": 1500}, {"top_p": 0.9}, {"top_k": 30000, "top_p": 0.95}, {"min_p": 0.3},
+    uniform = torch.tensor([0.02, 0.5, 0.93, 0.9999], device="cuda")
+    for given in ({"top_k": 60}, {"top_k": 1500}, {"top_p": 0.9}, {"top_p": 0.995}, {"top_k": 30000, "top_p": 0.95}, {"min_p": 0.3},
                   {"temperature": 0.01, "top_p": 0.6}, {"temperature": 30.0, "top_k": 20000, "top_p": 0.5}):
         check_sample(x, uniform, options_of(4, **given), fewest=0.5)
 
