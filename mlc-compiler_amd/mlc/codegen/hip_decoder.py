@@ -118,8 +118,10 @@ def plan_quantize(x: Operand, gate: Operand | None) -> Plan:
 
 #: Rows and columns up to which a workgroup reads all of a beside 16 rows of the weight, in 8 waves with
 #: 4 blocks each: 1 row, 4096 -> 6144 8.6 us and in tiles 10.8, 4 rows, 4096 -> 4096 6.5 and 9.9; 16 rows,
-#: 4096 -> 16384 21.3 and 13.8.
-FEW_ROWS, FEW_COLUMNS, FEW_BLOCKS, FEW_WAVES = 8, 16384, 4, 8
+#: 4096 -> 16384 21.3 and 13.8. In 16 waves where a unit has one workgroup and the sum more blocks than 8 waves
+#: ask for at once: 1 row, 12288 -> 4096 10.9 and with 8 waves 11.9, 16384 -> 4096 16.6 and 18.8; but 4096 -> 6144
+#: 9.6 and 8.6, 4096 -> 1024 6.0 and 5.7.
+FEW_ROWS, FEW_COLUMNS, FEW_BLOCKS, FEW_WAVES = 8, 16384, 4, (8, 16)
 #: Tiles of many rows by the product's instructions, exact or not (rows of both operands, waves along both):
 #: workgroups that a unit holds, and in us what one takes beside its steps, a step of one alone and of each of
 #: many. Measured over 768 to 12288 inputs, 128 to 8192 rows and 2304 to 24576 outputs.
@@ -155,9 +157,9 @@ def choose_tile(rows: int, n: int, blocks: int, dtype: torch.dtype) -> tuple[tup
     return best[1]
 
 
-def few_kernel(dtype) -> tuple[str, str]:
-    name = f"scaled_product_rows_{SHORT[dtype]}"
-    return f"SCALED_PRODUCT_ROWS({name}, {NAMES[dtype]}, {FEW_BLOCKS}, {FEW_WAVES})", name
+def few_kernel(dtype, waves: int) -> tuple[str, str]:
+    name = f"scaled_product_rows_{SHORT[dtype]}_w{waves}"
+    return f"SCALED_PRODUCT_ROWS({name}, {NAMES[dtype]}, {FEW_BLOCKS}, {waves})", name
 
 
 def tiles_kernel(dtype, tile: tuple) -> tuple[str, str]:
@@ -203,8 +205,9 @@ def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, b
         seq = rows
     pointers = ["a", "a_scales", "b", "b_scales", "bias" if bias is not None else None, "out0", None]
     if rows <= FEW_ROWS and n <= FEW_COLUMNS:
-        kernel, name = few_kernel(dtype)
-        grid, threads = _ceil(n, 16), 64 * FEW_WAVES
+        waves = FEW_WAVES[n <= 16 * UNITS and blocks > FEW_WAVES[0] * FEW_BLOCKS]
+        kernel, name = few_kernel(dtype, waves)
+        grid, threads = _ceil(n, 16), 64 * waves
     else:
         tile, splits = choose_tile(rows, n, blocks, dtype)
         reach = max(max(tile[:2]) * max(strides[1], b.strides[0], 4 * scale_strides[1]) if regular else
@@ -289,7 +292,8 @@ def all_kernels() -> list[tuple[str, str]]:
         for w, n in NORM_SHAPES:
             out += [("rows", norm_kernel(dtype, a, w, n, e)[0]) for a in aligns for e in (False, True)]
         out += [("rows", quantize_kernel(dtype, a, g)[0]) for a in aligns for g in (False, True)]
-        out += [("scaled_product", few_kernel(dtype)[0]), ("scaled_product", product_join_kernel(dtype)[0]),
+        out += [("scaled_product", few_kernel(dtype, waves)[0]) for waves in FEW_WAVES]
+        out += [("scaled_product", product_join_kernel(dtype)[0]),
                 ("sample", sample_kernel(dtype)[0])]
         out += [("scaled_product", tiles_kernel(dtype, t)[0]) for t in TILES[dtype == torch.float32]]
     return out

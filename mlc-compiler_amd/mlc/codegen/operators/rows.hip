@@ -12,9 +12,10 @@
 // in fp32, but for the sums of eight squares, whose range is any value's.
 // Infinities and NaN become codes of NaN and do not count for a scale.
 //
-// 8192 rows of 4096 in bf16 with a residual, to codes: 49.3 us, 4.7 TB/s, with 53 % of the time in vector
-// instructions (in 64 bits all through 54.8); with 8 waves of one pack instead of 4 of two 51.1. 6063 rows of 12288 in bf16,
-// gated: 73 us, 5.1 TB/s and 75 % (in 64 bits, and with a division for every pack, 97). A single row: 3 us.
+// 8192 rows of 4096 in bf16 with a residual, to codes: 48.8 us, 4.8 TB/s, with 53 % of the time in vector
+// instructions (in 64 bits all through 54.8); with 8 waves of one pack instead of 4 of two 51.1. 6063 rows
+// of 12288 in bf16, gated: 73 us, 5.1 TB/s and 75 % (in 64 bits, and with a division for every pack, 97). A
+// single row: 3 us.
 
 namespace mlc {
 
@@ -94,7 +95,8 @@ __device__ __forceinline__ void store_block(const float (&y)[8], bool in, uint8_
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       q[j] = y[j] * by;
-      if constexpr (KIND == GIVEN) q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
+      if constexpr (KIND == GIVEN)
+        q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
     }
   }
   if (!finite) {

@@ -439,12 +439,14 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t at = first + j, key = ~order_of(x[j]);
-          const bool in = ((((key ^ k) & k_mask) | ((at ^ i) & i_mask)) == 0) & (at < (uint32_t)size) & before.keeps(x[j], at);
+          const bool in = ((((key ^ k) & k_mask) | ((at ^ i) & i_mask)) == 0) & (at < (uint32_t)size) &
+                          before.keeps(x[j], at);
           const u64 some = __ballot(in);
           if (some == 0) continue;
           // equal logits, the reason to be here, at once: atomics on one word go one after the other
           const int digit = ((of_index ? at : key) >> shift) & digits, lane = __builtin_ctzll(some);
-          const bool same = in & (key == (uint32_t)__builtin_amdgcn_readlane(key, lane)) & (digit == __builtin_amdgcn_readlane(digit, lane));
+          const bool same = in & (key == (uint32_t)__builtin_amdgcn_readlane(key, lane)) &
+                            (digit == __builtin_amdgcn_readlane(digit, lane));
           const int n = __popcll(__ballot(same));
           if (in & (!same | ((tid & 63) == lane))) atomicAdd(&l.bins[digit], mass(x[j]) * (same ? n : 1));
         }
@@ -506,15 +508,20 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
     // tokens in each 512th of a power of two of the weight
     const float per = 512.0f * weigh.hi;
     constexpr int COUNTS = SAMPLE_COUNTS, EACH = COUNTS / SAMPLE_THREADS;
-    auto count_of = [&](float x) __attribute__((always_inline)) { return (int)__builtin_fminf((top - x) * per, (float)COUNTS); };
+    auto count_of = [&](float x) __attribute__((always_inline)) {
+      return (int)__builtin_fminf((top - x) * per, (float)COUNTS);
+    };
     // What is further away, or behind the row's end, is counted for each lane: the atomics of 64 on one
     // word take as long as on 64 words one after the other.
     const float far = (float)(COUNTS + (tid & 63));
-    auto count = [&](float x) __attribute__((always_inline)) { atomicAdd(&l.counts[(int)__builtin_fminf((top - x) * per, far)], 1u); };
+    auto count = [&](float x) __attribute__((always_inline)) {
+      atomicAdd(&l.counts[(int)__builtin_fminf((top - x) * per, far)], 1u);
+    };
     auto clear_counts = [&] {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < EACH; j += 4) *reinterpret_cast<uint4v*>(&l.counts[j * SAMPLE_THREADS + tid * 4]) = uint4v{0, 0, 0, 0};
+      for (int j = 0; j < EACH; j += 4)
+        *reinterpret_cast<uint4v*>(&l.counts[j * SAMPLE_THREADS + tid * 4]) = uint4v{0, 0, 0, 0};
       __syncthreads();
     };
     clear_counts();
@@ -652,8 +659,9 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
         if (want <= in_front || !__syncthreads_or(held > SAMPLE_EACH)) break;
         // the last quarter of the bin in front of the first is not yet among what lies in front
         const float rest = (float)(want - in_front) * 0x1p-40f;
-        early = first_bin == 0 ? 0.0f
-                : __builtin_fmaxf(rest - (float)l.counts[first_bin - 1] * __builtin_amdgcn_exp2f((float)(first_bin - 1) * -0x1p-9f + 0x1p-12f), 0.0f);
+        const int front_bin = first_bin > 0 ? first_bin - 1 : 0;
+        const float quarter = (float)l.counts[front_bin] * __builtin_amdgcn_exp2f((float)front_bin * -0x1p-9f + 0x1p-12f);
+        early = first_bin == 0 ? 0.0f : __builtin_fmaxf(rest - quarter, 0.0f);
         late = rest / (float)RATIO;
         from_bin = first_bin;
         __syncthreads();
@@ -666,7 +674,8 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
         // into fine bins of the window, of which one is then sorted
         const float wide = (float)SAMPLE_BINS / (float)(last_bin - first_bin + 2);
         auto fine_bin = [&](u64 key) {
-          return (int)__builtin_fminf(__builtin_fmaxf(((top - x_of(key)) * per - ((float)first_bin - 0.5f)) * wide, 0.0f), (float)(SAMPLE_BINS - 1));
+          const float at = ((top - x_of(key)) * per - ((float)first_bin - 0.5f)) * wide;
+          return (int)__builtin_fminf(__builtin_fmaxf(at, 0.0f), (float)(SAMPLE_BINS - 1));
         };
         clear_bins();
 #pragma unroll 1
@@ -709,7 +718,8 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
           }
         }
       }
-      if (!done) kept = find(before, 0, (double)top_p, [&](float x) __attribute__((always_inline)) { return units(weigh(x)); });
+      if (!done)
+        kept = find(before, 0, (double)top_p, [&](float x) __attribute__((always_inline)) { return units(weigh(x)); });
     }
   }
 

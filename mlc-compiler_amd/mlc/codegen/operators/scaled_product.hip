@@ -48,7 +48,8 @@ template <> struct Codes<true> {
   __device__ __forceinline__ Codes(int4v lo, int4v hi) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t a = (uint32_t)(i < 2 ? lo[2 * i] : hi[2 * i - 4]), b = (uint32_t)(i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]);
+      const uint32_t a = (uint32_t)(i < 2 ? lo[2 * i] : hi[2 * i - 4]);
+      const uint32_t b = (uint32_t)(i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]);
       x[i] = __builtin_bit_cast(half8, uint4v{codes<f16>::widen(a, 0), codes<f16>::widen(a, 1),
                                               codes<f16>::widen(b, 0), codes<f16>::widen(b, 1)});
     }
@@ -84,7 +85,7 @@ template <class T> __device__ __forceinline__ float bias_of(const ScaledProductA
 
 // Up to 16 rows: the weight is read once and is all that counts. A workgroup has 16 of its rows and
 // all of a's; its waves take U blocks of the sum in turn, whose operands they ask for at once, and
-// meet in LDS. 1 row, 4096 -> 6144 8.6 us, 12288 -> 4096 11.7, 4.3 TB/s.
+// meet in LDS. 1 row, 4096 -> 6144 8.6 us, 12288 -> 4096 10.9, 4.6 TB/s.
 template <class T, int U, int WAVES> __device__ __forceinline__ void scaled_product_rows(const ScaledProductArgs& a) {
   __shared__ __attribute__((aligned(16))) float4v parts[WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -190,9 +191,12 @@ __device__ __forceinline__ void scaled_product_tiles(const ScaledProductArgs& a)
     m += m0 - base;
     return a.regular ? m * (uint32_t)token : m / a.seq * (uint32_t)batch + m % a.seq * (uint32_t)token;
   };
-  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at<uint8_t>(a.a, a.a_off) + base * a.at), 0, OUTSIDE, 0x27000);
-  const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at<uint8_t>(a.b, a.b_off) + n0 * a.br), 0, OUTSIDE, 0x27000);
-  const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(at<float>(a.a_scales, a.as_off) + base * a.ast), 0, OUTSIDE, 0x27000);
+  auto buffer_at = [](const void* p) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, OUTSIDE, 0x27000);
+  };
+  const auto ra = buffer_at(at<uint8_t>(a.a, a.a_off) + base * a.at);
+  const auto rb = buffer_at(at<uint8_t>(a.b, a.b_off) + n0 * a.br);
+  const auto rs = buffer_at(at<float>(a.a_scales, a.as_off) + base * a.ast);
   const int own = threadIdx.x / 8, chunk = (threadIdx.x & 7) ^ (own >> 1 & 7);
   uint32_t va[LA], vb[LB];
 #pragma unroll
@@ -232,7 +236,8 @@ __device__ __forceinline__ void scaled_product_tiles(const ScaledProductArgs& a)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int m = at_row + q * 8 + lane / 8, block = i + lane % 8;
-          const uint32_t v = m0 + m < a.rows && block < blocks ? (offset(m, a.asb, a.ast) + block * (uint32_t)a.ass) * 4 : OUTSIDE;
+          const uint32_t far = (offset(m, a.asb, a.ast) + block * (uint32_t)a.ass) * 4;
+          const uint32_t v = m0 + m < a.rows && block < blocks ? far : OUTSIDE;
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(to + (at_row + q * 8) * GROUP * 4), 4, v, 0, 0, 0);
         }
       }

@@ -14,8 +14,9 @@ choice of a token.
     tokens = mlc.ops.sample(logits, uniform, temperature=t, top_p=p)
 
 In attention and the cache tensors are token-major, ``[batch, tokens, heads, dim]``, as a
-linear layer's output is viewed, rows elsewhere ``[rows, dim]`` or ``[batch, tokens, dim]``, with
-any strides whose last is 1; results are contiguous. ``heads`` of the queries is a multiple of ``kv_heads`` of keys and values: query head ``h`` reads
+linear layer's output is viewed, rows elsewhere ``[rows, dim]`` or ``[batch, tokens, dim]``,
+with any strides whose last is 1; results are contiguous. ``heads`` of the queries is a
+multiple of ``kv_heads`` of keys and values: query head ``h`` reads
 key head ``h // (heads // kv_heads)``.
 
 Called with GPU tensors, each launches this build's kernels on the current stream.

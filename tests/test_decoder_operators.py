@@ -160,7 +160,8 @@ def coded(n, k, rows, seed=0, spread=1.0):
 @pytest.mark.parametrize("rows,n,k", [
     (1, 1, 16), (1, 16, 128), (3, 17, 144), (15, 40, 256), (16, 128, 4096), (17, 130, 400), (32, 256, 1280),
     (33, 100, 1152), (48, 33, 1024), (64, 300, 2304), (65, 129, 272), (100, 7, 160), (128, 128, 2048),
-    (130, 257, 1008), (200, 1024, 128), (300, 256, 4112), (513, 640, 640), (1, 5, 12304)])
+    (130, 257, 1008), (200, 1024, 128), (300, 256, 4112), (513, 640, 640), (1, 5, 12304),
+    (3, 100, 4240), (8, 48, 8208)])
 @pytest.mark.parametrize("biased", (False, True))
 def test_scaled_product(dtype, rows, n, k, biased):
     a, a_scales = coded(rows, k, 1)
@@ -309,7 +310,8 @@ def test_tokens_that_are_equal_go_by_their_index():
 @pytest.mark.parametrize("kind", ("even", "steps", "masked", "far", "cliff", "one"))
 def test_borders_in_rows_of_many_kinds(dtype, kind):
     """As a model's, few different logits, few that are not masked, all but one far below the largest, some so and
-    some near, and one alone: with fewer tokens than top_k asks for, lists too short for what lies at a border, or nothing there."""
+    some near, and one alone: with fewer tokens than top_k asks for, lists too short for what lies at a border, or
+    nothing there."""
     size = 60000
     x = normal(4, size, dtype=dtype, spread=1.0)
     if kind == "even":
@@ -326,7 +328,8 @@ def test_borders_in_rows_of_many_kinds(dtype, kind):
         x[:] = -INF
         x[:, 59999] = -3.0
     uniform = torch.tensor([0.02, 0.5, 0.93, 0.9999], device="cuda")
-    for given in ({"top_k": 60}, {"top_k": 1500}, {"top_p": 0.9}, {"top_p": 0.995}, {"top_k": 30000, "top_p": 0.95}, {"min_p": 0.3},
+    for given in ({"top_k": 60}, {"top_k": 1500}, {"top_p": 0.9}, {"top_p": 0.995}, {"min_p": 0.3},
+                  {"top_k": 30000, "top_p": 0.95},
                   {"temperature": 0.01, "top_p": 0.6}, {"temperature": 30.0, "top_k": 20000, "top_p": 0.5}):
         check_sample(x, uniform, options_of(4, **given), fewest=0.5)
 
