@@ -116,12 +116,14 @@ def plan_quantize(x: Operand, gate: Operand | None) -> Plan:
 # products
 # --------------------------------------------------------------------------
 
-#: Rows and columns up to which a workgroup reads all of a beside 16 rows of the weight, in 8 waves with
-#: 4 blocks each: 1 row, 4096 -> 6144 8.6 us and in tiles 10.8, 4 rows, 4096 -> 4096 6.5 and 9.9; 16 rows,
-#: 4096 -> 16384 21.3 and 13.8. In 16 waves where a unit has one workgroup and the sum more blocks than 8 waves
-#: ask for at once: 1 row, 12288 -> 4096 10.9 and with 8 waves 11.9, 16384 -> 4096 16.6 and 18.8; but 4096 -> 6144
-#: 9.6 and 8.6, 4096 -> 1024 6.0 and 5.7.
-FEW_ROWS, FEW_COLUMNS, FEW_BLOCKS, FEW_WAVES = 8, 16384, 4, (8, 16)
+#: Few rows, up to 16: a workgroup reads all of them beside 16 rows of the weight, in 8 waves with 4 blocks each. Reading
+#: them again and again ends that: 1 row, 4096 -> 8192 8.9 us and in tiles 11.2, 16 rows, 4096 -> 4096 7.5 and 10.8,
+#: 8 rows, 4096 -> 8192 10.4 and 11.0; but 16 rows 12.0 and 11.4, 12288 -> 4096 15.8 and 14.9, 1 row, 4096 -> 16384 15.5
+#: and 13.7, and 12288 -> 5120, one and a quarter rounds of long sums, 17.4 and 15.0.
+FEW_ROWS, FEW_COLUMNS, FEW_SUM, FEW_VALUES, FEW_PRODUCTS = 16, 8192, 8192, 1 << 16, 1 << 29
+#: In 16 waves where a unit has one workgroup and the sum more blocks than 8 waves ask for at once: 1 row, 12288 -> 4096
+#: 10.9 us and with 8 waves 11.9, 16384 -> 4096 16.6 and 18.8; but 4096 -> 6144 9.6 and 8.6, 4096 -> 1024 6.0 and 5.7.
+FEW_BLOCKS, FEW_WAVES = 4, (8, 16)
 #: Tiles of many rows by the product's instructions, exact or not (rows of both operands, waves along both):
 #: workgroups that a unit holds, and in us what one takes beside its steps, a step of one alone and of each of
 #: many. Measured over 768 to 12288 inputs, 128 to 8192 rows and 2304 to 24576 outputs.
@@ -132,9 +134,15 @@ TILES = {False: {(256, 256, 4, 2): (1, 8.5, 1.7, 1.7), (128, 128, 2, 2): (2, 3.5
 JOIN_THREADS = 256
 
 
-def is_exact(rows: int, n: int, dtype: torch.dtype) -> bool:
+def takes_rows(rows: int, n: int, k: int) -> bool:
+    """Whether a workgroup reads all rows of a."""
+    return (rows <= FEW_ROWS and n <= FEW_COLUMNS and rows * n <= FEW_VALUES and rows * n * k < FEW_PRODUCTS
+            and (n <= 16 * UNITS or k <= FEW_SUM))
+
+
+def is_exact(rows: int, n: int, k: int, dtype: torch.dtype) -> bool:
     """Whether products are taken of widened codes: where that costs nothing, or fp32 results show it."""
-    return dtype == torch.float32 or (rows <= FEW_ROWS and n <= FEW_COLUMNS)
+    return dtype == torch.float32 or takes_rows(rows, n, k)
 
 
 def choose_tile(rows: int, n: int, blocks: int, dtype: torch.dtype) -> tuple[tuple, int]:
@@ -204,7 +212,7 @@ def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, b
     if regular:
         seq = rows
     pointers = ["a", "a_scales", "b", "b_scales", "bias" if bias is not None else None, "out0", None]
-    if rows <= FEW_ROWS and n <= FEW_COLUMNS:
+    if takes_rows(rows, n, k):
         waves = FEW_WAVES[n <= 16 * UNITS and blocks > FEW_WAVES[0] * FEW_BLOCKS]
         kernel, name = few_kernel(dtype, waves)
         grid, threads = _ceil(n, 16), 64 * waves

@@ -84,7 +84,7 @@ def quantized(x, gate=None):
 
 
 def product(a, a_scales, b, b_scales, bias=None):
-    """``(want, bound, groups)`` without the result's rounding. Within a block 128 products, exact in
+    """``(want, bound, groups, k)`` without the result's rounding. Within a block 128 products, exact in
     fp32, are added in any order: 128 F of their magnitudes' sum; a factor of two roundings, an
     addition for every block, of parts of them and of the bias.
 
@@ -105,12 +105,12 @@ def product(a, a_scales, b, b_scales, bias=None):
     if bias is not None:
         want = want + _host(bias)
         bound = bound + 2 * F * want.abs()
-    return want, bound, groups
+    return want, bound, groups, k
 
 
-def check_product(got, want, bound, groups, dtype):
+def check_product(got, want, bound, groups, k, dtype):
     assert got.dtype == dtype and got.is_contiguous() and got.shape == want.shape
-    if not is_exact(math.prod(want.shape[:-1]), want.shape[-1], dtype):
+    if not is_exact(math.prod(want.shape[:-1]), want.shape[-1], k, dtype):
         bound = bound + groups
     bound = bound * (1 + U[dtype]) + U[dtype] * want.abs() + LEAST[dtype]
     off = (_host(got) - want).abs()

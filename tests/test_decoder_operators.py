@@ -161,7 +161,7 @@ def coded(n, k, rows, seed=0, spread=1.0):
     (1, 1, 16), (1, 16, 128), (3, 17, 144), (15, 40, 256), (16, 128, 4096), (17, 130, 400), (32, 256, 1280),
     (33, 100, 1152), (48, 33, 1024), (64, 300, 2304), (65, 129, 272), (100, 7, 160), (128, 128, 2048),
     (130, 257, 1008), (200, 1024, 128), (300, 256, 4112), (513, 640, 640), (1, 5, 12304),
-    (3, 100, 4240), (8, 48, 8208)])
+    (3, 100, 4240), (8, 48, 8208), (16, 4100, 272), (9, 4100, 144)])
 @pytest.mark.parametrize("biased", (False, True))
 def test_scaled_product(dtype, rows, n, k, biased):
     a, a_scales = coded(rows, k, 1)
