@@ -326,10 +326,11 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   float from = NONE;
   if (!gathers && top_k && top_k <= SAMPLE_FEW) {
     // as many threads as top_k have a token at or above the end of the bin, a 64th, of their top_k-th
-    clear_bins();
-    atomicAdd(&l.bins[(int)__builtin_fminf((top - own_top) * 64.0f, (float)(SAMPLE_BINS - 1))], (u64)1);
+    l.bins[tid] = 0;  // two counts
     __syncthreads();
-    const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+    atomicAdd(&l.counts[(int)__builtin_fminf((top - own_top) * 64.0f, (float)(SAMPLE_BINS - 1))], 1u);
+    __syncthreads();
+    const u64 first = l.counts[2 * tid], second = l.counts[2 * tid + 1];
     u64 below;
     sum_over_threads(first + second, l, below);
     if (below < (u64)top_k && below + first + second >= (u64)top_k) l.digits[0] = 2 * tid + 1;
@@ -344,21 +345,29 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   }
   if (gathers) {
     int n;
+    if (tid == 0) l.digits[1] = 0;
     if (__syncthreads_count(own_top >= from) <= 256) {
       // few threads have one: their waves look through their packs, a token a lane
-      held = 0;
       for (u64 some = __ballot(own_top >= from); some; some &= some - 1) {
         const int first = (tid - (tid & 63) + __builtin_ctzll(some)) * 8;
 #pragma unroll 1
         for (int e = tid & 63; e < (size - first + SAMPLE_THREADS * 8 - 1) / (SAMPLE_THREADS * 8) * 8; e += 64) {
           const int i = first + e / 8 * (SAMPLE_THREADS * 8) + e % 8;
           const float x = i < size ? element<T>::widen(row[i]) : NONE;
-          put(i < size && x >= from, i);
+          const bool in = i < size && x >= from;
+          const u64 mask = __ballot(in);
+          if (mask) {
+            int at = 0;
+            const int lane = __builtin_ctzll(mask);
+            if ((tid & 63) == lane) at = atomicAdd(&l.digits[1], __popcll(mask));
+            at = __builtin_amdgcn_readlane(at, lane) +
+                 __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+            if (in && at < SAMPLE_LIST) l.list[at] = (u64)~order_of(x) << 32 | (uint32_t)i;
+          }
         }
-        held = __builtin_amdgcn_readfirstlane(held);
       }
-      settle();
-      n = collect(any_of);
+      __syncthreads();
+      n = l.digits[1];
     } else {
       n = gather([&](float x, int) __attribute__((always_inline)) { return x >= from; });
     }
