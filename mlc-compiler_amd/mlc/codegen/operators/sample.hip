@@ -345,24 +345,44 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   }
   if (gathers) {
     int n;
-    if (tid == 0) l.digits[1] = 0;
-    if (__syncthreads_count(own_top >= from) <= 256) {
-      // few threads have one: their waves look through their packs, a token a lane
-      for (u64 some = __ballot(own_top >= from); some; some &= some - 1) {
-        const int first = (tid - (tid & 63) + __builtin_ctzll(some)) * 8;
+    if (tid == 0) l.digits[1] = l.digits[2] = 0;
+    const int seers = __syncthreads_count(own_top >= from);
+    // a place behind the ``counter`` for each lane of ``mask``
+    auto place = [&](u64 mask, int* counter) __attribute__((always_inline)) {
+      const int lane = __builtin_ctzll(mask);
+      int first = 0;
+      if ((tid & 63) == lane) first = atomicAdd(counter, __popcll(mask));
+      return __builtin_amdgcn_readlane(first, lane) +
+             (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    };
+    if (seers <= 512) {
+      // few threads have one: all look through what those have seen, two tokens of theirs on their way
+      const u64 some = __ballot(own_top >= from);
+      if (some) {
+        const int at = place(some, &l.digits[2]);
+        if (own_top >= from) l.sorted[at] = tid;
+      }
+      __syncthreads();
+      const int per = (size + SAMPLE_THREADS * 8 - 1) / (SAMPLE_THREADS * 8) * 8, all = seers * per;
+      const float share = 1.0f / (float)per;
 #pragma unroll 1
-        for (int e = tid & 63; e < (size - first + SAMPLE_THREADS * 8 - 1) / (SAMPLE_THREADS * 8) * 8; e += 64) {
-          const int i = first + e / 8 * (SAMPLE_THREADS * 8) + e % 8;
-          const float x = i < size ? element<T>::widen(row[i]) : NONE;
-          const bool in = i < size && x >= from;
+      for (int begin = 0; begin < all; begin += 2 * SAMPLE_THREADS) {
+        int i[2];
+        float x[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int at = begin + u * SAMPLE_THREADS + tid;
+          const int nth = (int)(((float)at + 0.5f) * share), e = at - nth * per;  // at / per: below 2^21
+          i[u] = at < all ? (int)l.sorted[nth] * 8 + e / 8 * (SAMPLE_THREADS * 8) + e % 8 : size;
+          x[u] = i[u] < size ? element<T>::widen(row[i[u]]) : NONE;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bool in = i[u] < size && x[u] >= from;
           const u64 mask = __ballot(in);
           if (mask) {
-            int at = 0;
-            const int lane = __builtin_ctzll(mask);
-            if ((tid & 63) == lane) at = atomicAdd(&l.digits[1], __popcll(mask));
-            at = __builtin_amdgcn_readlane(at, lane) +
-                 __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-            if (in && at < SAMPLE_LIST) l.list[at] = (u64)~order_of(x) << 32 | (uint32_t)i;
+            const int at = place(mask, &l.digits[1]);
+            if (in && at < SAMPLE_LIST) l.list[at] = (u64)~order_of(x[u]) << 32 | (uint32_t)i[u];
           }
         }
       }
