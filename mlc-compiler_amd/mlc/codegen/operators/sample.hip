@@ -626,7 +626,10 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
           up_to[j] = own;
           most *= 0x1.ff4eacp-1f;  // 2^(-1/512)
         }
-        if (tid == 0) l.digits[0] = l.digits[1] = COUNTS;
+        if (tid == 0) {
+          l.digits[0] = l.digits[1] = COUNTS;
+          l.digits[3] = 0;
+        }
         u64 below;
         const double near = (double)sum_over_threads((u64)((double)own * 0x1p40), l, below) * 0x1p-40;
         if (turn == 0) {
@@ -680,6 +683,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
           }
         });
         settle();
+        if ((tid & 63) == 0) atomicAdd(&l.digits[3], held);
         u64 unused;
         all = sum_over_threads((u64)all_own, l, unused);
         in_front = sum_over_threads((u64)front_own, l, unused);
@@ -700,39 +704,49 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
       bool done = false;
       if (want > in_front && !__syncthreads_or(held > SAMPLE_EACH)) {
         want -= in_front;
-        // into fine bins of the window, of which one is then sorted
-        const float wide = (float)SAMPLE_BINS / (float)(last_bin - first_bin + 2);
-        auto fine_bin = [&](u64 key) {
-          const float at = ((top - x_of(key)) * per - ((float)first_bin - 0.5f)) * wide;
-          return (int)__builtin_fminf(__builtin_fmaxf(at, 0.0f), (float)(SAMPLE_BINS - 1));
-        };
-        clear_bins();
+        int m = 0;
+        if (l.digits[3] <= 256) {
+          m = collect([&](u64 key) { return key <= limit; });
+        } else {
+          // not all of the window, but one of fine bins that it is taken apart into
+          const float wide = (float)SAMPLE_BINS / (float)(last_bin - first_bin + 2);
+          auto fine_bin = [&](u64 key) {
+            const float at = ((top - x_of(key)) * per - ((float)first_bin - 0.5f)) * wide;
+            return (int)__builtin_fminf(__builtin_fmaxf(at, 0.0f), (float)(SAMPLE_BINS - 1));
+          };
+          clear_bins();
 #pragma unroll 1
-        for (int i = tid & 63; i < held; i += 64) {
-          const u64 key = l.gathered[wave][i];
-          if (key <= limit) atomicAdd(&l.bins[fine_bin(key)], units(weigh(x_of(key))));
+          for (int i = tid & 63; i < held; i += 64) {
+            const u64 key = l.gathered[wave][i];
+            if (key <= limit) atomicAdd(&l.bins[fine_bin(key)], units(weigh(x_of(key))));
+          }
+          if (tid == 0) l.found[0] = ~(u64)0;
+          __syncthreads();
+          const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
+          u64 below;
+          sum_over_threads(first + second, l, below);
+          if (below < want && below + first + second >= want) {
+            l.digits[0] = 2 * tid + (below + first < want);
+            l.found[0] = below + first < want ? below + first : below;
+          }
+          __syncthreads();
+          m = SAMPLE_LIST + 1;
+          if (l.found[0] != ~(u64)0) {
+            const int bin = l.digits[0];
+            want -= l.found[0];
+            m = collect([&](u64 key) { return key <= limit && fine_bin(key) == bin; });
+          }
         }
-        if (tid == 0) l.found[0] = ~(u64)0;
-        __syncthreads();
-        const u64 first = l.bins[2 * tid], second = l.bins[2 * tid + 1];
-        u64 below;
-        sum_over_threads(first + second, l, below);
-        if (below < want && below + first + second >= want) {
-          l.digits[0] = 2 * tid + (below + first < want);
-          l.found[0] = below + first < want ? below + first : below;
-        }
-        __syncthreads();
-        if (l.found[0] != ~(u64)0) {
-          const int bin = l.digits[0];
-          want -= l.found[0];
-          const int m = collect([&](u64 key) { return key <= limit && fine_bin(key) == bin; });
-          if (m <= SAMPLE_LIST) {
-            const u64 key = sort_list(m, l);
-            const u64 w = tid < m ? units(weigh(x_of(key))) : 0;
-            sum_over_threads(w, l, below);
-            if (below < want && below + w >= want) l.found[0] = key;
-            __syncthreads();
-            const u64 last = l.found[0];
+        if (m <= SAMPLE_LIST) {
+          const u64 key = sort_list(m, l);
+          const u64 w = tid < m ? units(weigh(x_of(key))) : 0;
+          if (tid == 0) l.found[0] = ~(u64)0;
+          u64 below;
+          sum_over_threads(w, l, below);
+          if (below < want && below + w >= want) l.found[0] = key;
+          __syncthreads();
+          const u64 last = l.found[0];
+          if (last != ~(u64)0) {
             kept = Border{x_of(last), (int)(uint32_t)last};
             done = true;
             if (weigh(kept.x) >= min_p) {
