@@ -12,9 +12,9 @@
 // in fp32, but for the sums of eight squares, whose range is any value's.
 // Infinities and NaN become codes of NaN and do not count for a scale.
 //
-// 8192 rows of 4096 in bf16 with a residual, to codes: 48.8 us, 4.8 TB/s, with 53 % of the time in vector
+// 8192 rows of 4096 in bf16 with a residual, to codes: 49.8 us, 4.7 TB/s, with 55 % of the time in vector
 // instructions (in 64 bits all through 54.8); with 8 waves of one pack instead of 4 of two 51.1. 6063 rows
-// of 12288 in bf16, gated: 73 us, 5.1 TB/s and 75 % (in 64 bits, and with a division for every pack, 97). A
+// of 12288 in bf16, gated: 74 us, 5.1 TB/s and 75 % (in 64 bits, and with a division for every pack, 97). A
 // single row: 3 us.
 
 namespace mlc {
@@ -67,9 +67,13 @@ enum { GIVEN, ROUNDED, FULL };
 // be exact. y * 448 and the middle times the largest are whole numbers of 14 and 16 bits where y has 11: the
 // quotient is in the middle or at least 2^-16 beside it. So one in fp32, off by 2^-22, is rounded to 18
 // digits, which puts it there or leaves it on its side. Of fp32 values it is taken in 64 bits.
+//
+// Of values rounded to fp32 a quotient is rounded once more, by a factor of two floats, so that few codes are
+// others than the real quotients'. What all values have in common, ``factor``, is left to the scale: codes do
+// not depend on it.
 template <int KIND>
-__device__ __forceinline__ void store_block(const float (&y)[8], bool in, uint8_t* codes, float* scale_at,
-                                            bool first) {
+__device__ __forceinline__ void store_block(const float (&y)[8], float factor, bool in, uint8_t* codes,
+                                            float* scale_at, bool first) {
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = __builtin_elementwise_maximum(top, __builtin_fabsf(y[j]));
@@ -85,19 +89,20 @@ __device__ __forceinline__ void store_block(const float (&y)[8], bool in, uint8_
     top = group_reduce<16, OpMax>(top);
   }
   float q[8];
-  if constexpr (KIND == FULL) {
-    const double by = __builtin_fmin(448.0 / (double)top, 0x1p126);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = (float)((double)y[j] * by);
-  } else {
+  if constexpr (KIND == GIVEN) {
     // 448 / top, whose reciprocal is a normal number: two roundings and the reciprocal's unit of a quotient
     const float by = __builtin_fminf(1.75f * __builtin_amdgcn_rcpf(top * 0x1p-8f), 0x1p126f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      q[j] = y[j] * by;
-      if constexpr (KIND == GIVEN)
-        q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
-    }
+    for (int j = 0; j < 8; ++j)
+      q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y[j] * by) + 0x20) & 0xffffffc0u);
+  } else {
+    const double r = __builtin_amdgcn_rcp((double)top);
+    double by = 448.0 * __builtin_fma(__builtin_fma(-(double)top, r, 1.0), r, r);  // NaN for zeros alone
+    by = factor == factor ? __builtin_fmin(by, (double)factor * 0x1p126) : (double)factor;
+    const float hi = (float)by, lo = (float)(by - (double)hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      q[j] = KIND == FULL ? (float)((double)y[j] * by) : __builtin_fmaf(y[j], hi, y[j] * lo);
   }
   if (!finite) {
 #pragma unroll
@@ -105,7 +110,7 @@ __device__ __forceinline__ void store_block(const float (&y)[8], bool in, uint8_
   }
   if (in) {
     *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
-    if (first) *scale_at = __builtin_fmaxf(top * (1.0f / 448.0f), 0x1p-126f);
+    if (first) *scale_at = __builtin_fmaxf(top * factor * (1.0f / 448.0f), 0x1p-126f);
   }
 }
 
@@ -202,15 +207,17 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   }
   const double mean = __builtin_fma(sum, a.part, a.eps);
   auto weight = [&](int n, int j) { return sizeof(T) < 4 && a.wide_weight ? wide[n][j] : element<T>::widen(z[n][j]); };
+  float factor = 1.0f;
   if constexpr (sizeof(T) < 4) {
     // a power of two near the root goes into h, so that the reciprocal is a normal number whatever the root
     const int power = __builtin_amdgcn_frexp_exp(mean) >> 1;
     const float by = __builtin_amdgcn_rsqf((float)__builtin_amdgcn_ldexp(mean, -2 * power));
+    factor = by;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       if (!EARLY) load_weight(n);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[n][j] = __builtin_amdgcn_ldexpf(h[n][j], -power) * by * weight(n, j);
+      for (int j = 0; j < 8; ++j) h[n][j] = __builtin_amdgcn_ldexpf(h[n][j], -power) * (EIGHT ? 1.0f : by) * weight(n, j);
     }
   } else {
     const double by = 1.0 / __builtin_sqrt(mean);
@@ -225,7 +232,7 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   for (int n = 0; n < N; ++n) {
     const int d = (lane + n * LANES) * 8;
     if constexpr (EIGHT) {
-      store_block<sizeof(T) < 4 ? ROUNDED : FULL>(h[n], d < dim, reinterpret_cast<uint8_t*>(a.out) + row * dim + d,
+      store_block<sizeof(T) < 4 ? ROUNDED : FULL>(h[n], factor, d < dim, reinterpret_cast<uint8_t*>(a.out) + row * dim + d,
                                                   a.scales + row * ((dim + 127) / 128) + d / 128, lane % 16 == 0);
     } else if (d < dim) {
       store_pack_of<A>(reinterpret_cast<T*>(a.out) + row * dim, h[n], d, dim);
@@ -247,7 +254,8 @@ __device__ __forceinline__ double sigmoid_of_full(float g) {
 
 // For 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is: g / (1 + t^2), and g
 // times t^2 of that below zero. The exponent's rounding is |g| / 2 times 2^-24 of t, so up to
-// |g| times that of the result.
+// |g| times that of the result: as many codes are others than the real quotients' as with the formula in fp32,
+// 1.2e-6 of them. With that and the reciprocal corrected 1.0e-6, but 81 us where it takes 74.
 __device__ __forceinline__ float silu(float g) {
   const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0x1.715476p-1f), f = g < 0.0f ? t : 1.0f;
   return g * f * (f * __builtin_amdgcn_rcpf(__builtin_fmaf(t, t, 1.0f)));
@@ -303,7 +311,7 @@ template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(c
       }
     }
     store_block<sizeof(T) == 4 ? FULL : GATED ? ROUNDED : GIVEN>(
-        y, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
+        y, 1.0f, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
         a.scales + (int64_t)rows[n] * blocks + ds[n] / 128, threadIdx.x % 16 == 0);
   }
 }
