@@ -8,13 +8,13 @@
 // Memory bounds both: a row is read once into registers, so that nothing is read again, and all of
 // its loads, the weight's too, are on their way before the first is used. What else is to be watched are the
 // instructions for each value: a wave's double takes one and its conversions take more.
-// fp32's sums, root, y and quotients are taken in 64 bits, and y is rounded once; 16-bit values'
-// in fp32, but for the sums of eight squares, whose range is any value's.
+// fp32's sums, root, y and quotients are taken in 64 bits, and a norm's y is rounded once; 16-bit values'
+// in fp32, but for the sums of eight squares, whose range is any value's, and for what fp32 does not tell.
 // Infinities and NaN become codes of NaN and do not count for a scale.
 //
 // 8192 rows of 4096 in bf16 with a residual, to codes: 49.8 us, 4.7 TB/s, with 55 % of the time in vector
 // instructions (in 64 bits all through 54.8); with 8 waves of one pack instead of 4 of two 51.1. 6063 rows
-// of 12288 in bf16, gated: 74 us, 5.1 TB/s and 78 % (in 64 bits, and with a division for every pack, 97). A
+// of 12288 in bf16, gated: 76 us, 4.9 TB/s. A
 // single row: 3 us.
 
 namespace mlc {
@@ -57,8 +57,8 @@ __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// What y is: of T's digits, or rounded to fp32 from more, or that of fp32 values.
-enum { GIVEN, ROUNDED, FULL };
+// What y is: of T's digits, or rounded to fp32 from more, or that of fp32 values, or some units of fp32 off.
+enum { GIVEN, ROUNDED, FULL, ROUGH };
 
 // The codes of a block of 128 values, 8 in each of 16 neighbouring lanes, of which the first
 // writes the scale. Lanes past the row's end have zeros and ``in`` false.
@@ -71,8 +71,14 @@ enum { GIVEN, ROUNDED, FULL };
 // Of values rounded to fp32 a quotient is rounded once more, by a factor of two floats, so that few codes are
 // others than the real quotients'. What all values have in common, ``factor``, is left to the scale: codes do
 // not depend on it.
+//
+// Of rough values, up to 30 units of 2^-23 off, one may be so near the middle of two codes that they do not tell which
+// is nearer: within NEAR units. Then nothing is stored and the result is true, for the whole block. It is
+// in 1 of 200 blocks, which are then taken in 64 bits: 6063 rows of 12288 76 us, without that 74.5, all of them 110.
+constexpr uint32_t NEAR = 32;
+
 template <int KIND>
-__device__ __forceinline__ void store_block(const float (&y)[8], float factor, bool in, uint8_t* codes,
+__device__ __forceinline__ bool store_block(const float (&y)[8], float factor, bool in, uint8_t* codes,
                                             float* scale_at, bool first) {
   float top = 0.0f;
 #pragma unroll
@@ -89,12 +95,25 @@ __device__ __forceinline__ void store_block(const float (&y)[8], float factor, b
     top = group_reduce<16, OpMax>(top);
   }
   float q[8];
-  if constexpr (KIND == GIVEN) {
+  if constexpr (KIND == GIVEN || KIND == ROUGH) {
     // 448 / top, whose reciprocal is a normal number: two roundings and the reciprocal's unit of a quotient
     const float by = __builtin_fminf(1.75f * __builtin_amdgcn_rcpf(top * 0x1p-8f), 0x1p126f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y[j] * by) + 0x20) & 0xffffffc0u);
+    for (int j = 0; j < 8; ++j) {
+      q[j] = y[j] * by;
+      if constexpr (KIND == GIVEN)
+        q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
+    }
+    if constexpr (KIND == ROUGH) {
+      uint32_t least = ~0u;  // of what lies behind a code's three digits, from NEAR below the middle on
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t behind = (__builtin_bit_cast(uint32_t, q[j]) << 12) - (0x80000000u - (NEAR << 12));
+        least = behind < least ? behind : least;
+      }
+      const uint64_t near = __ballot(least < NEAR << 13);
+      if (near >> (threadIdx.x & 48) & 0xffff) return true;
+    }
   } else {
     const double r = __builtin_amdgcn_rcp((double)top);
     double by = 448.0 * __builtin_fma(__builtin_fma(-(double)top, r, 1.0), r, r);  // NaN for zeros alone
@@ -112,6 +131,7 @@ __device__ __forceinline__ void store_block(const float (&y)[8], float factor, b
     *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
     if (first) *scale_at = __builtin_fmaxf(top * factor * (1.0f / 448.0f), 0x1p-126f);
   }
+  return false;
 }
 
 // 8 values of a row from d on, which end at ``dim``. A: bytes that packs lie on.
@@ -240,22 +260,68 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   }
 }
 
-// 1 / (1 + e^-g) for fp32's values, off by what the hardware's 2^h is for |h| up to 1/2: h is the rounded product
-// without its whole part, and corrected by what the rounding left (as exp_nonpos does).
-__device__ __forceinline__ double sigmoid_of_full(float g) {
-  const float x = __builtin_fminf(__builtin_fmaxf(-g, -104.0f), 690.0f), h = x * 0x1.715476p+0f;
-  float r = __builtin_fmaf(-h, 0x1.62e430p-1f, x);
-  r = __builtin_fmaf(-h, -0x1.05c610p-29f, r);
-  const float n = __builtin_rintf(h);
-  const double e = (double)__builtin_amdgcn_exp2f(h - n);
-  const double z = 1.0 + __builtin_amdgcn_ldexp(__builtin_fma(e, (double)r, e), (int)n), q = __builtin_amdgcn_rcp(z);
+// 1 / (1 + e^-g): 2^h from h's whole part and a polynomial of the rest, up to 1/2 to both sides, which is 2^-28 of
+// itself off (a least squares fit of degree 6, weighted for that).
+__device__ __forceinline__ double sigmoid(float g) {
+  const double h = __builtin_fmax(__builtin_fmin((double)g * -0x1.71547652b82fep+0, 1000.0), -1000.0);
+  const double n = __builtin_rint(h), f = h - n;
+  double p = 0x1.41c82d5786988p-13;
+  p = __builtin_fma(p, f, 0x1.5f69753d724cbp-10);
+  p = __builtin_fma(p, f, 0x1.3b2e341c3f47ep-7);
+  p = __builtin_fma(p, f, 0x1.c6ae81545310dp-5);
+  p = __builtin_fma(p, f, 0x1.ebfbd9497c82ap-3);
+  p = __builtin_fma(p, f, 0x1.62e431121ea6dp-1);
+  p = __builtin_fma(p, f, 0x1.00000003b033bp+0);
+  const double z = 1.0 + __builtin_amdgcn_ldexp(p, (int)n), q = __builtin_amdgcn_rcp(z);
   return __builtin_fma(__builtin_fma(-z, q, 1.0), q, q);  // one step of Newton's
 }
 
-// For 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is: g / (1 + t^2), and g
-// times t^2 of that below zero. The exponent's rounding is |g| / 2 times 2^-24 of t, so up to
-// |g| times that of the result: as many codes are others than the real quotients' as with the formula in fp32,
-// 1.2e-6 of them. With that and the reciprocal corrected 1.0e-6, but 81 us where it takes 74.
+// x of a lane of the same 16 by DPP, BY lanes on.
+template <int BY> __device__ __forceinline__ double turned(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x120 + BY, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), 0x120 + BY, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// store_block of values in 64 bits. What fp32 does not hold is an infinity.
+__device__ __forceinline__ void store_wide_block(const double (&y)[8], bool in, uint8_t* codes, float* scale_at,
+                                                 bool first) {
+  constexpr double MOST = 0x1.fffffep127;
+  double top = 0.0, zero = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    top = __builtin_fmax(top, __builtin_fabs(y[j]));
+    zero = __builtin_fma(y[j], 0.0, zero);  // or NaN
+  }
+  const bool odd = zero != 0.0 || top > MOST;
+  if (odd) {
+    top = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = __builtin_fabs(y[j]) <= MOST ? __builtin_fmax(top, __builtin_fabs(y[j])) : top;
+  }
+  top = __builtin_fmax(top, turned<8>(top));
+  top = __builtin_fmax(top, turned<4>(top));
+  top = __builtin_fmax(top, turned<2>(top));
+  top = __builtin_fmax(top, turned<1>(top));
+  const double r = __builtin_amdgcn_rcp(top);
+  const double by = __builtin_fmin(448.0 * __builtin_fma(__builtin_fma(-top, r, 1.0), r, r), 0x1p126);
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = (float)(y[j] * by);
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __builtin_fabs(y[j]) <= MOST ? q[j] : __builtin_nanf("");
+  }
+  if (in) {
+    *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
+    if (first) *scale_at = __builtin_fmaxf((float)(top * (1.0 / 448.0)), 0x1p-126f);
+  }
+}
+
+// g times that in fp32, for 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is:
+// g / (1 + t^2), and g times t^2 of that below zero. The exponent's rounding is |g| / 2 times 2^-24 of t, so up to
+// |g| times that of the result, for which 16 units and gates down to -35 are 30 of 2^-23.
 __device__ __forceinline__ float silu(float g) {
   const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0x1.715476p-1f), f = g < 0.0f ? t : 1.0f;
   return g * f * (f * __builtin_amdgcn_rcpf(__builtin_fmaf(t, t, 1.0f)));
@@ -300,19 +366,28 @@ template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(c
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const bool in = rows[n] < (uint32_t)a.rows && ds[n] < (uint32_t)a.dim;
-    float y[8];
+    uint8_t* const codes = reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n];
+    float* const scale = a.scales + (int64_t)rows[n] * blocks + ds[n] / 128;
+    if constexpr (GATED) {
+      if constexpr (sizeof(T) < 4) {
+        float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[j] = element<T>::widen(v[n][j]);
-      if constexpr (GATED && sizeof(T) < 4) y[j] *= silu(element<T>::widen(u[n][j]));
-      if constexpr (GATED && sizeof(T) == 4) {
-        const float gate = element<T>::widen(u[n][j]);
-        y[j] = (float)((double)y[j] * (double)gate * sigmoid_of_full(gate));
+        for (int j = 0; j < 8; ++j) y[j] = element<T>::widen(v[n][j]) * silu(element<T>::widen(u[n][j]));
+        if (!store_block<ROUGH>(y, 1.0f, in, codes, scale, threadIdx.x % 16 == 0)) continue;
       }
+      double y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float gate = element<T>::widen(u[n][j]);
+        y[j] = (double)element<T>::widen(v[n][j]) * (double)gate * sigmoid(gate);
+      }
+      store_wide_block(y, in, codes, scale, threadIdx.x % 16 == 0);
+    } else {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = element<T>::widen(v[n][j]);
+      store_block<sizeof(T) == 4 ? FULL : GIVEN>(y, 1.0f, in, codes, scale, threadIdx.x % 16 == 0);
     }
-    store_block<sizeof(T) == 4 ? FULL : GATED ? ROUNDED : GIVEN>(
-        y, 1.0f, in, reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n],
-        a.scales + (int64_t)rows[n] * blocks + ds[n] / 128, threadIdx.x % 16 == 0);
   }
 }
 

@@ -70,11 +70,10 @@ def check_eight(codes, scales, y, slack):
 
 
 def quantized(x, gate=None):
-    """What :func:`check_eight` takes. fp32: an exponential of 2 F, its correction's
-    second order and the result's rounding are within 12 F. 16-bit values': e^(-|g| / 2), twice, has an
+    """What :func:`check_eight` takes. fp32: in 64 bits, with a polynomial of 2^-28, within 2 F. 16-bit values': e^(-|g| / 2), twice, has an
     exponent that is 0.6 |g| F off, by the product's rounding and its factor's 0.22 F, and a unit of 2 F; with a sum,
     a reciprocal and four products that is within (16 + 1.25 |g|) F, until |g| = 175 leaves nothing."""
-    y, slack = _host(x), 12 * F
+    y, slack = _host(x), 2 * F
     if gate is not None:
         g = _host(gate)
         y = y * (g * torch.special.expit(g))
