@@ -59,7 +59,7 @@ __device__ __forceinline__ float of_order(uint32_t k) {
 }
 
 struct SampleLds {
-  alignas(16) char tail[32];  // the row's last pack
+  alignas(16) char tail[64];  // the row's last pack, and one of -infinity
   union {
     u64 bins[SAMPLE_BINS];  // and a list's weights
     uint32_t counts[SAMPLE_COUNTS + 64];
@@ -178,9 +178,9 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   const float min_p = a.min_p ? at<float>(a.min_p, a.m_off)[b * a.ms] : 0.0f;
   constexpr float NONE = -__builtin_inff();
 
-  // the row's last pack, with -infinity behind its end
+  // the row's last pack, with -infinity behind its end, and a whole pack of that
   T* const tail = reinterpret_cast<T*>(l.tail);
-  if (tid < 8) tail[tid] = size / 8 * 8 + tid < size ? row[size / 8 * 8 + tid] : element<T>::narrow(NONE);
+  if (tid < 16) tail[tid] = size / 8 * 8 + tid < size ? row[size / 8 * 8 + tid] : element<T>::narrow(NONE);
   __syncthreads();
   // f(8 logits, index of the first) of the packs of this thread from lo up to hi, a multiple of 8 from
   // lo or the row's end. One pack is on its way while one is in use.
@@ -208,7 +208,7 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
     for (int u = 0; u < 4; ++u) {
       const int at = i + u * SAMPLE_THREADS * 8;
       if (at + 8 <= size) load_n<(int)sizeof(T)>(x[u], row + at);
-      else load_n<16>(x[u], tail);  // again and again, past the end
+      else load_n<16>(x[u], at < size ? tail : tail + 8);  // the last one is one thread's, as in ``over``
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -325,7 +325,8 @@ template <class T> __device__ __forceinline__ void sample(const SampleArgs& a) {
   bool gathers = size <= SAMPLE_LIST;
   float from = NONE;
   if (!gathers && top_k && top_k <= SAMPLE_FEW) {
-    // as many threads as top_k have a token at or above the end of the bin, a 64th, of their top_k-th
+    // As many threads as top_k have a token at or above the end of the bin, a 64th, of their top_k-th: each one of
+    // its own packs, so that as many tokens are gathered.
     l.bins[tid] = 0;  // two counts
     __syncthreads();
     atomicAdd(&l.counts[(int)__builtin_fminf((top - own_top) * 64.0f, (float)(SAMPLE_BINS - 1))], 1u);
