@@ -142,12 +142,12 @@ __device__ __forceinline__ u64 sort_list(int n, SampleLds& l) {
 
 // e^((x - m) / T): 2^t goes to the hardware, with log2 e / T as two floats. t is rounded once.
 struct Weigh {
-  float m, hi, lo, least;  // the distance from which on a weight is 2^-64
+  float m, hi, lo, least;  // the distance, finite for a masked token too, from which on a weight is 0
   __device__ __forceinline__ Weigh(float m, float temperature) : m(m) {
     const double c = 1.4426950408889634074 / (double)temperature;
     hi = (float)c;
     lo = (float)(c - (double)hi);
-    least = -64.0f / hi;
+    least = -256.0f / hi;
   }
   __device__ __forceinline__ float operator()(float x) const {
     const float d = __builtin_fmaxf(x - m, least);

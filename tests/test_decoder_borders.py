@@ -12,6 +12,7 @@ from mlc import ops
 from test_decoder_operators import NEAR, TYPES, normal, options_of
 
 gpu = pytest.mark.gpu
+INF = float("inf")
 
 
 # --------------------------------------------------------------------------
@@ -46,3 +47,15 @@ def test_rows_whose_likely_tokens_lie_behind_the_last_whole_pack(dtype, size):
         for top_k in (2, 50, 512):
             for given in ({}, {"top_p": 0.9}, {"min_p": 0.01}, {"temperature": 0.8, "top_p": 0.95, "min_p": 0.002}):
                 check_shares(x, 257, top_k=top_k, **given)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_tokens_take_nothing_of_their_neighbours(dtype):
+    """A weight of 2^-41, half a step, beside masked tokens, at the random number 0."""
+    x = torch.full((1, 3000), -INF, dtype=dtype, device="cuda")
+    x[0, 8], x[0, 2992] = -41.0, 0.0
+    for given in ({}, {"top_k": 2000}, {"top_k": 600, "min_p": 0.0}):
+        # the temperature is log2 e, so that the weight is 2^-41
+        options = options_of(1, temperature=1.4426950408889634, **given)
+        assert ops.sample(x, torch.zeros(1, device="cuda"), **options).item() in (8, 2992)
