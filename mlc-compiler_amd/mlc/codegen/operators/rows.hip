@@ -14,7 +14,7 @@
 //
 // 8192 rows of 4096 in bf16 with a residual, to codes: 49.8 us, 4.7 TB/s, with 55 % of the time in vector
 // instructions (in 64 bits all through 54.8); with 8 waves of one pack instead of 4 of two 51.1. 6063 rows
-// of 12288 in bf16, gated: 76 us, 4.9 TB/s. A
+// of 12288 in bf16, gated: 75 us, 5.0 TB/s. A
 // single row: 3 us.
 
 namespace mlc {
@@ -57,8 +57,8 @@ __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// What y is: of T's digits, or rounded to fp32 from more, or that of fp32 values, or some units of fp32 off.
-enum { GIVEN, ROUNDED, FULL, ROUGH };
+// What y is: of T's digits, or rounded to fp32 from more, or that of fp32 values.
+enum { GIVEN, ROUNDED, FULL };
 
 // The codes of a block of 128 values, 8 in each of 16 neighbouring lanes, of which the first
 // writes the scale. Lanes past the row's end have zeros and ``in`` false.
@@ -71,14 +71,8 @@ enum { GIVEN, ROUNDED, FULL, ROUGH };
 // Of values rounded to fp32 a quotient is rounded once more, by a factor of two floats, so that few codes are
 // others than the real quotients'. What all values have in common, ``factor``, is left to the scale: codes do
 // not depend on it.
-//
-// Of rough values, up to 30 units of 2^-23 off, one may be so near the middle of two codes that they do not tell which
-// is nearer: within NEAR units. Then nothing is stored and the result is true, for the whole block. It is
-// in 1 of 200 blocks, which are then taken in 64 bits: 6063 rows of 12288 76 us, without that 74.5, all of them 110.
-constexpr uint32_t NEAR = 32;
-
 template <int KIND>
-__device__ __forceinline__ bool store_block(const float (&y)[8], float factor, bool in, uint8_t* codes,
+__device__ __forceinline__ void store_block(const float (&y)[8], float factor, bool in, uint8_t* codes,
                                             float* scale_at, bool first) {
   float top = 0.0f;
 #pragma unroll
@@ -95,24 +89,13 @@ __device__ __forceinline__ bool store_block(const float (&y)[8], float factor, b
     top = group_reduce<16, OpMax>(top);
   }
   float q[8];
-  if constexpr (KIND == GIVEN || KIND == ROUGH) {
+  if constexpr (KIND == GIVEN) {
     // 448 / top, whose reciprocal is a normal number: two roundings and the reciprocal's unit of a quotient
     const float by = __builtin_fminf(1.75f * __builtin_amdgcn_rcpf(top * 0x1p-8f), 0x1p126f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       q[j] = y[j] * by;
-      if constexpr (KIND == GIVEN)
-        q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
-    }
-    if constexpr (KIND == ROUGH) {
-      uint32_t least = ~0u;  // of what lies behind a code's three digits, from NEAR below the middle on
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t behind = (__builtin_bit_cast(uint32_t, q[j]) << 12) - (0x80000000u - (NEAR << 12));
-        least = behind < least ? behind : least;
-      }
-      const uint64_t near = __ballot(least < NEAR << 13);
-      if (near >> (threadIdx.x & 48) & 0xffff) return true;
+      q[j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, q[j]) + 0x20) & 0xffffffc0u);
     }
   } else {
     const double r = __builtin_amdgcn_rcp((double)top);
@@ -130,6 +113,39 @@ __device__ __forceinline__ bool store_block(const float (&y)[8], float factor, b
   if (in) {
     *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
     if (first) *scale_at = __builtin_fmaxf(top * factor * (1.0f / 448.0f), 0x1p-126f);
+  }
+}
+
+// store_block of gated 16-bit values in fp32, where that tells every code. A value is within (7.5 + 1.25 g) 2^-24 of
+// itself, with ``far`` this lane's largest g = -gate (``gated``). So is the largest, with that of the lanes that may have
+// it, and a quotient by four roundings more: 19 + 1.25 (g + g) units of 2^-23 of its power of two. Three digits behind
+// that power e4m3 ends, or below 2^-6 at 2^-9, where a value with 2^-6 added has its middles in the same place. Where
+// a quotient is so near to one nothing is stored and the result is true, for the whole block, which is then taken in 64
+// bits: 1 of 160 blocks, 6063 rows of 12288 75 us, as without that, all of them 110. So are infinities and NaN, gates
+// below -80, and blocks so small that fp32 loses digits.
+__device__ __forceinline__ bool store_rough_block(const float (&y)[8], float far, bool in, uint8_t* codes,
+                                                  float* scale_at, bool first) {
+  float own = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) own = __builtin_elementwise_maximum(own, __builtin_fabsf(y[j]));
+  const float top = group_reduce<16, OpMax>(own);
+  const float top_far = group_reduce<16, OpMax>(own < top * 0.9999f ? 0.0f : far);
+  const bool fine = far <= 80.0f && top < __builtin_inff() && (top >= 0x1p-60f || top == 0.0f);
+  const uint32_t near = (uint32_t)__builtin_fmaf(far + top_far, 1.25f, 21.0f) << 12, base = near - 0x80000000u;
+  const float by = 1.75f * __builtin_amdgcn_rcpf(__builtin_fmaxf(top, 0x1p-60f) * 0x1p-8f);
+  float q[8];
+  uint32_t least = ~0u;  // of what lies behind three digits, from ``near`` below the middle on
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    q[j] = y[j] * by;
+    const float m = __builtin_fabsf(q[j]);
+    const uint32_t behind = (__builtin_bit_cast(uint32_t, m + (m < 0x1p-6f ? 0x1p-6f : 0.0f)) << 12) + base;
+    least = behind < least ? behind : least;
+  }
+  if (__ballot(least < 2 * near || !fine) >> (threadIdx.x & 48) & 0xffff) return true;
+  if (in) {
+    *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
+    if (first) *scale_at = __builtin_fmaxf(top * (1.0f / 448.0f), 0x1p-126f);
   }
   return false;
 }
@@ -319,12 +335,11 @@ __device__ __forceinline__ void store_wide_block(const double (&y)[8], bool in, 
   }
 }
 
-// g times that in fp32, for 16-bit values, with t = e^(-|g| / 2), which is a normal number for all whose silu is:
-// g / (1 + t^2), and g times t^2 of that below zero. The exponent's rounding is |g| / 2 times 2^-24 of t, so up to
-// |g| times that of the result, for which 16 units and gates down to -35 are 30 of 2^-23.
-__device__ __forceinline__ float silu(float g) {
-  const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0x1.715476p-1f), f = g < 0.0f ? t : 1.0f;
-  return g * f * (f * __builtin_amdgcn_rcpf(__builtin_fmaf(t, t, 1.0f)));
+// x g times that in fp32, for 16-bit values and gates from -80 on. The exponent's roundings are 1.22 |g| 2^-24 of
+// e^-g, and of the result where that is large; its unit, a sum, a reciprocal's unit and two products are 7 more. Only x g
+// can leave fp32's range before the result does: upwards it is then infinite.
+__device__ __forceinline__ float gated(float x, float g) {
+  return x * g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -0x1.715476p+0f));
 }
 
 constexpr int QUANTIZE_BLOCK = 256, QUANTIZE_PACKS = 2;  // of 8 values, for each thread
@@ -368,25 +383,28 @@ template <class T, int A, bool GATED> __device__ __forceinline__ void quantize(c
     const bool in = rows[n] < (uint32_t)a.rows && ds[n] < (uint32_t)a.dim;
     uint8_t* const codes = reinterpret_cast<uint8_t*>(a.out) + (int64_t)rows[n] * a.dim + ds[n];
     float* const scale = a.scales + (int64_t)rows[n] * blocks + ds[n] / 128;
-    if constexpr (GATED) {
-      if constexpr (sizeof(T) < 4) {
-        float y[8];
+    float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = element<T>::widen(v[n][j]) * silu(element<T>::widen(u[n][j]));
-        if (!store_block<ROUGH>(y, 1.0f, in, codes, scale, threadIdx.x % 16 == 0)) continue;
+    for (int j = 0; j < 8; ++j) x[j] = element<T>::widen(v[n][j]);
+    if constexpr (GATED) {
+      float g[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = element<T>::widen(u[n][j]);
+      if constexpr (sizeof(T) < 4) {
+        float y[8], far = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[j] = gated(x[j], g[j]);
+          far = __builtin_fmaxf(far, -g[j]);
+        }
+        if (!store_rough_block(y, far, in, codes, scale, threadIdx.x % 16 == 0)) continue;
       }
       double y[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float gate = element<T>::widen(u[n][j]);
-        y[j] = (double)element<T>::widen(v[n][j]) * (double)gate * sigmoid(gate);
-      }
+      for (int j = 0; j < 8; ++j) y[j] = (double)x[j] * (double)g[j] * sigmoid(g[j]);
       store_wide_block(y, in, codes, scale, threadIdx.x % 16 == 0);
     } else {
-      float y[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = element<T>::widen(v[n][j]);
-      store_block<sizeof(T) == 4 ? FULL : GIVEN>(y, 1.0f, in, codes, scale, threadIdx.x % 16 == 0);
+      store_block<sizeof(T) == 4 ? FULL : GIVEN>(x, 1.0f, in, codes, scale, threadIdx.x % 16 == 0);
     }
   }
 }
