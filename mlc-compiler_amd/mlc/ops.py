@@ -702,7 +702,8 @@ def quantize_weight(weight):
     _require(k % 16 == 0 and k > 0, f"weight: a multiple of 16 inputs expected, got {k}")
     rows, blocks = decoder.blocks_of(n), decoder.blocks_of(k)
     with torch.no_grad():
-        whole = torch.zeros(rows * decoder.BLOCK, blocks * decoder.BLOCK, device=weight.device)
+        whole = torch.zeros(rows * decoder.BLOCK, blocks * decoder.BLOCK, dtype=torch.float32,
+                            device=weight.device)
         whole[:n, :k] = weight
         tiles = whole.view(rows, decoder.BLOCK, blocks, decoder.BLOCK)
         top = torch.where(tiles.isfinite(), tiles.abs(), 0.0).amax(dim=(1, 3))
@@ -779,8 +780,8 @@ class ScaledLinear(_KeepsTypes):
         self.register_buffer("codes", torch.zeros(outputs, inputs, dtype=torch.uint8, device=device)
                              .view(_E4M3))
         self.register_buffer("scales", torch.ones(decoder.blocks_of(outputs), decoder.blocks_of(inputs),
-                                                  device=device))
-        self.register_buffer("bias", torch.zeros(outputs, device=device) if bias else None)
+                                                  dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros(outputs, dtype=torch.float32, device=device) if bias else None)
 
     @classmethod
     def from_linear(cls, linear: torch.nn.Linear, dtype=None) -> "ScaledLinear":
@@ -816,7 +817,7 @@ class KeyValueCache(_KeepsTypes):
             self.register_buffer(name, torch.zeros(shape, dtype=torch.uint8, device=device)
                                  .view(_E4M3), persistent=False)
             self.register_buffer(f"{name[:-1]}_scales",
-                                 torch.ones(*shape[:2], capacity // block, device=device),
+                                 torch.ones(*shape[:2], capacity // block, dtype=torch.float32, device=device),
                                  persistent=False)
 
     def append(self, k, v, start, count=None) -> None:
