@@ -218,9 +218,11 @@ def plan_product(a: Operand, a_scales: Operand, b: Operand, b_scales: Operand, b
         grid, threads = _ceil(n, 16), 64 * waves
     else:
         tile, splits = choose_tile(rows, n, blocks, dtype)
-        reach = max(max(tile[:2]) * max(strides[1], b.strides[0], 4 * scale_strides[1]) if regular else
-                    max(_reach(a, strides), _reach(a_scales, scale_strides), max(tile[:2]) * b.strides[0]),
-                    4 * a_scales.strides[-1] * blocks) + k
+        # bytes from where the kernel counts to the end of a row, or to a row's last scale
+        most = max(tile[:2])
+        far, scales_far = ((most * strides[1], most * 4 * scale_strides[1]) if regular
+                           else (_reach(a, strides), _reach(a_scales, scale_strides)))
+        reach = max(max(far, most * b.strides[0]) + k, scales_far + 4 * a_scales.strides[-1] * blocks)
         if reach >= 1 << 31:
             raise OperatorError("scaled_product: rows that lie too far apart: make them contiguous")
         row_tiles = _ceil(rows, tile[0])
