@@ -78,6 +78,23 @@ struct Slab {
   bool is_static = false;
 };
 
+// While this thread or another captures a stream, freeing memory or a module is refused and ends that capture, unless
+// the calling thread says that it knows what it frees: what belongs to a runtime that nobody holds any longer, as
+// one of which a pass is recorded has to be held.
+class OutsideCaptures {
+ public:
+  OutsideCaptures() { held_ = hipThreadExchangeStreamCaptureMode(&mode_) == hipSuccess; }
+  ~OutsideCaptures() {
+    if (held_) (void)hipThreadExchangeStreamCaptureMode(&mode_);
+  }
+  OutsideCaptures(const OutsideCaptures&) = delete;
+  OutsideCaptures& operator=(const OutsideCaptures&) = delete;
+
+ private:
+  hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
+  bool held_ = false;
+};
+
 void slab_release(Slab* s) {
   if (s == nullptr) return;
   if (s->is_static) {
@@ -86,6 +103,7 @@ void slab_release(Slab* s) {
   }
   if (s->refs.fetch_sub(1) == 1) {
     if (s->ptr != nullptr) {
+      const OutsideCaptures outside;
       int prev = 0;
       (void)hipGetDevice(&prev);
       (void)hipSetDevice(s->device);
@@ -237,6 +255,7 @@ int mlc_ctx_create(int device, mlc_ctx** out) {
 
 int mlc_ctx_destroy(mlc_ctx* ctx) {
   if (ctx == nullptr) return MLC_OK;
+  const OutsideCaptures outside;
   (void)hipSetDevice(ctx->device);
   if (ctx->exec != nullptr) (void)hipGraphExecDestroy(ctx->exec);
   if (ctx->graph != nullptr) (void)hipGraphDestroy(ctx->graph);
@@ -265,6 +284,7 @@ int mlc_module_load(mlc_ctx* ctx, const void* image, size_t size, mlc_module** o
 
 int mlc_module_unload(mlc_module* mod) {
   if (mod == nullptr) return MLC_OK;
+  const OutsideCaptures outside;
   (void)hipSetDevice(mod->device);
   hipError_t e = hipModuleUnload(mod->mod);
   delete mod;
