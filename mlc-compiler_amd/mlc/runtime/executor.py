@@ -48,6 +48,7 @@ import torch
 from ..config import Config
 from ..ir.graph import Graph, Value
 from ..kernels import ExternKernel, Schedule
+from . import hip_runtime
 
 
 #: launches of a pass above which it is always a graph
@@ -336,9 +337,7 @@ class CompiledModel:
         self.device = torch.device(device)
         if runner is None:
             self.backend = select_backend(cfg, self.device)
-            from .hip_runtime import HipRuntime
-
-            self._module = HipRuntime(schedule, cfg, self.device)
+            self._module = hip_runtime.HipRuntime(schedule, cfg, self.device)
         else:
             self.backend, self._module = getattr(runner, "name", "custom"), runner
         # library calls reading no tensor always give the same result: they run
@@ -608,6 +607,8 @@ class CompiledModel:
         return self._collect(table)
 
     def __call__(self, *inputs: torch.Tensor):
+        if hip_runtime._late:
+            hip_runtime.close_late()
         self._raise_pending()
         if not (self.cfg.cuda_graphs and self.device.type == "cuda"):
             out = self.forward(*inputs)

@@ -56,8 +56,17 @@ _late: list[HipRuntime] = []
 
 
 def close_late() -> None:
-    while _late:
-        _late.pop().close()
+    """Close them, unless the current stream captures. Any thread may come by; whether one
+    of them closes is no matter of the call that happens to."""
+    while _late and not torch.cuda.is_current_stream_capturing():
+        try:
+            runtime = _late.pop()
+        except IndexError:  # another thread has taken the last one
+            return
+        try:
+            runtime.close()
+        except Exception:
+            pass
 
 
 @dataclass
@@ -104,8 +113,7 @@ class HipRuntime:
         self.device = device
         self.index = device.index if device.index is not None else torch.cuda.current_device()
         self.lib = native.load_library()
-        if not torch.cuda.is_current_stream_capturing():
-            close_late()
+        close_late()
         self.module = build_module(schedule, cfg)
         #: the generated HIP module text (``TritonRuntime.source``)
         self.source: str = self.module.source

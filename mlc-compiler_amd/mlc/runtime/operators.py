@@ -144,6 +144,9 @@ def raise_pending(modules: OperatorModules) -> None:
 
 def check_errors() -> None:
     """Wait for every device that operators ran on and raise for an invalid input."""
+    from . import hip_runtime
+
+    hip_runtime.close_late()
     for index, modules in list(_devices.items()):
         torch.cuda.synchronize(index)
         if modules.pending():

@@ -49,3 +49,65 @@ def test_a_compiled_step_that_is_collected_beside_a_capture(where):
         assert all(torch.equal(x, y) for x, y in zip(eager, want)) and torch.equal(twice, want[1] * 2.0)
     ops.check_errors()
     assert not hip_runtime._late
+
+
+def _runtime(close):
+    r = hip_runtime.HipRuntime.__new__(hip_runtime.HipRuntime)
+    r.close = close
+    return r
+
+
+def test_runtimes_are_closed_by_whoever_comes_first(monkeypatch):
+    """Another thread may take the last one between a look and the taking."""
+    class Taken(list):
+        def __len__(self):
+            return 1
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(hip_runtime, "_late", Taken())
+    hip_runtime.close_late()
+
+
+def test_a_runtime_that_does_not_close_is_nobody_elses_matter(monkeypatch):
+    closed, late = [], []
+
+    def fails():
+        raise RuntimeError("not closed")
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(hip_runtime, "_late", late)
+    late += [_runtime(lambda: closed.append(1)), _runtime(fails), _runtime(lambda: closed.append(2))]
+    hip_runtime.close_late()
+    assert set(closed) == {1, 2} and not late
+
+
+def test_late_runtimes_are_closed_by_a_wait_outside_of_captures(monkeypatch):
+    """Where nothing is compiled any more their memory would stay."""
+    closed, late, capturing = [], [], [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(hip_runtime, "_late", late)
+    late.append(_runtime(lambda: closed.append(1)))
+    ops.check_errors()
+    assert not closed
+    capturing[0] = False
+    ops.check_errors()
+    assert closed and not late
+
+
+@gpu
+def test_late_runtimes_are_closed_by_a_compiled_call():
+    args = step_inputs(tokens=3)
+    kept, held = mlc.compile(Step().cuda(), args), [mlc.compile(Step().cuda(), args)]
+    for compiled in (kept, *held):
+        compiled(*args)
+    compiled = None
+    x = torch.ones(4, device="cuda")
+    x * 2.0
+    gc.collect()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x * 2.0
+        held.clear()
+        gc.collect()
+    assert hip_runtime._late
+    kept(*args)
+    assert not hip_runtime._late
