@@ -76,9 +76,10 @@ def test_a_runtime_that_does_not_close_is_nobody_elses_matter(monkeypatch):
 
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(hip_runtime, "_late", late)
-    late += [_runtime(lambda: closed.append(1)), _runtime(fails), _runtime(lambda: closed.append(2))]
+    held = [_runtime(lambda: closed.append(1)), _runtime(fails), _runtime(lambda: closed.append(2))]
+    late += held  # what is held does not end by itself, which would swallow the failure
     hip_runtime.close_late()
-    assert set(closed) == {1, 2} and not late
+    assert sorted(closed) == [1, 2] and not late
 
 
 def test_late_runtimes_are_closed_by_a_wait_outside_of_captures(monkeypatch):
