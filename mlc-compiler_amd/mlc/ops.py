@@ -720,8 +720,14 @@ def scaled_product(a, a_scales, b, b_scales, bias=None, *, dtype=torch.bfloat16)
         out[m, n] = sum_j a[m, j] * a_scales[m, j / 128] * b[n, j] * b_scales[n / 128, j / 128] + bias[n]
 
     Scales are float32, ``[..., ceil(k / 128)]`` (:func:`quantize`) and ``[ceil(outputs / 128),
-    ceil(k / 128)]`` (:func:`quantize_weight`), of any value; ``bias [outputs]`` is in ``dtype`` or
-    float32. The result is ``dtype``: float16, bfloat16 or float32. Sums are held in fp32.
+    ceil(k / 128)]`` (:func:`quantize_weight`), of any value; a block's two are multiplied in fp32. ``bias
+    [outputs]`` is in ``dtype`` or float32. The result is ``dtype``: float16, bfloat16 or float32.
+
+    Sums are held in fp32. In float32, and for few rows in any type, every product counts whole.
+    In float16 and bfloat16 of more rows the matrix units take eight neighbouring products at once and
+    cut each at 2^-13 of the largest one's power of two: a random sum is 1.3e-5 to 3e-5 of itself off, but one of
+    large terms that cancel by as much of those, and a row's result depends in its last places on how many rows
+    come with it.
     """
     number = _result_number(dtype)
     out = _now("scaled_product", (a, a_scales, b, b_scales, bias), (number,), 1)

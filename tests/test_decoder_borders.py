@@ -182,3 +182,27 @@ def test_every_code_of_values_and_gates_far_apart(dtype):
         fine = gated(a, b).abs().view(512, 2, 128).amax(-1).repeat_interleave(128, 1) < 2.0 ** 127
         a = torch.where(fine, a, 1.0)  # of what is beyond fp32 the codes are NaN
         check_codes(ops.quantize(a, b)[0], gated(a, b), 2 * F)
+
+
+# --------------------------------------------------------------------------
+# sums whose large terms cancel
+# --------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", (4, 40, 300))
+def test_products_whose_large_terms_cancel(dtype, rows):
+    """What is left of pairs of opposite terms shows how products are added: whole in fp32 and for few rows, else each
+    cut at 2^-13 of the largest of eight (``groups``)."""
+    n, k = 200, 1024
+    a = normal(rows, k, dtype=FULL, seed=12).clamp(-3, 3)
+    a[:, ::4] *= 100.0
+    a[:, 1::4] = a[:, ::4]
+    b = normal(n, k, dtype=FULL, seed=13).clamp(-3, 3)
+    b[:, ::4] *= 100.0
+    b[:, 1::4] = -b[:, ::4]
+    a, b = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+    a_scales, b_scales = torch.ones(rows, 8, device="cuda"), torch.ones(2, 8, device="cuda")
+    want, *bounds = ref.product(a, a_scales, b, b_scales)
+    got = ops.scaled_product(a, a_scales, b, b_scales, dtype=dtype)
+    ref.check_product(got, want, *bounds, dtype)
