@@ -9,7 +9,10 @@
 // ``uniform`` of the kept weight lies.
 //
 // Sums are of whole numbers of 2^-40, so they are exact whatever their order: results do not depend
-// on the order of atomics.
+// on the order of atomics. What is rounded to one is a token's weight where tokens lie in a list, and in passes over a
+// row the weight of eight neighbouring tokens, added in fp32: beside a weight of 1 one of 2^-25 counts as nothing
+// there, and sums are up to 2^-21 of themselves off. With each token's own, in 64 bits, 256 rows of 131072 with top_p take
+// 61 us instead of 54, without options 29 instead of 26.
 //
 // A workgroup has a row: no word passes between workgroups, one launch does it, and 256 rows fill the card. Only
 // the first pass, for the largest logit, is bound by memory; then caches hold the row, and each instruction of

@@ -750,10 +750,12 @@ def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=N
     * ``min_p`` (float32[batch]): of those the ones of ``min_p`` times the largest weight or more.
 
     The token is the first, by index, up to which more than ``uniform`` of the kept weight lies.
-    Weights count in steps of 2^-40 of the largest. Logits of -infinity are never taken; a row of
-    nothing else gets -1. So does a row with NaN or +infinity among its logits, a random number
-    outside its range, or an option that is NaN, negative or, for ``top_p`` and ``min_p``, above 1,
-    for the temperature above 2^100: ``ExecutionError`` is raised by a later call or :func:`check_errors`.
+    Weights count in steps of 2^-40 of the largest, and of 2^-24 of the weight of the eight neighbouring
+    tokens that they may be added with in fp32: one of 2^-25 beside one of 1 may never be drawn. A token whose
+    border lies within 2^-20 of the random number, or of ``top_p`` or ``min_p``, may go to either side. Logits of
+    -infinity are never taken; a row of nothing else gets -1. So does a row with NaN or +infinity among its
+    logits, a random number outside its range, or an option that is NaN, negative or, for ``top_p`` and ``min_p``,
+    above 1, for the temperature above 2^100: ``ExecutionError`` is raised by a later call or :func:`check_errors`.
     """
     out = _now("sample", (logits, uniform, temperature, top_k, top_p, min_p), (), 1)
     if out is not None:

@@ -63,6 +63,19 @@ def test_masked_tokens_take_nothing_of_their_neighbours(dtype):
         assert ops.sample(x, torch.zeros(1, device="cuda"), **options).item() in (8, 2992)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_weights_beside_a_large_one(dtype):
+    """Eight tokens that a pass over the row adds in fp32, of which seven have 2^-18 of the first: a random number in
+    the middle of a token's share, 2^-19 from both ends, draws it."""
+    x = torch.full((1, 3000), -INF, dtype=dtype, device="cuda")
+    x[0, 64], x[0, 65:72] = 0.0, -18.0
+    uniform = torch.tensor([(1 + (i + 0.5) * 2.0 ** -18) / (1 + 7 * 2.0 ** -18) for i in range(7)]).cuda()
+    for given in ({}, {"top_p": 0.9999999}, {"top_k": 600}, {"min_p": 2.0 ** -20}):
+        options = options_of(7, temperature=1.4426950408889634, **given)  # weights of 2^x
+        assert ops.sample(x.expand(7, -1), uniform, **options).tolist() == list(range(65, 72))
+
+
 # --------------------------------------------------------------------------
 # the code that a quotient goes to
 # --------------------------------------------------------------------------
