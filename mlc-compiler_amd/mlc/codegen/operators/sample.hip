@@ -143,7 +143,8 @@ __device__ __forceinline__ u64 sort_list(int n, SampleLds& l) {
   return own;
 }
 
-// e^((x - m) / T): 2^t goes to the hardware, with log2 e / T as two floats. t is rounded once.
+// e^((x - m) / T): 2^t goes to the hardware, with log2 e / T as two floats. t is rounded once. Weights do not rise
+// where logits fall (looked at for every t from 0 to -128), so that what min_p keeps is in front of the rest.
 struct Weigh {
   float m, hi, lo, least;  // the distance, finite for a masked token too, from which on a weight is 0
   __device__ __forceinline__ Weigh(float m, float temperature) : m(m) {
