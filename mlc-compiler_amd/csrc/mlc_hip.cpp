@@ -95,6 +95,24 @@ class OutsideCaptures {
   bool held_ = false;
 };
 
+// Where something is freed, which may be in anybody's call: the caller's device is the current one again afterwards.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    held_ = hipGetDevice(&before_) == hipSuccess;
+    (void)hipSetDevice(device);
+  }
+  ~OnDevice() {
+    if (held_) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+
+ private:
+  int before_ = 0;
+  bool held_ = false;
+};
+
 void slab_release(Slab* s) {
   if (s == nullptr) return;
   if (s->is_static) {
@@ -104,11 +122,8 @@ void slab_release(Slab* s) {
   if (s->refs.fetch_sub(1) == 1) {
     if (s->ptr != nullptr) {
       const OutsideCaptures outside;
-      int prev = 0;
-      (void)hipGetDevice(&prev);
-      (void)hipSetDevice(s->device);
+      const OnDevice there(s->device);
       (void)hipFree(s->ptr);
-      (void)hipSetDevice(prev);
     }
     delete s;
   }
@@ -256,7 +271,7 @@ int mlc_ctx_create(int device, mlc_ctx** out) {
 int mlc_ctx_destroy(mlc_ctx* ctx) {
   if (ctx == nullptr) return MLC_OK;
   const OutsideCaptures outside;
-  (void)hipSetDevice(ctx->device);
+  const OnDevice there(ctx->device);
   if (ctx->exec != nullptr) (void)hipGraphExecDestroy(ctx->exec);
   if (ctx->graph != nullptr) (void)hipGraphDestroy(ctx->graph);
   slab_release(ctx->slab);
@@ -285,7 +300,7 @@ int mlc_module_load(mlc_ctx* ctx, const void* image, size_t size, mlc_module** o
 int mlc_module_unload(mlc_module* mod) {
   if (mod == nullptr) return MLC_OK;
   const OutsideCaptures outside;
-  (void)hipSetDevice(mod->device);
+  const OnDevice there(mod->device);
   hipError_t e = hipModuleUnload(mod->mod);
   delete mod;
   if (e != hipSuccess) return hip_fail(e, "hipModuleUnload");

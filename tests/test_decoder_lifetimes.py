@@ -112,3 +112,17 @@ def test_late_runtimes_are_closed_by_a_compiled_call():
     assert hip_runtime._late
     kept(*args)
     assert not hip_runtime._late
+
+
+@gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_a_runtime_that_is_closed_leaves_the_current_device():
+    last = torch.device("cuda", torch.cuda.device_count() - 1)
+    model = torch.nn.Sequential(torch.nn.Linear(64, 64), torch.nn.ReLU()).to(last)
+    with torch.cuda.device(last):
+        held = [mlc.compile(model, (torch.ones(2, 64, device=last),))]
+        held[0](torch.ones(2, 64, device=last))
+    torch.cuda.set_device(0)
+    held.clear()
+    gc.collect()
+    assert torch.cuda.current_device() == 0
