@@ -112,7 +112,7 @@ __device__ __forceinline__ void store_block(const float (&y)[8], float factor, b
   }
   if (in) {
     *reinterpret_cast<uint2v*>(codes) = uint2v{to_e4m3(q[0], q[1], q[2], q[3]), to_e4m3(q[4], q[5], q[6], q[7])};
-    if (first) *scale_at = __builtin_fmaxf(top * factor * (1.0f / 448.0f), 0x1p-126f);
+    if (first) *scale_at = __builtin_fmaxf(top * (1.0f / 448.0f) * factor, 0x1p-126f);
   }
 }
 
@@ -245,8 +245,9 @@ __device__ __forceinline__ void rms_norm(const RowsArgs& a) {
   auto weight = [&](int n, int j) { return sizeof(T) < 4 && a.wide_weight ? wide[n][j] : element<T>::widen(z[n][j]); };
   float factor = 1.0f;
   if constexpr (sizeof(T) < 4) {
-    // a power of two near the root goes into h, so that the reciprocal is a normal number whatever the root
-    const int power = __builtin_amdgcn_frexp_exp(mean) >> 1;
+    // A power of two near the root goes into h, so that the reciprocal is a normal number whatever the root: from 1 to 2,
+    // so that h times the weight is not beyond fp32 where the norm is not.
+    const int power = (__builtin_amdgcn_frexp_exp(mean) + 1) >> 1;
     const float by = __builtin_amdgcn_rsqf((float)__builtin_amdgcn_ldexp(mean, -2 * power));
     factor = by;
 #pragma unroll

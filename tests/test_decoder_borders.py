@@ -106,7 +106,7 @@ def check_codes(codes, y, bound):
         want, distance = nearest(q)
         wrong = (got & 127) != want
         assert not (wrong & ((distance > bound) | (bound == 0))).any(), \
-            (int(wrong.sum()), distance[wrong].max().log2(), q[wrong][:4], LADDER[(got & 127).long()][wrong][:4])
+            (int(wrong.sum()), distance[wrong].max().log2(), q[wrong][:4], got[wrong][:4])
         assert ((got >> 7 == 1) == (part < 0))[want > 0].all()
 
 
@@ -219,3 +219,25 @@ def test_products_whose_large_terms_cancel(dtype, rows):
     want, *bounds = ref.product(a, a_scales, b, b_scales)
     got = ops.scaled_product(a, a_scales, b, b_scales, dtype=dtype)
     ref.check_product(got, want, *bounds, dtype)
+
+
+# --------------------------------------------------------------------------
+# norms near the end of fp32
+# --------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norms_near_the_largest_values(dtype):
+    """Weights near fp32's largest: a norm that fp32 holds has codes and a scale, whatever the row's root is."""
+    for size in (0.6, 0.7, 0.8, 1.0, 1.3, 1.5, 3.0, 1000.0):
+        sign = normal(4, 256, dtype=FULL, seed=14).sign()
+        x = (size * sign).to(dtype)
+        w = torch.full((256,), 3.0e38, device="cuda")
+        w[::3] = 1.0e38
+        w[130:] = 1.0
+        codes, scales = ops.rms_norm(x, w, quantized=True)
+        y, _ = ref.norm(x, w)
+        # a rounding of the weight's product, of the largest's and of the quotient
+        check_codes(codes, y, 6 * F)
+        want = y.abs().view(4, 2, 128).amax(-1) / 448
+        assert ((scales.cpu().double() - want).abs() <= 16 * F * want).all()
