@@ -662,7 +662,7 @@ def rms_norm(x, weight, residual=None, *, eps: float = 1e-6, quantized: bool = F
     """``h / sqrt(mean(h^2) + eps) * weight`` for rows ``h`` of ``x [rows, dim]`` or
     ``[batch, tokens, dim]`` (fp16, bf16 or fp32, ``dim`` up to 32768), with ``weight``
     ``[dim]`` in the type of ``x`` or float32. With ``residual``, of the shape and type of
-    ``x``, ``h = x + residual``, and the sum, rounded to that type, comes back behind the
+    ``x``, ``h = x + residual`` in fp32, and the sum, rounded to that type, comes back behind the
     norm; the norm itself is taken of the sum as it is before that.
 
     Returns the norm in the type of ``x``, or with ``quantized`` (``dim`` a multiple of 16)
